@@ -23,6 +23,7 @@ LIB_PATH = os.environ.get("FORTAI_HIP_LIBRARY") or \
 OK, INVALID, RUNTIME_ERROR = 0, 1, 2
 
 _vp, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
+_d = C.c_double
 _fp, _i64p, _u16p = C.POINTER(C.c_float), C.POINTER(C.c_int64), C.POINTER(C.c_uint16)
 _vpp = C.POINTER(C.c_void_p)
 
@@ -121,6 +122,9 @@ _SIGNATURES = {
     "fortai_hip_qwen35_decoder_set_mode": [_vp, _i],
     "fortai_hip_qwen35_batch_set_mode": [_vp, _i],
     "fortai_hip_qwen35_batch_set_prefill_mode": [_vp, _i],
+    "fortai_hip_rope_create": [_vp, _i, _i, _d, _i, _d, _i, _d, _d, _d, _vpp],
+    "fortai_hip_rope_destroy": [_vp],
+    "fortai_hip_rope_device": [_vp, _i, _vp, _i64, _i64, _i, _i, _i, _vp, _vp, _f, _vp, _i64, _i64],
 }
 _RESTYPE = {"fortai_hip_q8_last_error": C.c_char_p, "fortai_hip_q8_tokens_bytes": C.c_size_t,
             "fortai_hip_q8_pack_bytes": C.c_size_t}
@@ -133,6 +137,8 @@ DECODER_DIRECT = 1
 DECODER_MATVEC_ONLY = 2
 DECODER_FAMILIES = {"matvec": 2, "gdn": 4, "attention": 8, "head": 16}
 PREFILL_MODES = {"exact": 0, "matvec": 1, "fast": 2}
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 
 
 class BackendError(RuntimeError):
@@ -568,4 +574,42 @@ class BatchDecoder:
     def free(self) -> None:
         if self.h:
             self.ctx.lib.fortai_hip_qwen35_batch_destroy(self.h)
+            self.h = None
+
+
+def _dev(x):
+    """A device address: None, an integer (a tensor's data_ptr()), a c_void_p or a DeviceBuffer."""
+    return x.h if isinstance(x, DeviceBuffer) else x
+
+
+class Rope:
+    """Rotary positions of query and key heads, with an optional per-head RMSNorm
+    in front.  ``scaling``: 'none', 'linear' (factor) or 'yarn' (factor,
+    original_context, beta_fast, beta_slow)."""
+
+    def __init__(self, ctx: Context, rope_dim: int, interleaved: bool = False, base: float = 1.0e4,
+                 scaling: str = "none", factor: float = 1.0, original_context: int = 0, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, attention_factor: float = 1.0):
+        self.ctx, self.rope_dim = ctx, rope_dim
+        h = C.c_void_p()
+        ctx.call("fortai_hip_rope_create", ctx.h, rope_dim, 1 if interleaved else 0, base, ROPE_SCALINGS[scaling],
+                 factor, original_context, beta_fast, beta_slow, attention_factor, C.byref(h))
+        self.h = h
+
+    def apply(self, x, positions, rows: int, heads: int, head_size: int, out, dtype: str = "f32",
+              row_pitch: Optional[int] = None, head_pitch: Optional[int] = None, out_row_pitch: Optional[int] = None,
+              out_head_pitch: Optional[int] = None, norm=None, eps: float = 1e-6) -> None:
+        """x [rows][heads][head_size] (dense unless pitches are given) at
+        positions[rows] (int32) -> out; out may be x itself."""
+        hp = head_size if head_pitch is None else head_pitch
+        rp = heads * hp if row_pitch is None else row_pitch
+        ohp = head_size if out_head_pitch is None else out_head_pitch
+        orp = heads * ohp if out_row_pitch is None else out_row_pitch
+        self.ctx.check(self.ctx.lib.fortai_hip_rope_device(self.h, DTYPES[dtype], _dev(x), rp, hp, rows, heads,
+                                                           head_size, _dev(positions), _dev(norm), eps, _dev(out),
+                                                           orp, ohp), "fortai_hip_rope_device")
+
+    def free(self) -> None:
+        if self.h:
+            self.ctx.lib.fortai_hip_rope_destroy(self.h)
             self.h = None

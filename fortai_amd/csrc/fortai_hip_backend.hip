@@ -6,6 +6,7 @@
 // (backend/cuda/fortai_cuda_backend.cu:805-1736) in arguments, ownership and
 // return codes; each carries the citation of the function it replaces.
 #include "../../include/fortai_hip_backend.h"
+#include "fortai_hip_context.h"
 #include "fortai_hip_internal.h"
 #include "fortai_hip_kernels.h"
 
@@ -31,29 +32,6 @@ constexpr int kArgmaxParts = 4096;
 struct plan_step {
     std::string operation, kernel;
     int batch = 1;
-};
-
-struct fortai_hip_q8_context {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    hipEvent_t start = nullptr, stop = nullptr;
-    int *position = nullptr;    // device: current token position
-    int64_t *token = nullptr;   // device: current token id
-    int8_t *scratch_act = nullptr;
-    size_t scratch_act_bytes = 0;
-    float *scratch_out = nullptr;
-    size_t scratch_out_bytes = 0;
-    float *scratch_aux = nullptr;
-    size_t scratch_aux_bytes = 0;
-    float *argmax_value = nullptr;
-    int32_t *argmax_index = nullptr;
-    void *scratch_q8l = nullptr;  // quantized FFN hidden of the ABI FFN paths
-    size_t scratch_q8l_bytes = 0;
-    void *noalloc_scratch = nullptr;  // device address of this GPU's `scratch` array (set at create)
-    hipEvent_t noalloc_done = nullptr;  // recorded after this context's last use of that array
-    hipGraph_t graph = nullptr;
-    hipGraphExec_t graph_exec = nullptr;
-    char error[256] = {};
 };
 
 struct fortai_hip_q8_weights {
@@ -201,14 +179,6 @@ struct fortai_hip_qwen35_batch {
 
 namespace {
 
-int fail(fortai_hip_q8_context *ctx, int code, const char *op, hipError_t err = hipSuccess) {
-    if (ctx) {
-        if (err == hipSuccess) std::snprintf(ctx->error, sizeof(ctx->error), "%s", op);
-        else std::snprintf(ctx->error, sizeof(ctx->error), "%s: %s", op, hipGetErrorString(err));
-    }
-    return code;
-}
-
 thread_local unsigned g_families = kFamAll;
 inline bool fam(unsigned f) { return (g_families & f) != 0; }
 // PlanIR recording (src/fortai_plan_ir.f90:7-21): while a plan is being
@@ -241,23 +211,6 @@ int copy_plan(const std::vector<plan_step> &plan, char *buffer, size_t bytes, si
     if (bytes < t.size() + 1) return FORTAI_HIP_INVALID;
     std::memcpy(buffer, t.c_str(), t.size() + 1);
     return FORTAI_HIP_OK;
-}
-
-int done(fortai_hip_q8_context *ctx, hipError_t err, const char *op) {
-    return err == hipSuccess ? FORTAI_HIP_OK : fail(ctx, FORTAI_HIP_RUNTIME_ERROR, op, err);
-}
-
-template <typename T>
-hipError_t alloc(T **ptr, size_t count) {
-    *ptr = nullptr;
-    if (count == 0) return hipSuccess;
-    return hipMalloc(reinterpret_cast<void **>(ptr), count * sizeof(T));
-}
-
-template <typename T>
-void release(T *&ptr) {
-    if (ptr) (void)hipFree(ptr);
-    ptr = nullptr;
 }
 
 // The planes of several Q8_0 matrices of one width, one after the other, as

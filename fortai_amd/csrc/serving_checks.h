@@ -1,0 +1,93 @@
+// Argument checks and launch rules of the serving operators, free of device
+// code so that they also compile for the host alone.  A check returns what is
+// wrong with the arguments, or nullptr.
+#pragma once
+
+#include <cmath>
+#include <cstddef>
+#include <cstdint>
+
+namespace fortai_hip {
+
+constexpr int64_t kMaxPitch = int64_t{1} << 31;  // elements: products with int counts stay within 64 bits
+constexpr int kMaxRows = 1 << 23;                // a launch's threads stay below 2^32
+
+inline bool dtype_ok(int d) { return d >= 0 && d <= 2; }
+inline size_t dtype_bytes(int d) { return d == 0 ? 4 : 2; }
+inline bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline bool pitch_ok(int64_t pitch) { return pitch >= 0 && pitch <= kMaxPitch; }
+
+// Whether rows x heads vectors of `head` elements at these pitches touch no
+// element twice (either pitch may be the outer one).
+inline bool apart(int64_t rows, int64_t heads, int64_t head, int64_t row_pitch, int64_t head_pitch) {
+    const bool by_row = (heads == 1 || head_pitch >= head) &&
+        (rows == 1 || row_pitch >= (heads - 1) * (heads == 1 ? 0 : head_pitch) + head);
+    const bool by_head = (rows == 1 || row_pitch >= head) &&
+        (heads == 1 || head_pitch >= (rows - 1) * (rows == 1 ? 0 : row_pitch) + head);
+    return by_row || by_head;
+}
+
+// Whether four consecutive elements at this address and at every multiple of
+// these pitches are aligned to all four.
+inline bool vector4_ok(const void *p, int dtype, int64_t pitch_a, int64_t pitch_b) {
+    return aligned(p, 4 * dtype_bytes(dtype)) && pitch_a % 4 == 0 && pitch_b % 4 == 0;
+}
+
+// ---------------------------------------------------------- rotary positions
+inline const char *check_rope_create(int rope_dimension, double base, int scaling, double factor, int original_context,
+    double beta_fast, double beta_slow, double attention_factor) {
+    if (rope_dimension < 2 || rope_dimension > 256 || rope_dimension % 2) return "rope: dimension even, 2 to 256";
+    if (!(base > 0.0) || !std::isfinite(base)) return "rope: base above 0";
+    if (!(attention_factor > 0.0) || !std::isfinite(attention_factor)) return "rope: attention factor above 0";
+    if (scaling < 0 || scaling > 2) return "rope: unknown scaling";
+    if (scaling != 0 && (!(factor > 0.0) || !std::isfinite(factor))) return "rope: scaling factor above 0";
+    if (scaling == 2 && (original_context < 1 || !(base > 1.0) || !(beta_slow > 0.0) || !(beta_fast > beta_slow) ||
+        !std::isfinite(beta_fast)))
+        return "rope: scaling by parts needs original_context, base > 1 and beta_fast > beta_slow > 0";
+    return nullptr;
+}
+
+// theta_i / 2 pi of the rope_dimension / 2 pairs
+inline void rope_turns(int rope_dimension, double base, int scaling, double factor, int original_context,
+    double beta_fast, double beta_slow, double *turns) {
+    const double two_pi = 6.283185307179586476925286766559, r = rope_dimension;
+    double low = 0.0, high = 0.0;
+    if (scaling == 2) {
+        // the pair index that makes this many turns within the original context
+        const auto pair = [&](double t) { return r * std::log(original_context / (t * two_pi)) / (2.0 * std::log(base)); };
+        low = std::fmax(std::floor(pair(beta_fast)), 0.0);
+        high = std::fmin(std::ceil(pair(beta_slow)), r - 1.0);
+    }
+    for (int i = 0; i < rope_dimension / 2; ++i) {
+        double theta = std::pow(base, -2.0 * i / r);
+        if (scaling == 1) theta /= factor;
+        if (scaling == 2) {
+            const double ramp = std::fmin(std::fmax((i - low) / std::fmax(high - low, 1e-3), 0.0), 1.0);
+            theta = theta / factor * ramp + theta * (1.0 - ramp);
+        }
+        turns[i] = theta / two_pi;
+    }
+}
+
+inline const char *check_rope(int rotary, int dtype, const void *input, int64_t in_row, int64_t in_head, int rows,
+    int heads, int head_size, const void *positions, const void *norm, float epsilon, const void *output,
+    int64_t out_row, int64_t out_head) {
+    if (!dtype_ok(dtype)) return "rope: unknown dtype";
+    if (rows < 0 || rows > kMaxRows || heads < 1 || heads > kMaxRows) return "rope: rows 0 to 2^23, heads 1 to 2^23";
+    if (head_size < 4 || head_size > 256 || head_size % 4 || head_size < rotary)
+        return "rope: head size a multiple of 4, from the rope dimension to 256";
+    if (rows == 0) return nullptr;
+    if (!input || !output || !positions) return "rope: null array";
+    if (!aligned(input, dtype_bytes(dtype)) || !aligned(output, dtype_bytes(dtype)) || !aligned(positions, 4) ||
+        !aligned(norm, 4))
+        return "rope: misaligned array";
+    if (norm && !(epsilon > 0.0f)) return "rope: the norm needs epsilon > 0";
+    if (!pitch_ok(in_row) || !pitch_ok(in_head) || !pitch_ok(out_row) || !pitch_ok(out_head))
+        return "rope: pitches 0 to 2^31";
+    if (!apart(rows, heads, head_size, out_row, out_head)) return "rope: output vectors overlap";
+    if (input == output && ((rows > 1 && in_row != out_row) || (heads > 1 && in_head != out_head)))
+        return "rope: in place, both sides have the same pitches";
+    return nullptr;
+}
+
+}  // namespace fortai_hip

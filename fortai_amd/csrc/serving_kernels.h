@@ -1,0 +1,30 @@
+// Host-side launchers of the serving operators' kernels (rope.hip, kv8_cache.hip,
+// kv8_attention.hip, verify.hip).  Every launcher enqueues on the given stream and
+// returns hipGetLastError() of the launch; the entry points that call them
+// (fortai_hip_serving.hip) have checked the arguments.
+#pragma once
+
+#include "element_types.h"
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace fortai_hip {
+
+struct RopeParams {
+    const void *x = nullptr;
+    void *out = nullptr;
+    const int32_t *positions = nullptr;  // [rows]
+    const float *norm = nullptr;         // [head], or null: no norm
+    const double *turns = nullptr;       // [rotary / 2]: theta_i / (2 pi)
+    float attention = 1.0f, eps = 0.0f;
+    int rows = 0, heads = 0, head = 0, rotary = 0;
+    int64_t x_row = 0, x_head = 0, out_row = 0, out_head = 0;  // pitches in elements
+    bool interleaved = false;
+    bool half4 = false;  // rotary / 2 is a multiple of 4
+};
+// vec: x and out allow four-element accesses
+hipError_t launch_rope(const RopeParams &p, Dtype dtype, bool vec, hipStream_t stream);
+
+}  // namespace fortai_hip

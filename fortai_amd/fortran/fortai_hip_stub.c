@@ -808,3 +808,30 @@ FORTAI_HIP_WEAK int fortai_hip_q8_context_scratch_bytes(const fortai_hip_q8_cont
     if (bytes) *bytes = 0;
     return FORTAI_HIP_RUNTIME_ERROR;
 }
+
+FORTAI_HIP_WEAK int fortai_hip_rope_create(fortai_hip_q8_context *context, int rope_dimension,
+    int interleaved, double base, int scaling, double factor, int original_context,
+    double beta_fast, double beta_slow, double attention_factor, fortai_hip_rope **rope)
+{
+    (void)context; (void)rope_dimension; (void)interleaved; (void)base; (void)scaling; (void)factor;
+    (void)original_context; (void)beta_fast; (void)beta_slow; (void)attention_factor;
+    if (rope) *rope = NULL;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_rope_destroy(fortai_hip_rope *rope)
+{
+    (void)rope;
+    return FORTAI_HIP_OK;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype,
+    const void *device_input, int64_t input_row_pitch, int64_t input_head_pitch, int rows,
+    int heads, int head_size, const void *device_positions, const void *device_norm, float epsilon,
+    void *device_output, int64_t output_row_pitch, int64_t output_head_pitch)
+{
+    (void)rope; (void)dtype; (void)device_input; (void)input_row_pitch; (void)input_head_pitch;
+    (void)rows; (void)heads; (void)head_size; (void)device_positions; (void)device_norm;
+    (void)epsilon; (void)device_output; (void)output_row_pitch; (void)output_head_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}

@@ -37,6 +37,7 @@ typedef struct fortai_hip_qwen35_attention fortai_hip_qwen35_attention;
 typedef struct fortai_hip_f16_weights fortai_hip_f16_weights;          /* [extension] */
 typedef struct fortai_hip_qwen35_decoder fortai_hip_qwen35_decoder;    /* [extension] */
 typedef struct fortai_hip_qwen35_batch fortai_hip_qwen35_batch;        /* [extension] */
+typedef struct fortai_hip_rope fortai_hip_rope;                        /* [extension] */
 
 enum {
     FORTAI_HIP_OK = 0,
@@ -464,6 +465,45 @@ int fortai_hip_qwen35_attention_set_test_options(fortai_hip_qwen35_attention *la
 int fortai_hip_qwen35_decoder_set_mode(fortai_hip_qwen35_decoder *decoder, int flags);
 int fortai_hip_qwen35_batch_set_mode(fortai_hip_qwen35_batch *batch_decoder, int flags);
 int fortai_hip_qwen35_batch_set_prefill_mode(fortai_hip_qwen35_batch *batch_decoder, int mode);
+
+/* ============ [extension] serving operators ==========================
+ * The operators of a step that runs several tokens of several sequences over a
+ * shared cache.  As everywhere, they are enqueued on the context's stream; data
+ * that another stream produced has to be complete (or waited for) before the
+ * call.  The caller's current device stays current.  Arrays of activations are
+ * fp32, fp16 or bf16, computed on in fp32 and rounded once, to nearest even.
+ * Pitches count elements, at most 2^31; base addresses are aligned to their
+ * element.  Row counts go up to 2^23. */
+#define FORTAI_HIP_DTYPE_F32 0
+#define FORTAI_HIP_DTYPE_F16 1
+#define FORTAI_HIP_DTYPE_BF16 2
+
+/* Rotary positions.  create: the angle of pair i at position p is p theta_i,
+ * theta_i = base^(-2i / rope_dimension); the pairs are dims (i, i +
+ * rope_dimension / 2), or (2i, 2i + 1) with interleaved != 0.  Scaling for long
+ * contexts: FORTAI_HIP_ROPE_LINEAR divides every theta_i by factor;
+ * FORTAI_HIP_ROPE_YARN (interpolation by parts, as published for YaRN) divides
+ * those pairs that make fewer than beta_slow turns within original_context
+ * positions, keeps those that make more than beta_fast, and ramps between.
+ * attention_factor multiplies sine and cosine.  Numbers that a scaling does not
+ * use are ignored.  rope_dimension: even, 2 to 256.
+ * device: rows x heads vectors of head_size (a multiple of 4, rope_dimension to
+ * 256); row r is at device_positions[r] (int32).  device_norm (fp32
+ * [head_size], may be NULL): each vector is RMS-normalised over head_size with
+ * these weights first.  Dims from rope_dimension on are not rotated.  The
+ * output may be the input itself (same pitches), or an array apart from it.  A
+ * context that replays the call in a graph keeps the handle. */
+#define FORTAI_HIP_ROPE_PLAIN 0
+#define FORTAI_HIP_ROPE_LINEAR 1
+#define FORTAI_HIP_ROPE_YARN 2
+int fortai_hip_rope_create(fortai_hip_q8_context *context, int rope_dimension, int interleaved,
+    double base, int scaling, double factor, int original_context, double beta_fast, double beta_slow,
+    double attention_factor, fortai_hip_rope **rope);
+int fortai_hip_rope_destroy(fortai_hip_rope *rope);
+int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype, const void *device_input,
+    int64_t input_row_pitch, int64_t input_head_pitch, int rows, int heads, int head_size,
+    const void *device_positions, const void *device_norm, float epsilon, void *device_output,
+    int64_t output_row_pitch, int64_t output_head_pitch);
 
 #ifdef __cplusplus
 }
