@@ -125,9 +125,25 @@ _SIGNATURES = {
     "fortai_hip_rope_create": [_vp, _i, _i, _d, _i, _d, _i, _d, _d, _d, _vpp],
     "fortai_hip_rope_destroy": [_vp],
     "fortai_hip_rope_device": [_vp, _i, _vp, _i64, _i64, _i, _i, _i, _vp, _vp, _f, _vp, _i64, _i64],
+    "fortai_hip_kv8_bytes": [_i, _i, _i, _i, _i],
+    "fortai_hip_kv8_create": [_vp, _i, _i, _i, _i, _i, _vp, _sz, _vpp],
+    "fortai_hip_kv8_destroy": [_vp],
+    "fortai_hip_kv8_append_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64],
+    "fortai_hip_kv8_read_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64],
+    "fortai_hip_kv8_copy_pages": [_vp, _vp, _vp, _i],
+    "fortai_hip_kv8_pages_create": [_i, _i, _i, _i, _vpp],
+    "fortai_hip_kv8_pages_destroy": [_vp],
+    "fortai_hip_kv8_pages_extend": [_vp, _i, _i, _vp, _vp, _vp],
+    "fortai_hip_kv8_pages_fork": [_vp, _i, _i, _i64],
+    "fortai_hip_kv8_pages_truncate": [_vp, _i, _i64],
+    "fortai_hip_kv8_pages_compact": [_vp, _vp, _vp, _i, _vp],
+    "fortai_hip_kv8_pages_length": [_vp, _i],
+    "fortai_hip_kv8_pages_free_count": [_vp],
+    "fortai_hip_kv8_pages_tables": [_vp, _vp, _i, _vp, _i],
 }
 _RESTYPE = {"fortai_hip_q8_last_error": C.c_char_p, "fortai_hip_q8_tokens_bytes": C.c_size_t,
-            "fortai_hip_q8_pack_bytes": C.c_size_t}
+            "fortai_hip_q8_pack_bytes": C.c_size_t, "fortai_hip_kv8_bytes": C.c_size_t,
+            "fortai_hip_kv8_pages_length": C.c_int64}
 
 _lib: Optional[C.CDLL] = None
 
@@ -612,4 +628,123 @@ class Rope:
     def free(self) -> None:
         if self.h:
             self.ctx.lib.fortai_hip_rope_destroy(self.h)
+            self.h = None
+
+
+class Kv8Batch(C.Structure):
+    """Which rows of a call belong to which sequence of an 8-bit cache, and where
+    its tokens lie (fortai_hip_kv8_batch): device int32 row_starts [sequences + 1],
+    lengths [sequences] (tokens before the rows) and tables [sequences][table_pitch]."""
+
+    _fields_ = [("sequences", _i), ("rows", _i), ("max_rows", _i), ("table_pitch", _i), ("row_starts", _vp),
+                ("lengths", _vp), ("tables", _vp)]
+
+    def __init__(self, sequences: int, rows: int, max_rows: int, row_starts, lengths, tables, table_pitch: int):
+        super().__init__(sequences, rows, max_rows, table_pitch, _dev(row_starts), _dev(lengths), _dev(tables))
+
+
+class Kv8Cache:
+    """8-bit paged key/value cache (fortai_hip_kv8_cache), over the caller's
+    device storage of Kv8Cache.bytes() bytes or over its own."""
+
+    def __init__(self, ctx: Context, layers: int, pages: int, page_tokens: int, kv_heads: int, head_size: int,
+                 storage=None, storage_bytes: int = 0):
+        self.ctx = ctx
+        self.layers, self.pages, self.page_tokens = layers, pages, page_tokens
+        self.kv_heads, self.head_size = kv_heads, head_size
+        h = C.c_void_p()
+        ctx.call("fortai_hip_kv8_create", ctx.h, layers, pages, page_tokens, kv_heads, head_size, _dev(storage),
+                 storage_bytes, C.byref(h))
+        self.h = h
+
+    @staticmethod
+    def bytes(layers: int, pages: int, page_tokens: int, kv_heads: int, head_size: int) -> int:
+        """Bytes of the storage (0: no such cache)."""
+        return load().fortai_hip_kv8_bytes(layers, pages, page_tokens, kv_heads, head_size)
+
+    def append(self, layer: int, batch: Kv8Batch, keys, values, dtype: str = "f32", key_pitch: Optional[int] = None,
+               value_pitch: Optional[int] = None) -> None:
+        """Store rows of keys and values [rows][kv_heads][head_size] (dense unless pitches are given)."""
+        width = self.kv_heads * self.head_size
+        self.ctx.check(self.ctx.lib.fortai_hip_kv8_append_device(
+            self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(keys), width if key_pitch is None else key_pitch,
+            _dev(values), width if value_pitch is None else value_pitch), "fortai_hip_kv8_append_device")
+
+    def read(self, layer: int, batch: Kv8Batch, keys, values, dtype: str = "f32", key_pitch: Optional[int] = None,
+             value_pitch: Optional[int] = None) -> None:
+        """The batch's rows as the values that their codes stand for."""
+        width = self.kv_heads * self.head_size
+        self.ctx.check(self.ctx.lib.fortai_hip_kv8_read_device(
+            self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(keys), width if key_pitch is None else key_pitch,
+            _dev(values), width if value_pitch is None else value_pitch), "fortai_hip_kv8_read_device")
+
+    def copy_pages(self, source, target) -> None:
+        """Page target[i] becomes a copy of page source[i], in every layer (host int32 arrays)."""
+        f = np.ascontiguousarray(source, dtype=np.int32)
+        t = np.ascontiguousarray(target, dtype=np.int32)
+        if f.shape != t.shape or f.ndim != 1:
+            raise ValueError("need as many source as target pages")
+        self.ctx.check(self.ctx.lib.fortai_hip_kv8_copy_pages(self.h, f.ctypes.data, t.ctypes.data, len(f)),
+                       "fortai_hip_kv8_copy_pages")
+
+    def free(self) -> None:
+        if self.h:
+            self.ctx.lib.fortai_hip_kv8_destroy(self.h)
+            self.h = None
+
+
+class Kv8Pages:
+    """Page bookkeeping of a pool (fortai_hip_kv8_pages): host only, no GPU."""
+
+    def __init__(self, pages: int, page_tokens: int, sequences: int, table_pitch: int):
+        self.lib, self.pages, self.table_pitch = load(), pages, table_pitch
+        h = C.c_void_p()
+        self._check(self.lib.fortai_hip_kv8_pages_create(pages, page_tokens, sequences, table_pitch, C.byref(h)),
+                    "fortai_hip_kv8_pages_create")
+        self.h = h
+
+    @staticmethod
+    def _check(rc: int, what: str) -> None:
+        if rc != OK:
+            raise BackendError(rc, what)
+
+    def extend(self, sequence: int, tokens: int):
+        """Room for more tokens; the (from, to) page pairs that have to be copied first (none or one)."""
+        f, t, n = C.c_int32(), C.c_int32(), C.c_int()
+        self._check(self.lib.fortai_hip_kv8_pages_extend(self.h, sequence, tokens, C.byref(f), C.byref(t), C.byref(n)),
+                    "fortai_hip_kv8_pages_extend")
+        return [(f.value, t.value)] if n.value else []
+
+    def fork(self, sequence: int, fork: int, length: int) -> None:
+        self._check(self.lib.fortai_hip_kv8_pages_fork(self.h, sequence, fork, length), "fortai_hip_kv8_pages_fork")
+
+    def truncate(self, sequence: int, length: int = 0) -> None:
+        self._check(self.lib.fortai_hip_kv8_pages_truncate(self.h, sequence, length), "fortai_hip_kv8_pages_truncate")
+
+    def compact(self, capacity: Optional[int] = None):
+        """Move live pages to the pool's lower end; the moves as (from, to) arrays."""
+        n = C.c_int()
+        capacity = self.pages if capacity is None else capacity
+        f, t = np.empty(max(capacity, 1), dtype=np.int32), np.empty(max(capacity, 1), dtype=np.int32)
+        self._check(self.lib.fortai_hip_kv8_pages_compact(self.h, _ptr(f), _ptr(t), capacity, C.byref(n)),
+                    "fortai_hip_kv8_pages_compact")
+        return f[:n.value].copy(), t[:n.value].copy()
+
+    def length(self, sequence: int) -> int:
+        return self.lib.fortai_hip_kv8_pages_length(self.h, sequence)
+
+    def free_count(self) -> int:
+        return self.lib.fortai_hip_kv8_pages_free_count(self.h)
+
+    def tables(self, sequences) -> np.ndarray:
+        """The pages of these sequences, int32 [len(sequences)][table_pitch], -1 behind the last."""
+        s = np.ascontiguousarray(sequences, dtype=np.int32)
+        out = np.empty((len(s), self.table_pitch), dtype=np.int32)
+        self._check(self.lib.fortai_hip_kv8_pages_tables(self.h, _ptr(s), len(s), _ptr(out), self.table_pitch),
+                    "fortai_hip_kv8_pages_tables")
+        return out
+
+    def free(self) -> None:
+        if self.h:
+            self.lib.fortai_hip_kv8_pages_destroy(self.h)
             self.h = None

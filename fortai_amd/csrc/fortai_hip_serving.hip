@@ -43,6 +43,52 @@ struct fortai_hip_rope {
     double *turns = nullptr;
 };
 
+struct fortai_hip_kv8_cache {
+    fortai_hip_q8_context *context = nullptr;
+    int device = 0;
+    Kv8Shape shape;
+    uint8_t *storage = nullptr;
+    bool owned = false;
+
+    Kv8View layer(int index) const {
+        Kv8View v;
+        const size_t at = static_cast<size_t>(index);
+        v.keys = reinterpret_cast<int8_t *>(storage) + at * shape.layer_codes();
+        v.values = v.keys + shape.codes();
+        v.key_max = reinterpret_cast<float *>(storage + 2 * shape.codes()) + at * shape.layer_tops();
+        v.value_max = v.key_max + shape.layers * shape.layer_tops();
+        v.pages = shape.pages;
+        v.page_tokens = shape.page_tokens;
+        v.kv_heads = shape.kv_heads;
+        v.head = shape.head;
+        return v;
+    }
+};
+
+namespace {
+
+Kv8Rows batch_rows(const fortai_hip_kv8_batch *b) {
+    Kv8Rows r;
+    r.starts = static_cast<const int32_t *>(b->device_row_starts);
+    r.lengths = static_cast<const int32_t *>(b->device_lengths);
+    r.tables = static_cast<const int32_t *>(b->device_tables);
+    r.sequences = b->sequences;
+    r.rows = b->rows;
+    r.max_rows = b->max_rows;
+    r.pitch = b->table_pitch;
+    return r;
+}
+
+const char *check_batch(const fortai_hip_kv8_batch *b) {
+    if (!b) return "kv8: no batch";
+    return check_kv8_batch(b->sequences, b->rows, b->max_rows, b->table_pitch, b->device_row_starts, b->device_lengths,
+        b->device_tables);
+}
+
+bool empty(const fortai_hip_kv8_batch *b) { return b->sequences == 0 || b->rows == 0 || b->max_rows == 0; }
+
+}  // namespace
+
 extern "C" {
 
 // ---------------------------------------------------------- rotary positions
@@ -116,6 +162,105 @@ int fortai_hip_rope_device(fortai_hip_rope *h, int dtype, const void *input, int
         vector4_ok(output, dtype, output_row_pitch, output_head_pitch);
     const DeviceScope scope(c->device);
     return done(c, launch_rope(p, static_cast<Dtype>(dtype), vec, c->stream), "rotary positions");
+}
+
+// --------------------------------------------------------------- 8-bit cache
+size_t fortai_hip_kv8_bytes(int layers, int pages, int page_tokens, int kv_heads, int head_size) {
+    Kv8Shape s;
+    s.layers = layers;
+    s.pages = pages;
+    s.page_tokens = page_tokens;
+    s.kv_heads = kv_heads;
+    s.head = head_size;
+    return kv8_bytes(s);
+}
+
+int fortai_hip_kv8_create(fortai_hip_q8_context *c, int layers, int pages, int page_tokens, int kv_heads, int head_size,
+    void *device_storage, size_t storage_bytes, fortai_hip_kv8_cache **cache) {
+    if (!c || !cache) return FORTAI_HIP_INVALID;
+    *cache = nullptr;
+    Kv8Shape s;
+    s.layers = layers;
+    s.pages = pages;
+    s.page_tokens = page_tokens;
+    s.kv_heads = kv_heads;
+    s.head = head_size;
+    if (const char *wrong = check_kv8_shape(s)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    const size_t bytes = kv8_bytes(s);
+    if (bytes == 0) return fail(c, FORTAI_HIP_INVALID, "kv8: the cache is larger than any memory");
+    if (device_storage && (storage_bytes < bytes || !aligned(device_storage, 16)))
+        return fail(c, FORTAI_HIP_INVALID, "kv8: storage smaller than fortai_hip_kv8_bytes, or not aligned to 16 bytes");
+    auto *h = new (std::nothrow) fortai_hip_kv8_cache;
+    if (!h) return fail(c, FORTAI_HIP_RUNTIME_ERROR, "kv8: out of host memory");
+    h->context = c;
+    h->device = c->device;
+    h->shape = s;
+    h->storage = static_cast<uint8_t *>(device_storage);
+    const DeviceScope scope(c->device);
+    hipError_t e = hipSuccess;
+    if (!device_storage) {
+        e = alloc(&h->storage, bytes);
+        h->owned = e == hipSuccess;
+        if (e == hipSuccess) e = launch_kv8_clear(h->storage, bytes, c->stream);
+    }
+    if (e != hipSuccess) {
+        if (h->owned) release(h->storage);
+        delete h;
+        return fail(c, FORTAI_HIP_RUNTIME_ERROR, "kv8 create", e);
+    }
+    *cache = h;
+    return FORTAI_HIP_OK;
+}
+
+int fortai_hip_kv8_destroy(fortai_hip_kv8_cache *h) {
+    if (!h) return FORTAI_HIP_OK;
+    const DeviceScope scope(h->device);
+    if (h->owned) release(h->storage);
+    delete h;
+    return FORTAI_HIP_OK;
+}
+
+int fortai_hip_kv8_append_device(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch, int dtype,
+    const void *keys, int64_t key_pitch, const void *values, int64_t value_pitch) {
+    if (!h) return FORTAI_HIP_INVALID;
+    fortai_hip_q8_context *c = h->context;
+    if (const char *wrong = check_batch(batch)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (empty(batch)) return FORTAI_HIP_OK;
+    if (const char *wrong = check_kv8_rows(h->shape, layer, dtype, keys, key_pitch, values, value_pitch, false))
+        return fail(c, FORTAI_HIP_INVALID, wrong);
+    const bool vec = vector4_ok(keys, dtype, key_pitch, 0) && vector4_ok(values, dtype, value_pitch, 0);
+    const DeviceScope scope(c->device);
+    return done(c, launch_kv8_append(h->layer(layer), batch_rows(batch), static_cast<Dtype>(dtype), keys, key_pitch,
+        values, value_pitch, vec, c->stream), "kv8 append");
+}
+
+int fortai_hip_kv8_read_device(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch, int dtype,
+    void *keys, int64_t key_pitch, void *values, int64_t value_pitch) {
+    if (!h) return FORTAI_HIP_INVALID;
+    fortai_hip_q8_context *c = h->context;
+    if (const char *wrong = check_batch(batch)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (empty(batch)) return FORTAI_HIP_OK;
+    if (const char *wrong = check_kv8_rows(h->shape, layer, dtype, keys, key_pitch, values, value_pitch, true))
+        return fail(c, FORTAI_HIP_INVALID, wrong);
+    const bool vec = vector4_ok(keys, dtype, key_pitch, 0) && vector4_ok(values, dtype, value_pitch, 0);
+    const DeviceScope scope(c->device);
+    return done(c, launch_kv8_read(h->layer(layer), batch_rows(batch), static_cast<Dtype>(dtype), keys, key_pitch,
+        values, value_pitch, vec, c->stream), "kv8 read");
+}
+
+int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *h, const int32_t *from, const int32_t *to, int count) {
+    if (!h || count < 0) return FORTAI_HIP_INVALID;
+    if (count == 0) return FORTAI_HIP_OK;
+    fortai_hip_q8_context *c = h->context;
+    if (!from || !to) return fail(c, FORTAI_HIP_INVALID, "kv8 copy: null array");
+    try {
+        if (const char *wrong = check_page_pairs(from, to, count, h->shape.pages)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    } catch (...) {
+        return fail(c, FORTAI_HIP_RUNTIME_ERROR, "kv8 copy: out of host memory");
+    }
+    const DeviceScope scope(c->device);
+    return done(c, launch_kv8_copy_pages(h->layer(0), h->shape.layer_codes(), h->shape.layer_tops(), h->shape.layers, from,
+        to, count, c->stream), "kv8 copy pages");
 }
 
 }  // extern "C"

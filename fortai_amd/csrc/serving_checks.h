@@ -3,9 +3,11 @@
 // wrong with the arguments, or nullptr.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
+#include <vector>
 
 namespace fortai_hip {
 
@@ -87,6 +89,69 @@ inline const char *check_rope(int rotary, int dtype, const void *input, int64_t 
     if (!apart(rows, heads, head_size, out_row, out_head)) return "rope: output vectors overlap";
     if (input == output && ((rows > 1 && in_row != out_row) || (heads > 1 && in_head != out_head)))
         return "rope: in place, both sides have the same pitches";
+    return nullptr;
+}
+
+// --------------------------------------------------------------- 8-bit cache
+struct Kv8Shape {
+    int layers = 0, pages = 0, page_tokens = 0, kv_heads = 0, head = 0;
+    size_t layer_tops() const { return static_cast<size_t>(pages) * kv_heads; }
+    size_t layer_codes() const { return layer_tops() * page_tokens * head; }
+    size_t codes() const { return layers * layer_codes(); }  // bytes of the key codes, and of the value codes
+    size_t bytes() const { return 2 * codes() + 2 * sizeof(float) * layers * layer_tops(); }
+};
+
+inline const char *check_kv8_shape(const Kv8Shape &s) {
+    if (s.layers < 1 || s.layers > 4096 || s.kv_heads < 1 || s.kv_heads > 1024) return "kv8: layers 1 to 4096, heads 1 to 1024";
+    if (s.pages < 1) return "kv8: no pages";
+    if (s.page_tokens != 16 && s.page_tokens != 32 && s.page_tokens != 64) return "kv8: pages of 16, 32 or 64 tokens";
+    if (s.head != 64 && s.head != 128 && s.head != 256) return "kv8: heads of 64, 128 or 256";
+    return nullptr;  // at most 2^(12 + 10 + 31 + 6 + 8) = 2^67 bytes: kv8_bytes() says which do not fit
+}
+
+// 0 where 64 bits do not hold it (no storage is that large)
+inline size_t kv8_bytes(const Kv8Shape &s) {
+    if (check_kv8_shape(s)) return 0;
+    const double about = 2.0 * s.layers * s.pages * s.kv_heads * (static_cast<double>(s.page_tokens) * s.head + 4.0);
+    return about < 9.0e15 ? s.bytes() : 0;
+}
+
+inline const char *check_kv8_batch(int sequences, int rows, int max_rows, int table_pitch, const void *starts,
+    const void *lengths, const void *tables) {
+    if (sequences < 0 || sequences > 16384) return "kv8: sequences 0 to 16384";
+    if (rows < 0 || rows > kMaxRows || max_rows < 0 || max_rows > rows) return "kv8: rows 0 to 2^23, max_rows 0 to rows";
+    if (sequences == 0 || rows == 0 || max_rows == 0) return nullptr;
+    if (table_pitch < 1 || table_pitch > (1 << 24)) return "kv8: table pitch 1 to 2^24";
+    if (!starts || !lengths || !tables) return "kv8: null array";
+    if (!aligned(starts, 4) || !aligned(lengths, 4) || !aligned(tables, 4)) return "kv8: misaligned array";
+    return nullptr;
+}
+
+// the rows of keys and values that are appended (written == false) or read into
+inline const char *check_kv8_rows(const Kv8Shape &s, int layer, int dtype, const void *keys, int64_t key_pitch,
+    const void *values, int64_t value_pitch, bool written) {
+    const int64_t width = static_cast<int64_t>(s.kv_heads) * s.head;
+    if (layer < 0 || layer >= s.layers) return "kv8: no such layer";
+    if (!dtype_ok(dtype)) return "kv8: unknown dtype";
+    if (!keys || !values) return "kv8: null array";
+    if (!aligned(keys, dtype_bytes(dtype)) || !aligned(values, dtype_bytes(dtype))) return "kv8: misaligned array";
+    if (!pitch_ok(key_pitch) || !pitch_ok(value_pitch) || (written && (key_pitch < width || value_pitch < width)))
+        return written ? "kv8: pitches from kv_heads * head to 2^31" : "kv8: pitches 0 to 2^31";
+    return nullptr;
+}
+
+// Pairs that can be copied in any order: ids within the pool, no page written
+// twice, none both read and written.  May throw std::bad_alloc.
+inline const char *check_page_pairs(const int32_t *from, const int32_t *to, int count, int pages) {
+    for (int i = 0; i < count; ++i)
+        if (from[i] < 0 || from[i] >= pages || to[i] < 0 || to[i] >= pages) return "kv8 copy: a page outside the pool";
+    if (count == 1) return from[0] == to[0] ? "kv8 copy: a page is both read and written" : nullptr;
+    std::vector<int32_t> written(to, to + count);
+    std::sort(written.begin(), written.end());
+    for (int i = 1; i < count; ++i)
+        if (written[i] == written[i - 1]) return "kv8 copy: a page is written twice";
+    for (int i = 0; i < count; ++i)
+        if (std::binary_search(written.begin(), written.end(), from[i])) return "kv8 copy: a page is both read and written";
     return nullptr;
 }
 

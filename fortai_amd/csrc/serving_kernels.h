@@ -5,6 +5,7 @@
 #pragma once
 
 #include "element_types.h"
+#include "kv8_device.h"
 
 #include <hip/hip_runtime.h>
 #include <stddef.h>
@@ -26,5 +27,15 @@ struct RopeParams {
 };
 // vec: x and out allow four-element accesses
 hipError_t launch_rope(const RopeParams &p, Dtype dtype, bool vec, hipStream_t stream);
+
+// vec: keys and values allow four-element accesses
+hipError_t launch_kv8_append(const Kv8View &cache, const Kv8Rows &batch, Dtype dtype, const void *keys, int64_t key_pitch,
+    const void *values, int64_t value_pitch, bool vec, hipStream_t stream);
+hipError_t launch_kv8_read(const Kv8View &cache, const Kv8Rows &batch, Dtype dtype, void *keys, int64_t key_pitch,
+    void *values, int64_t value_pitch, bool vec, hipStream_t stream);
+// cache: the first layer; layer_codes, layer_tops: bytes and maxima of a layer's planes; from, to: host arrays
+hipError_t launch_kv8_copy_pages(const Kv8View &cache, size_t layer_codes, size_t layer_tops, int layers,
+    const int32_t *from, const int32_t *to, int count, hipStream_t stream);
+hipError_t launch_kv8_clear(void *storage, size_t bytes, hipStream_t stream);
 
 }  // namespace fortai_hip

@@ -835,3 +835,112 @@ FORTAI_HIP_WEAK int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype,
     (void)epsilon; (void)device_output; (void)output_row_pitch; (void)output_head_pitch;
     return FORTAI_HIP_RUNTIME_ERROR;
 }
+
+FORTAI_HIP_WEAK size_t fortai_hip_kv8_bytes(int layers, int pages, int page_tokens, int kv_heads,
+    int head_size)
+{
+    (void)layers; (void)pages; (void)page_tokens; (void)kv_heads; (void)head_size;
+    return 0;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_create(fortai_hip_q8_context *context, int layers, int pages,
+    int page_tokens, int kv_heads, int head_size, void *device_storage, size_t storage_bytes,
+    fortai_hip_kv8_cache **cache)
+{
+    (void)context; (void)layers; (void)pages; (void)page_tokens; (void)kv_heads; (void)head_size;
+    (void)device_storage; (void)storage_bytes;
+    if (cache) *cache = NULL;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_destroy(fortai_hip_kv8_cache *cache)
+{
+    (void)cache;
+    return FORTAI_HIP_OK;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_append_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, const void *device_keys, int64_t key_pitch,
+    const void *device_values, int64_t value_pitch)
+{
+    (void)cache; (void)layer; (void)batch; (void)dtype; (void)device_keys; (void)key_pitch;
+    (void)device_values; (void)value_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_read_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, void *device_keys, int64_t key_pitch,
+    void *device_values, int64_t value_pitch)
+{
+    (void)cache; (void)layer; (void)batch; (void)dtype; (void)device_keys; (void)key_pitch;
+    (void)device_values; (void)value_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *cache, const int32_t *from,
+    const int32_t *to, int count)
+{
+    (void)cache; (void)from; (void)to; (void)count;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_create(int pages, int page_tokens, int sequences,
+    int table_pitch, fortai_hip_kv8_pages **pool)
+{
+    (void)pages; (void)page_tokens; (void)sequences; (void)table_pitch;
+    if (pool) *pool = NULL;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_destroy(fortai_hip_kv8_pages *pool)
+{
+    (void)pool;
+    return FORTAI_HIP_OK;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_extend(fortai_hip_kv8_pages *pool, int sequence,
+    int tokens, int32_t *from, int32_t *to, int *copies)
+{
+    (void)pool; (void)sequence; (void)tokens; (void)from; (void)to; (void)copies;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_fork(fortai_hip_kv8_pages *pool, int sequence, int fork,
+    int64_t length)
+{
+    (void)pool; (void)sequence; (void)fork; (void)length;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_truncate(fortai_hip_kv8_pages *pool, int sequence,
+    int64_t length)
+{
+    (void)pool; (void)sequence; (void)length;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_compact(fortai_hip_kv8_pages *pool, int32_t *from,
+    int32_t *to, int capacity, int *copies)
+{
+    (void)pool; (void)from; (void)to; (void)capacity; (void)copies;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int64_t fortai_hip_kv8_pages_length(const fortai_hip_kv8_pages *pool, int sequence)
+{
+    (void)pool; (void)sequence;
+    return 0;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_free_count(const fortai_hip_kv8_pages *pool)
+{
+    (void)pool;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool,
+    const int *sequences, int count, int32_t *tables, int table_pitch)
+{
+    (void)pool; (void)sequences; (void)count; (void)tables; (void)table_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}

@@ -38,6 +38,8 @@ typedef struct fortai_hip_f16_weights fortai_hip_f16_weights;          /* [exten
 typedef struct fortai_hip_qwen35_decoder fortai_hip_qwen35_decoder;    /* [extension] */
 typedef struct fortai_hip_qwen35_batch fortai_hip_qwen35_batch;        /* [extension] */
 typedef struct fortai_hip_rope fortai_hip_rope;                        /* [extension] */
+typedef struct fortai_hip_kv8_cache fortai_hip_kv8_cache;              /* [extension] */
+typedef struct fortai_hip_kv8_pages fortai_hip_kv8_pages;              /* [extension] */
 
 enum {
     FORTAI_HIP_OK = 0,
@@ -504,6 +506,88 @@ int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype, const void *device_
     int64_t input_row_pitch, int64_t input_head_pitch, int rows, int heads, int head_size,
     const void *device_positions, const void *device_norm, float epsilon, void *device_output,
     int64_t output_row_pitch, int64_t output_head_pitch);
+
+/* 8-bit paged key/value cache.  Keys and values are held as int8 codes with one
+ * fp32 magnitude for each page of page_tokens (16, 32 or 64) tokens and head:
+ * value = code * (magnitude / 127).  A cache has `layers` layers of `pages`
+ * pages of kv_heads heads of head_size (64, 128 or 256).  Its storage is
+ * fortai_hip_kv8_bytes bytes (0: no such cache), aligned to 16, in this order:
+ *   key codes    [layers][pages][kv_heads][page_tokens][head_size]
+ *   value codes  [layers][pages][kv_heads][head_size][page_tokens]
+ *   key magnitudes, then value magnitudes, fp32 [layers][pages][kv_heads].
+ * create: over the caller's device storage, which is taken as it is and stays
+ * the caller's, or with NULL over storage of its own, cleared.
+ *
+ * A batch says which rows of a call belong to which sequence and where its
+ * tokens lie.  Rows row_starts[s] .. row_starts[s + 1] - 1 are sequence s's next
+ * tokens; lengths[s] tokens of it precede them, so that its i-th row is token
+ * lengths[s] + i, in page tables[s][token / page_tokens].  All three arrays are
+ * device memory, read when the call's kernels run.  max_rows: at least the rows
+ * of any sequence (rows past it are left out).  Ids outside the pool (-1, say)
+ * are pages that are not there, as are those past table_pitch.
+ *
+ * append: rows of keys and values [rows][kv_heads][head_size] at row pitches.
+ * The page's magnitude is the largest of its tokens so far; when new tokens
+ * raise it, the codes that the page holds are rounded to the new one.  Codes are
+ * the nearest integers to 127 x / magnitude, ties to even, in exact arithmetic.
+ * NaN is stored as zero, an infinity as the page's largest magnitude.  A page
+ * whose first token is among the rows starts anew; tokens without a page, and
+ * those before token 0, are not stored.  Slots behind the last token keep their
+ * bytes.  Two sequences of a batch must not write to the same page.
+ * read: the same rows as values (tokens without a page read as zero, those
+ * before token 0 are left as they were).
+ * copy_pages: page to[i] becomes a copy of page from[i] in every layer; host
+ * arrays, used before the call returns.  No page may be written twice, or be
+ * both read and written. */
+typedef struct fortai_hip_kv8_batch {
+    int sequences, rows, max_rows, table_pitch;
+    const void *device_row_starts; /* int32 [sequences + 1] */
+    const void *device_lengths;    /* int32 [sequences] */
+    const void *device_tables;     /* int32 [sequences][table_pitch] */
+} fortai_hip_kv8_batch;
+
+size_t fortai_hip_kv8_bytes(int layers, int pages, int page_tokens, int kv_heads, int head_size);
+int fortai_hip_kv8_create(fortai_hip_q8_context *context, int layers, int pages, int page_tokens,
+    int kv_heads, int head_size, void *device_storage, size_t storage_bytes,
+    fortai_hip_kv8_cache **cache);
+int fortai_hip_kv8_destroy(fortai_hip_kv8_cache *cache);
+int fortai_hip_kv8_append_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, const void *device_keys, int64_t key_pitch,
+    const void *device_values, int64_t value_pitch);
+int fortai_hip_kv8_read_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, void *device_keys, int64_t key_pitch,
+    void *device_values, int64_t value_pitch);
+int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *cache, const int32_t *from, const int32_t *to,
+    int count);
+
+/* Which pages whose tokens lie in: host bookkeeping for one pool and up to
+ * `sequences` sequences of at most table_pitch pages; no GPU is needed, and a
+ * refused call (INVALID) changes nothing.
+ * extend: room for `tokens` more tokens.  A last page that is partly filled and
+ * shared with another sequence is replaced by one of its own: *copies is then 1
+ * and (*from, *to) has to go through copy_pages, for every cache of the pool,
+ * before the next append; otherwise 0.  INVALID when pages run out.
+ * fork: the empty sequence `fork` starts with the first `length` tokens of
+ * `sequence`, on the same pages.  truncate: drops tokens from `length` on (0:
+ * the whole sequence) and gives back pages that nobody holds any more.
+ * compact: moves live pages from the pool's upper end into the lowest free ones,
+ * at most `capacity` of them; the moves go through copy_pages before the next
+ * append or attention, and tables that were taken before are stale.
+ * tables: the pages of count sequences, rows of table_pitch, -1 behind the last.
+ * length (-1: no such sequence) and free_count ask. */
+int fortai_hip_kv8_pages_create(int pages, int page_tokens, int sequences, int table_pitch,
+    fortai_hip_kv8_pages **pool);
+int fortai_hip_kv8_pages_destroy(fortai_hip_kv8_pages *pool);
+int fortai_hip_kv8_pages_extend(fortai_hip_kv8_pages *pool, int sequence, int tokens, int32_t *from,
+    int32_t *to, int *copies);
+int fortai_hip_kv8_pages_fork(fortai_hip_kv8_pages *pool, int sequence, int fork, int64_t length);
+int fortai_hip_kv8_pages_truncate(fortai_hip_kv8_pages *pool, int sequence, int64_t length);
+int fortai_hip_kv8_pages_compact(fortai_hip_kv8_pages *pool, int32_t *from, int32_t *to,
+    int capacity, int *copies);
+int64_t fortai_hip_kv8_pages_length(const fortai_hip_kv8_pages *pool, int sequence);
+int fortai_hip_kv8_pages_free_count(const fortai_hip_kv8_pages *pool);
+int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool, const int *sequences, int count,
+    int32_t *tables, int table_pitch);
 
 #ifdef __cplusplus
 }
