@@ -130,6 +130,7 @@ _SIGNATURES = {
     "fortai_hip_kv8_destroy": [_vp],
     "fortai_hip_kv8_append_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64],
     "fortai_hip_kv8_read_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64],
+    "fortai_hip_kv8_attention_device": [_vp, _i, _vp, _i, _vp, _i64, _i64, _vp, _i, _f, _i, _vp, _i64],
     "fortai_hip_kv8_copy_pages": [_vp, _vp, _vp, _i],
     "fortai_hip_kv8_pages_create": [_i, _i, _i, _i, _vpp],
     "fortai_hip_kv8_pages_destroy": [_vp],
@@ -677,6 +678,18 @@ class Kv8Cache:
         self.ctx.check(self.ctx.lib.fortai_hip_kv8_read_device(
             self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(keys), width if key_pitch is None else key_pitch,
             _dev(values), width if value_pitch is None else value_pitch), "fortai_hip_kv8_read_device")
+
+    def attention(self, layer: int, batch: Kv8Batch, query, heads: int, out, scale: float, max_length: int,
+                  dtype: str = "f32", gate=None, query_pitch: Optional[int] = None,
+                  query_head_pitch: Optional[int] = None, out_pitch: Optional[int] = None) -> None:
+        """Attention of the batch's rows: query [rows][heads][head_size] (dense unless pitches are given; gate,
+        where given, at the same pitches) -> out [rows][heads][head_size].  max_length: about the longest
+        sequence with its rows, for cutting the work."""
+        hp = self.head_size if query_head_pitch is None else query_head_pitch
+        self.ctx.check(self.ctx.lib.fortai_hip_kv8_attention_device(
+            self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(query), heads * hp if query_pitch is None else query_pitch,
+            hp, _dev(gate), heads, scale, max_length, _dev(out), heads * self.head_size if out_pitch is None else out_pitch),
+            "fortai_hip_kv8_attention_device")
 
     def copy_pages(self, source, target) -> None:
         """Page target[i] becomes a copy of page source[i], in every layer (host int32 arrays)."""

@@ -6,8 +6,8 @@
 #include "serving_checks.h"
 #include "serving_kernels.h"
 
+#include <mutex>
 #include <new>
-#include <vector>
 
 using namespace fortai_hip;
 
@@ -49,6 +49,10 @@ struct fortai_hip_kv8_cache {
     Kv8Shape shape;
     uint8_t *storage = nullptr;
     bool owned = false;
+    // partial results of split attention calls, [kKv8PartialRows][head + 2]: made
+    // with the cache and never again, so that a captured call keeps its address
+    float *partial = nullptr;
+    std::mutex launches;  // a call's two launches follow each other on the stream
 
     Kv8View layer(int index) const {
         Kv8View v;
@@ -203,8 +207,10 @@ int fortai_hip_kv8_create(fortai_hip_q8_context *c, int layers, int pages, int p
         h->owned = e == hipSuccess;
         if (e == hipSuccess) e = launch_kv8_clear(h->storage, bytes, c->stream);
     }
+    if (e == hipSuccess) e = alloc(&h->partial, static_cast<size_t>(kKv8PartialRows) * (head_size + 2));
     if (e != hipSuccess) {
         if (h->owned) release(h->storage);
+        release(h->partial);
         delete h;
         return fail(c, FORTAI_HIP_RUNTIME_ERROR, "kv8 create", e);
     }
@@ -216,6 +222,7 @@ int fortai_hip_kv8_destroy(fortai_hip_kv8_cache *h) {
     if (!h) return FORTAI_HIP_OK;
     const DeviceScope scope(h->device);
     if (h->owned) release(h->storage);
+    release(h->partial);
     delete h;
     return FORTAI_HIP_OK;
 }
@@ -246,6 +253,37 @@ int fortai_hip_kv8_read_device(fortai_hip_kv8_cache *h, int layer, const fortai_
     const DeviceScope scope(c->device);
     return done(c, launch_kv8_read(h->layer(layer), batch_rows(batch), static_cast<Dtype>(dtype), keys, key_pitch,
         values, value_pitch, vec, c->stream), "kv8 read");
+}
+
+int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch, int dtype,
+    const void *query, int64_t query_pitch, int64_t query_head_pitch, const void *gate, int heads, float scale,
+    int max_length, void *output, int64_t output_pitch) {
+    if (!h) return FORTAI_HIP_INVALID;
+    fortai_hip_q8_context *c = h->context;
+    if (const char *wrong = check_batch(batch)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (empty(batch)) return FORTAI_HIP_OK;
+    if (const char *wrong = check_kv8_attention(h->shape, layer, dtype, batch->rows, batch->max_rows, query, query_pitch,
+            query_head_pitch, gate, heads, scale, max_length, output, output_pitch))
+        return fail(c, FORTAI_HIP_INVALID, wrong);
+    Kv8AttentionParams p;
+    p.cache = h->layer(layer);
+    p.batch = batch_rows(batch);
+    p.q = query;
+    p.gate = gate;
+    p.out = output;
+    p.q_row = query_pitch;
+    p.q_head = query_head_pitch;
+    p.out_row = output_pitch;
+    p.group = heads / h->shape.kv_heads;
+    p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074 / 127.0);
+    p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0);
+    p.partial = h->partial;
+    p.partial_ml = h->partial + static_cast<size_t>(kKv8PartialRows) * h->shape.head;
+    const Kv8Plan plan = kv8_plan(dtype == FORTAI_HIP_DTYPE_F32, batch->sequences, h->shape.kv_heads,
+        static_cast<int64_t>(batch->max_rows) * p.group, max_length);
+    const DeviceScope scope(c->device);
+    const std::lock_guard<std::mutex> lock(h->launches);
+    return done(c, launch_kv8_attention(p, static_cast<Dtype>(dtype), plan, c->stream), "kv8 attention");
 }
 
 int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *h, const int32_t *from, const int32_t *to, int count) {

@@ -18,6 +18,9 @@ namespace fortai_hip {
 constexpr int kKv8MaxTokens = 1 << 30;  // the longest table: 2^24 pages of 64 tokens
 constexpr int kKv8PairsPerLaunch = 448;  // page pairs that fit a launch's arguments beside the rest
 
+constexpr int kKv8MaxSplits = 256;       // workgroups that may share a sequence's head
+constexpr int kKv8PartialRows = 16384;   // rows of partial results that a cache has room for
+
 struct Kv8View {
     int8_t *keys = nullptr, *values = nullptr;         // [pages][kv_heads][P][D], [pages][kv_heads][D][P]
     float *key_max = nullptr, *value_max = nullptr;    // [pages][kv_heads]
@@ -49,5 +52,32 @@ struct Kv8Rows {
         return id >= 0 && id < pages ? id : -1;
     }
 };
+
+// How an attention call is cut: `rows` rows of a kv head a workgroup, row_tiles
+// such tiles, `splits` workgroups over the cached tokens of each.
+struct Kv8Plan {
+    int rows = 0, row_tiles = 0, splits = 0;
+    bool split_halves = false;  // queries and weights as two fp16 halves
+};
+
+// fp32 queries are always split into halves (8 rows in an instruction's 16
+// columns), others where 8 columns are enough.  Tokens are split until 512
+// workgroups (two a CU) are there, as far as every one has a tile for each of its
+// four waves and the partial results fit.
+inline Kv8Plan kv8_plan(bool fp32, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
+    Kv8Plan p;
+    p.split_halves = fp32 || rows <= 8;
+    if (p.split_halves) p.rows = rows <= 8 ? 8 : 16;
+    else p.rows = rows <= 16 ? 16 : 32;
+    p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
+    const int64_t base = static_cast<int64_t>(p.row_tiles) * kv_heads * sequences;
+    const int64_t wanted = (512 + base - 1) / base, useful = (max_length + 255) / 256;
+    const int64_t room = kKv8PartialRows / (base * p.rows);
+    int64_t s = wanted < useful ? wanted : useful;
+    s = s < room ? s : room;
+    s = s < kKv8MaxSplits ? s : kKv8MaxSplits;
+    p.splits = s < 1 ? 1 : static_cast<int>(s);
+    return p;
+}
 
 }  // namespace fortai_hip

@@ -140,6 +140,26 @@ inline const char *check_kv8_rows(const Kv8Shape &s, int layer, int dtype, const
     return nullptr;
 }
 
+inline const char *check_kv8_attention(const Kv8Shape &s, int layer, int dtype, int rows, int max_rows, const void *query,
+    int64_t query_pitch, int64_t query_head_pitch, const void *gate, int heads, float scale, int max_length,
+    const void *output, int64_t output_pitch) {
+    if (layer < 0 || layer >= s.layers) return "kv8: no such layer";
+    if (!dtype_ok(dtype)) return "kv8: unknown dtype";
+    if (heads < 1 || heads % s.kv_heads || heads > 65535) return "kv8: heads a multiple of the cache's, at most 65535";
+    const int64_t group = heads / s.kv_heads;
+    if (group * max_rows > kMaxRows || (group * max_rows + 7) / 8 * s.kv_heads > 65535)
+        return "kv8: more rows in a sequence than a call takes";
+    if (!(std::fabs(scale) <= 1e30f)) return "kv8: scale is not a number, or beyond 1e30";
+    if (max_length < 0) return "kv8: max_length below 0";
+    if (!query || !output) return "kv8: null array";
+    const size_t e = dtype_bytes(dtype);
+    if (!aligned(query, e) || !aligned(gate, e) || !aligned(output, e)) return "kv8: misaligned array";
+    if (!pitch_ok(query_pitch) || !pitch_ok(query_head_pitch)) return "kv8: pitches 0 to 2^31";
+    if (!pitch_ok(output_pitch) || (rows > 1 && output_pitch < static_cast<int64_t>(heads) * s.head))
+        return "kv8: output pitch from heads * head to 2^31";
+    return nullptr;
+}
+
 // Pairs that can be copied in any order: ids within the pool, no page written
 // twice, none both read and written.  May throw std::bad_alloc.
 inline const char *check_page_pairs(const int32_t *from, const int32_t *to, int count, int pages) {

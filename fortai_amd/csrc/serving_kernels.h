@@ -36,6 +36,20 @@ hipError_t launch_kv8_read(const Kv8View &cache, const Kv8Rows &batch, Dtype dty
 // cache: the first layer; layer_codes, layer_tops: bytes and maxima of a layer's planes; from, to: host arrays
 hipError_t launch_kv8_copy_pages(const Kv8View &cache, size_t layer_codes, size_t layer_tops, int layers,
     const int32_t *from, const int32_t *to, int count, hipStream_t stream);
+
+struct Kv8AttentionParams {
+    Kv8View cache;
+    Kv8Rows batch;
+    const void *q = nullptr, *gate = nullptr;  // gate: null, or at q's pitches
+    void *out = nullptr;
+    int64_t q_row = 0, q_head = 0, out_row = 0;
+    int group = 0;            // query heads of a kv head
+    float scale_log2 = 0.0f;  // softmax scale * log2(e) / 127
+    bool vec = false;         // q, gate and out allow four-element accesses
+    float *partial = nullptr, *partial_ml = nullptr;  // [kKv8PartialRows][head], [kKv8PartialRows][2]
+    int splits = 0, row_tiles = 0;  // set by the launcher
+};
+hipError_t launch_kv8_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8Plan &plan, hipStream_t stream);
 hipError_t launch_kv8_clear(void *storage, size_t bytes, hipStream_t stream);
 
 }  // namespace fortai_hip

@@ -944,3 +944,14 @@ FORTAI_HIP_WEAK int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool
     (void)pool; (void)sequences; (void)count; (void)tables; (void)table_pitch;
     return FORTAI_HIP_RUNTIME_ERROR;
 }
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, const void *device_query, int64_t query_pitch,
+    int64_t query_head_pitch, const void *device_gate, int heads, float scale, int max_length,
+    void *device_output, int64_t output_pitch)
+{
+    (void)cache; (void)layer; (void)batch; (void)dtype; (void)device_query; (void)query_pitch;
+    (void)query_head_pitch; (void)device_gate; (void)heads; (void)scale; (void)max_length;
+    (void)device_output; (void)output_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}

@@ -560,6 +560,23 @@ int fortai_hip_kv8_read_device(fortai_hip_kv8_cache *cache, int layer,
 int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *cache, const int32_t *from, const int32_t *to,
     int count);
 
+/* Attention of a batch's rows over the cached tokens of their sequences: row i of
+ * sequence s attends to tokens 0 .. lengths[s] + i (its own included, so append
+ * first; tokens without a page are left out).  Query head h goes with kv head
+ * h / (heads / kv_heads).  out = softmax(scale q.k) v, times sigmoid(gate) where
+ * device_gate is not NULL (an array at the queries' pitches: in the layers'
+ * [heads][q | gate] projection, the query's address + head_size).  Queries at
+ * row and head pitches, outputs [rows][heads][head_size] at a row pitch.  Rows
+ * that see no token give zeros; rows that belong to no sequence are left as they
+ * were.  max_length: about the largest lengths[s] + rows, for cutting the work; a
+ * wrong one costs time only.  Queries that are not finite give NaN in their row
+ * and head.  fp32 queries are computed to fp32's accuracy.  A sequence's rows
+ * times heads / kv_heads, in groups of 8 and over the kv heads, go up to 65535. */
+int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, int dtype, const void *device_query, int64_t query_pitch,
+    int64_t query_head_pitch, const void *device_gate, int heads, float scale, int max_length,
+    void *device_output, int64_t output_pitch);
+
 /* Which pages whose tokens lie in: host bookkeeping for one pool and up to
  * `sequences` sequences of at most table_pitch pages; no GPU is needed, and a
  * refused call (INVALID) changes nothing.
