@@ -132,6 +132,9 @@ _SIGNATURES = {
     "fortai_hip_kv8_read_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64],
     "fortai_hip_kv8_attention_device": [_vp, _i, _vp, _i, _vp, _i64, _i64, _vp, _i, _f, _i, _vp, _i64],
     "fortai_hip_kv8_copy_pages": [_vp, _vp, _vp, _i],
+    "fortai_hip_verifier_create": [_vp, _i, _i, _i, _vpp],
+    "fortai_hip_verifier_destroy": [_vp],
+    "fortai_hip_verify_drafts_device": [_vp, _i, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp],
     "fortai_hip_kv8_pages_create": [_i, _i, _i, _i, _vpp],
     "fortai_hip_kv8_pages_destroy": [_vp],
     "fortai_hip_kv8_pages_extend": [_vp, _i, _i, _vp, _vp, _vp],
@@ -760,4 +763,33 @@ class Kv8Pages:
     def free(self) -> None:
         if self.h:
             self.lib.fortai_hip_kv8_pages_destroy(self.h)
+            self.h = None
+
+
+class Verifier:
+    """Verification of drafted tokens against the target's logits
+    (fortai_hip_verify_drafts_device), for up to max_rows rows of max_sequences
+    sequences and one vocabulary."""
+
+    def __init__(self, ctx: Context, max_rows: int, max_sequences: int, vocab: int):
+        self.ctx, self.vocab = ctx, vocab
+        h = C.c_void_p()
+        ctx.call("fortai_hip_verifier_create", ctx.h, max_rows, max_sequences, vocab, C.byref(h))
+        self.h = h
+
+    def run(self, target_logits, tokens, uniforms, row_starts, sequences: int, rows: int, emitted, accepted,
+            dtype: str = "f32", draft_logits=None, temperatures=None, logprobs=None,
+            target_pitch: Optional[int] = None, draft_pitch: Optional[int] = None) -> None:
+        """Device arrays: target_logits and draft_logits [rows][vocab] (dense unless pitches are given), tokens int64
+        [rows], uniforms fp32 [rows], row_starts int32 [sequences + 1], temperatures fp32 [sequences] -> emitted int64
+        [rows], accepted int32 [sequences], logprobs fp32 [rows]."""
+        self.ctx.check(self.ctx.lib.fortai_hip_verify_drafts_device(
+            self.h, DTYPES[dtype], _dev(target_logits), self.vocab if target_pitch is None else target_pitch,
+            _dev(draft_logits), self.vocab if draft_pitch is None else draft_pitch, _dev(tokens), _dev(uniforms),
+            _dev(temperatures), sequences, _dev(row_starts), rows, _dev(emitted), _dev(accepted), _dev(logprobs)),
+            "fortai_hip_verify_drafts_device")
+
+    def free(self) -> None:
+        if self.h:
+            self.ctx.lib.fortai_hip_verifier_destroy(self.h)
             self.h = None

@@ -69,6 +69,16 @@ struct fortai_hip_kv8_cache {
     }
 };
 
+struct fortai_hip_verifier {
+    fortai_hip_q8_context *context = nullptr;
+    int device = 0;
+    int max_rows = 0, max_sequences = 0, vocab = 0, chunk = 0, chunks = 0;
+    // made with the verifier and never again, so that a captured call keeps their addresses
+    VerifyPart *parts = nullptr;
+    double *weights = nullptr;
+    std::mutex launches;  // a call's launches follow each other on the stream
+};
+
 namespace {
 
 Kv8Rows batch_rows(const fortai_hip_kv8_batch *b) {
@@ -299,6 +309,79 @@ int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *h, const int32_t *from, cons
     const DeviceScope scope(c->device);
     return done(c, launch_kv8_copy_pages(h->layer(0), h->shape.layer_codes(), h->shape.layer_tops(), h->shape.layers, from,
         to, count, c->stream), "kv8 copy pages");
+}
+
+// -------------------------------------------------------- draft verification
+int fortai_hip_verifier_create(fortai_hip_q8_context *c, int max_rows, int max_sequences, int vocab,
+    fortai_hip_verifier **verifier) {
+    if (!c || !verifier) return FORTAI_HIP_INVALID;
+    *verifier = nullptr;
+    if (const char *wrong = check_verifier(max_rows, max_sequences, vocab)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    auto *h = new (std::nothrow) fortai_hip_verifier;
+    if (!h) return fail(c, FORTAI_HIP_RUNTIME_ERROR, "verify: out of host memory");
+    h->context = c;
+    h->device = c->device;
+    h->max_rows = max_rows;
+    h->max_sequences = max_sequences;
+    h->vocab = vocab;
+    h->chunk = verify_chunk(max_rows, vocab);
+    h->chunks = (vocab + h->chunk - 1) / h->chunk;
+    const DeviceScope scope(c->device);
+    hipError_t e = alloc(&h->parts, 2 * static_cast<size_t>(max_rows) * h->chunks);
+    if (e == hipSuccess) e = alloc(&h->weights, static_cast<size_t>(max_sequences) * h->chunks);
+    if (e != hipSuccess) {
+        release(h->parts);
+        release(h->weights);
+        delete h;
+        return fail(c, FORTAI_HIP_RUNTIME_ERROR, "verifier create", e);
+    }
+    *verifier = h;
+    return FORTAI_HIP_OK;
+}
+
+int fortai_hip_verifier_destroy(fortai_hip_verifier *h) {
+    if (!h) return FORTAI_HIP_OK;
+    const DeviceScope scope(h->device);
+    release(h->parts);
+    release(h->weights);
+    delete h;
+    return FORTAI_HIP_OK;
+}
+
+int fortai_hip_verify_drafts_device(fortai_hip_verifier *h, int dtype, const void *target_logits, int64_t target_pitch,
+    const void *draft_logits, int64_t draft_pitch, const void *tokens, const void *uniforms, const void *temperatures,
+    int sequences, const void *row_starts, int rows, void *emitted, void *accepted, void *logprobs) {
+    if (!h) return FORTAI_HIP_INVALID;
+    fortai_hip_q8_context *c = h->context;
+    if (const char *wrong = check_verify(h->max_rows, h->max_sequences, h->vocab, dtype, target_logits, target_pitch,
+            draft_logits, draft_pitch, tokens, uniforms, temperatures, sequences, row_starts, rows, emitted, accepted, logprobs))
+        return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (sequences == 0) return FORTAI_HIP_OK;
+    VerifyParams p;
+    p.target = target_logits;
+    p.draft = draft_logits;
+    p.target_pitch = target_pitch;
+    p.draft_pitch = draft_pitch;
+    p.tokens = static_cast<const int64_t *>(tokens);
+    p.uniforms = static_cast<const float *>(uniforms);
+    p.temperatures = static_cast<const float *>(temperatures);
+    p.row_starts = static_cast<const int32_t *>(row_starts);
+    p.emitted = static_cast<int64_t *>(emitted);
+    p.accepted = static_cast<int32_t *>(accepted);
+    p.logprobs = static_cast<float *>(logprobs);
+    p.parts = h->parts;
+    p.weights = h->weights;
+    p.rows = rows;
+    p.max_rows = h->max_rows;
+    p.sequences = sequences;
+    p.vocab = h->vocab;
+    p.chunk = h->chunk;
+    p.chunks = h->chunks;
+    const bool vec = vector4_ok(target_logits, dtype, target_pitch, 0) &&
+        (!draft_logits || vector4_ok(draft_logits, dtype, draft_pitch, 0));
+    const DeviceScope scope(c->device);
+    const std::lock_guard<std::mutex> lock(h->launches);
+    return done(c, launch_verify(p, static_cast<Dtype>(dtype), vec, c->stream), "draft verification");
 }
 
 }  // extern "C"

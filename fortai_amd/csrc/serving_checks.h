@@ -175,4 +175,37 @@ inline const char *check_page_pairs(const int32_t *from, const int32_t *to, int 
     return nullptr;
 }
 
+// -------------------------------------------------------- draft verification
+inline const char *check_verifier(int max_rows, int max_sequences, int vocab) {
+    if (max_rows < 1 || max_rows > 65535) return "verify: rows 1 to 65535";
+    if (max_sequences < 1 || max_sequences > 65535) return "verify: sequences 1 to 65535";
+    if (vocab < 1 || vocab > (1 << 28)) return "verify: vocabulary 1 to 2^28";
+    return nullptr;
+}
+
+// Tokens a workgroup takes of a row: 4096, or 1024 where that leaves fewer than
+// two workgroups a CU.
+inline int verify_chunk(int max_rows, int vocab) {
+    return static_cast<int64_t>(max_rows) * ((vocab + 4095) / 4096) >= 512 ? 4096 : 1024;
+}
+
+inline const char *check_verify(int max_rows, int max_sequences, int vocab, int dtype, const void *target,
+    int64_t target_pitch, const void *draft, int64_t draft_pitch, const void *tokens, const void *uniforms,
+    const void *temperatures, int sequences, const void *row_starts, int rows, const void *emitted, const void *accepted,
+    const void *logprobs) {
+    if (!dtype_ok(dtype)) return "verify: unknown dtype";
+    if (sequences < 0 || sequences > max_sequences || rows < 0 || rows > max_rows)
+        return "verify: more rows or sequences than the verifier was made for";
+    if (sequences == 0) return nullptr;
+    if (!row_starts || !accepted || (rows > 0 && (!target || !tokens || !uniforms || !emitted))) return "verify: null array";
+    const size_t e = dtype_bytes(dtype);
+    if (!aligned(target, e) || !aligned(draft, e) || !aligned(tokens, 8) || !aligned(uniforms, 4) ||
+        !aligned(temperatures, 4) || !aligned(row_starts, 4) || !aligned(emitted, 8) || !aligned(accepted, 4) ||
+        !aligned(logprobs, 4))
+        return "verify: misaligned array";
+    if (target_pitch < vocab || !pitch_ok(target_pitch) || (draft && (draft_pitch < vocab || !pitch_ok(draft_pitch))))
+        return "verify: pitches from the vocabulary to 2^31";
+    return nullptr;
+}
+
 }  // namespace fortai_hip

@@ -52,4 +52,28 @@ struct Kv8AttentionParams {
 hipError_t launch_kv8_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8Plan &plan, hipStream_t stream);
 hipError_t launch_kv8_clear(void *storage, size_t bytes, hipStream_t stream);
 
+
+// a row's chunk of the vocabulary: its largest logit, the first token that has it, sum of exp((x - top) / T)
+struct VerifyPart {
+    double sum;
+    float top;
+    int32_t place;
+};
+
+struct VerifyParams {
+    const void *target = nullptr, *draft = nullptr;  // [rows][vocab]; draft null: drafts without probabilities
+    int64_t target_pitch = 0, draft_pitch = 0;
+    const int64_t *tokens = nullptr;        // [rows]
+    const float *uniforms = nullptr;        // [rows]
+    const float *temperatures = nullptr;    // [sequences], or null: 1
+    const int32_t *row_starts = nullptr;    // [sequences + 1]
+    int64_t *emitted = nullptr;             // [rows]
+    int32_t *accepted = nullptr;            // [sequences]
+    float *logprobs = nullptr;              // [rows], or null
+    VerifyPart *parts = nullptr;            // [2][max_rows][chunks]
+    double *weights = nullptr;              // [sequences][chunks]
+    int rows = 0, max_rows = 0, sequences = 0, vocab = 0, chunk = 0, chunks = 0;
+};
+hipError_t launch_verify(const VerifyParams &p, Dtype dtype, bool vec, hipStream_t stream);
+
 }  // namespace fortai_hip

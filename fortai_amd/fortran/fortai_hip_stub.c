@@ -955,3 +955,30 @@ FORTAI_HIP_WEAK int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache,
     (void)device_output; (void)output_pitch;
     return FORTAI_HIP_RUNTIME_ERROR;
 }
+
+FORTAI_HIP_WEAK int fortai_hip_verifier_create(fortai_hip_q8_context *context, int max_rows,
+    int max_sequences, int vocab, fortai_hip_verifier **verifier)
+{
+    (void)context; (void)max_rows; (void)max_sequences; (void)vocab;
+    if (verifier) *verifier = NULL;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_verifier_destroy(fortai_hip_verifier *verifier)
+{
+    (void)verifier;
+    return FORTAI_HIP_OK;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_verify_drafts_device(fortai_hip_verifier *verifier, int dtype,
+    const void *device_target_logits, int64_t target_pitch, const void *device_draft_logits,
+    int64_t draft_pitch, const void *device_tokens, const void *device_uniforms,
+    const void *device_temperatures, int sequences, const void *device_row_starts, int rows,
+    void *device_emitted, void *device_accepted, void *device_logprobs)
+{
+    (void)verifier; (void)dtype; (void)device_target_logits; (void)target_pitch;
+    (void)device_draft_logits; (void)draft_pitch; (void)device_tokens; (void)device_uniforms;
+    (void)device_temperatures; (void)sequences; (void)device_row_starts; (void)rows;
+    (void)device_emitted; (void)device_accepted; (void)device_logprobs;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}

@@ -40,6 +40,7 @@ typedef struct fortai_hip_qwen35_batch fortai_hip_qwen35_batch;        /* [exten
 typedef struct fortai_hip_rope fortai_hip_rope;                        /* [extension] */
 typedef struct fortai_hip_kv8_cache fortai_hip_kv8_cache;              /* [extension] */
 typedef struct fortai_hip_kv8_pages fortai_hip_kv8_pages;              /* [extension] */
+typedef struct fortai_hip_verifier fortai_hip_verifier;                /* [extension] */
 
 enum {
     FORTAI_HIP_OK = 0,
@@ -605,6 +606,39 @@ int64_t fortai_hip_kv8_pages_length(const fortai_hip_kv8_pages *pool, int sequen
 int fortai_hip_kv8_pages_free_count(const fortai_hip_kv8_pages *pool);
 int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool, const int *sequences, int count,
     int32_t *tables, int table_pitch);
+
+/* Verification of drafted tokens.  Rows row_starts[s] .. row_starts[s + 1] - 1
+ * (device int32 [sequences + 1]) are the step of sequence s: its first row ran
+ * the last token that stands, the others its drafts.  device_tokens (int64
+ * [rows]) are the step's tokens, so that the draft which row r's logits judge is
+ * tokens[r + 1]; row r of draft_logits is the distribution it was drawn from.
+ * Without draft_logits (NULL) drafts count as certain.  A sequence's last row
+ * judges no draft: what its draft logits hold does not matter.
+ * With p = softmax(target / T) and q = softmax(draft / T) a draft x stands while
+ * uniforms[r] q(x) < p(x).  At the first that does not, a token is drawn from
+ * max(p - q, 0) (from p where that is zero everywhere); if all stand, from p of
+ * the last row.  Drawn is the lowest token whose cumulative weight exceeds u times
+ * the total, with u the uniform of the sequence's last row; all in 64 bits.
+ * device_uniforms: fp32 [rows] in [0, 1).  device_temperatures: fp32 [sequences]
+ * (NULL: 1); T <= 0 takes the first of the largest logits instead, and a draft
+ * stands if it is that.
+ * Outputs: emitted (int64 [rows]) has for each sequence the drafts that stand, the
+ * drawn token, then -1; accepted (int32 [sequences]) how many stand; logprobs
+ * (fp32 [rows], may be NULL) log p of each emitted token, 0 behind them (T <= 0:
+ * at T = 1).  A logit of -infinity or NaN has no weight, +infinity counts as the
+ * largest number; a deciding row without any weight emits -1 with -infinity.  A
+ * draft outside the vocabulary does not stand.  Rows of no sequence are left as
+ * they were.  Logits are fp32, fp16 or bf16 at row pitches; a verifier is made
+ * for at most max_rows rows, max_sequences sequences (both up to 65535) and one
+ * vocabulary (up to 2^28). */
+int fortai_hip_verifier_create(fortai_hip_q8_context *context, int max_rows, int max_sequences,
+    int vocab, fortai_hip_verifier **verifier);
+int fortai_hip_verifier_destroy(fortai_hip_verifier *verifier);
+int fortai_hip_verify_drafts_device(fortai_hip_verifier *verifier, int dtype,
+    const void *device_target_logits, int64_t target_pitch, const void *device_draft_logits,
+    int64_t draft_pitch, const void *device_tokens, const void *device_uniforms,
+    const void *device_temperatures, int sequences, const void *device_row_starts, int rows,
+    void *device_emitted, void *device_accepted, void *device_logprobs);
 
 #ifdef __cplusplus
 }
