@@ -54,4 +54,12 @@ __device__ __forceinline__ void store4(typename Element<DT>::type *p, f32x4_t v)
     }
 }
 
+// A workgroup barrier that orders LDS accesses only: loads from memory that are in
+// flight stay so (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 }  // namespace fortai_hip

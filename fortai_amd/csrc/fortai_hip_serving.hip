@@ -76,6 +76,8 @@ struct fortai_hip_verifier {
     // made with the verifier and never again, so that a captured call keeps their addresses
     VerifyPart *parts = nullptr;
     double *weights = nullptr;
+    VerifyDecision *decisions = nullptr;
+    VerifyRow *row_stats = nullptr;
     std::mutex launches;  // a call's launches follow each other on the stream
 };
 
@@ -329,9 +331,13 @@ int fortai_hip_verifier_create(fortai_hip_q8_context *c, int max_rows, int max_s
     const DeviceScope scope(c->device);
     hipError_t e = alloc(&h->parts, 2 * static_cast<size_t>(max_rows) * h->chunks);
     if (e == hipSuccess) e = alloc(&h->weights, static_cast<size_t>(max_sequences) * h->chunks);
+    if (e == hipSuccess) e = alloc(&h->decisions, static_cast<size_t>(max_sequences));
+    if (e == hipSuccess) e = alloc(&h->row_stats, static_cast<size_t>(max_rows));
     if (e != hipSuccess) {
         release(h->parts);
         release(h->weights);
+        release(h->decisions);
+        release(h->row_stats);
         delete h;
         return fail(c, FORTAI_HIP_RUNTIME_ERROR, "verifier create", e);
     }
@@ -344,6 +350,8 @@ int fortai_hip_verifier_destroy(fortai_hip_verifier *h) {
     const DeviceScope scope(h->device);
     release(h->parts);
     release(h->weights);
+    release(h->decisions);
+    release(h->row_stats);
     delete h;
     return FORTAI_HIP_OK;
 }
@@ -371,13 +379,15 @@ int fortai_hip_verify_drafts_device(fortai_hip_verifier *h, int dtype, const voi
     p.logprobs = static_cast<float *>(logprobs);
     p.parts = h->parts;
     p.weights = h->weights;
+    p.decisions = h->decisions;
+    p.row_stats = h->row_stats;
     p.rows = rows;
     p.max_rows = h->max_rows;
     p.sequences = sequences;
     p.vocab = h->vocab;
     p.chunk = h->chunk;
     p.chunks = h->chunks;
-    const bool vec = vector4_ok(target_logits, dtype, target_pitch, 0) &&
+    const bool vec = h->vocab % 4 == 0 && vector4_ok(target_logits, dtype, target_pitch, 0) &&
         (!draft_logits || vector4_ok(draft_logits, dtype, draft_pitch, 0));
     const DeviceScope scope(c->device);
     const std::lock_guard<std::mutex> lock(h->launches);

@@ -15,7 +15,7 @@
 // workgroup owns a page and head (keys or values), so that no two write a word.
 //
 // Bound by memory for prompts, by the chain of dependent loads (rows, table, A,
-// values) for single tokens.  A wave takes blocks of 16 tokens x 64 dims, a lane
+// values) for single tokens.  A wave takes a block of 16 tokens x 64 dims, a lane
 // 4 x 4 of them: reads of 256 (fp32) or 128 bytes in a row and, for both orders,
 // writes of whole words with the transpose inside the lane.
 #include "fortai_hip_internal.h"
@@ -28,46 +28,57 @@ namespace {
 
 constexpr int kPageThreads = 256;
 constexpr int kPageWaves = kPageThreads / 64;
-constexpr int kBlocksPerWave = 4;  // 64 tokens x 256 dims over 4 waves
+constexpr int kAppendWaves = 16;  // 64 tokens x 256 dims, a block of 16 x 64 a wave
 
-// round(|v| n / a) for finite v, ties to even, of the exact quotient; v n and
-// (2 k + 1) a are exact in 64 bits (7 + 24 and 8 + 24 bits).
-// inverse: n / a rounded to fp32, so |v| inverse is off by at most 127 * 2^-23.
-__device__ __forceinline__ int nearest_code(float v, float n, float a, float inverse) {
-    v = fabsf(v);
-    if (a < 1e-30f) {  // n / a may overflow fp32; the fp64 quotient cannot round onto a tie that it is not
-        return a > 0.0f ? static_cast<int>(__builtin_rint(static_cast<double>(v) * n / a)) : 0;
+// The integer nearest to v n / a, ties to even, of the exact quotient; v >= 0 and
+// n <= 127 a, all scaled so that a is in [1/2, 1).  inverse: n / a rounded, so the
+// first guess is off by one at most.  The border odd a = (2 k + 1) a is split into
+// p + e exactly, and 2 v n - p, which near the border is a difference of two
+// products of 32 bits, fits fp32: what is compared is exact where it is close.
+__device__ __forceinline__ int nearest_code(float v, float twice_n, float a, float inverse) {
+    const float k = floorf(v * inverse), odd = __builtin_fmaf(2.0f, k, 1.0f);
+    const float p = odd * a, e = __builtin_fmaf(odd, a, -p), r = __builtin_fmaf(v, twice_n, -p);
+    const int i = static_cast<int>(k);
+    return i + (r > e || (r == e && (i & 1)) ? 1 : 0);
+}
+
+// a page's magnitude as [1/2, 1) and its exponent, and what codes are made with
+struct CodeScale {
+    float a, inverse;
+    int exponent;
+    __device__ __forceinline__ explicit CodeScale(float top) {
+        exponent = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
+        a = top > 0.0f ? __builtin_ldexpf(top, -exponent) : 1.0f;
+        inverse = 127.0f / a;
     }
-    const float y = v * inverse, whole = floorf(y), part = y - whole;
-    int k = static_cast<int>(whole) + (part > 0.5f ? 1 : 0);
-    if (fabsf(part - 0.5f) < 2e-4f) {
-        k = static_cast<int>(whole);
-        const double twice = 2.0 * static_cast<double>(v) * n, border = (2.0 * k + 1.0) * static_cast<double>(a);
-        if (twice > border || (twice == border && (k & 1))) ++k;
+    // An infinity stands for the largest magnitude.  NaN has been made zero.
+    __device__ __forceinline__ uint32_t code(float x) const {
+        int k = nearest_code(__builtin_ldexpf(fabsf(x), -exponent), 254.0f, a, inverse);
+        k = fabsf(x) == __builtin_inff() ? 127 : k;
+        return static_cast<uint32_t>(x < 0.0f ? -k : k) & 0xffu;
     }
-    return min(k, 127);
-}
+};
 
-// An infinity stands for the largest magnitude, NaN for zero.
-__device__ __forceinline__ uint32_t code_byte(float x, float a, float inverse) {
-    if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? 0u : (x > 0.0f ? 127u : 0x81u);
-    const int k = nearest_code(x, 127.0f, a, inverse);
-    return static_cast<uint32_t>(x < 0.0f ? -k : k) & 0xffu;
-}
+// old codes under a raised magnitude: code * was / a
+struct Requantizer {
+    float twice_was, a, ratio;
+    __device__ __forceinline__ Requantizer(float was, const CodeScale &s)
+        : twice_was(__builtin_ldexpf(was, 1 - s.exponent)), a(s.a), ratio(0.5f * twice_was / s.a) {}
+    __device__ __forceinline__ uint32_t code(uint32_t byte) const {
+        const int c = static_cast<int8_t>(byte);
+        const int k = nearest_code(fabsf(static_cast<float>(c)), twice_was, a, ratio);
+        return static_cast<uint32_t>(c < 0 ? -k : k) & 0xffu;
+    }
+    __device__ __forceinline__ uint32_t word(uint32_t w) const {
+        return code(w) | code(w >> 8) << 8 | code(w >> 16) << 16 | code(w >> 24) << 24;
+    }
+};
 
-__device__ __forceinline__ uint32_t requantized_byte(uint32_t byte, float was, float a, float ratio) {
-    const int c = static_cast<int8_t>(byte);
-    const int k = nearest_code(static_cast<float>(c), was, a, ratio);
-    return static_cast<uint32_t>(c < 0 ? -k : k) & 0xffu;
-}
-
-template <Dtype DT, bool VEC>
-__global__ __launch_bounds__(kPageThreads) void kv8_append_kernel(Kv8View cache, Kv8Rows batch,
-    const typename Element<DT>::type *__restrict__ keys, int64_t key_pitch,
-    const typename Element<DT>::type *__restrict__ values, int64_t value_pitch) {
-    __shared__ float wave_top[kPageWaves];
+template <Dtype DT, bool VEC, bool VALUES>
+__device__ __forceinline__ void append_page(const Kv8View &cache, const Kv8Rows &batch,
+    const typename Element<DT>::type *__restrict__ x, int64_t pitch) {
+    __shared__ float wave_top[kAppendWaves];
     const int seq = blockIdx.z >> 1, head = blockIdx.y;
-    const bool is_value = blockIdx.z & 1;
     const int P = cache.page_tokens, D = cache.head;
     int begin, count;
     batch.range(seq, &begin, &count);
@@ -80,83 +91,81 @@ __global__ __launch_bounds__(kPageThreads) void kv8_append_kernel(Kv8View cache,
     if (id < 0) return;
     const int old = length > first ? new_from : 0;  // slots [0, old) hold tokens already
     const size_t which = static_cast<size_t>(id) * cache.kv_heads + head;
-    float *top_at = (is_value ? cache.value_max : cache.key_max) + which;
-    uint32_t *codes = reinterpret_cast<uint32_t *>((is_value ? cache.values : cache.keys) + which * P * D);
+    float *top_at = (VALUES ? cache.value_max : cache.key_max) + which;
+    uint32_t *codes = reinterpret_cast<uint32_t *>((VALUES ? cache.values : cache.keys) + which * P * D);
     const float was = old > 0 ? *top_at : 0.0f;
-    const typename Element<DT>::type *x = (is_value ? values : keys) + static_cast<int64_t>(head) * D;
-    const int64_t pitch = is_value ? value_pitch : key_pitch;
+    x += static_cast<int64_t>(head) * D + static_cast<int64_t>(begin + first - length) * pitch;  // slot 0's row
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int dim_blocks = D / 64, blocks = (P / 16) * dim_blocks;
-    f32x4_t v[kBlocksPerWave][4];  // [block][token of the four][dim of the four]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dim_blocks = D / 64;
+    const int slot = (wave / dim_blocks) * 16 + (lane >> 4) * 4, d = (wave % dim_blocks) * 64 + (lane & 15) * 4;
+    f32x4_t v[4];  // [token of the four][dim of the four]
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (slot + i >= new_from && slot + i < new_until) v[i] = load4<DT, VEC>(x + static_cast<int64_t>(slot + i) * pitch + d);
+    }
     float top = 0.0f;
 #pragma unroll
-    for (int b = 0; b < kBlocksPerWave; ++b) {
-        const int block = b * kPageWaves + wave;
-        const int slot = (block / dim_blocks) * 16 + (lane >> 4) * 4, d = (block % dim_blocks) * 64 + (lane & 15) * 4;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[b][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (block < blocks && slot + i >= new_from && slot + i < new_until)
-                v[b][i] = load4<DT, VEC>(x + static_cast<int64_t>(begin + first + slot + i - length) * pitch + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float m = fabsf(v[b][i][j]);
-                if (m <= 3.402823466e38f) top = fmaxf(top, m);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const float m = fabsf(v[i][j]);
+            v[i][j] = m == m ? v[i][j] : 0.0f;
+            top = m < __builtin_inff() ? fmaxf(top, m) : top;
         }
-    }
     top = wave_max(top);
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
     float a = was;
-#pragma unroll
-    for (int w = 0; w < kPageWaves; ++w) a = fmaxf(a, wave_top[w]);
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) a = fmaxf(a, wave_top[w]);
     const bool grown = old > 0 && a > was;
-    const float inverse = 127.0f / a, ratio = was / a;  // not used where a is zero or tiny
+    const CodeScale scale(a);
+    const Requantizer again(was, scale);
     if (threadIdx.x == 0) *top_at = a;
 
+    const bool some_new = slot + 3 >= new_from && slot < new_until;
+    if (!some_new && !(grown && slot < old)) return;
+    // the slots of this lane's four that are new, and those rounded again
+    uint32_t fresh = 0, rounded = 0;
 #pragma unroll
-    for (int b = 0; b < kBlocksPerWave; ++b) {
-        const int block = b * kPageWaves + wave;
-        const int slot = (block / dim_blocks) * 16 + (lane >> 4) * 4, d = (block % dim_blocks) * 64 + (lane & 15) * 4;
-        const bool some_new = slot + 3 >= new_from && slot < new_until;
-        if (block >= blocks || (!some_new && !(grown && slot < old))) continue;
-        if (!is_value) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t *at = codes + (static_cast<size_t>(slot + i) * D + d) / 4;
-                if (slot + i >= new_from && slot + i < new_until) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w |= code_byte(v[b][i][j], a, inverse) << (8 * j);
-                    *at = w;
-                } else if (grown && slot + i < old) {
-                    const uint32_t c = *at;
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w |= requantized_byte(c >> (8 * j), was, a, ratio) << (8 * j);
-                    *at = w;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t *at = codes + (static_cast<size_t>(d + j) * P + slot) / 4;
-                const bool all_new = slot >= new_from && slot + 3 < new_until;
-                const uint32_t c = all_new ? 0u : *at;  // slots that are neither new nor rounded again keep their codes
-                uint32_t w = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t byte = c >> (8 * i);
-                    if (slot + i >= new_from && slot + i < new_until) byte = code_byte(v[b][i][j], a, inverse);
-                    else if (grown && slot + i < old) byte = requantized_byte(byte, was, a, ratio);
-                    w |= (byte & 0xffu) << (8 * i);
-                }
-                *at = w;
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        if (slot + i >= new_from && slot + i < new_until) fresh |= 0xffu << (8 * i);
+        if (grown && slot + i < old) rounded |= 0xffu << (8 * i);
     }
+    uint32_t w[4];  // keys: of a token, values: of a dim
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = VALUES ? scale.code(v[0][i]) | scale.code(v[1][i]) << 8 | scale.code(v[2][i]) << 16 | scale.code(v[3][i]) << 24
+                      : scale.code(v[i][0]) | scale.code(v[i][1]) << 8 | scale.code(v[i][2]) << 16 | scale.code(v[i][3]) << 24;
+    uint32_t *at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        at[i] = codes + (VALUES ? static_cast<size_t>(d + i) * P + slot : static_cast<size_t>(slot + i) * D + d) / 4;
+    if (fresh == 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *at[i] = w[i];
+        return;
+    }
+    // slots that are neither new nor rounded again keep their codes
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t mine = i == 0 ? w[0] : i == 1 ? w[1] : i == 2 ? w[2] : w[3];
+        uint32_t *to = i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3];
+        const uint32_t take = VALUES ? fresh : (fresh >> (8 * i) & 1 ? 0xffffffffu : 0u);
+        const uint32_t turn = VALUES ? rounded : (rounded >> (8 * i) & 1 ? 0xffffffffu : 0u);
+        if ((take | turn) == 0) continue;
+        uint32_t kept = *to;
+        if (turn) kept = (again.word(kept) & turn) | (kept & ~turn);
+        *to = (mine & take) | (kept & ~take);
+    }
+}
+
+template <Dtype DT, bool VEC>
+__global__ __launch_bounds__(kAppendWaves * 64) void kv8_append_kernel(Kv8View cache, Kv8Rows batch,
+    const typename Element<DT>::type *__restrict__ keys, int64_t key_pitch,
+    const typename Element<DT>::type *__restrict__ values, int64_t value_pitch) {
+    if (blockIdx.z & 1) append_page<DT, VEC, true>(cache, batch, values, value_pitch);
+    else append_page<DT, VEC, false>(cache, batch, keys, key_pitch);
 }
 
 // Rows of the cache as values, the transpose of the value codes inside the lane
@@ -253,7 +262,7 @@ template <Dtype DT>
 void append_typed(const Kv8View &cache, const Kv8Rows &batch, const void *keys, int64_t key_pitch, const void *values,
     int64_t value_pitch, bool vec, hipStream_t stream) {
     typedef typename Element<DT>::type E;
-    const dim3 grid = page_grid(cache, batch), block(kPageThreads);
+    const dim3 grid = page_grid(cache, batch), block(cache.page_tokens / 16 * (cache.head / 64) * 64);
     const E *k = static_cast<const E *>(keys), *v = static_cast<const E *>(values);
     if (vec) hipLaunchKernelGGL((kv8_append_kernel<DT, true>), grid, block, 0, stream, cache, batch, k, key_pitch, v, value_pitch);
     else hipLaunchKernelGGL((kv8_append_kernel<DT, false>), grid, block, 0, stream, cache, batch, k, key_pitch, v, value_pitch);

@@ -60,6 +60,22 @@ struct VerifyPart {
     int32_t place;
 };
 
+// a row: its largest logit, the first token that has it, sum of exp((x - top) / T)
+struct VerifyRow {
+    double sum;
+    float top;
+    int32_t place;
+};
+
+// a sequence's rows [begin, end) and the one that decides (-1: it has no rows)
+struct VerifyDecision {
+    VerifyRow target, draft;  // of that row
+    double uniform;           // for the token that is drawn
+    int32_t begin, end, row;
+    int32_t rejected;         // the draft that was turned down there, -1: none in the vocabulary
+    int32_t against_draft;    // whether one was: what p has over q is drawn from
+};
+
 struct VerifyParams {
     const void *target = nullptr, *draft = nullptr;  // [rows][vocab]; draft null: drafts without probabilities
     int64_t target_pitch = 0, draft_pitch = 0;
@@ -72,6 +88,8 @@ struct VerifyParams {
     float *logprobs = nullptr;              // [rows], or null
     VerifyPart *parts = nullptr;            // [2][max_rows][chunks]
     double *weights = nullptr;              // [sequences][chunks]
+    VerifyDecision *decisions = nullptr;    // [sequences]
+    VerifyRow *row_stats = nullptr;         // [max_rows], of the target's rows up to the deciding one
     int rows = 0, max_rows = 0, sequences = 0, vocab = 0, chunk = 0, chunks = 0;
 };
 hipError_t launch_verify(const VerifyParams &p, Dtype dtype, bool vec, hipStream_t stream);

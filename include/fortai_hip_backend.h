@@ -620,8 +620,8 @@ int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool, const int *seq
  * the last row.  Drawn is the lowest token whose cumulative weight exceeds u times
  * the total, with u the uniform of the sequence's last row; all in 64 bits.
  * device_uniforms: fp32 [rows] in [0, 1).  device_temperatures: fp32 [sequences]
- * (NULL: 1); T <= 0 takes the first of the largest logits instead, and a draft
- * stands if it is that.
+ * (NULL: 1; above 10^9: 10^9); T <= 0 takes the first of the largest logits
+ * instead, and a draft stands if it is that.
  * Outputs: emitted (int64 [rows]) has for each sequence the drafts that stand, the
  * drawn token, then -1; accepted (int32 [sequences]) how many stand; logprobs
  * (fp32 [rows], may be NULL) log p of each emitted token, 0 behind them (T <= 0:
