@@ -288,10 +288,11 @@ int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *h, int layer, const fo
     p.out_row = output_pitch;
     p.group = heads / h->shape.kv_heads;
     p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074 / 127.0);
-    p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0);
+    p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0) &&
+        vector4_ok(gate, dtype, 0, 0);
     p.partial = h->partial;
     p.partial_ml = h->partial + static_cast<size_t>(kKv8PartialRows) * h->shape.head;
-    const Kv8Plan plan = kv8_plan(dtype == FORTAI_HIP_DTYPE_F32, batch->sequences, h->shape.kv_heads,
+    const Kv8Plan plan = kv8_plan(dtype == FORTAI_HIP_DTYPE_F32, h->shape.head, batch->sequences, h->shape.kv_heads,
         static_cast<int64_t>(batch->max_rows) * p.group, max_length);
     const DeviceScope scope(c->device);
     const std::lock_guard<std::mutex> lock(h->launches);

@@ -8,27 +8,28 @@
 // One pass over the cache with a running maximum.  The rows of a kv head (tokens
 // x heads of its group) are the columns of 16-wide matrix instructions, its
 // cached tokens the rows:
-//   S^T [token][row] = K Q^T,   O^T [dim][row] += V^T P^T
-// in v_mfma_f32_16x16x32_f16, the codes turned into fp16 (exact) in registers.
+//   S^T [token][row] = K Q^T in v_mfma_i32_16x16x64_i8, q as digits to the base 256
+//   O^T [dim][row] += V^T P^T in v_mfma_f32_16x16x32_f16, the codes turned into fp16
+// so that key codes are operands as they are and S is exact up to the query's digits.
 // A tile is 64 tokens.  Lane (r = lane & 15, g = lane >> 4) of tile part u (0..3)
 // feeds key token 16 (r >> 2) + 4 u + (r & 3), so that S leaves the instruction
 // with lane group g holding the 16 consecutive tokens 16 g .. 16 g + 15 of row r:
 // those are exactly the value codes that lane reads as one 16-byte word per dim
 // (pages are [dim][token]), in the order in which the next instruction takes its
-// k index.  Neither P nor a code ever goes through LDS.
+// k index.  P never goes through LDS.
 //
-// Numerics.  A row of q is scaled by a power of two to a magnitude below 1 and
-// rounded to fp16.  With SPLIT the 16 columns are 8 rows and, in the other 8, what
-// that rounding left over (times 2^11), and p is split the same way, so that
-// products keep 22 bits: used for fp32 queries, and where no more than 8 rows are
-// there to fill the columns.  Without it p is one fp16 number (2^-11 of itself).
-// A_v enters the running maximum by its exponent: the numerator's terms are
-// p_j A_v / 127, and what is rounded to fp16 is that product over the largest such
-// product (times 2^14, away from fp16's subnormals), so that pages of very
-// different magnitude lose nothing against each other.  All sums are fp32.
+// Numerics.  SPLIT: the 16 columns are 8 rows twice, for four digits of q (31 bits)
+// and for p in two fp16 halves (22 bits): used for fp32 queries, and where no more
+// than 8 rows are there to fill the columns.  Without it two digits (bf16) or three
+// (fp16), and p is one fp16 number (2^-11 of itself).  A_v enters the running maximum
+// by its exponent: the numerator's terms are p_j A_v / 127, and what is rounded to
+// fp16 is that product over the largest such product (times 2^14, away from fp16's
+// subnormals), so that pages of very different magnitude lose nothing against each
+// other.  All sums are fp32.
 //
-// Bound by the cache's bytes for few rows: 32 KiB of codes a tile and head of 256.
-// The four waves of a workgroup take tiles in turn; `splits` workgroups share a
+// Bound by what a wave has to issue for a tile (about 1,000 instructions, a third of
+// them turning value codes into fp16) rather than by the cache's bytes.  The four waves
+// of a workgroup take tiles in turn, two workgroups a CU; `splits` workgroups share a
 // sequence's head, joined by a second launch.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
@@ -40,6 +41,7 @@ namespace {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTileTokens = 64;
 constexpr int kWaves = 4;
@@ -64,10 +66,19 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // exponent that A_v adds to the running maximum, and what is left of A_v
 __device__ __forceinline__ int value_exponent(float top) { return min(max(__builtin_amdgcn_frexp_expf(top), -100), 100); }
 
+// Four dims of one row and head, gated and stored.  some: the row saw a token.
 template <Dtype DT>
-__device__ __forceinline__ float gated(float y, const typename Element<DT>::type *gate) {
-    const float g = static_cast<float>(*gate);
-    return y / (1.0f + expf(-g));
+__device__ __forceinline__ void finish(const Kv8AttentionParams &p, f32x4_t y, bool some, int64_t row, int head, int out, int dim) {
+    typedef typename Element<DT>::type E;
+    if (p.gate && some) {
+        const E *at = static_cast<const E *>(p.gate) + row * p.q_row + static_cast<int64_t>(head) * p.q_head + dim;
+        const f32x4_t g = p.vec ? load4<DT, true>(at) : load4<DT, false>(at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = y[i] / (1.0f + expf(-g[i]));
+    }
+    E *to = static_cast<E *>(p.out) + row * p.out_row + out;
+    if (p.vec) store4<DT, true>(to, y);
+    else store4<DT, false>(to, y);
 }
 
 // The rows of one sequence: the first in the batch's arrays, how many of a kv head; how many tokens the last row
@@ -88,156 +99,289 @@ __device__ __forceinline__ RowTile row_tile(const Kv8AttentionParams &p, int seq
     return t;
 }
 
-template <int D, Dtype DT, bool SPLIT, int RT>
-__global__ __launch_bounds__(kWaves * 64, RT == 1 ? 2 : 1) void kv8_attention_kernel(Kv8AttentionParams p) {
+// Until at most N of this wave's loads from memory are on their way (gfx9 s_waitcnt:
+// vmcnt in bits 3:0 and 15:14, the other counters left alone), with no LDS access
+// moved across it.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+    asm volatile("" ::: "memory");
+}
+
+// LDS reads done: what they read may be overwritten
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// 16 bytes a lane from base + offset (+ INST) to LDS at `to`, lane after lane.
+// Written out because the compiler, which cannot tell one buffer's loads from
+// another's, would have every LDS read wait for all of them; wait_loads() says which
+// have to be there.  There is no destination register.
+template <int INST>
+__device__ __forceinline__ void load_to_lds(uint32_t to, uint64_t base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
+                 :
+                 : "s"(to), "v"(offset), "s"(base), "n"(INST)
+                 : "memory");  // m0 too, which nothing else here uses
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)(p)));
+}
+
+__device__ __forceinline__ float read_only(const float *p) {
+    return *(const __attribute__((address_space(4))) float *)(p);
+}
+
+// Queries of a workgroup's rows into LDS as int8 operands, [set][chunk][lane][16]:
+// a row scaled by a power of two to magnitudes below 1, times 127, as digits to the
+// base 256, the leading one in [-127, 127].  A digit a set in the row's column: two
+// for bf16 (2^-16 of the row's largest, where a value's own last place is 2^-8 of
+// itself), three for fp16; with SPLIT four, two a set in columns r and r + 8.
+// 16 threads a row, 32 where there are no more than 8 rows.
+template <Dtype DT, bool SPLIT>
+constexpr int kSets = !SPLIT && DT == Dtype::F16 ? 3 : 2;
+
+template <int D, Dtype DT, bool SPLIT>
+__device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const RowTile &tile, int row0, int kvh,
+    uint32_t *operands, float *factors) {
     typedef typename Element<DT>::type E;
-    constexpr int kCols = SPLIT ? 8 : 16;           // rows in an instruction's 16 columns
-    constexpr int kRows = kCols * RT;
+    constexpr int kRows = SPLIT ? 8 : 16, kS = kSets<DT, SPLIT>, kDigits = SPLIT ? 2 * kS : kS;
+    constexpr float kOne = 127.0f * (kDigits == 4 ? 16777216.0f : kDigits == 3 ? 65536.0f : 256.0f);
+    constexpr int kThreads = D >= 128 && kRows == 8 ? 32 : 16, kSteps = D / 4 / kThreads;
+#pragma unroll 1
+    for (int base = 0; base < kRows; base += kWaves * 64 / kThreads) {
+        const int local = base + static_cast<int>(threadIdx.x) / kThreads, part = threadIdx.x % kThreads, row = row0 + local;
+        if (local >= kRows) break;  // whole waves
+        const bool there = row < tile.total;
+        const int token = there ? row / p.group : 0, head = kvh * p.group + (there ? row % p.group : 0);
+        const E *at = static_cast<const E *>(p.q) + static_cast<int64_t>(tile.begin + token) * p.q_row +
+            static_cast<int64_t>(head) * p.q_head;
+        f32x4_t v[kSteps];
+        float top = 0.0f;
+        if (p.vec) {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) v[c] = load4<DT, true>(at + 4 * (kThreads * c + part));
+        } else {
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) v[c] = load4<DT, false>(at + 4 * (kThreads * c + part));
+        }
+        float poison = 0.0f;  // NaN where an element is not finite: the digits cannot say so
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                top = fmaxf(top, fabsf(v[c][i]));
+                poison += v[c][i] * 0.0f;
+            }
+        top = fmaxf(top, xor_lane<1>(top));
+        top = fmaxf(top, xor_lane<2>(top));
+        top = fmaxf(top, xor_lane<4>(top));
+        top = fmaxf(top, xor_lane<8>(top));
+        if constexpr (kThreads == 32) top = fmaxf(top, xor_lane<16>(top));
+        poison += xor_lane<1>(poison);
+        poison += xor_lane<2>(poison);
+        poison += xor_lane<4>(poison);
+        poison += xor_lane<8>(poison);
+        if constexpr (kThreads == 32) poison += xor_lane<16>(poison);
+        const int e = __builtin_amdgcn_frexp_expf(top);
+        if (part == 0) factors[local] = __builtin_ldexpf(p.scale_log2, e) * (1.0f / 127.0f) + poison;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+            uint32_t digits[kDigits];
+#pragma unroll
+            for (int k = 0; k < kDigits; ++k) digits[k] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int x = poison == 0.0f ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(v[c][i], -e) * kOne)) : 0;
+#pragma unroll
+                for (int k = kDigits - 1; k >= 0; --k) {
+                    const int digit = k > 0 ? static_cast<int8_t>(x) : x;
+                    digits[k] |= (static_cast<uint32_t>(digit) & 0xffu) << (8 * i);
+                    x = (x - digit) >> 8;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kDigits; ++k) {
+                const int set = SPLIT ? k >> 1 : k, column = SPLIT ? local + 8 * (k & 1) : local;
+                const int four = kThreads * c + part;  // of the row's groups of four dims: 16 a chunk, 4 a lane
+                operands[(set * (D / 64) + (four >> 4)) * 256 + (((four & 15) >> 2) * 16 + column) * 4 + (four & 3)] = digits[k];
+            }
+        }
+    }
+}
+
+// Every wave has its tile's codes brought to LDS of its own by loads that leave no
+// trace in registers: 1 KiB a load, whole rows, so that lines are read whole (a
+// lane's operands lie in 16 rows: read from memory directly, they took five times as
+// many accesses).  What a lane reads from LDS is 16 bytes of row r; the units of 16
+// bytes are permuted within a row (by the load's source address) so that lanes of
+// neighbouring rows find different banks.
+//
+// Keys: token T of the tile in rows of D, unit x at x ^ f(T) with f from T's lane,
+//   r(T) = (T / 16) 4 + T % 4.  Values: pages of P tokens one behind the other, dim d
+//   in rows of P, unit x at x ^ f(d).
+template <int D>
+__device__ __forceinline__ int key_turn(int r) {
+    return D == 256 ? r : D == 128 ? r >> 1 : r >> 2;
+}
+
+template <int D, Dtype DT, bool SPLIT>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8AttentionParams p) {
+    typedef typename Element<DT>::type E;
+    constexpr int kRows = SPLIT ? 8 : 16;           // in an instruction's 16 columns
     constexpr int kChunks = D / 64, kDims = D / 16;
-    __shared__ f32x4_t join[kWaves][RT][kDims][4 * kCols];
+    constexpr int kUnits = D / 16;                  // of a key row
+    __shared__ union {
+        u32x4_t codes[kWaves][kTileTokens * kUnits];  // a tile's keys, then its values
+        f32x4_t join[kWaves][kDims][64];              // a wave's results for 16 columns
+    } lds;
+    constexpr int kS = kSets<DT, SPLIT>;
+    __shared__ i32x4_t operands[kS][kChunks][64];
+    __shared__ float factors[kRows];
     __shared__ float join_m[kWaves][kRows], join_l[kWaves][kRows];
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kRows;
-    const int split = blockIdx.x;
+    const int split = blockIdx.x, step = p.splits * kWaves, first = split * kWaves + wave;
+    const int P = p.cache.page_tokens, shift_p = 31 - __builtin_clz(P), row_shift = shift_p - 4;
+    // the pages of a tile's four groups of 16 tokens
+    int page0, page1, page2, page3;
+    const auto find_page = [&](int token) {
+        return __builtin_amdgcn_readfirstlane(p.batch.page(seq, token >> shift_p, p.cache.pages));
+    };
+    const auto find_pages = [&](int n) {
+        page0 = find_page(n * kTileTokens);
+        page1 = find_page(n * kTileTokens + 16);
+        page2 = find_page(n * kTileTokens + 32);
+        page3 = find_page(n * kTileTokens + 48);
+    };
+    find_pages(first);
     const RowTile tile = row_tile(p, seq, row0, kRows);
     if (row0 >= tile.total) return;
     if (split > 0 && split * kWaves >= tile.tiles) return;  // the join does not look at it
 
-    // ---- queries: column r's row, as fp16 halves
+    const size_t page_stride = static_cast<size_t>(p.cache.kv_heads) * P * D;
+    const uint64_t keys = reinterpret_cast<uint64_t>(p.cache.keys) + static_cast<size_t>(kvh) * P * D;
+    const uint64_t values = reinterpret_cast<uint64_t>(p.cache.values) + static_cast<size_t>(kvh) * P * D;
+    const u32x4_t *value_codes = lds.codes[wave];
+    const i32x4_t *key_codes = reinterpret_cast<const i32x4_t *>(value_codes);
+    const uint32_t codes_to = __builtin_amdgcn_readfirstlane(lds_address(value_codes));
+    // a load takes 1024 / D tokens, D / 64 loads a group of 16, in which the lanes' units turn alike
+    uint32_t key_from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        key_from[i] = (lane / kUnits) * D + 16 * ((lane % kUnits) ^ (key_turn<D>(4 * i + (lane / kUnits & 3)) & (kUnits - 1)));
+    // value rows are P / 16 units
+    const int row_units = P / 16;
+    const uint32_t value_from = (lane >> row_shift) * P + 16 * ((lane & (row_units - 1)) ^ ((lane >> 4) & (row_units - 1)));
+    // a quarter of a tile: 16 D bytes of a page, the tokens' keys or the part of the values' page that is as long
+    const auto load_quarter = [&](uint64_t plane, int page, int i, uint32_t from) {
+        const uint64_t base = plane + static_cast<uint64_t>(max(page, 0)) * page_stride + ((16 * i) & (P - 1)) * D;
+        const uint32_t to = codes_to + i * 16 * D;
+        load_to_lds<0>(to, base, from);
+        if constexpr (D >= 128) load_to_lds<1024>(to, base, from);
+        if constexpr (D >= 256) load_to_lds<2048>(to, base, from);
+        if constexpr (D >= 256) load_to_lds<3072>(to, base, from);
+    };
+    const auto load_keys = [&]() {
+        load_quarter(keys, page0, 0, key_from[0]);
+        load_quarter(keys, page1, 1, key_from[1]);
+        load_quarter(keys, page2, 2, key_from[2]);
+        load_quarter(keys, page3, 3, key_from[3]);
+    };
+    const auto load_values = [&]() {
+        load_quarter(values, page0, 0, value_from);
+        load_quarter(values, page1, 1, value_from);
+        load_quarter(values, page2, 2, value_from);
+        load_quarter(values, page3, 3, value_from);
+    };
+    if (first < tile.tiles) load_keys();
+
+    stage_queries<D, DT, SPLIT>(p, tile, row0, kvh, reinterpret_cast<uint32_t *>(operands), factors);
+    lds_barrier();
+
     const int col = SPLIT ? r & 7 : r;
     const bool low = SPLIT && r >= 8;
-    f16x8_t q[RT][kChunks][2];
-    float factor[RT];  // of S: softmax scale, log2 e, the query's power of two, 1 / 127
-    int position[RT];  // the last token that the row sees
+    const float share = low ? 1.0f / kLoScale : 1.0f;
+    // what the digits of the first and the last set weigh
+    const float weight0 = low ? 1.0f / 256.0f : 1.0f, weight = SPLIT ? weight0 / 65536.0f : kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f;
+    const int row = row0 + col;
+    const float factor = factors[col];  // of S: softmax scale, log2 e, the query's power of two, 1 / 127^2
+    const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
+    f32x4_t o[kDims];
+    float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int row = row0 + t * kCols + col;
-        const bool there = row < tile.total;
-        const int token = there ? row / p.group : 0, head = kvh * p.group + (there ? row % p.group : 0);
-        const E *at = static_cast<const E *>(p.q) + static_cast<int64_t>(tile.begin + token) * p.q_row +
-            static_cast<int64_t>(head) * p.q_head + 16 * g;
-        position[t] = there ? tile.length + token : -1;
-        f32x4_t v[kChunks][4];
-        float top = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[c][k] = p.vec ? load4<DT, true>(at + 64 * c + 4 * k) : load4<DT, false>(at + 64 * c + 4 * k);
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(v[c][k][0]), fabsf(v[c][k][1])), fmaxf(fabsf(v[c][k][2]), fabsf(v[c][k][3]))));
-            }
-        top = fmaxf(top, xor_lane<16>(top));
-        top = fmaxf(top, xor_lane<32>(top));
-        const int e = __builtin_amdgcn_frexp_expf(top);
-        factor[t] = __builtin_ldexpf(p.scale_log2, e);
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = __builtin_ldexpf(v[c][k][i], -e);
-                    const _Float16 hi = static_cast<_Float16>(x);
-                    const _Float16 lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLoScale);
-                    q[t][c][k >> 1][(k & 1) * 4 + i] = low ? lo : hi;
-                }
-    }
+    for (int d = 0; d < kDims; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int P = p.cache.page_tokens;
-    const size_t page_stride = static_cast<size_t>(p.cache.kv_heads) * P * D;
-    const int8_t *keys = p.cache.keys + static_cast<size_t>(kvh) * P * D + 16 * g;
-    const int8_t *values = p.cache.values + static_cast<size_t>(kvh) * P * D + static_cast<size_t>(r) * P;
-    const float *key_max = p.cache.key_max + kvh, *value_max = p.cache.value_max + kvh;
-    const float share = SPLIT ? (low ? 1.0f / kLoScale : 1.0f) : 1.0f;
+    // where this lane's operands lie
+    const int key_at = (16 * (r >> 2) + (r & 3)) * kUnits, key_turned = key_turn<D>(r) & (kUnits - 1);
+    const int value_at = ((g >> row_shift) << row_shift) * D + (r << row_shift) +
+        ((g & (row_units - 1)) ^ ((r >> (4 - row_shift)) & (row_units - 1)));
 
-    f32x4_t o[RT][kDims];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) o[t][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    const int step = p.splits * kWaves;
-    const int first = split * kWaves + wave;
-    // pages of this lane's key tokens (16 (r >> 2) ..) and of its value tokens (16 g ..)
-    int key_page = p.batch.page(seq, (first * kTileTokens + 16 * (r >> 2)) / P, p.cache.pages);
-    int value_page = p.batch.page(seq, (first * kTileTokens + 16 * g) / P, p.cache.pages);
-    u32x4_t k[4][kChunks];
-    if (first < tile.tiles) {
-        const int8_t *at = keys + static_cast<size_t>(max(key_page, 0)) * page_stride;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                k[u][c] = *reinterpret_cast<const u32x4_t *>(
-                    at + ((first * kTileTokens + 16 * (r >> 2) + 4 * u + (r & 3)) % P) * D + 64 * c);
-    }
+#pragma unroll 1
     for (int n = first; n < tile.tiles; n += step) {
         const int token = n * kTileTokens + 16 * g;  // the first of this lane's 16
-        const int page = max(value_page, 0);
-        u32x4_t v[kDims];
-        const int8_t *at = values + static_cast<size_t>(page) * page_stride + token % P;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) v[d] = *reinterpret_cast<const u32x4_t *>(at + static_cast<size_t>(16 * d) * P);
-        // a page that holds no token yet may hold anything: its magnitudes are not used, and its codes are
-        // finite whatever they are
-        const bool there = value_page >= 0 && token < tile.seen;
-        float key_top = key_max[static_cast<size_t>(page) * p.cache.kv_heads];
-        float value_top = value_max[static_cast<size_t>(page) * p.cache.kv_heads];
-        key_top = there ? key_top : 0.0f;
-        value_top = there ? value_top : 0.0f;
-        // the next tile's pages
+        // the magnitudes of the four groups' pages, asked for together; a page that holds no token yet may hold
+        // anything: its magnitudes are not used, and its codes are finite whatever they are
+        const auto top_at = [&](const float *tops, int page) {
+            return read_only(tops + static_cast<size_t>(max(page, 0)) * p.cache.kv_heads + kvh);
+        };
+        float key_top0 = top_at(p.cache.key_max, page0), key_top1 = top_at(p.cache.key_max, page1);
+        float key_top2 = top_at(p.cache.key_max, page2), key_top3 = top_at(p.cache.key_max, page3);
+        float value_top0 = top_at(p.cache.value_max, page0), value_top1 = top_at(p.cache.value_max, page1);
+        float value_top2 = top_at(p.cache.value_max, page2), value_top3 = top_at(p.cache.value_max, page3);
         const int next = n + step;
-        key_page = p.batch.page(seq, (next * kTileTokens + 16 * (r >> 2)) / P, p.cache.pages);
-        value_page = p.batch.page(seq, (next * kTileTokens + 16 * g) / P, p.cache.pages);
+        wait_loads<0>();  // the keys have landed
 
-        f32x4_t s[RT][4];
+        i32x4_t s[kS][4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int set = 0; set < kS; ++set)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) s[t][u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < 4; ++u) s[set][u] = i32x4_t{0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const f16x8_t a0 = codes_to_half(k[u][c][0], k[u][c][1]), a1 = codes_to_half(k[u][c][2], k[u][c][3]);
+        for (int c = 0; c < kChunks; ++c) {
+            i32x4_t k[4];
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, q[t][c][0], s[t][u], 0, 0, 0);
-                    s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, q[t][c][1], s[t][u], 0, 0, 0);
-                }
+            for (int u = 0; u < 4; ++u) k[u] = key_codes[key_at + 4 * u * kUnits + ((4 * c + g) ^ key_turned)];
+#pragma unroll
+            for (int set = 0; set < kS; ++set) {
+                const i32x4_t q = operands[set][c][lane];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[set][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u], q, s[set][u], 0, 0, 0);
             }
         }
-        if (next < tile.tiles) {
-            const int8_t *from = keys + static_cast<size_t>(max(key_page, 0)) * page_stride;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    k[u][c] = *reinterpret_cast<const u32x4_t *>(
-                        from + ((next * kTileTokens + 16 * (r >> 2) + 4 * u + (r & 3)) % P) * D + 64 * c);
-        }
-
+        wait_lds();
+        load_values();
+        asm volatile("" : "+s"(key_top0), "+s"(key_top1), "+s"(key_top2), "+s"(key_top3));  // not one by one where they
+        asm volatile("" : "+s"(value_top0), "+s"(value_top1), "+s"(value_top2), "+s"(value_top3));  // are chosen from
+        const auto mine = [&](auto a0, auto a1, auto a2, auto a3) {
+            const auto x = g & 1 ? a1 : a0, y = g & 1 ? a3 : a2;
+            return g & 2 ? y : x;
+        };
+        const bool there = mine(page0, page1, page2, page3) >= 0 && token < tile.seen;
+        const float key_top = there ? mine(key_top0, key_top1, key_top2, key_top3) : 0.0f;
+        const float value_top = there ? mine(value_top0, value_top1, value_top2, value_top3) : 0.0f;
+        find_pages(next);
         const int exponent = value_exponent(value_top);
         const float shift = static_cast<float>(exponent);
         const float inverse = __builtin_ldexpf(1.0f, -exponent), rest = __builtin_ldexpf(value_top, -exponent) * kPScale;
-        f16x8_t b[RT][2];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const float f = factor[t] * key_top;
-            const int seen = there ? position[t] + 1 - token : 0;  // of this lane's 16 tokens
+        f16x8_t b[2];
+        {
+            const float f = factor * key_top;
+            const int seen = there ? position + 1 - token : 0;  // of this lane's 16 tokens
             float x[16];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float y = s[t][u][i];
-                    if constexpr (SPLIT) {
-                        y = y * share;
-                        y = y + xor_lane<8>(y);
-                    }
+                    // sums of up to 256 products of two digits: exact in fp32
+                    float y = static_cast<float>(s[kS - 1][u][i]) * weight;
+                    if constexpr (kS == 3) y = __builtin_fmaf(static_cast<float>(s[1][u][i]), 1.0f / 256.0f, y);
+                    y = SPLIT ? __builtin_fmaf(static_cast<float>(s[0][u][i]), weight0, y) : y + static_cast<float>(s[0][u][i]);
+                    if constexpr (SPLIT) y = y + xor_lane<8>(y);
                     x[4 * u + i] = __builtin_fmaf(y, f, shift);
                 }
             if (__any(seen < 16)) {
@@ -249,10 +393,10 @@ __global__ __launch_bounds__(kWaves * 64, RT == 1 ? 2 : 1) void kv8_attention_ke
             for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
             top = fmaxf(top, xor_lane<16>(top));
             top = fmaxf(top, xor_lane<32>(top));
-            const float now = fmaxf(m[t], top);
+            const float now = fmaxf(m, top);
             const float base = now == -__builtin_inff() ? 0.0f : now;  // nothing seen yet: p = 0, not exp(nan)
-            const float alpha = exp2_fast(m[t] - base);
-            m[t] = now;
+            const float alpha = exp2_fast(m - base);
+            m = now;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -264,109 +408,84 @@ __global__ __launch_bounds__(kWaves * 64, RT == 1 ? 2 : 1) void kv8_attention_ke
                     const _Float16 left = static_cast<_Float16>((y - static_cast<float>(h)) * kLoScale);
                     h = low ? left : h;
                 }
-                b[t][j >> 3][j & 7] = h;
+                b[j >> 3][j & 7] = h;
             }
-            l[t] = l[t] * alpha + sum * inverse;
-            if (__any(alpha != 1.0f)) {
+            l = l * alpha + sum * inverse;
+            if (n != first && __any(alpha != 1.0f)) {
 #pragma unroll
                 for (int d = 0; d < kDims; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[t][d][i] *= alpha;
+                    for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
             }
         }
+        wait_loads<0>();  // the values have landed
+        u32x4_t v[kDims];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) v[d] = value_codes[value_at + ((16 * d) << row_shift)];
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int d = 0; d < kDims; ++d) {
             const f16x8_t a0 = codes_to_half(v[d][0], v[d][1]), a1 = codes_to_half(v[d][2], v[d][3]);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b[t][0], o[t][d], 0, 0, 0);
-                o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b[t][1], o[t][d], 0, 0, 0);
-            }
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b[0], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b[1], o[d], 0, 0, 0);
+        }
+        if (next < tile.tiles) {
+            wait_lds();
+            load_keys();
         }
     }
 
     // ---- join the waves
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        l[t] += xor_lane<16>(l[t]);
-        l[t] += xor_lane<32>(l[t]);
-        if (g == 0 && !low) {
-            join_m[wave][t * kCols + col] = m[t];
-            join_l[wave][t * kCols + col] = l[t];
-        }
+    l += xor_lane<16>(l);
+    l += xor_lane<32>(l);
+    if (g == 0 && !low) {
+        join_m[wave][col] = m;
+        join_l[wave][col] = l;
     }
-    __syncthreads();
-    float total[RT], top[RT];
+    lds_barrier();
+    float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int row = t * kCols + col;
-        top[t] = -__builtin_inff();
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, join_m[w][col]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top[t] = fmaxf(top[t], join_m[w][row]);
-        const float base = top[t] == -__builtin_inff() ? 0.0f : top[t];
-        total[t] = 0.0f;
+    for (int w = 0; w < kWaves; ++w) total += join_l[w][col] * exp2_fast(join_m[w][col] - base);
+    const float scale = exp2_fast(m - base) * share;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) total[t] += join_l[w][row] * exp2_fast(join_m[w][row] - base);
-        const float mine = exp2_fast(m[t] - base) * share;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-            f32x4_t y = o[t][d] * mine;
-            if constexpr (SPLIT) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = y[i] + xor_lane<8>(y[i]);
-            }
-            if (!low) join[wave][t][d][g * kCols + col] = y;
-        }
-    }
-    __syncthreads();
+    for (int d = 0; d < kDims; ++d) lds.join[wave][d][lane] = o[d] * scale;
+    lds_barrier();
+    if (low || row >= tile.total) return;
     const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
+    const int head = kvh * p.group + row % p.group;
+    const int64_t at = tile.begin + row / p.group;
+    const float norm = total > 0.0f || total != total ? 1.0f / (total * (kPScale * 127.0f)) : 0.0f;
+#pragma unroll 1
+    for (int d = wave * kChunks; d < (wave + 1) * kChunks; ++d) {
+        f32x4_t y = lds.join[0][d][lane];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int row = row0 + t * kCols + col;
-        if (low || row >= tile.total) continue;
-        const int head = kvh * p.group + row % p.group;
-        const int64_t at = tile.begin + row / p.group;
+        for (int w = 1; w < kWaves; ++w) y += lds.join[w][d][lane];
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int k0 = 0; k0 < kChunks; ++k0) {
-            const int d = wave * kChunks + k0;
-            f32x4_t y = join[0][t][d][g * kCols + col];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) y += join[w][t][d][g * kCols + col];
-            const int dim = 16 * d + 4 * g;
-            if (p.splits > 1) {
-                *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + t * kCols + col) * D + dim) = y;
-            } else {
-                const float norm = total[t] > 0.0f || total[t] != total[t] ? 1.0f / (total[t] * (kPScale * 127.0f)) : 0.0f;
-                y = y * norm;
-                if (p.gate) {
-                    const E *gate = static_cast<const E *>(p.gate) + at * p.q_row + static_cast<int64_t>(head) * p.q_head + dim;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = norm != 0.0f ? gated<DT>(y[i], gate + i) : 0.0f;
-                }
-                E *to = static_cast<E *>(p.out) + at * p.out_row + static_cast<int64_t>(head) * D + dim;
-                if (p.vec) store4<DT, true>(to, y);
-                else store4<DT, false>(to, y);
-            }
+            for (int w = 0; w < kWaves; ++w) y += lds.join[w][d][lane + 8];
         }
-        if (p.splits > 1 && wave == 0 && g == 0) {
-            float *ml = p.partial_ml + (item * kRows + t * kCols + col) * 2;
-            ml[0] = top[t];
-            ml[1] = total[t];
-        }
+        const int dim = 16 * d + 4 * g;
+        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + col) * D + dim) = y;
+        else finish<DT>(p, y * norm, norm != 0.0f, at, head, head * D + dim, dim);
+    }
+    if (p.splits > 1 && wave == 0 && g == 0) {
+        float *ml = p.partial_ml + (item * kRows + col) * 2;
+        ml[0] = top;
+        ml[1] = total;
     }
 }
 
-// The splits of one row and head: a workgroup of eight waves, each over every
-// eighth split, four dims a lane.
-constexpr int kJoinWaves = 8;
-template <int D, Dtype DT>
-__global__ __launch_bounds__(kJoinWaves * 64) void kv8_attention_join_kernel(Kv8AttentionParams p, int tile_rows) {
-    typedef typename Element<DT>::type E;
-    constexpr int kLanes = D / 4;                    // of one vector
-    constexpr int kGroups = kJoinWaves * 64 / kLanes;  // splits side by side
+// The splits of one row and head, 64 dims a workgroup: four dims a lane, 16 or 32
+// splits side by side, so that up to 128 are on their way at once.
+template <int D, Dtype DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8AttentionParams p, int tile_rows) {
+    constexpr int kLanes = 16, kGroups = THREADS / kLanes;
     __shared__ float weight[kKv8MaxSplits];
     __shared__ f32x4_t sums[kGroups][kLanes];
-    const int seq = blockIdx.z, kvh = blockIdx.y, row = blockIdx.x;
+    const int seq = blockIdx.z, kvh = blockIdx.y / (D / 64), slice = blockIdx.y % (D / 64), row = blockIdx.x;
     const int row0 = row / tile_rows * tile_rows;
     const RowTile tile = row_tile(p, seq, row0, tile_rows);
     if (row >= tile.total) return;
@@ -378,53 +497,59 @@ __global__ __launch_bounds__(kJoinWaves * 64) void kv8_attention_join_kernel(Kv8
     const size_t ml_step = static_cast<size_t>(tile_rows) * 2;
 
     const int lane = threadIdx.x & 63;
+    const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes, dim = 64 * slice + 4 * at;
+    const float *from = p.partial + (item * tile_rows + row % tile_rows) * D + dim;
+    const size_t step = static_cast<size_t>(tile_rows) * D;
+    // the first four splits of a group, before the weights are known
+    f32x4_t early[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        early[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (group + k * kGroups < active) early[k] = *reinterpret_cast<const f32x4_t *>(from + (group + k * kGroups) * step);
+    }
     float top = -__builtin_inff();
+#pragma unroll 1
     for (int i = lane; i < active; i += 64) top = fmaxf(top, ml[i * ml_step]);
     top = wave_max(top);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     float total = 0.0f;
+#pragma unroll 1
     for (int i = lane; i < active; i += 64) {
         const float w = exp2_fast(ml[i * ml_step] - base);
         total += ml[i * ml_step + 1] * w;
         if (threadIdx.x < 64) weight[i] = w;
     }
     total = wave_sum(total);
-    __syncthreads();
-    const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes;
-    const float *from = p.partial + (item * tile_rows + row % tile_rows) * D + 4 * at;
-    const size_t step = static_cast<size_t>(tile_rows) * D;
+    lds_barrier();
     f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = group; i < active; i += kGroups) y += *reinterpret_cast<const f32x4_t *>(from + i * step) * weight[i];
-    sums[group][at] = y;
-    __syncthreads();
-    if (group != 0) return;
 #pragma unroll
-    for (int k = 1; k < kGroups; ++k) y += sums[k][at];
+    for (int k = 0; k < 4; ++k)
+        if (group + k * kGroups < active) y += early[k] * weight[group + k * kGroups];
+#pragma unroll 1
+    for (int i = group + 4 * kGroups; i < active; i += kGroups) y += *reinterpret_cast<const f32x4_t *>(from + i * step) * weight[i];
+    sums[group][at] = y;
+    lds_barrier();
+    if (threadIdx.x >= kLanes) return;
+    const int used = min(active, kGroups);
+#pragma unroll 4
+    for (int k = 1; k < used; ++k) y += sums[k][at];
     const float norm = total > 0.0f || total != total ? 1.0f / (total * (kPScale * 127.0f)) : 0.0f;
     y = y * norm;
     const int head = kvh * p.group + row % p.group;
-    const int64_t index = tile.begin + row / p.group;
-    if (p.gate) {
-        const E *gate = static_cast<const E *>(p.gate) + index * p.q_row + static_cast<int64_t>(head) * p.q_head + 4 * at;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = norm != 0.0f ? gated<DT>(y[i], gate + i) : 0.0f;
-    }
-    E *to = static_cast<E *>(p.out) + index * p.out_row + static_cast<int64_t>(head) * D + 4 * at;
-    if (p.vec) store4<DT, true>(to, y);
-    else store4<DT, false>(to, y);
+    finish<DT>(p, y, norm != 0.0f, tile.begin + row / p.group, head, head * D + dim, dim);
 }
 
-template <int D, Dtype DT, bool SPLIT, int RT>
+template <int D, Dtype DT, bool SPLIT>
 hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t stream) {
     const dim3 grid(plan.splits, plan.row_tiles * p.cache.kv_heads, p.batch.sequences);
     p.splits = plan.splits;
     p.row_tiles = plan.row_tiles;
-    hipLaunchKernelGGL((kv8_attention_kernel<D, DT, SPLIT, RT>), grid, dim3(kWaves * 64), 0, stream, p);
+    hipLaunchKernelGGL((kv8_attention_kernel<D, DT, SPLIT>), grid, dim3(kWaves * 64), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.splits > 1) {
-        const dim3 rows(p.batch.max_rows * p.group, p.cache.kv_heads, p.batch.sequences);
-        hipLaunchKernelGGL((kv8_attention_join_kernel<D, DT>), rows, dim3(kJoinWaves * 64), 0, stream, p, plan.rows);
+        const dim3 rows(p.batch.max_rows * p.group, p.cache.kv_heads * (D / 64), p.batch.sequences);
+        if (plan.splits <= 64) hipLaunchKernelGGL((kv8_attention_join_kernel<D, DT, 256>), rows, dim3(256), 0, stream, p, plan.rows);
+        else hipLaunchKernelGGL((kv8_attention_join_kernel<D, DT, 512>), rows, dim3(512), 0, stream, p, plan.rows);
         e = hipGetLastError();
     }
     return e;
@@ -433,10 +558,9 @@ hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t st
 template <int D, Dtype DT>
 hipError_t launch_typed(const Kv8AttentionParams &p, const Kv8Plan &plan, hipStream_t stream) {
     if constexpr (DT == Dtype::F32) {
-        return plan.rows == 8 ? launch_rows<D, DT, true, 1>(p, plan, stream) : launch_rows<D, DT, true, 2>(p, plan, stream);
+        return launch_rows<D, DT, true>(p, plan, stream);
     } else {
-        if (plan.split_halves) return launch_rows<D, DT, true, 1>(p, plan, stream);
-        return plan.rows == 16 ? launch_rows<D, DT, false, 1>(p, plan, stream) : launch_rows<D, DT, false, 2>(p, plan, stream);
+        return plan.rows == 8 ? launch_rows<D, DT, true>(p, plan, stream) : launch_rows<D, DT, false>(p, plan, stream);
     }
 }
 

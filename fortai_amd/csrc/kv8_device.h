@@ -27,6 +27,16 @@ struct Kv8View {
     int pages = 0, page_tokens = 0, kv_heads = 0, head = 0;
 };
 
+// A word that no kernel writes while this one runs: where its address is the same
+// for a whole wave it comes through the scalar cache.
+FORTAI_HD int32_t read_only(const int32_t *p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return *(const __attribute__((address_space(4))) int32_t *)(p);
+#else
+    return *p;
+#endif
+}
+
 struct Kv8Rows {
     const int32_t *starts = nullptr;   // [sequences + 1]
     const int32_t *lengths = nullptr;  // [sequences]: tokens before the sequence's first row
@@ -35,21 +45,21 @@ struct Kv8Rows {
 
     // the sequence's rows [begin, begin + count) of the batch's arrays
     FORTAI_HD void range(int seq, int *begin, int *count) const {
-        int b = starts[seq], e = starts[seq + 1];
+        int b = read_only(starts + seq), e = read_only(starts + seq + 1);
         b = b < 0 ? 0 : b > rows ? rows : b;
         e = e < b ? b : e > rows ? rows : e;
         *begin = b;
         *count = e - b < max_rows ? e - b : max_rows;
     }
     FORTAI_HD int length(int seq) const {
-        const int n = lengths[seq];
+        const int n = read_only(lengths + seq);
         return n < -kKv8MaxTokens ? -kKv8MaxTokens : n > kKv8MaxTokens ? kKv8MaxTokens : n;
     }
     // the pool's page that holds the sequence's page `index`, or -1
     FORTAI_HD int page(int seq, int index, int pages) const {
-        if (index < 0 || index >= pitch) return -1;
-        const int id = tables[static_cast<int64_t>(seq) * pitch + index];
-        return id >= 0 && id < pages ? id : -1;
+        const int at = index < 0 ? 0 : index >= pitch ? pitch - 1 : index;
+        const int id = read_only(tables + static_cast<int64_t>(seq) * pitch + at);
+        return at == index && id >= 0 && id < pages ? id : -1;
     }
 };
 
@@ -57,21 +67,21 @@ struct Kv8Rows {
 // such tiles, `splits` workgroups over the cached tokens of each.
 struct Kv8Plan {
     int rows = 0, row_tiles = 0, splits = 0;
-    bool split_halves = false;  // queries and weights as two fp16 halves
 };
 
-// fp32 queries are always split into halves (8 rows in an instruction's 16
-// columns), others where 8 columns are enough.  Tokens are split until 512
-// workgroups (two a CU) are there, as far as every one has a tile for each of its
-// four waves and the partial results fit.
-inline Kv8Plan kv8_plan(bool fp32, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
+// fp32 queries always have 8 rows in an instruction's 16 columns (each twice, for the
+// two halves of its numbers), others where 8 are enough.  Tokens are split until there
+// are two workgroups a CU for heads of 256 (more for smaller ones, which take less
+// LDS), as far as every one has a tile for each of its four waves and the partial
+// results fit: one workgroup a CU costs 29.7 us where two cost 25.0 (eight sequences of
+// up to 8190 tokens); one tile a wave costs 13.0 us where three cost 19.4 (600 tokens).
+inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
     Kv8Plan p;
-    p.split_halves = fp32 || rows <= 8;
-    if (p.split_halves) p.rows = rows <= 8 ? 8 : 16;
-    else p.rows = rows <= 16 ? 16 : 32;
+    p.rows = fp32 || rows <= 8 ? 8 : 16;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
     const int64_t base = static_cast<int64_t>(p.row_tiles) * kv_heads * sequences;
-    const int64_t wanted = (512 + base - 1) / base, useful = (max_length + 255) / 256;
+    const int64_t fill = 512 * (256 / head);
+    const int64_t wanted = (fill + base - 1) / base, useful = (max_length + 255) / 256;
     const int64_t room = kKv8PartialRows / (base * p.rows);
     int64_t s = wanted < useful ? wanted : useful;
     s = s < room ? s : room;

@@ -147,7 +147,7 @@ inline const char *check_kv8_attention(const Kv8Shape &s, int layer, int dtype, 
     if (!dtype_ok(dtype)) return "kv8: unknown dtype";
     if (heads < 1 || heads % s.kv_heads || heads > 65535) return "kv8: heads a multiple of the cache's, at most 65535";
     const int64_t group = heads / s.kv_heads;
-    if (group * max_rows > kMaxRows || (group * max_rows + 7) / 8 * s.kv_heads > 65535)
+    if (group * max_rows > kMaxRows || (group * max_rows + 7) / 8 * s.kv_heads > 65535 || 4 * s.kv_heads > 65535)
         return "kv8: more rows in a sequence than a call takes";
     if (!(std::fabs(scale) <= 1e30f)) return "kv8: scale is not a number, or beyond 1e30";
     if (max_length < 0) return "kv8: max_length below 0";

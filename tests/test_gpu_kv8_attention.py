@@ -87,8 +87,10 @@ class Case:
                     row = self.starts[s] + i
                     want[row, h] = p @ v[see]
                     # scores: the queries keep 2^-23 of their row's largest; head fp32 additions; three roundings of the score
+                    # (bf16 with more rows than 8 columns hold: two digits, 2^-16 of a power of two up to twice the largest)
                     size = self.scale * (np.abs(k[see]) @ np.abs(q))
-                    delta = np.max(self.scale * np.abs(q).max() * np.abs(k[see]).sum(1) * 2.0 ** -23 + size * self.head * 2.0 ** -24
+                    kept = 2.0 ** -15 if self.dtype == "bf16" and self.single() else 2.0 ** -23
+                    delta = np.max(self.scale * np.abs(q).max() * np.abs(k[see]).sum(1) * kept + size * self.head * 2.0 ** -24
                                    + (np.abs(x) + 150) * 3 * 2.0 ** -24)
                     # numerator and denominator: exp2 and the product with A, then sums of see terms in 16ths, joined
                     bound[row, h] = (p @ np.abs(v[see])) * (2 * delta + 8 * 2.0 ** -24 + 2 * (see.sum() / 16 + 64) * 2.0 ** -24)
@@ -97,9 +99,13 @@ class Case:
             want, bound = want * sigmoid, (bound + np.abs(want) * 2.0 ** -21) * sigmoid
         return want, bound
 
+    def single(self):
+        """Whether the kernel has weights as one fp16 number."""
+        return self.dtype != "f32" and max(self.counts) * self.heads // self.kv > 8
+
     def check(self, got, layer=0):
         want, bound = self.formula(layer)
-        if self.dtype != "f32" and max(self.counts) * self.heads // self.kv > 8:
+        if self.single():
             # more rows than 8 columns hold: p as one fp16 number, off by 2^-11 of itself, sum p = 1, |v| <= magnitude
             bound = bound + np.max(np.abs(self.value_max[np.isfinite(self.value_max)])) * 2.0 ** -11
         bound = bound + (np.abs(want) + bound) * HALF_STEP[self.dtype] + (2.0 ** -25 if self.dtype == "f16" else 1e-37)
