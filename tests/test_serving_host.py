@@ -245,3 +245,80 @@ extern "C" void look(const int32_t *starts, const int32_t *lengths, const int32_
     assert out[1] == 0  # starts that fall: no rows
     lib.look(ptr(starts), ptr(lengths), ptr(tables), 5, 10, 4, 2, 4, 0, 5, ptr(out))
     assert out[:2].tolist() == [0, 4]  # from below zero: clipped to the batch, then to max_rows
+
+
+def test_attention_checks_and_plan(tmp_path):
+    lib = compiled(tmp_path, '''
+#include "kv8_device.h"
+#include "serving_checks.h"
+using namespace fortai_hip;
+extern "C" {
+const char *check(int kv, int layer, int dtype, int rows, int most, const void *q, int64_t qp, int64_t qh, const void *gate, int heads,
+    float scale, int length, const void *out, int64_t op) {
+    Kv8Shape s; s.layers = 2; s.pages = 8; s.page_tokens = 16; s.kv_heads = kv; s.head = 64;
+    return check_kv8_attention(s, layer, dtype, rows, most, q, qp, qh, gate, heads, scale, length, out, op); }
+void plan(int fp32, int head, int sequences, int kv, int64_t rows, int64_t length, int *out) {
+    const Kv8Plan p = kv8_plan(fp32 != 0, head, sequences, kv, rows, length);
+    out[0] = p.rows; out[1] = p.row_tiles; out[2] = p.splits; out[3] = kKv8PartialRows; out[4] = kKv8MaxSplits; }
+}''')
+    lib.check.restype = C.c_char_p
+    lib.check.argtypes = [C.c_int] * 5 + [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_float, C.c_int, C.c_void_p, C.c_int64]
+    good = dict(kv=2, layer=1, dtype=2, rows=9, most=5, q=16, qp=512, qh=64, gate=None, heads=8, scale=0.125, length=100, out=16, op=512)
+    check = lambda **kw: lib.check(*{**good, **kw}.values())
+    assert check() is None and check(qp=0, qh=0, gate=18, length=0, scale=-1.0) is None and check(rows=1, most=1, op=0) is None
+    assert check(kv=1024, heads=1024, rows=8 * 63, most=8 * 63, op=1 << 16) is None  # 63 tiles of 1024 heads are within the grid
+    nan = float("nan")
+    for bad in (dict(layer=2), dict(layer=-1), dict(dtype=3), dict(heads=9), dict(heads=0), dict(heads=65536), dict(scale=nan),
+                dict(scale=float("inf")), dict(length=-1), dict(q=None), dict(out=None), dict(q=17), dict(gate=17), dict(out=17),
+                dict(qp=-1), dict(qh=1 << 32), dict(op=511), dict(op=1 << 32), dict(kv=1024, heads=1024, rows=8 * 64, most=8 * 64, op=1 << 16),
+                dict(rows=1 << 22, most=1 << 22, heads=64)):
+        assert check(**bad), bad
+    out = (C.c_int * 5)()
+    lib.plan.argtypes = [C.c_int] * 4 + [C.c_int64] * 2 + [C.c_void_p]
+    rng = random.Random(1)
+    for _ in range(3000):
+        fp32, head, kv = rng.randrange(2), rng.choice([64, 128, 256]), rng.choice([1, 2, 3, 8, 64, 1024])
+        sequences, rows, length = rng.choice([1, 2, 37, 16384]), int(2 ** rng.uniform(0, 23)), int(2 ** rng.uniform(0, 31)) - 1
+        lib.plan(fp32, head, sequences, kv, rows, length, out)
+        tile, tiles, splits, room, most = out[:]
+        assert tile in (8, 16) and (tile == 8) == bool(fp32 or rows <= 8) and tiles == -(-rows // tile)
+        assert 1 <= splits <= most and (splits == 1 or splits * tiles * tile * kv * sequences <= room)
+        assert splits <= max(1, -(-length // 256))  # every split has a tile for each of its waves
+
+
+def test_verify_checks(tmp_path):
+    lib = compiled(tmp_path, '''
+#include "serving_checks.h"
+using namespace fortai_hip;
+extern "C" {
+const char *create(int rows, int sequences, int vocab) { return check_verifier(rows, sequences, vocab); }
+int chunk(int rows, int vocab) { return verify_chunk(rows, vocab); }
+const char *check(int dtype, const void *t, int64_t tp, const void *d, int64_t dp, const void *tokens, const void *u, const void *temp,
+    int sequences, const void *starts, int rows, const void *e, const void *a, const void *l) {
+    return check_verify(40, 8, 1000, dtype, t, tp, d, dp, tokens, u, temp, sequences, starts, rows, e, a, l); }
+}''')
+    lib.create.restype = lib.check.restype = C.c_char_p
+    assert lib.create(1, 1, 1) is None and lib.create(65535, 65535, 1 << 28) is None
+    for bad in ((0, 1, 1), (65536, 1, 1), (1, 0, 1), (1, 65536, 1), (1, 1, 0), (1, 1, (1 << 28) + 1)):
+        assert lib.create(*bad), bad
+    assert lib.chunk(1, 1) == 1024 and lib.chunk(40, 248320) == 4096 and lib.chunk(65535, 1 << 28) == 4096
+    lib.check.argtypes = [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                          C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
+    good = dict(dtype=0, target=16, tp=1000, draft=None, dp=0, tokens=16, u=16, temp=None, sequences=8, starts=16, rows=40, e=16, a=16,
+                l=None)
+    check = lambda **kw: lib.check(*{**good, **kw}.values())
+    assert check() is None and check(draft=16, dp=1000, temp=16, l=16) is None and check(rows=0, target=None, tokens=None, u=None, e=None) is None
+    assert check(sequences=0, starts=None) is None and check(dtype=1, target=18) is None
+    for bad in (dict(dtype=3), dict(sequences=9), dict(sequences=-1), dict(rows=41), dict(rows=-1), dict(starts=None), dict(a=None),
+                dict(target=None), dict(tokens=None), dict(u=None), dict(e=None), dict(target=18), dict(draft=17, dp=1000), dict(tokens=20),
+                dict(u=18), dict(temp=18), dict(starts=18), dict(e=20), dict(a=18), dict(l=18), dict(tp=999), dict(tp=1 << 32),
+                dict(draft=16, dp=999), dict(draft=16, dp=1 << 32)):
+        assert check(**bad), bad
+
+
+def test_fortran_pages_and_refusals():
+    """The Fortran module's page bookkeeping and its refusals, through the library as built."""
+    from fortai_amd import build
+    r = subprocess.run([build.SERVING_SMOKE], capture_output=True, text=True, timeout=120)
+    print(r.stdout, r.stderr)
+    assert r.returncode == 0 and "fortran serving smoke ok" in r.stdout
