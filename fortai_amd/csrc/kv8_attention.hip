@@ -27,10 +27,12 @@
 // subnormals), so that pages of very different magnitude lose nothing against each
 // other.  All sums are fp32.
 //
-// Bound by what a wave has to issue for a tile (about 1,000 instructions, a third of
-// them turning value codes into fp16) rather than by the cache's bytes.  The four waves
-// of a workgroup take tiles in turn, two workgroups a CU; `splits` workgroups share a
-// sequence's head, joined by a second launch.
+// Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
+// workgroups a CU; `splits` workgroups share a sequence's head, joined by a second
+// launch.  Bound by what a wave has to issue for a tile (about 1,000 instructions, a
+// third of them turning value codes into fp16) and, where a wave has one tile or two, by
+// the way there and back.  Eight sequences of up to 8190 tokens, 16 heads of 256: 24.9
+// us for 80 MB; five rows over 32,760 tokens 21.2 us for 33.5 MB; 600 tokens 12.4 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"
@@ -42,11 +44,15 @@ namespace {
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kTileTokens = 64;
 constexpr int kWaves = 4;
+constexpr int kWideRows = kKv8WideRows;
+constexpr int kArithmeticMayCross = 6;       // a scheduling barrier for all but vector and scalar arithmetic
 constexpr float kLoScale = 2048.0f;          // 2^11: the left-over halves of a split
 constexpr float kPScale = 16384.0f;          // 2^14
+constexpr float kWideScale = 2048.0f;        // 2^11, where p may reach 2^4
 
 // 8 codes as fp16: with the sign bit turned a code is code + 128, which under the
 // exponent byte 0x64 reads 1024 + code + 128.
@@ -139,21 +145,21 @@ __device__ __forceinline__ float read_only(const float *p) {
 // base 256, the leading one in [-127, 127].  A digit a set in the row's column: two
 // for bf16 (2^-16 of the row's largest, where a value's own last place is 2^-8 of
 // itself), three for fp16; with SPLIT four, two a set in columns r and r + 8.
-// 16 threads a row, 32 where there are no more than 8 rows.
+// 16 threads a row, 32 where there are no more than 8 rows; `thread` of THREADS.
 template <Dtype DT, bool SPLIT>
 constexpr int kSets = !SPLIT && DT == Dtype::F16 ? 3 : 2;
 
-template <int D, Dtype DT, bool SPLIT>
-__device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const RowTile &tile, int row0, int kvh,
+template <int D, Dtype DT, bool SPLIT, int THREADS>
+__device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const RowTile &tile, int row0, int kvh, int thread,
     uint32_t *operands, float *factors) {
     typedef typename Element<DT>::type E;
     constexpr int kRows = SPLIT ? 8 : 16, kS = kSets<DT, SPLIT>, kDigits = SPLIT ? 2 * kS : kS;
     constexpr float kOne = 127.0f * (kDigits == 4 ? 16777216.0f : kDigits == 3 ? 65536.0f : 256.0f);
     constexpr int kThreads = D >= 128 && kRows == 8 ? 32 : 16, kSteps = D / 4 / kThreads;
 #pragma unroll 1
-    for (int base = 0; base < kRows; base += kWaves * 64 / kThreads) {
-        const int local = base + static_cast<int>(threadIdx.x) / kThreads, part = threadIdx.x % kThreads, row = row0 + local;
-        if (local >= kRows) break;  // whole waves
+    for (int base = 0; base < kRows; base += THREADS / kThreads) {
+        const int local = base + thread / kThreads, part = thread % kThreads, row = row0 + local;
+        if (local >= kRows) break;
         const bool there = row < tile.total;
         const int token = there ? row / p.group : 0, head = kvh * p.group + (there ? row % p.group : 0);
         const E *at = static_cast<const E *>(p.q) + static_cast<int64_t>(tile.begin + token) * p.q_row +
@@ -186,7 +192,8 @@ __device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const
         poison += xor_lane<8>(poison);
         if constexpr (kThreads == 32) poison += xor_lane<16>(poison);
         const int e = __builtin_amdgcn_frexp_expf(top);
-        if (part == 0) factors[local] = __builtin_ldexpf(p.scale_log2, e) * (1.0f / 127.0f) + poison;
+        const float one = p.scale_log2 < 0.0f ? -kOne : kOne;  // so that factors are not negative
+        if (part == 0) factors[local] = __builtin_ldexpf(fabsf(p.scale_log2), e) * (1.0f / 127.0f) + poison;
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
             uint32_t digits[kDigits];
@@ -194,7 +201,7 @@ __device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const
             for (int k = 0; k < kDigits; ++k) digits[k] = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                int x = poison == 0.0f ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(v[c][i], -e) * kOne)) : 0;
+                int x = poison == 0.0f ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(v[c][i], -e) * one)) : 0;
 #pragma unroll
                 for (int k = kDigits - 1; k >= 0; --k) {
                     const int digit = k > 0 ? static_cast<int8_t>(x) : x;
@@ -216,15 +223,16 @@ __device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const
 // trace in registers: 1 KiB a load, whole rows, so that lines are read whole (a
 // lane's operands lie in 16 rows: read from memory directly, they took five times as
 // many accesses).  What a lane reads from LDS is 16 bytes of row r; the units of 16
-// bytes are permuted within a row (by the load's source address) so that lanes of
-// neighbouring rows find different banks.
+// bytes are permuted within a row (by the load's source address) so that the lanes
+// that are served together find different banks: 64 banks, 16 lanes at a time, rows
+// 0-3 and 12-15 of one g with rows 4-11 of its neighbour.
 //
 // Keys: token T of the tile in rows of D, unit x at x ^ f(T) with f from T's lane,
 //   r(T) = (T / 16) 4 + T % 4.  Values: pages of P tokens one behind the other, dim d
-//   in rows of P, unit x at x ^ f(d).
+//   in rows of P, unit x at x ^ f(d) (f = 0 for pages of 16 and 32).
 template <int D>
 __device__ __forceinline__ int key_turn(int r) {
-    return D == 256 ? r : D == 128 ? r >> 1 : r >> 2;
+    return D == 256 ? r : D == 128 ? r >> 1 : 3 * (r >> 3);
 }
 
 template <int D, Dtype DT, bool SPLIT>
@@ -276,7 +284,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         key_from[i] = (lane / kUnits) * D + 16 * ((lane % kUnits) ^ (key_turn<D>(4 * i + (lane / kUnits & 3)) & (kUnits - 1)));
     // value rows are P / 16 units
     const int row_units = P / 16;
-    const uint32_t value_from = (lane >> row_shift) * P + 16 * ((lane & (row_units - 1)) ^ ((lane >> 4) & (row_units - 1)));
+    const uint32_t value_from = (lane >> row_shift) * P + 16 * ((lane & (row_units - 1)) ^ (P == 64 ? 3 * (lane >> 5) : 0));
     // a quarter of a tile: 16 D bytes of a page, the tokens' keys or the part of the values' page that is as long
     const auto load_quarter = [&](uint64_t plane, int page, int i, uint32_t from) {
         const uint64_t base = plane + static_cast<uint64_t>(max(page, 0)) * page_stride + ((16 * i) & (P - 1)) * D;
@@ -300,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     };
     if (first < tile.tiles) load_keys();
 
-    stage_queries<D, DT, SPLIT>(p, tile, row0, kvh, reinterpret_cast<uint32_t *>(operands), factors);
+    stage_queries<D, DT, SPLIT, kWaves * 64>(p, tile, row0, kvh, threadIdx.x, reinterpret_cast<uint32_t *>(operands), factors);
     lds_barrier();
 
     const int col = SPLIT ? r & 7 : r;
@@ -319,7 +327,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     // where this lane's operands lie
     const int key_at = (16 * (r >> 2) + (r & 3)) * kUnits, key_turned = key_turn<D>(r) & (kUnits - 1);
     const int value_at = ((g >> row_shift) << row_shift) * D + (r << row_shift) +
-        ((g & (row_units - 1)) ^ ((r >> (4 - row_shift)) & (row_units - 1)));
+        ((g & (row_units - 1)) ^ (P == 64 ? 3 * (r >> 3) : 0));
 
 #pragma unroll 1
     for (int n = first; n < tile.tiles; n += step) {
@@ -478,6 +486,253 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     }
 }
 
+// Many rows (a prompt's chunk): 64 rows a workgroup, which share every tile.  For the
+// scores and their weights a wave has 16 of the rows and the whole tile: its queries
+// stay in registers, the keys come from LDS (double buffered).  The weights go to the
+// other waves through LDS, because for the results a wave has all 64 rows and a
+// quarter of the dims: the values that it needs are its own then, which it loads and
+// turns into fp16 once for 64 rows.
+//
+// Scores: f y + shift with y the digits' sum, f > 0 and shift the same for a lane's 16
+// tokens (one page), so that only y is masked and searched for its largest; A_v's
+// mantissa goes into the exponent too, and its sum is divided by it again.
+//
+// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 255 us, 0.9 PFLOP/s with a
+// product of two digits counted once; the 16-row kernel takes 409, a version in which
+// every wave read the whole tile's values from LDS 265.  Matrix instructions are 45 %
+// of a SIMD's time, the 290 vector instructions of a wave's tile the rest: with two
+// waves a SIMD the two overlap little, more with priority for the products (12 us).
+template <int D, Dtype DT>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
+    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<DT, false>;
+    constexpr int kKeyUnits = kTileTokens * kUnits;
+    constexpr int kMine = D / 64;  // a wave's 16s of dims
+    __shared__ union {
+        struct {
+            u32x4_t keys[2][kKeyUnits];
+            f16x8_t weights[kWaves][2][64];  // of a wave's rows
+            f32x4_t alphas[16];              // of row r of the four waves
+        } tile;
+        struct {
+            u32x4_t first_keys[kKeyUnits];  // loaded meanwhile
+            i32x4_t operands[kWaves][kS][kChunks][64];
+        } start;
+        f32x4_t rows[kWaves][kDims][64];
+    } lds;
+    __shared__ float factors[kWaves][16];
+
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kWideRows;
+    const int split = blockIdx.x, step = p.splits;
+    const int P = p.cache.page_tokens, shift_p = 31 - __builtin_clz(P);
+    const RowTile tile = row_tile(p, seq, row0, kWideRows);
+    if (row0 >= tile.total) return;
+    if (split > 0 && split >= tile.tiles) return;  // the join does not look at it
+
+    const size_t page_stride = static_cast<size_t>(p.cache.kv_heads) * P * D;
+    const uint64_t keys = reinterpret_cast<uint64_t>(p.cache.keys) + static_cast<size_t>(kvh) * P * D;
+    const int8_t *values = p.cache.values + static_cast<size_t>(kvh) * P * D;
+    // the page of tile n's tokens 16 g .. 16 g + 15: its word of the table, looked at once it is there (where the
+    // table ends, tile.seen ends too)
+    const auto page_id = [&](int n) { return p.batch.page_word(seq, (n * kTileTokens + 16 * g) >> shift_p); };
+    const auto checked = [&](int id) { return id >= 0 && id < p.cache.pages ? id : -1; };
+    const uint32_t key_from = (lane / kUnits) * D + 16 * ((lane % kUnits) ^ (key_turn<D>(4 * wave + (lane / kUnits & 3)) & (kUnits - 1)));
+    const uint32_t keys_to = __builtin_amdgcn_readfirstlane(lds_address(lds.tile.keys[0]));
+    // this wave's 16 tokens of a tile
+    const auto load_keys = [&](int page, int buffer) {
+        const int mine = __builtin_amdgcn_readlane(page, 16 * wave);
+        const uint64_t base = keys + static_cast<uint64_t>(max(mine, 0)) * page_stride + ((16 * wave) & (P - 1)) * D;
+        const uint32_t to = keys_to + (buffer * kKeyUnits + wave * 16 * kUnits) * 16;
+        load_to_lds<0>(to, base, key_from);
+        if constexpr (D >= 128) load_to_lds<1024>(to, base, key_from);
+        if constexpr (D >= 256) load_to_lds<2048>(to, base, key_from);
+        if constexpr (D >= 256) load_to_lds<3072>(to, base, key_from);
+    };
+    // this wave's dims of a tile's values as they are operands: the lane's 16 tokens of dim r of each 16
+    u32x4_t codes[kMine];
+    const auto load_values = [&](int page) {
+        const int8_t *from = values + static_cast<size_t>(max(page, 0)) * page_stride +
+            static_cast<size_t>(wave * (D / 4) + r) * P + ((16 * g) & (P - 1));
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) codes[i] = *reinterpret_cast<const u32x4_t *>(from + 16 * i * P);
+    };
+    float key_top, value_top;  // of this lane's page
+    const auto load_tops = [&](int page) {
+        const size_t at = static_cast<size_t>(max(page, 0)) * p.cache.kv_heads + kvh;
+        key_top = p.cache.key_max[at];
+        value_top = p.cache.value_max[at];
+    };
+    int page = checked(page_id(split)), next_id = -1;  // the page of this tile, and the word that says the next one's
+    if (split < tile.tiles) {
+        load_keys(page, 0);
+        load_tops(page);
+        next_id = page_id(split + step);
+        load_values(page);
+    }
+    stage_queries<D, DT, false, 64>(p, tile, row0 + 16 * wave, kvh, lane, reinterpret_cast<uint32_t *>(lds.start.operands[wave]),
+        factors[wave]);
+    wait_lds();  // its own wave's rows only
+    i32x4_t q[kS][kChunks];
+#pragma unroll
+    for (int set = 0; set < kS; ++set)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) q[set][c] = lds.start.operands[wave][set][c][lane];
+    const int row = row0 + 16 * wave + r;
+    const float factor = factors[wave][r] * (kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f);  // per unit of the last digit
+    const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
+    f32x4_t o[kWaves][kMine];  // of row r of every wave's
+    float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kWaves; ++t)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) o[t][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const int key_at = (16 * (r >> 2) + (r & 3)) * kUnits, key_turned = key_turn<D>(r) & (kUnits - 1);
+
+    int buffer = 0;
+#pragma unroll 1
+    for (int n = split; n < tile.tiles; n += step) {
+        const bool more = n + step < tile.tiles;
+        wait_loads<kMine>();  // all but the values, which were asked for last
+        lds_barrier();  // every wave's keys are there, and its products with the tile before done
+        const int token = n * kTileTokens + 16 * g;  // the first of this lane's 16
+        const bool there = page >= 0 && token < tile.seen;
+        const float k_top = there ? key_top : 0.0f, v_top = there ? value_top : 0.0f;
+        page = checked(next_id);
+        if (more) {
+            load_keys(page, buffer ^ 1);
+            load_tops(page);
+            next_id = page_id(n + 2 * step);
+        }
+
+        const i32x4_t *key_codes = reinterpret_cast<const i32x4_t *>(lds.tile.keys[buffer]);
+        i32x4_t s[kS][4], k[2][4];
+        const auto read_keys = [&](int c) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) k[c & 1][u] = key_codes[key_at + 4 * u * kUnits + ((4 * c + g) ^ key_turned)];
+        };
+#pragma unroll
+        for (int set = 0; set < kS; ++set)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[set][u] = i32x4_t{0, 0, 0, 0};
+        read_keys(0);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            if (c + 1 < kChunks) read_keys(c + 1);
+            __builtin_amdgcn_sched_barrier(kArithmeticMayCross);
+#pragma unroll
+            for (int set = 0; set < kS; ++set)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[set][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c & 1][u], q[set][c], s[set][u], 0, 0, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        // digits' sums: up to 256 * 127^2 the leading one's, which leaves room for one more digit in 32 bits
+        float y[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float last = static_cast<float>(s[kS - 2][u][i] * 256 + s[kS - 1][u][i]);
+                y[4 * u + i] = kS == 3 ? __builtin_fmaf(static_cast<float>(s[0][u][i]), 65536.0f, last) : last;
+            }
+        const int seen = there ? position + 1 - token : 0;  // of this lane's 16 tokens
+        if (__any(seen < 16)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] = j < seen ? y[j] : -__builtin_inff();
+        }
+        const float product = factor * k_top, f = product == 0.0f ? 1.2e-38f : product;  // not 0 * infinity where masked
+        const int exponent = value_exponent(v_top);
+        const float shift = static_cast<float>(exponent);
+        float top = y[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, y[j]);
+        top = __builtin_fmaf(top, f, shift);
+        top = fmaxf(top, xor_lane<16>(top));
+        top = fmaxf(top, xor_lane<32>(top));
+        // a new base only where the old one is left behind by more than 2^4
+        const float now = top > m + 4.0f ? top : m;
+        const float base = now == -__builtin_inff() ? 0.0f : now;  // nothing seen yet: p = 0, not exp(nan)
+        const float alpha = exp2_fast(m - base);
+        m = now;
+        // what is left of A_v, scaled; pages of zeros have weights, but no values
+        const float rest = __builtin_ldexpf(v_top, -exponent) * kWideScale;
+        const bool silent = rest == 0.0f;
+        const float c = (shift - base) + (silent ? 0.0f : __builtin_amdgcn_logf(rest));
+        float sum = 0.0f;
+        f16x8_t b[2];
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const f32x2_t e = {exp2_fast(__builtin_fmaf(y[j], f, c)), exp2_fast(__builtin_fmaf(y[j + 1], f, c))};
+            sum += e[0] + e[1];
+            const f16x2_t h = __builtin_convertvector(e, f16x2_t);
+            b[j >> 3][j & 7] = h[0];
+            b[j >> 3][(j & 7) + 1] = h[1];
+        }
+        if (__any(silent)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) b[j >> 3][j & 7] = silent ? static_cast<_Float16>(0.0f) : b[j >> 3][j & 7];
+        }
+        l = l * alpha + sum * __builtin_ldexpf(silent ? 1.0f : __builtin_amdgcn_rcpf(rest), -exponent);
+        lds.tile.weights[wave][0][lane] = b[0];
+        lds.tile.weights[wave][1][lane] = b[1];
+        if (g == 0) reinterpret_cast<float *>(&lds.tile.alphas[r])[wave] = alpha;
+        lds_barrier();  // every wave's weights are there
+        __builtin_amdgcn_s_setprio(1);
+        f16x8_t weights[kWaves][2];
+        const f32x4_t alphas = lds.tile.alphas[r];
+#pragma unroll
+        for (int t = 0; t < kWaves; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) weights[t][half] = lds.tile.weights[t][half][lane];
+        if (__any(alphas[0] != 1.0f || alphas[1] != 1.0f || alphas[2] != 1.0f || alphas[3] != 1.0f)) {
+#pragma unroll
+            for (int t = 0; t < kWaves; ++t)
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) o[t][i] *= alphas[t];
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const f16x8_t a0 = codes_to_half(codes[i][0], codes[i][1]), a1 = codes_to_half(codes[i][2], codes[i][3]);
+#pragma unroll
+            for (int t = 0; t < kWaves; ++t) o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, weights[t][0], o[t][i], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < kWaves; ++t) o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, weights[t][1], o[t][i], 0, 0, 0);
+        }
+        if (more) load_values(page);
+        buffer ^= 1;
+    }
+    __builtin_amdgcn_s_setprio(0);
+
+    l += xor_lane<16>(l);
+    l += xor_lane<32>(l);
+    const float norm = p.splits > 1 ? kPScale / kWideScale : l > 0.0f || l != l ? 1.0f / (l * (kWideScale * 127.0f)) : 0.0f;
+    lds_barrier();  // the last tile's products are done
+#pragma unroll
+    for (int t = 0; t < kWaves; ++t)
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) lds.rows[t][wave * kMine + i][lane] = o[t][i];
+    const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
+    if (p.splits > 1 && g == 0) {
+        float *ml = p.partial_ml + (item * kWideRows + 16 * wave + r) * 2;
+        ml[0] = m;
+        ml[1] = l;
+    }
+    lds_barrier();
+    // the 16 rows that the wave has the sums of: a row's dims, four a lane, in as many rows at a time as a wave holds
+    constexpr int kLanes = D / 4, kTogether = 64 / kLanes;
+    const int four = lane % kLanes, dim = 4 * four;
+#pragma unroll 1
+    for (int k = 0; k < 16; k += kTogether) {
+        const int local = k + lane / kLanes, at = row0 + 16 * wave + local;
+        const float scale = __shfl(norm, local);
+        if (at >= tile.total) break;
+        const f32x4_t y = lds.rows[wave][four >> 2][16 * (four & 3) + local] * scale;
+        const int head = kvh * p.group + at % p.group;
+        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kWideRows + 16 * wave + local) * D + dim) = y;
+        else finish<DT>(p, y, scale != 0.0f, tile.begin + at / p.group, head, head * D + dim, dim);
+    }
+}
+
 // The splits of one row and head, 64 dims a workgroup: four dims a lane, 16 or 32
 // splits side by side, so that up to 128 are on their way at once.
 template <int D, Dtype DT, int THREADS>
@@ -489,7 +744,8 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     const int row0 = row / tile_rows * tile_rows;
     const RowTile tile = row_tile(p, seq, row0, tile_rows);
     if (row >= tile.total) return;
-    const int active = min(p.splits, max((tile.tiles + kWaves - 1) / kWaves, 1));
+    const int together = tile_rows == kWideRows ? 1 : kWaves;  // tiles that a workgroup's waves take at once
+    const int active = min(p.splits, max((tile.tiles + together - 1) / together, 1));
     const size_t y_index = static_cast<size_t>(row / tile_rows) * p.cache.kv_heads + kvh;
     const size_t tiles_y = static_cast<size_t>(p.row_tiles) * p.cache.kv_heads;
     const size_t item = (static_cast<size_t>(seq) * tiles_y + y_index) * p.splits;
@@ -539,12 +795,13 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     finish<DT>(p, y, norm != 0.0f, tile.begin + row / p.group, head, head * D + dim, dim);
 }
 
-template <int D, Dtype DT, bool SPLIT>
+template <int D, Dtype DT, int ROWS>
 hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t stream) {
     const dim3 grid(plan.splits, plan.row_tiles * p.cache.kv_heads, p.batch.sequences);
     p.splits = plan.splits;
     p.row_tiles = plan.row_tiles;
-    hipLaunchKernelGGL((kv8_attention_kernel<D, DT, SPLIT>), grid, dim3(kWaves * 64), 0, stream, p);
+    if constexpr (ROWS == kWideRows) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT>), grid, dim3(kWaves * 64), 0, stream, p);
+    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, ROWS == 8>), grid, dim3(kWaves * 64), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.splits > 1) {
         const dim3 rows(p.batch.max_rows * p.group, p.cache.kv_heads * (D / 64), p.batch.sequences);
@@ -558,9 +815,11 @@ hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t st
 template <int D, Dtype DT>
 hipError_t launch_typed(const Kv8AttentionParams &p, const Kv8Plan &plan, hipStream_t stream) {
     if constexpr (DT == Dtype::F32) {
-        return launch_rows<D, DT, true>(p, plan, stream);
+        return launch_rows<D, DT, 8>(p, plan, stream);
     } else {
-        return plan.rows == 8 ? launch_rows<D, DT, true>(p, plan, stream) : launch_rows<D, DT, false>(p, plan, stream);
+        return plan.rows == 8 ? launch_rows<D, DT, 8>(p, plan, stream)
+            : plan.rows == 16 ? launch_rows<D, DT, 16>(p, plan, stream)
+                              : launch_rows<D, DT, kWideRows>(p, plan, stream);
     }
 }
 

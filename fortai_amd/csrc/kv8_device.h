@@ -21,6 +21,8 @@ constexpr int kKv8PairsPerLaunch = 448;  // page pairs that fit a launch's argum
 constexpr int kKv8MaxSplits = 256;       // workgroups that may share a sequence's head
 constexpr int kKv8PartialRows = 16384;   // rows of partial results that a cache has room for
 
+constexpr int kKv8WideRows = 64;         // rows of a workgroup where there are many
+
 struct Kv8View {
     int8_t *keys = nullptr, *values = nullptr;         // [pages][kv_heads][P][D], [pages][kv_heads][D][P]
     float *key_max = nullptr, *value_max = nullptr;    // [pages][kv_heads]
@@ -55,11 +57,15 @@ struct Kv8Rows {
         const int n = read_only(lengths + seq);
         return n < -kKv8MaxTokens ? -kKv8MaxTokens : n > kKv8MaxTokens ? kKv8MaxTokens : n;
     }
+    // the table's word for the sequence's page `index`, or for the nearest that the table has
+    FORTAI_HD int page_word(int seq, int index) const {
+        const int at = index < 0 ? 0 : index >= pitch ? pitch - 1 : index;
+        return read_only(tables + static_cast<int64_t>(seq) * pitch + at);
+    }
     // the pool's page that holds the sequence's page `index`, or -1
     FORTAI_HD int page(int seq, int index, int pages) const {
-        const int at = index < 0 ? 0 : index >= pitch ? pitch - 1 : index;
-        const int id = read_only(tables + static_cast<int64_t>(seq) * pitch + at);
-        return at == index && id >= 0 && id < pages ? id : -1;
+        const int id = page_word(seq, index);
+        return index >= 0 && index < pitch && id >= 0 && id < pages ? id : -1;
     }
 };
 
@@ -70,18 +76,24 @@ struct Kv8Plan {
 };
 
 // fp32 queries always have 8 rows in an instruction's 16 columns (each twice, for the
-// two halves of its numbers), others where 8 are enough.  Tokens are split until there
-// are two workgroups a CU for heads of 256 (more for smaller ones, which take less
-// LDS), as far as every one has a tile for each of its four waves and the partial
-// results fit: one workgroup a CU costs 29.7 us where two cost 25.0 (eight sequences of
-// up to 8190 tokens); one tile a wave costs 13.0 us where three cost 19.4 (600 tokens).
+// two halves of its numbers), others where 8 are enough.  More than 32 rows take the
+// kernel with 64 rows a workgroup, if the cached tokens are so many that 16-row
+// workgroups would have four tiles of 64 a SIMD (heads of 256: 40 rows over 30,000
+// tokens, 5.5 tiles a SIMD, 29.8 us against 36.7; 256 rows over 1,000 tokens, one tile
+// a SIMD, 21.5 against 19.6).
+// Tokens are split until there are two workgroups a CU for heads of 256 (more for
+// smaller ones, which take less LDS), as far as every one has a tile for each of its
+// four waves (two tiles of 64 rows) and the partial results fit: one workgroup a CU
+// costs 29.7 us where two cost 25.0 (eight sequences of up to 8190 tokens); one tile a
+// wave costs 13.0 us where three cost 19.4 (600 tokens).
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
     Kv8Plan p;
-    p.rows = fp32 || rows <= 8 ? 8 : 16;
+    const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
+    const bool much = rows > 32 && (rows + 15) / 16 * heads >= 4096 / ((max_length + 63) / 64 + 1);
+    p.rows = fp32 || rows <= 8 ? 8 : much ? kKv8WideRows : 16;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-    const int64_t base = static_cast<int64_t>(p.row_tiles) * kv_heads * sequences;
-    const int64_t fill = 512 * (256 / head);
-    const int64_t wanted = (fill + base - 1) / base, useful = (max_length + 255) / 256;
+    const int64_t base = p.row_tiles * heads, fill = 512 * (256 / head), least = p.rows == kKv8WideRows ? 128 : 256;
+    const int64_t wanted = (fill + base - 1) / base, useful = (max_length + least - 1) / least;
     const int64_t room = kKv8PartialRows / (base * p.rows);
     int64_t s = wanted < useful ? wanted : useful;
     s = s < room ? s : room;

@@ -88,9 +88,9 @@ class Case:
                     want[row, h] = p @ v[see]
                     # scores: the queries keep 2^-23 of their row's largest; head fp32 additions; three roundings of the score
                     # (bf16 with more rows than 8 columns hold: two digits, 2^-16 of a power of two up to twice the largest)
-                    size = self.scale * (np.abs(k[see]) @ np.abs(q))
+                    size = abs(self.scale) * (np.abs(k[see]) @ np.abs(q))
                     kept = 2.0 ** -15 if self.dtype == "bf16" and self.single() else 2.0 ** -23
-                    delta = np.max(self.scale * np.abs(q).max() * np.abs(k[see]).sum(1) * kept + size * self.head * 2.0 ** -24
+                    delta = np.max(abs(self.scale) * np.abs(q).max() * np.abs(k[see]).sum(1) * kept + size * self.head * 2.0 ** -24
                                    + (np.abs(x) + 150) * 3 * 2.0 ** -24)
                     # numerator and denominator: exp2 and the product with A, then sums of see terms in 16ths, joined
                     bound[row, h] = (p @ np.abs(v[see])) * (2 * delta + 8 * 2.0 ** -24 + 2 * (see.sum() / 16 + 64) * 2.0 ** -24)
@@ -131,6 +131,42 @@ def test_several_rows(ctx, dtype, heads, kv, head, page, counts, lengths):
     c = Case(ctx, heads, kv, head, page, counts, lengths, dtype, gate=False, seed=len(counts) + head)
     c.upload()
     c.check(c.run())
+    c.cache.free()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,head,page,counts,lengths,gate", [
+    (8, 2, 256, 64, [40, 2, 11], [700, 0, 61], True), (16, 4, 64, 16, [9, 1], [100, 3], False), (4, 2, 128, 32, [17, 40, 1, 6], [0, 333, 5, 64], True),
+    (3, 3, 256, 16, [130], [70], False), (8, 1, 128, 16, [33, 64], [511, 0], True), (6, 2, 256, 32, [45, 0, 22], [-5, 9, 130], True),
+    (32, 32, 64, 64, [70, 40, 66, 1], [0, 64, 30, 200], False), (32, 32, 256, 64, [70, 40, 66, 1], [0, 64, 30, 200], True)])
+def test_many_rows(ctx, dtype, heads, kv, head, page, counts, lengths, gate):
+    """As for long contexts, where 64 rows share a tile: max_length says so.  Split, and (32 heads) not split."""
+    c = Case(ctx, heads, kv, head, page, counts, lengths, dtype, gate=gate, seed=heads + head + page)
+    c.upload()
+    c.check(c.run(max_length=1 << 20))
+    c.cache.free()
+
+
+@pytest.mark.parametrize("head", [64, 128, 256])
+def test_many_rows_where_pages_are_odd(ctx, head):
+    """Pages that are not there or hold zeros, unlike magnitudes, queries that are not finite, a negative scale."""
+    c = Case(ctx, 8, 2, head, 16, [30, 19], [250, 90], "bf16", seed=head)
+    c.tables[0, 2:4] = [-1, c.pages + 5]
+    c.key_max[:, c.tables[0, 5:8]] = 0.0
+    c.value_max[:, c.tables[0, 6:9]] = 0.0
+    c.value_max[:, c.tables[0, 10]] = 1e4
+    c.value_max[:, c.tables[0, 11]] = 1e-30
+    c.key_max[:, c.tables[1, 3]] *= 3.0
+    c.scale = -c.scale
+    c.q[45, 3, 0, 7] = float("inf")
+    c.q[46, 0, 0, 0] = float("nan")
+    c.upload()
+    got = c.run(max_length=1 << 20)
+    assert np.isnan(got[45, 3]).all() and np.isnan(got[46, 0]).all()
+    c.q[45, 3] = c.q[46, 0] = 0.0
+    want, _ = c.formula()
+    got[45, 3], got[46, 0] = want[45, 3], want[46, 0]
+    c.check(got)
     c.cache.free()
 
 
@@ -195,6 +231,20 @@ def test_pages_of_unlike_magnitudes(ctx, dtype, count):
     assert np.all(c.run() == 0.0)
     # one loud page that the scores all but rule out, one quiet one that they choose
     c.value_max[0, :, 0] = 1e-4
+    c.cache.free()
+
+
+@pytest.mark.parametrize("dtype,counts", [("f32", [5, 1]), ("f16", [40, 3]), ("bf16", [1, 2]), ("bf16", [7, 1]), ("bf16", [70, 30])])
+@pytest.mark.parametrize("head", [64, 256])
+def test_pages_of_zeros_and_a_negative_scale(ctx, dtype, counts, head):
+    """Magnitudes of zero: keys that score zero, values that add nothing but count; and the smallest scores win."""
+    c = Case(ctx, 8, 2, head, 16, counts, [250, 90], dtype, seed=21, gate=True)
+    c.scale = -c.scale
+    c.key_max[:, c.tables[0, 1:4]] = 0.0
+    c.value_max[:, c.tables[0, 3:9]] = 0.0
+    c.value_max[:, c.tables[1, :2]] = 0.0
+    c.upload()
+    c.check(c.run())
     c.cache.free()
 
 
