@@ -27,7 +27,6 @@ namespace fortai_hip {
 namespace {
 
 constexpr int kPageThreads = 256;
-constexpr int kPageWaves = kPageThreads / 64;
 constexpr int kAppendWaves = 16;  // 64 tokens x 256 dims, a block of 16 x 64 a wave
 
 // The integer nearest to v n / a, ties to even, of the exact quotient; v >= 0 and
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(kAppendWaves * 64) void kv8_append_kernel(Kv8View c
 // Rows of the cache as values, the transpose of the value codes inside the lane
 // as in the append.
 template <Dtype DT, bool VEC>
-__global__ __launch_bounds__(kPageThreads) void kv8_read_kernel(Kv8View cache, Kv8Rows batch,
+__global__ __launch_bounds__(kAppendWaves * 64) void kv8_read_kernel(Kv8View cache, Kv8Rows batch,
     typename Element<DT>::type *__restrict__ keys, int64_t key_pitch, typename Element<DT>::type *__restrict__ values,
     int64_t value_pitch) {
     const int seq = blockIdx.z >> 1, head = blockIdx.y;
@@ -191,25 +190,22 @@ __global__ __launch_bounds__(kPageThreads) void kv8_read_kernel(Kv8View cache, K
     typename Element<DT>::type *out = (is_value ? values : keys) + static_cast<int64_t>(head) * D;
     const int64_t pitch = is_value ? value_pitch : key_pitch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int dim_blocks = D / 64, blocks = (P / 16) * dim_blocks;
-    for (int block = wave; block < blocks; block += kPageWaves) {
-        const int slot = (block / dim_blocks) * 16 + (lane >> 4) * 4, d = (block % dim_blocks) * 64 + (lane & 15) * 4;
-        if (slot + 3 < slot_from || slot >= slot_until) continue;
-        uint32_t w[4];  // keys: of a token, values: of a dim
+    const int dim_blocks = D / 64, slot = (wave / dim_blocks) * 16 + (lane >> 4) * 4, d = (wave % dim_blocks) * 64 + (lane & 15) * 4;
+    if (slot + 3 < slot_from || slot >= slot_until) return;
+    uint32_t w[4];  // keys: of a token, values: of a dim
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            w[k] = codes[(is_value ? static_cast<size_t>(d + k) * P + slot : static_cast<size_t>(slot + k) * D + d) / 4];
+    for (int k = 0; k < 4; ++k)
+        w[k] = codes[(is_value ? static_cast<size_t>(d + k) * P + slot : static_cast<size_t>(slot + k) * D + d) / 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (slot + i < slot_from || slot + i >= slot_until) continue;
-            f32x4_t y;
+    for (int i = 0; i < 4; ++i) {
+        if (slot + i < slot_from || slot + i >= slot_until) continue;
+        f32x4_t y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t byte = is_value ? w[j] >> (8 * i) : w[i] >> (8 * j);
-                y[j] = id < 0 ? 0.0f : static_cast<float>(static_cast<int8_t>(byte)) * scale;
-            }
-            store4<DT, VEC>(out + static_cast<int64_t>(begin + first + slot + i - length) * pitch + d, y);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t byte = is_value ? w[j] >> (8 * i) : w[i] >> (8 * j);
+            y[j] = id < 0 ? 0.0f : static_cast<float>(static_cast<int8_t>(byte)) * scale;
         }
+        store4<DT, VEC>(out + static_cast<int64_t>(begin + first + slot + i - length) * pitch + d, y);
     }
 }
 
@@ -272,7 +268,7 @@ template <Dtype DT>
 void read_typed(const Kv8View &cache, const Kv8Rows &batch, void *keys, int64_t key_pitch, void *values,
     int64_t value_pitch, bool vec, hipStream_t stream) {
     typedef typename Element<DT>::type E;
-    const dim3 grid = page_grid(cache, batch), block(kPageThreads);
+    const dim3 grid = page_grid(cache, batch), block(cache.page_tokens / 16 * (cache.head / 64) * 64);
     E *k = static_cast<E *>(keys), *v = static_cast<E *>(values);
     if (vec) hipLaunchKernelGGL((kv8_read_kernel<DT, true>), grid, block, 0, stream, cache, batch, k, key_pitch, v, value_pitch);
     else hipLaunchKernelGGL((kv8_read_kernel<DT, false>), grid, block, 0, stream, cache, batch, k, key_pitch, v, value_pitch);
