@@ -101,6 +101,13 @@ const char *check_batch(const fortai_hip_kv8_batch *b) {
         b->device_tables);
 }
 
+// Making a handle is no work of a graph: its copy or clearing would wait for a replay.
+const char *check_no_capture(fortai_hip_q8_context *c) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c->stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone) return nullptr;
+    return "handles are created before a capture begins";
+}
+
 bool empty(const fortai_hip_kv8_batch *b) { return b->sequences == 0 || b->rows == 0 || b->max_rows == 0; }
 
 }  // namespace
@@ -116,6 +123,7 @@ int fortai_hip_rope_create(fortai_hip_q8_context *c, int rope_dimension, int int
     if (const char *wrong = check_rope_create(rope_dimension, base, scaling, factor, original_context, beta_fast,
             beta_slow, attention_factor))
         return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (const char *wrong = check_no_capture(c)) return fail(c, FORTAI_HIP_INVALID, wrong);
     double turns[128];
     rope_turns(rope_dimension, base, scaling, factor, original_context, beta_fast, beta_slow, turns);
     const int pairs = rope_dimension / 2;
@@ -202,6 +210,7 @@ int fortai_hip_kv8_create(fortai_hip_q8_context *c, int layers, int pages, int p
     s.kv_heads = kv_heads;
     s.head = head_size;
     if (const char *wrong = check_kv8_shape(s)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (const char *wrong = check_no_capture(c)) return fail(c, FORTAI_HIP_INVALID, wrong);
     const size_t bytes = kv8_bytes(s);
     if (bytes == 0) return fail(c, FORTAI_HIP_INVALID, "kv8: the cache is larger than any memory");
     if (device_storage && (storage_bytes < bytes || !aligned(device_storage, 16)))
@@ -320,6 +329,7 @@ int fortai_hip_verifier_create(fortai_hip_q8_context *c, int max_rows, int max_s
     if (!c || !verifier) return FORTAI_HIP_INVALID;
     *verifier = nullptr;
     if (const char *wrong = check_verifier(max_rows, max_sequences, vocab)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (const char *wrong = check_no_capture(c)) return fail(c, FORTAI_HIP_INVALID, wrong);
     auto *h = new (std::nothrow) fortai_hip_verifier;
     if (!h) return fail(c, FORTAI_HIP_RUNTIME_ERROR, "verify: out of host memory");
     h->context = c;

@@ -477,8 +477,9 @@ int fortai_hip_qwen35_batch_set_prefill_mode(fortai_hip_qwen35_batch *batch_deco
  * fp32, fp16 or bf16, computed on in fp32 and rounded once, to nearest even.
  * Pitches count elements, at most 2^31; base addresses are aligned to their
  * element.  Row counts go up to 2^23.  Where nothing else is said, what a call
- * writes overlaps nothing that it reads.  Handles are destroyed before their
- * context. */
+ * writes overlaps nothing that it reads.  Handles are created while no capture is
+ * under way, and destroyed before their context; the page bookkeeping is used by
+ * one thread at a time. */
 #define FORTAI_HIP_DTYPE_F32 0
 #define FORTAI_HIP_DTYPE_F16 1
 #define FORTAI_HIP_DTYPE_BF16 2

@@ -4,6 +4,7 @@ rejected tokens and are moved by a compaction.  Every stage is held to its defin
 in 64 bits on the inputs that the stage before it left; the cache byte for byte."""
 
 import subprocess
+import threading
 
 import numpy as np
 import pytest
@@ -238,6 +239,59 @@ def test_a_captured_step_is_replayed():
             assert torch.equal(a, b)
     m.close()
     ctx.close()
+
+
+def test_handles_are_not_made_inside_a_capture():
+    ctx = B.Context(0)
+    rope = B.Rope(ctx, 64)
+    x, positions = torch.ones(4, 64, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    ctx.capture_begin()
+    for make in (lambda: B.Rope(ctx, 64), lambda: B.Kv8Cache(ctx, 1, 2, 16, 1, 64), lambda: B.Verifier(ctx, 4, 1, 100)):
+        with pytest.raises(B.BackendError):
+            make()
+    rope.apply(x.data_ptr(), positions.data_ptr(), 4, 1, 64, out.data_ptr())
+    ctx.capture_end()
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        ctx.graph_launch()
+        ctx.synchronize()
+        assert torch.equal(out[0], x[0]) and bool((out[1:] != x[1:]).any())
+    rope.free()
+    ctx.close()
+
+
+def test_three_caches_and_three_threads(ctx):
+    """Two caches of one context and a third of another one, called from three host threads at once."""
+    other = B.Context(0)
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(4, 8, 64, generator=g).cuda()
+    kv = torch.randn(2, 4, 2, 64, generator=g).cuda()
+    ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3, 4], [0, 0], [[1, 2], [0, 3]])]
+    batch = B.Kv8Batch(2, 4, 3, *(i.data_ptr() for i in ints), 2)
+    torch.cuda.synchronize()
+    made = [(c, B.Kv8Cache(c, 1, 4, 16, 2, 64), torch.zeros(4, 8, 64, device="cuda")) for c in (ctx, ctx, other)]
+    torch.cuda.synchronize()
+
+    def work(c, cache, out):
+        for _ in range(20):
+            cache.append(0, batch, kv[0].data_ptr(), kv[1].data_ptr())
+            cache.attention(0, batch, q.data_ptr(), 8, out.data_ptr(), 0.125, 1 << 16)
+
+    threads = [threading.Thread(target=work, args=m) for m in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for c, _, _ in made:
+        c.synchronize()
+    assert torch.equal(made[0][2], made[1][2]) and torch.equal(made[0][2], made[2][2])
+    assert bool((made[0][2].abs().amax(-1) > 0).all())  # single elements may be codes of zero
+    for _, cache, _ in made:
+        cache.free()
+    other.close()
 
 
 def test_fortran_callers():
