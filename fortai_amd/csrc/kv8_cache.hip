@@ -17,7 +17,11 @@
 // Bound by memory for prompts, by the chain of dependent loads (rows, table, A,
 // values) for single tokens.  A wave takes a block of 16 tokens x 64 dims, a lane
 // 4 x 4 of them: reads of 256 (fp32) or 128 bytes in a row and, for both orders,
-// writes of whole words with the transpose inside the lane.
+// writes of whole words with the transpose inside the lane.  One block a wave, so that
+// a page is in flight at once (four blocks one after the other: the read back of
+// 2,300 prompt tokens 12.4 us instead of 10.8, an append of them 45 us, 27 KB of code,
+// instead of 16).  A token of each of eight sequences: append 6.4 us, read back 5.6.
+// Page copies: 1.06 GB in 174 us, 6.1 TB/s.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"

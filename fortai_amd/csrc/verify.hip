@@ -18,7 +18,9 @@
 // sequence the row that decides, worked out again by every workgroup from the
 // chunks' sums, and the weights of that row summed by chunk; (3) the chunk, the
 // token and the outputs.  Bound by reading the logits once, and about as much by
-// the exponentials in 64 bits.
+// the exponentials in 64 bits: eight sequences of up to five rows of 248,320 tokens
+// with their drafts' logits, 58 MB, take 21 + 10 + 8.5 us under a trace, 37 back to back;
+// five rows of 16,384 tokens 13.2 us.
 #include "fortai_hip_internal.h"
 #include "serving_kernels.h"
 
