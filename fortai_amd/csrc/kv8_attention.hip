@@ -292,8 +292,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         const uint32_t to = codes_to + i * 16 * D;
         load_to_lds<0>(to, base, from);
         if constexpr (D >= 128) load_to_lds<1024>(to, base, from);
-        if constexpr (D >= 256) load_to_lds<2048>(to, base, from);
-        if constexpr (D >= 256) load_to_lds<3072>(to, base, from);
+        if constexpr (D >= 256) load_to_lds<2 * 1024>(to, base, from);
+        if constexpr (D >= 256) load_to_lds<3 * 1024>(to, base, from);
     };
     const auto load_keys = [&]() {
         load_quarter(keys, page0, 0, key_from[0]);
@@ -547,8 +547,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         const uint32_t to = keys_to + (buffer * kKeyUnits + wave * 16 * kUnits) * 16;
         load_to_lds<0>(to, base, key_from);
         if constexpr (D >= 128) load_to_lds<1024>(to, base, key_from);
-        if constexpr (D >= 256) load_to_lds<2048>(to, base, key_from);
-        if constexpr (D >= 256) load_to_lds<3072>(to, base, key_from);
+        if constexpr (D >= 256) load_to_lds<2 * 1024>(to, base, key_from);
+        if constexpr (D >= 256) load_to_lds<3 * 1024>(to, base, key_from);
     };
     // this wave's dims of a tile's values as they are operands: the lane's 16 tokens of dim r of each 16
     u32x4_t codes[kMine];
