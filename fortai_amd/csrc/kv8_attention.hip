@@ -641,7 +641,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 #pragma unroll
             for (int j = 0; j < 16; ++j) y[j] = j < seen ? y[j] : -__builtin_inff();
         }
-        const float product = factor * k_top, f = product == 0.0f ? 1.2e-38f : product;  // not 0 * infinity where masked
+        // not 0 or NaN times infinity where masked
+        const float product = seen > 0 ? factor * k_top : 0.0f, f = product == 0.0f ? 1.2e-38f : product;
         const int exponent = value_exponent(v_top);
         const float shift = static_cast<float>(exponent);
         float top = y[0];

@@ -274,6 +274,54 @@ def test_queries_that_are_not_finite(ctx):
     c.cache.free()
 
 
+@pytest.mark.parametrize("counts,max_length", [([9, 2], 40), ([45, 2], 40), ([45, 2], 1 << 20)])
+def test_rows_without_tokens_are_zeros_whatever_they_ask(ctx, counts, max_length):
+    """A sequence that begins before token 0: its first rows see nothing, NaN and infinities among their queries."""
+    c = Case(ctx, 8, 2, 128, 16, counts, [-6, 20], "bf16", seed=4)
+    c.q[0], c.q[5, :, 0, 3] = float("nan"), float("-inf")
+    c.upload()
+    got = c.run(max_length=max_length)
+    assert not got[:6].any()
+    c.q[:6] = 0.0
+    c.check(got)
+    c.cache.free()
+
+
+def test_pages_beyond_32_bits(ctx):
+    """A pool of 5 GiB a layer: the second layer's last pages against the same tokens in its first ones."""
+    layers, pages, page, kv, head, heads = 2, 40000, 64, 4, 256, 16
+    cache = B.Kv8Cache(ctx, layers, pages, page, kv, head)
+    g = torch.Generator().manual_seed(6)
+    rows = 100
+    k, v, q = (torch.randn(rows, n, head, generator=g).bfloat16().cuda() for n in (kv, kv, heads))
+    ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, rows], [0], [[0, 1]], [[pages - 1, pages - 2]])]
+    results = []
+    for table in ints[2:]:
+        batch = B.Kv8Batch(1, rows, rows, ints[0].data_ptr(), ints[1].data_ptr(), table.data_ptr(), 2)
+        back = torch.zeros(2, rows, kv, head, dtype=torch.bfloat16, device="cuda")
+        outs = torch.zeros(3, rows, heads, head, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        cache.append(1, batch, k.data_ptr(), v.data_ptr(), dtype="bf16")
+        cache.read(1, batch, back[0].data_ptr(), back[1].data_ptr(), dtype="bf16")
+        for out, max_length in zip(outs, (100, 1 << 20)):
+            cache.attention(1, batch, q.data_ptr(), heads, out.data_ptr(), 0.0625, max_length, dtype="bf16")
+        last = B.Kv8Batch(1, rows, 2, ints[0].data_ptr(), ints[1].data_ptr(), table.data_ptr(), 2)
+        cache.attention(1, last, q.data_ptr(), heads, outs[2].data_ptr(), 0.0625, 100, dtype="bf16")
+        ctx.synchronize()
+        results.append((back, outs))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert bool(results[0][1][:2].abs().amax(-1).all()) and bool(results[0][1][2, :2].abs().amax(-1).all())
+    cache.copy_pages([pages - 1], [pages - 3])
+    far = torch.tensor([[pages - 3, pages - 2]], dtype=torch.int32, device="cuda")
+    batch = B.Kv8Batch(1, rows, rows, ints[0].data_ptr(), ints[1].data_ptr(), far.data_ptr(), 2)
+    back = torch.zeros_like(results[0][0])
+    torch.cuda.synchronize()
+    cache.read(1, batch, back[0].data_ptr(), back[1].data_ptr(), dtype="bf16")
+    ctx.synchronize()
+    assert torch.equal(back, results[0][0])
+    cache.free()
+
+
 def test_pitches_and_layers(ctx):
     """Unaligned queries and outputs at pitches of their own; the second layer of two."""
     c = Case(ctx, 4, 2, 64, 16, [3, 2], [40, 100], "bf16", seed=8, layers=2)
