@@ -25,7 +25,8 @@
 // by its exponent: the numerator's terms are p_j A_v / 127, and what is rounded to
 // fp16 is that product over the largest such product (times 2^14, away from fp16's
 // subnormals), so that pages of very different magnitude lose nothing against each
-// other.  All sums are fp32.
+// other.  Products below 2^-49 of the largest (2^-38 as one number) count as zero.
+// All sums are fp32.
 //
 // Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
 // workgroups a CU; `splits` workgroups share a sequence's head, joined by a second
@@ -49,7 +50,6 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kTileTokens = 64;
 constexpr int kWaves = 4;
-constexpr int kWideRows = kKv8WideRows;
 constexpr int kArithmeticMayCross = 6;       // a scheduling barrier for all but vector and scalar arithmetic
 constexpr float kLoScale = 2048.0f;          // 2^11: the left-over halves of a split
 constexpr float kPScale = 16384.0f;          // 2^14
@@ -487,8 +487,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     }
 }
 
-// Many rows (a prompt's chunk): 64 rows a workgroup, which share every tile.  For the
-// scores and their weights a wave has 16 of the rows and the whole tile: its queries
+// Many rows (a prompt's chunk): 64 rows a workgroup (32 with SPLIT), which share every
+// tile.  For the scores and their weights a wave has 16 (8) of the rows and the whole tile: its queries
 // stay in registers, the keys come from LDS (double buffered).  The weights go to the
 // other waves through LDS, because for the results a wave has all 64 rows and a
 // quarter of the dims: the values that it needs are its own then, which it loads and
@@ -503,9 +503,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // every wave read the whole tile's values from LDS 265.  Matrix instructions are 45 %
 // of a SIMD's time, the 290 vector instructions of a wave's tile the rest: with two
 // waves a SIMD the two overlap little, more with priority for the products (12 us).
-template <int D, Dtype DT>
+template <int D, Dtype DT, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
-    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<DT, false>;
+    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<DT, SPLIT>;
+    constexpr int kMyRows = SPLIT ? 8 : 16, kRows = kWaves * kMyRows;
     constexpr int kKeyUnits = kTileTokens * kUnits;
     constexpr int kMine = D / 64;  // a wave's 16s of dims
     __shared__ union {
@@ -524,10 +525,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kWideRows;
+    const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kRows;
     const int split = blockIdx.x, step = p.splits;
     const int P = p.cache.page_tokens, shift_p = 31 - __builtin_clz(P);
-    const RowTile tile = row_tile(p, seq, row0, kWideRows);
+    const RowTile tile = row_tile(p, seq, row0, kRows);
     if (row0 >= tile.total) return;
     if (split > 0 && split >= tile.tiles) return;  // the join does not look at it
 
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         next_id = page_id(split + step);
         load_values(page);
     }
-    stage_queries<D, DT, false, 64>(p, tile, row0 + 16 * wave, kvh, lane, reinterpret_cast<uint32_t *>(lds.start.operands[wave]),
+    stage_queries<D, DT, SPLIT, 64>(p, tile, row0 + kMyRows * wave, kvh, lane, reinterpret_cast<uint32_t *>(lds.start.operands[wave]),
         factors[wave]);
     wait_lds();  // its own wave's rows only
     i32x4_t q[kS][kChunks];
@@ -579,8 +580,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
     for (int set = 0; set < kS; ++set)
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) q[set][c] = lds.start.operands[wave][set][c][lane];
-    const int row = row0 + 16 * wave + r;
-    const float factor = factors[wave][r] * (kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f);  // per unit of the last digit
+    const int col = SPLIT ? r & 7 : r, row = row0 + kMyRows * wave + col;
+    const bool low = SPLIT && r >= 8;
+    const float factor = factors[wave][col] * (SPLIT ? 1.0f : kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f);  // per unit of the last digit
+    const float weight0 = low ? 1.0f / 256.0f : 1.0f;  // of a first digit, where they are four
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kWaves][kMine];  // of row r of every wave's
     float m = -__builtin_inff(), l = 0.0f;
@@ -627,14 +630,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
                 for (int u = 0; u < 4; ++u) s[set][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c & 1][u], q[set][c], s[set][u], 0, 0, 0);
         }
         __builtin_amdgcn_s_setprio(0);
-        // digits' sums: up to 256 * 127^2 the leading one's, which leaves room for one more digit in 32 bits
+        // digits' sums: up to 256 * 127^2 the leading one's, which leaves room for one more digit in 32 bits; four digits
+        // are two of the row's column and two of the one 8 further on
         float y[16];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float last = static_cast<float>(s[kS - 2][u][i] * 256 + s[kS - 1][u][i]);
-                y[4 * u + i] = kS == 3 ? __builtin_fmaf(static_cast<float>(s[0][u][i]), 65536.0f, last) : last;
+                if constexpr (SPLIT) {
+                    const float half = __builtin_fmaf(static_cast<float>(s[0][u][i]), weight0,
+                        static_cast<float>(s[1][u][i]) * (weight0 / 65536.0f));
+                    y[4 * u + i] = half + xor_lane<8>(half);
+                } else {
+                    const float last = static_cast<float>(s[kS - 2][u][i] * 256 + s[kS - 1][u][i]);
+                    y[4 * u + i] = kS == 3 ? __builtin_fmaf(static_cast<float>(s[0][u][i]), 65536.0f, last) : last;
+                }
             }
         const int seen = there ? position + 1 - token : 0;  // of this lane's 16 tokens
         if (__any(seen < 16)) {
@@ -666,7 +676,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         for (int j = 0; j < 16; j += 2) {
             const f32x2_t e = {exp2_fast(__builtin_fmaf(y[j], f, c)), exp2_fast(__builtin_fmaf(y[j + 1], f, c))};
             sum += e[0] + e[1];
-            const f16x2_t h = __builtin_convertvector(e, f16x2_t);
+            f16x2_t h = __builtin_convertvector(e, f16x2_t);
+            if constexpr (SPLIT) {
+                const f32x2_t left = (e - __builtin_convertvector(h, f32x2_t)) * kLoScale;
+                h = low ? __builtin_convertvector(left, f16x2_t) : h;
+            }
             b[j >> 3][j & 7] = h[0];
             b[j >> 3][(j & 7) + 1] = h[1];
         }
@@ -714,23 +728,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 #pragma unroll
         for (int i = 0; i < kMine; ++i) lds.rows[t][wave * kMine + i][lane] = o[t][i];
     const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
-    if (p.splits > 1 && g == 0) {
-        float *ml = p.partial_ml + (item * kWideRows + 16 * wave + r) * 2;
+    if (p.splits > 1 && g == 0 && !low) {
+        float *ml = p.partial_ml + (item * kRows + kMyRows * wave + col) * 2;
         ml[0] = m;
         ml[1] = l;
     }
     lds_barrier();
-    // the 16 rows that the wave has the sums of: a row's dims, four a lane, in as many rows at a time as a wave holds
+    // the rows that the wave has the sums of: a row's dims, four a lane, in as many rows at a time as a wave holds
     constexpr int kLanes = D / 4, kTogether = 64 / kLanes;
     const int four = lane % kLanes, dim = 4 * four;
 #pragma unroll 1
-    for (int k = 0; k < 16; k += kTogether) {
-        const int local = k + lane / kLanes, at = row0 + 16 * wave + local;
+    for (int k = 0; k < kMyRows; k += kTogether) {
+        const int local = k + lane / kLanes, at = row0 + kMyRows * wave + local;
         const float scale = __shfl(norm, local);
         if (at >= tile.total) break;
-        const f32x4_t y = lds.rows[wave][four >> 2][16 * (four & 3) + local] * scale;
+        f32x4_t y = lds.rows[wave][four >> 2][16 * (four & 3) + local];
+        if constexpr (SPLIT) y += lds.rows[wave][four >> 2][16 * (four & 3) + local + 8] * (1.0f / kLoScale);
+        y *= scale;
         const int head = kvh * p.group + at % p.group;
-        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kWideRows + 16 * wave + local) * D + dim) = y;
+        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + kMyRows * wave + local) * D + dim) = y;
         else finish<DT>(p, y, scale != 0.0f, tile.begin + at / p.group, head, head * D + dim, dim);
     }
 }
@@ -746,7 +762,7 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     const int row0 = row / tile_rows * tile_rows;
     const RowTile tile = row_tile(p, seq, row0, tile_rows);
     if (row >= tile.total) return;
-    const int together = tile_rows == kWideRows ? 1 : kWaves;  // tiles that a workgroup's waves take at once
+    const int together = tile_rows > 16 ? 1 : kWaves;  // tiles that a workgroup's waves take at once
     const int active = min(p.splits, max((tile.tiles + together - 1) / together, 1));
     const size_t y_index = static_cast<size_t>(row / tile_rows) * p.cache.kv_heads + kvh;
     const size_t tiles_y = static_cast<size_t>(p.row_tiles) * p.cache.kv_heads;
@@ -802,8 +818,9 @@ hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t st
     const dim3 grid(plan.splits, plan.row_tiles * p.cache.kv_heads, p.batch.sequences);
     p.splits = plan.splits;
     p.row_tiles = plan.row_tiles;
-    if constexpr (ROWS == kWideRows) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT>), grid, dim3(kWaves * 64), 0, stream, p);
-    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, ROWS == 8>), grid, dim3(kWaves * 64), 0, stream, p);
+    constexpr bool kSplit = ROWS == 8 || ROWS == 32;
+    if constexpr (ROWS > 16) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT, kSplit>), grid, dim3(kWaves * 64), 0, stream, p);
+    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, kSplit>), grid, dim3(kWaves * 64), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.splits > 1) {
         const dim3 rows(p.batch.max_rows * p.group, p.cache.kv_heads * (D / 64), p.batch.sequences);
@@ -817,11 +834,11 @@ hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t st
 template <int D, Dtype DT>
 hipError_t launch_typed(const Kv8AttentionParams &p, const Kv8Plan &plan, hipStream_t stream) {
     if constexpr (DT == Dtype::F32) {
-        return launch_rows<D, DT, 8>(p, plan, stream);
+        return plan.rows == 8 ? launch_rows<D, DT, 8>(p, plan, stream) : launch_rows<D, DT, 32>(p, plan, stream);
     } else {
         return plan.rows == 8 ? launch_rows<D, DT, 8>(p, plan, stream)
             : plan.rows == 16 ? launch_rows<D, DT, 16>(p, plan, stream)
-                              : launch_rows<D, DT, kWideRows>(p, plan, stream);
+                              : launch_rows<D, DT, 64>(p, plan, stream);
     }
 }
 

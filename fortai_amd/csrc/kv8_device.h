@@ -21,7 +21,6 @@ constexpr int kKv8PairsPerLaunch = 448;  // page pairs that fit a launch's argum
 constexpr int kKv8MaxSplits = 256;       // workgroups that may share a sequence's head
 constexpr int kKv8PartialRows = 16384;   // rows of partial results that a cache has room for
 
-constexpr int kKv8WideRows = 64;         // rows of a workgroup where there are many
 
 struct Kv8View {
     int8_t *keys = nullptr, *values = nullptr;         // [pages][kv_heads][P][D], [pages][kv_heads][D][P]
@@ -76,11 +75,12 @@ struct Kv8Plan {
 };
 
 // fp32 queries always have 8 rows in an instruction's 16 columns (each twice, for the
-// two halves of its numbers), others where 8 are enough.  More than 32 rows take the
-// kernel with 64 rows a workgroup, if the cached tokens are so many that 16-row
-// workgroups would have four tiles of 64 a SIMD (heads of 256: 40 rows over 30,000
-// tokens, 5.5 tiles a SIMD, 29.8 us against 36.7; 256 rows over 1,000 tokens, one tile
-// a SIMD, 21.5 against 19.6).
+// two halves of its numbers), others where 8 are enough.  More than twice as many rows
+// take the kernel with four times as many a workgroup, if the cached tokens are so many
+// that the smaller workgroups would have four tiles of 64 a SIMD (heads of 256: 40 rows
+// of 16 bits over 30,000 tokens, 5.5 tiles a SIMD, 29.8 us against 36.7; 256 rows over
+// 1,000 tokens, one tile a SIMD, 21.5 against 19.6; fp32, 64 rows over 30,000 tokens,
+// 41.3 against 44.4, 8,000 over 7,000 561 against 853).
 // Tokens are split until there are two workgroups a CU for heads of 256 (more for
 // smaller ones, which take less LDS), as far as every one has a tile for each of its
 // four waves (two tiles of 64 rows) and the partial results fit: one workgroup a CU
@@ -89,10 +89,11 @@ struct Kv8Plan {
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
     Kv8Plan p;
     const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
-    const bool much = rows > 32 && (rows + 15) / 16 * heads >= 4096 / ((max_length + 63) / 64 + 1);
-    p.rows = fp32 || rows <= 8 ? 8 : much ? kKv8WideRows : 16;
+    const int few = fp32 || rows <= 8 ? 8 : 16;
+    const bool much = rows > 2 * few && (rows + few - 1) / few * heads >= 4096 / ((max_length + 63) / 64 + 1);
+    p.rows = much ? 4 * few : few;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-    const int64_t base = p.row_tiles * heads, fill = 512 * (256 / head), least = p.rows == kKv8WideRows ? 128 : 256;
+    const int64_t base = p.row_tiles * heads, fill = 512 * (256 / head), least = much ? 128 : 256;
     const int64_t wanted = (fill + base - 1) / base, useful = (max_length + least - 1) / least;
     const int64_t room = kKv8PartialRows / (base * p.rows);
     int64_t s = wanted < useful ? wanted : useful;

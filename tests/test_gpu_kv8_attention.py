@@ -94,6 +94,9 @@ class Case:
                                    + (np.abs(x) + 150) * 3 * 2.0 ** -24)
                     # numerator and denominator: exp2 and the product with A, then sums of see terms in 16ths, joined
                     bound[row, h] = (p @ np.abs(v[see])) * (2 * delta + 8 * 2.0 ** -24 + 2 * (see.sum() / 16 + 64) * 2.0 ** -24)
+                    # weights are pairs of fp16: the lower half's smallest step is 2^-24 of 2^-11, and the largest weight times
+                    # magnitude stands at 2^11 at least (2^14 with few rows), so each is off by half of 2^-46 of that
+                    bound[row, h] += see.sum() * 2.0 ** -47 * np.max(self.value_max[layer, pick, h // group])
         if self.gate:
             sigmoid = 1 / (1 + np.exp(-q64[:, :, 1]))
             want, bound = want * sigmoid, (bound + np.abs(want) * 2.0 ** -21) * sigmoid
@@ -134,7 +137,7 @@ def test_several_rows(ctx, dtype, heads, kv, head, page, counts, lengths):
     c.cache.free()
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("heads,kv,head,page,counts,lengths,gate", [
     (8, 2, 256, 64, [40, 2, 11], [700, 0, 61], True), (16, 4, 64, 16, [9, 1], [100, 3], False), (4, 2, 128, 32, [17, 40, 1, 6], [0, 333, 5, 64], True),
     (3, 3, 256, 16, [130], [70], False), (8, 1, 128, 16, [33, 64], [511, 0], True), (6, 2, 256, 32, [45, 0, 22], [-5, 9, 130], True),
@@ -147,10 +150,11 @@ def test_many_rows(ctx, dtype, heads, kv, head, page, counts, lengths, gate):
     c.cache.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("head", [64, 128, 256])
-def test_many_rows_where_pages_are_odd(ctx, head):
+def test_many_rows_where_pages_are_odd(ctx, head, dtype):
     """Pages that are not there or hold zeros, unlike magnitudes, queries that are not finite, a negative scale."""
-    c = Case(ctx, 8, 2, head, 16, [30, 19], [250, 90], "bf16", seed=head)
+    c = Case(ctx, 8, 2, head, 16, [30, 19], [250, 90], dtype, seed=head)
     c.tables[0, 2:4] = [-1, c.pages + 5]
     c.key_max[:, c.tables[0, 5:8]] = 0.0
     c.value_max[:, c.tables[0, 6:9]] = 0.0
@@ -274,10 +278,11 @@ def test_queries_that_are_not_finite(ctx):
     c.cache.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("counts,max_length", [([9, 2], 40), ([45, 2], 40), ([45, 2], 1 << 20)])
-def test_rows_without_tokens_are_zeros_whatever_they_ask(ctx, counts, max_length):
+def test_rows_without_tokens_are_zeros_whatever_they_ask(ctx, counts, max_length, dtype):
     """A sequence that begins before token 0: its first rows see nothing, NaN and infinities among their queries."""
-    c = Case(ctx, 8, 2, 128, 16, counts, [-6, 20], "bf16", seed=4)
+    c = Case(ctx, 8, 2, 128, 16, counts, [-6, 20], dtype, seed=4)
     c.q[0], c.q[5, :, 0, 3] = float("nan"), float("-inf")
     c.upload()
     got = c.run(max_length=max_length)

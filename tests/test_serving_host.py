@@ -281,9 +281,10 @@ void plan(int fp32, int head, int sequences, int kv, int64_t rows, int64_t lengt
         sequences, rows, length = rng.choice([1, 2, 37, 16384]), int(2 ** rng.uniform(0, 23)), int(2 ** rng.uniform(0, 31)) - 1
         lib.plan(fp32, head, sequences, kv, rows, length, out)
         tile, tiles, splits, room, most = out[:]
-        assert tile in ((8,) if fp32 or rows <= 8 else (16,) if rows <= 32 else (16, 64)) and tiles == -(-rows // tile)
+        few = 8 if fp32 or rows <= 8 else 16
+        assert tile in ((few,) if rows <= 2 * few else (few, 4 * few)) and tiles == -(-rows // tile)
         assert 1 <= splits <= most and (splits == 1 or splits * tiles * tile * kv * sequences <= room)
-        assert splits <= max(1, -(-length // (128 if tile == 64 else 256)))  # every split has work for its waves
+        assert splits <= max(1, -(-length // (128 if tile > 16 else 256)))  # every split has work for its waves
 
 
 def test_verify_checks(tmp_path):
