@@ -33,7 +33,8 @@
 // launch (the last workgroup joining instead: every workgroup writes its L2 back for
 // that, 88 us where two launches take 25).  Bound by what a wave has to issue for a tile (about 1,000 instructions, a
 // third of them turning value codes into fp16) and, where a wave has one tile or two, by
-// the way there and back.  Eight sequences of up to 8190 tokens, 16 heads of 256: 24.9
+// the way there and back.  (Values read into registers as they are operands, in pieces of
+// 16 bytes out of rows of 64: 27.9 us where it is 24.9 now.)  Eight sequences of up to 8190 tokens, 16 heads of 256: 24.9
 // us for 80 MB; five rows over 32,760 tokens 21.2 us for 33.5 MB; 600 tokens 12.4 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
@@ -503,6 +504,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // every wave read the whole tile's values from LDS 265.  Matrix instructions are 45 %
 // of a SIMD's time, the 290 vector instructions of a wave's tile the rest: with two
 // waves a SIMD the two overlap little, more with priority for the products (12 us).
+// Values by loads to LDS, as the keys, took 273 us.
 template <int D, Dtype DT, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
     constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<DT, SPLIT>;

@@ -83,7 +83,7 @@ struct Kv8Plan {
 // 41.3 against 44.4, 8,000 over 7,000 561 against 853).
 // Tokens are split until there are two workgroups a CU for heads of 256 (more for
 // smaller ones, which take less LDS), as far as every one has a tile for each of its
-// four waves (two tiles of 64 rows) and the partial results fit: one workgroup a CU
+// four waves (two tiles where the waves share them) and the partial results fit: one workgroup a CU
 // costs 29.7 us where two cost 25.0 (eight sequences of up to 8190 tokens); one tile a
 // wave costs 13.0 us where three cost 19.4 (600 tokens).
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
