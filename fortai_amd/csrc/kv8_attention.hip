@@ -31,11 +31,12 @@
 // Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
 // workgroups a CU; `splits` workgroups share a sequence's head, joined by a second
 // launch (the last workgroup joining instead: every workgroup writes its L2 back for
-// that, 88 us where two launches take 25).  Bound by what a wave has to issue for a tile (about 1,000 instructions, a
-// third of them turning value codes into fp16) and, where a wave has one tile or two, by
-// the way there and back.  (Values read into registers as they are operands, in pieces of
-// 16 bytes out of rows of 64: 27.9 us where it is 24.9 now.)  Eight sequences of up to 8190 tokens, 16 heads of 256: 24.9
-// us for 80 MB; five rows over 32,760 tokens 21.2 us for 33.5 MB; 600 tokens 12.4 us.
+// that, 88 us where two launches take 25).  Bound by what a wave has to issue for a
+// tile (about 1,000 instructions, a third of them turning value codes into fp16) and,
+// where a wave has one tile or two, by the way there and back.  Eight sequences of up
+// to 8190 tokens, 16 heads of 256: 24.8 us for 80 MB (27.9 with values read into
+// registers as they are operands, in pieces of 16 bytes out of rows of 64); five rows
+// over 32,760 tokens 21.2 us for 33.5 MB; 600 tokens 12.5 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"
