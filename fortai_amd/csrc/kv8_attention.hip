@@ -20,12 +20,15 @@
 //
 // Numerics.  SPLIT: the 16 columns are 8 rows twice, for four digits of q (31 bits)
 // and for p in two fp16 halves (22 bits): used for fp32 queries, and where no more
-// than 8 rows are there to fill the columns.  Without it two digits (bf16) or three
-// (fp16), and p is one fp16 number (2^-11 of itself).  A_v enters the running maximum
+// than 8 rows are there to fill the columns.  Without it three digits (23 bits), and
+// p's halves are operands one after the other: with two digits and the upper half alone
+// five rows over 32,760 tokens take 21.1 us instead of 22.0 and 2000 behind 6000 250
+// instead of 359, but the results are off by 2^-12 of themselves and not the same as the
+// same row's in a call of fewer.  A_v enters the running maximum
 // by its exponent: the numerator's terms are p_j A_v / 127, and what is rounded to
 // fp16 is that product over the largest such product (times 2^14, away from fp16's
 // subnormals), so that pages of very different magnitude lose nothing against each
-// other.  Products below 2^-49 of the largest (2^-38 as one number) count as zero.
+// other.  Products below 2^-49 of the largest (2^-38 without SPLIT) count as zero.
 // All sums are fp32.
 //
 // Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
@@ -36,7 +39,7 @@
 // where a wave has one tile or two, by the way there and back.  Eight sequences of up
 // to 8190 tokens, 16 heads of 256: 24.8 us for 80 MB (27.9 with values read into
 // registers as they are operands, in pieces of 16 bytes out of rows of 64); five rows
-// over 32,760 tokens 21.2 us for 33.5 MB; 600 tokens 12.5 us.
+// over 32,760 tokens 22.0 us for 33.5 MB; 600 tokens 12.5 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"
@@ -68,6 +71,14 @@ __device__ __forceinline__ f16x8_t codes_to_half(uint32_t a, uint32_t b) {
     const f16x2_t p2 = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + bias;
     const f16x2_t p3 = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + bias;
     return f16x8_t{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+
+// A product that is rounded to fp32 before anything is done with it: the compiler folds
+// a multiplication into a conversion to fp16 (one rounding), but not into every use of it,
+// and a lower half that is left over from another upper half is off by a whole step.
+__device__ __forceinline__ float rounded(float product) {
+    asm("" : "+v"(product));
+    return product;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -145,19 +156,19 @@ __device__ __forceinline__ float read_only(const float *p) {
 
 // Queries of a workgroup's rows into LDS as int8 operands, [set][chunk][lane][16]:
 // a row scaled by a power of two to magnitudes below 1, times 127, as digits to the
-// base 256, the leading one in [-127, 127].  A digit a set in the row's column: two
-// for bf16 (2^-16 of the row's largest, where a value's own last place is 2^-8 of
-// itself), three for fp16; with SPLIT four, two a set in columns r and r + 8.
+// base 256, the leading one in [-127, 127].  A digit a set in the row's column: three
+// (2^-24 of that power of two: bf16 elements down to 2^-9 of the row's largest are
+// exact, fp16 ones to 2^-6); with SPLIT four, two a set in columns r and r + 8.
 // 16 threads a row, 32 where there are no more than 8 rows; `thread` of THREADS.
-template <Dtype DT, bool SPLIT>
-constexpr int kSets = !SPLIT && DT == Dtype::F16 ? 3 : 2;
+template <bool SPLIT>
+constexpr int kSets = SPLIT ? 2 : 3;
 
 template <int D, Dtype DT, bool SPLIT, int THREADS>
 __device__ __forceinline__ void stage_queries(const Kv8AttentionParams &p, const RowTile &tile, int row0, int kvh, int thread,
     uint32_t *operands, float *factors) {
     typedef typename Element<DT>::type E;
-    constexpr int kRows = SPLIT ? 8 : 16, kS = kSets<DT, SPLIT>, kDigits = SPLIT ? 2 * kS : kS;
-    constexpr float kOne = 127.0f * (kDigits == 4 ? 16777216.0f : kDigits == 3 ? 65536.0f : 256.0f);
+    constexpr int kRows = SPLIT ? 8 : 16, kS = kSets<SPLIT>, kDigits = SPLIT ? 2 * kS : kS;
+    constexpr float kOne = 127.0f * (kDigits == 4 ? 16777216.0f : 65536.0f);
     constexpr int kThreads = D >= 128 && kRows == 8 ? 32 : 16, kSteps = D / 4 / kThreads;
 #pragma unroll 1
     for (int base = 0; base < kRows; base += THREADS / kThreads) {
@@ -248,7 +259,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         u32x4_t codes[kWaves][kTileTokens * kUnits];  // a tile's keys, then its values
         f32x4_t join[kWaves][kDims][64];              // a wave's results for 16 columns
     } lds;
-    constexpr int kS = kSets<DT, SPLIT>;
+    constexpr int kS = kSets<SPLIT>;
     __shared__ i32x4_t operands[kS][kChunks][64];
     __shared__ float factors[kRows];
     __shared__ float join_m[kWaves][kRows], join_l[kWaves][kRows];
@@ -318,7 +329,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     const bool low = SPLIT && r >= 8;
     const float share = low ? 1.0f / kLoScale : 1.0f;
     // what the digits of the first and the last set weigh
-    const float weight0 = low ? 1.0f / 256.0f : 1.0f, weight = SPLIT ? weight0 / 65536.0f : kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f;
+    const float weight0 = low ? 1.0f / 256.0f : 1.0f, weight = (SPLIT ? weight0 : 1.0f) / 65536.0f;
     const int row = row0 + col;
     const float factor = factors[col];  // of S: softmax scale, log2 e, the query's power of two, 1 / 127^2
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
@@ -379,7 +390,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         const int exponent = value_exponent(value_top);
         const float shift = static_cast<float>(exponent);
         const float inverse = __builtin_ldexpf(1.0f, -exponent), rest = __builtin_ldexpf(value_top, -exponent) * kPScale;
-        f16x8_t b[2];
+        f16x8_t b[SPLIT ? 2 : 4];  // the weights of tokens 0..7 and 8..15, then their lower halves
         {
             const float f = factor * key_top;
             const int seen = there ? position + 1 - token : 0;  // of this lane's 16 tokens
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
                 for (int i = 0; i < 4; ++i) {
                     // sums of up to 256 products of two digits: exact in fp32
                     float y = static_cast<float>(s[kS - 1][u][i]) * weight;
-                    if constexpr (kS == 3) y = __builtin_fmaf(static_cast<float>(s[1][u][i]), 1.0f / 256.0f, y);
+                    if constexpr (!SPLIT) y = __builtin_fmaf(static_cast<float>(s[1][u][i]), 1.0f / 256.0f, y);
                     y = SPLIT ? __builtin_fmaf(static_cast<float>(s[0][u][i]), weight0, y) : y + static_cast<float>(s[0][u][i]);
                     if constexpr (SPLIT) y = y + xor_lane<8>(y);
                     x[4 * u + i] = __builtin_fmaf(y, f, shift);
@@ -413,12 +424,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
             for (int j = 0; j < 16; ++j) {
                 const float e = exp2_fast(x[j] - base);
                 sum += e;
-                const float y = e * rest;
+                const float y = rounded(e * rest);
                 _Float16 h = static_cast<_Float16>(y);
-                if constexpr (SPLIT) {
-                    const _Float16 left = static_cast<_Float16>((y - static_cast<float>(h)) * kLoScale);
-                    h = low ? left : h;
-                }
+                const float left = y - static_cast<float>(h);
+                if constexpr (SPLIT) h = low ? static_cast<_Float16>(left * kLoScale) : h;
+                else b[2 + (j >> 3)][j & 7] = static_cast<_Float16>(left);
                 b[j >> 3][j & 7] = h;
             }
             l = l * alpha + sum * inverse;
@@ -439,6 +449,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
             const f16x8_t a0 = codes_to_half(v[d][0], v[d][1]), a1 = codes_to_half(v[d][2], v[d][3]);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b[0], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b[1], o[d], 0, 0, 0);
+            if constexpr (!SPLIT) {
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, b[2], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, b[3], o[d], 0, 0, 0);
+            }
         }
         if (next < tile.tiles) {
             wait_lds();
@@ -500,22 +514,22 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // tokens (one page), so that only y is masked and searched for its largest; A_v's
 // mantissa goes into the exponent too, and its sum is divided by it again.
 //
-// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 255 us, 0.9 PFLOP/s with a
-// product of two digits counted once; the 16-row kernel takes 409, a version in which
-// every wave read the whole tile's values from LDS 265.  Matrix instructions are 45 %
-// of a SIMD's time, the 290 vector instructions of a wave's tile the rest: with two
-// waves a SIMD the two overlap little, more with priority for the products (12 us).
-// Values by loads to LDS, as the keys, took 273 us.
+// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 359 us, 0.64 PFLOP/s with a
+// product of three digits or two halves counted once.  Where the products had two digits
+// and one half (250 us; the 16-row kernel 409) a version in which every wave read the
+// whole tile's values from LDS took 265, values by loads to LDS, as the keys, 273, and
+// priority for the products was worth 12.
 template <int D, Dtype DT, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
-    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<DT, SPLIT>;
+    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<SPLIT>;
     constexpr int kMyRows = SPLIT ? 8 : 16, kRows = kWaves * kMyRows;
     constexpr int kKeyUnits = kTileTokens * kUnits;
     constexpr int kMine = D / 64;  // a wave's 16s of dims
+    constexpr int kHalves = SPLIT ? 1 : 2;  // of a weight, in a column
     __shared__ union {
         struct {
             u32x4_t keys[2][kKeyUnits];
-            f16x8_t weights[kWaves][2][64];  // of a wave's rows
+            f16x8_t weights[kHalves][kWaves][2][64];  // of a wave's rows
             f32x4_t alphas[16];              // of row r of the four waves
         } tile;
         struct {
@@ -585,7 +599,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         for (int c = 0; c < kChunks; ++c) q[set][c] = lds.start.operands[wave][set][c][lane];
     const int col = SPLIT ? r & 7 : r, row = row0 + kMyRows * wave + col;
     const bool low = SPLIT && r >= 8;
-    const float factor = factors[wave][col] * (SPLIT ? 1.0f : kS == 3 ? 1.0f / 65536.0f : 1.0f / 256.0f);  // per unit of the last digit
+    const float factor = factors[wave][col] * (SPLIT ? 1.0f : 1.0f / 65536.0f);  // per unit of the last digit
     const float weight0 = low ? 1.0f / 256.0f : 1.0f;  // of a first digit, where they are four
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kWaves][kMine];  // of row r of every wave's
@@ -645,8 +659,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
                         static_cast<float>(s[1][u][i]) * (weight0 / 65536.0f));
                     y[4 * u + i] = half + xor_lane<8>(half);
                 } else {
-                    const float last = static_cast<float>(s[kS - 2][u][i] * 256 + s[kS - 1][u][i]);
-                    y[4 * u + i] = kS == 3 ? __builtin_fmaf(static_cast<float>(s[0][u][i]), 65536.0f, last) : last;
+                    const float last = static_cast<float>(s[1][u][i] * 256 + s[kS - 1][u][i]);
+                    y[4 * u + i] = __builtin_fmaf(static_cast<float>(s[0][u][i]), 65536.0f, last);
                 }
             }
         const int seen = there ? position + 1 - token : 0;  // of this lane's 16 tokens
@@ -674,35 +688,46 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         const bool silent = rest == 0.0f;
         const float c = (shift - base) + (silent ? 0.0f : __builtin_amdgcn_logf(rest));
         float sum = 0.0f;
-        f16x8_t b[2];
+        f16x8_t b[kHalves][2];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
             const f32x2_t e = {exp2_fast(__builtin_fmaf(y[j], f, c)), exp2_fast(__builtin_fmaf(y[j + 1], f, c))};
             sum += e[0] + e[1];
             f16x2_t h = __builtin_convertvector(e, f16x2_t);
+            const f32x2_t left = e - __builtin_convertvector(h, f32x2_t);
             if constexpr (SPLIT) {
-                const f32x2_t left = (e - __builtin_convertvector(h, f32x2_t)) * kLoScale;
-                h = low ? __builtin_convertvector(left, f16x2_t) : h;
+                h = low ? __builtin_convertvector(left * kLoScale, f16x2_t) : h;
+            } else {
+                const f16x2_t rest_of = __builtin_convertvector(left, f16x2_t);
+                b[kHalves - 1][j >> 3][j & 7] = rest_of[0];
+                b[kHalves - 1][j >> 3][(j & 7) + 1] = rest_of[1];
             }
-            b[j >> 3][j & 7] = h[0];
-            b[j >> 3][(j & 7) + 1] = h[1];
+            b[0][j >> 3][j & 7] = h[0];
+            b[0][j >> 3][(j & 7) + 1] = h[1];
         }
         if (__any(silent)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) b[j >> 3][j & 7] = silent ? static_cast<_Float16>(0.0f) : b[j >> 3][j & 7];
+            for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) b[half][j >> 3][j & 7] = silent ? static_cast<_Float16>(0.0f) : b[half][j >> 3][j & 7];
         }
         l = l * alpha + sum * __builtin_ldexpf(silent ? 1.0f : __builtin_amdgcn_rcpf(rest), -exponent);
-        lds.tile.weights[wave][0][lane] = b[0];
-        lds.tile.weights[wave][1][lane] = b[1];
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) {
+            lds.tile.weights[half][wave][0][lane] = b[half][0];
+            lds.tile.weights[half][wave][1][lane] = b[half][1];
+        }
         if (g == 0) reinterpret_cast<float *>(&lds.tile.alphas[r])[wave] = alpha;
         lds_barrier();  // every wave's weights are there
         __builtin_amdgcn_s_setprio(1);
-        f16x8_t weights[kWaves][2];
+        f16x8_t weights[kHalves][kWaves][2];
         const f32x4_t alphas = lds.tile.alphas[r];
 #pragma unroll
-        for (int t = 0; t < kWaves; ++t)
+        for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) weights[t][half] = lds.tile.weights[t][half][lane];
+            for (int t = 0; t < kWaves; ++t)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) weights[half][t][k] = lds.tile.weights[half][t][k][lane];
         if (__any(alphas[0] != 1.0f || alphas[1] != 1.0f || alphas[2] != 1.0f || alphas[3] != 1.0f)) {
 #pragma unroll
             for (int t = 0; t < kWaves; ++t)
@@ -713,9 +738,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         for (int i = 0; i < kMine; ++i) {
             const f16x8_t a0 = codes_to_half(codes[i][0], codes[i][1]), a1 = codes_to_half(codes[i][2], codes[i][3]);
 #pragma unroll
-            for (int t = 0; t < kWaves; ++t) o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, weights[t][0], o[t][i], 0, 0, 0);
+            for (int half = 0; half < kHalves; ++half) {
 #pragma unroll
-            for (int t = 0; t < kWaves; ++t) o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, weights[t][1], o[t][i], 0, 0, 0);
+                for (int t = 0; t < kWaves; ++t)
+                    o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, weights[half][t][0], o[t][i], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < kWaves; ++t)
+                    o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, weights[half][t][1], o[t][i], 0, 0, 0);
+            }
         }
         if (more) load_values(page);
         buffer ^= 1;

@@ -574,7 +574,9 @@ int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *cache, const int32_t *from, 
  * that see no token give zeros; rows that belong to no sequence are left as they
  * were.  max_length: about the largest lengths[s] + rows, for cutting the work; a
  * wrong one costs time only.  Queries that are not finite give NaN in their row
- * and head.  fp32 queries are computed to fp32's accuracy.  A sequence's rows
+ * and head.  Whatever the type and the rows beside a row, its scores and weights
+ * have fp32's accuracy: a query's elements count to 2^-24 (fp32: 2^-31) of a
+ * power of two above its largest, weights to 2^-22 of themselves.  A sequence's rows
  * times heads / kv_heads, in groups of 8 and over the kv heads, go up to 65535. */
 int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
     const fortai_hip_kv8_batch *batch, int dtype, const void *device_query, int64_t query_pitch,

@@ -1,0 +1,111 @@
+"""Attention over the 8-bit cache held, row by row and head by head, to what fp32
+arithmetic rounded once may be off: 16-bit types and however many rows a call has, too."""
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv8_attention import HALF_STEP, TYPES, Case
+
+LOG2E = 1.4426950408889634
+
+
+def tight(c, layer=0):
+    """The formula in 64 bits, and how far a row and head may be off before its one rounding to the output's type.
+
+    Scores: three digits to the base 256 of the query over a power of two above its row's largest (127 2^16 steps; four
+    digits, 127 2^24 steps, for fp32, behind one fp32 rounding), and eight fp32 roundings on the way to the exponent,
+    each 2^-24 of partial sums that |scale| sum |q k| bounds; the exponent's distance from its base is rounded once.
+    Weights: exp2, its base, the magnitude's mantissa and two fp16 halves: eight times 2^-23.  Sums of n tokens: n / 16
+    additions and 16 joins, 2^-23 of the terms' sum.  A lower half below fp16's range is lost: 2^-34 of the largest
+    product of weight and magnitude, a token.  An error of the weight of token j moves the result by p_j (v_j - out)."""
+    rows, group, page, d = int(c.starts[-1]), c.heads // c.kv, c.page, c.head
+    want, bound = np.zeros((rows, c.heads, d)), np.zeros((rows, c.heads, d))
+    q64 = c.q.double().numpy()
+    for s, (count, length) in enumerate(zip(c.counts, c.lengths)):
+        seen_pages = [(j, p) for j, p in enumerate(c.tables[s]) if 0 <= p < c.pages]
+        if not seen_pages or length + count <= 0:
+            continue
+        token = np.concatenate([np.arange(j * page, (j + 1) * page) for j, _ in seen_pages])
+        pick = [p for _, p in seen_pages]
+        for g in range(c.kv):
+            top_k, top_v = (x[layer, pick, g].astype(np.float64) for x in (c.key_max, c.value_max))
+            k = (c.keys[layer, pick, g] * (top_k / 127)[:, None, None]).reshape(-1, d)
+            v = (c.values[layer, pick, g] * (top_v / 127)[:, None, None]).transpose(0, 2, 1).reshape(-1, d)
+            magnitude = np.repeat(top_v, page)
+            for h in range(g * group, (g + 1) * group):
+                for i in range(count):
+                    see = token <= length + i
+                    if not see.any():
+                        continue
+                    row, q = c.starts[s] + i, q64[c.starts[s] + i, h, 0]
+                    x = (k[see] @ q) * c.scale
+                    p = np.exp(x - x.max())
+                    p /= p.sum()
+                    out = p @ v[see]
+                    size = abs(c.scale) * (np.abs(k[see]) @ np.abs(q))
+                    power = 2.0 ** np.frexp(np.abs(q).max())[1]
+                    steps = 127 * 2.0 ** (24 if c.dtype == "f32" else 16) / power
+                    lost = np.abs(np.rint(q * steps) / steps - q) + (np.abs(q) * 2.0 ** -24 if c.dtype == "f32" else 0.0)
+                    delta = abs(c.scale) * (np.abs(k[see]) @ lost) + (8 * size + (x.max() - x) + 1) * 2.0 ** -24
+                    gross = p @ np.abs(v[see])
+                    off = (p * (delta + 2.0 ** -20)) @ (np.abs(v[see]) + np.abs(out))
+                    off += (see.sum() / 16 + 16) * 2.0 ** -23 * (gross + np.abs(out))
+                    off += see.sum() * 2.0 ** -34 * np.max(p * magnitude[see])
+                    want[row, h], bound[row, h] = out, off
+    if c.gate:
+        sigmoid = 1 / (1 + np.exp(-q64[:, :, 1]))
+        want, bound = want * sigmoid, (bound + np.abs(want) * 2.0 ** -21) * sigmoid
+    return want, bound
+
+
+def allowed(c, layer=0):
+    want, bound = tight(c, layer)
+    return want, bound + (np.abs(want) + bound) * HALF_STEP[c.dtype] + (2.0 ** -25 if c.dtype == "f16" else 1e-37)
+
+
+def check(c, got, layer=0):
+    want, bound = allowed(c, layer)
+    assert np.all(np.abs(got - want) <= bound), float(np.nanmax(np.abs(got - want) / bound))
+
+
+# calls that take the kernel with 16 rows a workgroup, and (a long max_length) the one with 64
+FEW, MANY = None, 1 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_length", [FEW, MANY])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,head,page,counts,lengths", [
+    (8, 2, 256, 64, [5, 9, 1], [2, 0, 61]), (16, 4, 128, 16, [9, 40], [3, 1]), (12, 1, 64, 32, [17, 3], [30, 100])])
+def test_rows_are_computed_in_fp32(ctx, dtype, heads, kv, head, page, counts, lengths, max_length):
+    """Few tokens, so that no error of a weight is lost in the sum; more rows than eight columns hold."""
+    c = Case(ctx, heads, kv, head, page, counts, lengths, dtype, gate=False, seed=heads + head)
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_length", [FEW, MANY])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_queries_with_one_large_element(ctx, dtype, max_length):
+    """An element 2^9 times the others, where the keys are zero: the others decide."""
+    c = Case(ctx, 8, 2, 128, 32, [20, 3], [100, 7], dtype, seed=2)
+    c.keys[..., 5] = 0
+    c.q[:, :, 0, 5] = 2.0 ** 9 * c.q[:, :, 0].float().abs().amax(-1).to(TYPES[dtype])
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_row_alone_and_among_others(ctx, dtype):
+    """The same token decoded alone, with three drafts of another sequence and beside a prompt's chunk: the same bound."""
+    for counts in ([1, 1], [1, 3], [1, 90]):
+        for max_length in (FEW, MANY):
+            c = Case(ctx, 8, 2, 128, 32, counts, [130, 6], dtype, seed=11)
+            c.upload()
+            check(c, c.run(max_length=max_length))
+            c.cache.free()
