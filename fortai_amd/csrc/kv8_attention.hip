@@ -22,14 +22,18 @@
 // and for p in two fp16 halves (22 bits): used for fp32 queries, and where no more
 // than 8 rows are there to fill the columns.  Without it three digits (23 bits), and
 // p's halves are operands one after the other: with two digits and the upper half alone
-// five rows over 32,760 tokens take 21.1 us instead of 22.0 and 2000 behind 6000 250
-// instead of 359, but the results are off by 2^-12 of themselves and not the same as the
-// same row's in a call of fewer.  A_v enters the running maximum
-// by its exponent: the numerator's terms are p_j A_v / 127, and what is rounded to
-// fp16 is that product over the largest such product (times 2^14, away from fp16's
-// subnormals), so that pages of very different magnitude lose nothing against each
-// other.  Products below 2^-49 of the largest (2^-38 without SPLIT) count as zero.
-// All sums are fp32.
+// five rows over 32,760 tokens take 0.9 us less and 2000 behind 6000 109 us less, but the
+// results are off by 2^-12 of themselves and not the same as the same row's in a call of
+// fewer.  The numerator's terms are p_j A_v / 127: what is rounded to fp16 is p_j A_v over
+// the largest such product so far (times 2^14, away from fp16's subnormals), so that pages
+// of very different magnitude lose nothing against each other.  The denominator has a
+// maximum of its own, a lane's: a page of zeros counts there, whatever its score, and
+// raises no product's.  Both are whole powers of two, with a score's and a
+// magnitude's exponent apart, and what a page's weights are held against first is their
+// own largest score: any finite score and magnitude will do.  (Magnitudes in the scores'
+// maximum instead, up to 2^100: 4 % faster, infinities beyond, and products beside a page
+// of zeros lost.)  Products count as zero below 2^-48 of the largest, 2^-37 without SPLIT;
+// in the kernel for many rows below 2^-45 and 2^-34.  All sums are fp32.
 //
 // Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
 // workgroups a CU; `splits` workgroups share a sequence's head, joined by a second
@@ -37,9 +41,9 @@
 // that, 88 us where two launches take 25).  Bound by what a wave has to issue for a
 // tile (about 1,000 instructions, a third of them turning value codes into fp16) and,
 // where a wave has one tile or two, by the way there and back.  Eight sequences of up
-// to 8190 tokens, 16 heads of 256: 24.8 us for 80 MB (27.9 with values read into
-// registers as they are operands, in pieces of 16 bytes out of rows of 64); five rows
-// over 32,760 tokens 22.0 us for 33.5 MB; 600 tokens 12.5 us.
+// to 8190 tokens, 16 heads of 256: 26.1 us for 80 MB (values read into registers as they
+// are operands, in pieces of 16 bytes out of rows of 64: 12 % more); five rows over
+// 32,760 tokens 22.9 us for 33.5 MB; 600 tokens 13.2 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"
@@ -83,8 +87,50 @@ __device__ __forceinline__ float rounded(float product) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// exponent that A_v adds to the running maximum, and what is left of A_v
-__device__ __forceinline__ int value_exponent(float top) { return min(max(__builtin_amdgcn_frexp_expf(top), -100), 100); }
+// What products p_j A_v are held against: 2^(score + value), with a whole number near a
+// score and the exponent of a magnitude (score -infinity: nothing yet).  The two are
+// kept apart: their sum would lose the exponent beside a large score.
+struct Base {
+    float score, value;
+};
+
+// log2 of a over b; exact wherever it matters, NaN where neither is there
+__device__ __forceinline__ float above(const Base &a, const Base &b) { return (a.score - b.score) + (a.value - b.value); }
+
+// the larger of this lane's and that of the lane N further on
+template <int N>
+__device__ __forceinline__ Base larger_of_lanes(const Base &a) {
+    const Base b = {xor_lane<N>(a.score), xor_lane<N>(a.value)};
+    return above(b, a) > 0.0f ? b : a;
+}
+
+// A softmax's denominator, sum 2^base.
+struct Denominator {
+    float base = -__builtin_inff(), sum = 0.0f;
+    __device__ __forceinline__ void add(float other_base, float other_sum) {
+        const float top = fmaxf(base, other_base), zero = top == -__builtin_inff() ? 0.0f : top;  // not exp(nan)
+        sum = sum * exp2_fast(base - zero) + other_sum * exp2_fast(other_base - zero);
+        base = top;
+    }
+    template <int N>
+    __device__ __forceinline__ void add_lane() { add(xor_lane<N>(base), xor_lane<N>(sum)); }
+};
+
+// What turns a sum of products over 2^base into a result: y norm 2^exponent.  No token: 0.
+struct Quotient {
+    float norm;
+    int exponent;
+    __device__ __forceinline__ Quotient(const Base &base, const Denominator &l, float scale)
+        : norm(l.sum > 0.0f || l.sum != l.sum ? 1.0f / (l.sum * (scale * 127.0f)) : 0.0f),
+          exponent(static_cast<int>(fminf(fmaxf((base.score - l.base) + base.value, -1000.0f), 1000.0f))) {}
+    __device__ __forceinline__ Quotient(float n, int e) : norm(n), exponent(e) {}
+    __device__ __forceinline__ f32x4_t operator()(f32x4_t y) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf(y[i] * norm, exponent);
+        return y;
+    }
+    __device__ __forceinline__ bool some() const { return norm != 0.0f; }
+};
 
 // Four dims of one row and head, gated and stored.  some: the row saw a token.
 template <Dtype DT>
@@ -262,7 +308,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     constexpr int kS = kSets<SPLIT>;
     __shared__ i32x4_t operands[kS][kChunks][64];
     __shared__ float factors[kRows];
-    __shared__ float join_m[kWaves][kRows], join_l[kWaves][kRows];
+    __shared__ f32x4_t joins[kWaves][kRows];  // a wave's base (score, value) and denominator (base, sum)
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -334,7 +380,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     const float factor = factors[col];  // of S: softmax scale, log2 e, the query's power of two, 1 / 127^2
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kDims];
-    float m = -__builtin_inff(), l = 0.0f;
+    Base m = {-__builtin_inff(), 0.0f};  // of o
+    Denominator l;                       // of this lane's tokens
 #pragma unroll
     for (int d = 0; d < kDims; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -387,9 +434,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         const float key_top = there ? mine(key_top0, key_top1, key_top2, key_top3) : 0.0f;
         const float value_top = there ? mine(value_top0, value_top1, value_top2, value_top3) : 0.0f;
         find_pages(next);
-        const int exponent = value_exponent(value_top);
-        const float shift = static_cast<float>(exponent);
-        const float inverse = __builtin_ldexpf(1.0f, -exponent), rest = __builtin_ldexpf(value_top, -exponent) * kPScale;
         f16x8_t b[SPLIT ? 2 : 4];  // the weights of tokens 0..7 and 8..15, then their lower halves
         {
             const float f = factor * key_top;
@@ -404,7 +448,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
                     if constexpr (!SPLIT) y = __builtin_fmaf(static_cast<float>(s[1][u][i]), 1.0f / 256.0f, y);
                     y = SPLIT ? __builtin_fmaf(static_cast<float>(s[0][u][i]), weight0, y) : y + static_cast<float>(s[0][u][i]);
                     if constexpr (SPLIT) y = y + xor_lane<8>(y);
-                    x[4 * u + i] = __builtin_fmaf(y, f, shift);
+                    x[4 * u + i] = y * f;
                 }
             if (__any(seen < 16)) {
 #pragma unroll
@@ -413,16 +457,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
             float top = x[0];
 #pragma unroll
             for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-            top = fmaxf(top, xor_lane<16>(top));
-            top = fmaxf(top, xor_lane<32>(top));
-            const float now = fmaxf(m, top);
-            const float base = now == -__builtin_inff() ? 0.0f : now;  // nothing seen yet: p = 0, not exp(nan)
-            const float alpha = exp2_fast(m - base);
-            m = now;
+            const bool some = top > -__builtin_inff();
+            const float whole = some ? __builtin_rintf(top) : 0.0f;
+            // a page of zeros counts in the denominator, but has no products
+            const Base own = {some && value_top > 0.0f ? whole : -__builtin_inff(),
+                static_cast<float>(__builtin_amdgcn_frexp_expf(value_top))};
+            const Base now = larger_of_lanes<32>(larger_of_lanes<16>(own));
+            const bool higher = above(now, m) > 0.0f;
+            const float alpha = higher ? exp2_fast(above(m, now)) : 1.0f;
+            if (higher) m = now;
+            const float rest = own.score > -__builtin_inff()
+                ? exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(value_top) * kPScale) : 0.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const float e = exp2_fast(x[j] - base);
+                const float e = exp2_fast(x[j] - whole);
                 sum += e;
                 const float y = rounded(e * rest);
                 _Float16 h = static_cast<_Float16>(y);
@@ -431,7 +480,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
                 else b[2 + (j >> 3)][j & 7] = static_cast<_Float16>(left);
                 b[j >> 3][j & 7] = h;
             }
-            l = l * alpha + sum * inverse;
+            l.add(some ? whole : -__builtin_inff(), sum);
             if (n != first && __any(alpha != 1.0f)) {
 #pragma unroll
                 for (int d = 0; d < kDims; ++d)
@@ -461,20 +510,20 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     }
 
     // ---- join the waves
-    l += xor_lane<16>(l);
-    l += xor_lane<32>(l);
-    if (g == 0 && !low) {
-        join_m[wave][col] = m;
-        join_l[wave][col] = l;
-    }
+    l.add_lane<16>();
+    l.add_lane<32>();
+    if (g == 0 && !low) joins[wave][col] = f32x4_t{m.score, m.value, l.base, l.sum};
     lds_barrier();
-    float top = -__builtin_inff(), total = 0.0f;
+    Base top = {-__builtin_inff(), 0.0f};
+    Denominator total;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, join_m[w][col]);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += join_l[w][col] * exp2_fast(join_m[w][col] - base);
-    const float scale = exp2_fast(m - base) * share;
+    for (int w = 0; w < kWaves; ++w) {
+        const f32x4_t join = joins[w][col];
+        const Base other = {join[0], join[1]};
+        if (above(other, top) > 0.0f) top = other;
+        total.add(join[2], join[3]);
+    }
+    const float scale = m.score > -__builtin_inff() ? exp2_fast(above(m, top)) * share : 0.0f;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) lds.join[wave][d][lane] = o[d] * scale;
     lds_barrier();
@@ -482,7 +531,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
     const int head = kvh * p.group + row % p.group;
     const int64_t at = tile.begin + row / p.group;
-    const float norm = total > 0.0f || total != total ? 1.0f / (total * (kPScale * 127.0f)) : 0.0f;
+    const Quotient quotient(top, total, kPScale);
 #pragma unroll 1
     for (int d = wave * kChunks; d < (wave + 1) * kChunks; ++d) {
         f32x4_t y = lds.join[0][d][lane];
@@ -494,13 +543,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         }
         const int dim = 16 * d + 4 * g;
         if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + col) * D + dim) = y;
-        else finish<DT>(p, y * norm, norm != 0.0f, at, head, head * D + dim, dim);
+        else finish<DT>(p, quotient(y), quotient.some(), at, head, head * D + dim, dim);
     }
-    if (p.splits > 1 && wave == 0 && g == 0) {
-        float *ml = p.partial_ml + (item * kRows + col) * 2;
-        ml[0] = top;
-        ml[1] = total;
-    }
+    if (p.splits > 1 && wave == 0 && g == 0)
+        p.partial_ml[item * kRows + col] = f32x4_t{top.score, top.value, total.base, total.sum};
 }
 
 // Many rows (a prompt's chunk): 64 rows a workgroup (32 with SPLIT), which share every
@@ -510,11 +556,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // quarter of the dims: the values that it needs are its own then, which it loads and
 // turns into fp16 once for 64 rows.
 //
-// Scores: f y + shift with y the digits' sum, f > 0 and shift the same for a lane's 16
-// tokens (one page), so that only y is masked and searched for its largest; A_v's
-// mantissa goes into the exponent too, and its sum is divided by it again.
+// Scores: f y with y the digits' sum and f > 0 the same for a lane's 16 tokens (one
+// page), so that only y is masked and searched for its largest.
 //
-// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 359 us, 0.64 PFLOP/s with a
+// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 382 us, 0.6 PFLOP/s with a
 // product of three digits or two halves counted once.  Where the products had two digits
 // and one half (250 us; the 16-row kernel 409) a version in which every wave read the
 // whole tile's values from LDS took 265, values by loads to LDS, as the keys, 273, and
@@ -603,7 +648,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
     const float weight0 = low ? 1.0f / 256.0f : 1.0f;  // of a first digit, where they are four
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kWaves][kMine];  // of row r of every wave's
-    float m = -__builtin_inff(), l = 0.0f;
+    Base m = {-__builtin_inff(), 0.0f};
+    Denominator l;  // of this lane's tokens
 #pragma unroll
     for (int t = 0; t < kWaves; ++t)
 #pragma unroll
@@ -670,29 +716,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         }
         // not 0 or NaN times infinity where masked
         const float product = seen > 0 ? factor * k_top : 0.0f, f = product == 0.0f ? 1.2e-38f : product;
-        const int exponent = value_exponent(v_top);
-        const float shift = static_cast<float>(exponent);
         float top = y[0];
 #pragma unroll
         for (int j = 1; j < 16; ++j) top = fmaxf(top, y[j]);
-        top = __builtin_fmaf(top, f, shift);
-        top = fmaxf(top, xor_lane<16>(top));
-        top = fmaxf(top, xor_lane<32>(top));
+        top *= f;
+        const bool some = top > -__builtin_inff();
+        const float whole = some ? __builtin_rintf(top) : 0.0f;
+        // a page of zeros counts in the denominator, but has no products
+        const Base own = {some && v_top > 0.0f ? whole : -__builtin_inff(), static_cast<float>(__builtin_amdgcn_frexp_expf(v_top))};
+        const Base now = larger_of_lanes<32>(larger_of_lanes<16>(own));
         // a new base only where the old one is left behind by more than 2^4
-        const float now = top > m + 4.0f ? top : m;
-        const float base = now == -__builtin_inff() ? 0.0f : now;  // nothing seen yet: p = 0, not exp(nan)
-        const float alpha = exp2_fast(m - base);
-        m = now;
-        // what is left of A_v, scaled; pages of zeros have weights, but no values
-        const float rest = __builtin_ldexpf(v_top, -exponent) * kWideScale;
-        const bool silent = rest == 0.0f;
-        const float c = (shift - base) + (silent ? 0.0f : __builtin_amdgcn_logf(rest));
+        const bool higher = above(now, m) > 4.0f;
+        const float alpha = higher ? exp2_fast(above(m, now)) : 1.0f;
+        if (higher) m = now;
+        const float rest = own.score > -__builtin_inff()
+            ? exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(v_top) * kWideScale) : 0.0f;
         float sum = 0.0f;
         f16x8_t b[kHalves][2];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-            const f32x2_t e = {exp2_fast(__builtin_fmaf(y[j], f, c)), exp2_fast(__builtin_fmaf(y[j + 1], f, c))};
-            sum += e[0] + e[1];
+            // the same rounded product as the largest one: beyond 2^24 the exact one may lie far above it
+            const float e0 = exp2_fast(y[j] * f - whole), e1 = exp2_fast(y[j + 1] * f - whole);
+            sum += e0 + e1;
+            const f32x2_t e = {rounded(e0 * rest), rounded(e1 * rest)};
             f16x2_t h = __builtin_convertvector(e, f16x2_t);
             const f32x2_t left = e - __builtin_convertvector(h, f32x2_t);
             if constexpr (SPLIT) {
@@ -705,13 +751,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
             b[0][j >> 3][j & 7] = h[0];
             b[0][j >> 3][(j & 7) + 1] = h[1];
         }
-        if (__any(silent)) {
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) b[half][j >> 3][j & 7] = silent ? static_cast<_Float16>(0.0f) : b[half][j >> 3][j & 7];
-        }
-        l = l * alpha + sum * __builtin_ldexpf(silent ? 1.0f : __builtin_amdgcn_rcpf(rest), -exponent);
+        l.add(some ? whole : -__builtin_inff(), sum);
 #pragma unroll
         for (int half = 0; half < kHalves; ++half) {
             lds.tile.weights[half][wave][0][lane] = b[half][0];
@@ -752,20 +792,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
     }
     __builtin_amdgcn_s_setprio(0);
 
-    l += xor_lane<16>(l);
-    l += xor_lane<32>(l);
-    const float norm = p.splits > 1 ? kPScale / kWideScale : l > 0.0f || l != l ? 1.0f / (l * (kWideScale * 127.0f)) : 0.0f;
+    l.add_lane<16>();
+    l.add_lane<32>();
+    const Quotient quotient = p.splits > 1 ? Quotient(kPScale / kWideScale, 0) : Quotient(m, l, kWideScale);
     lds_barrier();  // the last tile's products are done
 #pragma unroll
     for (int t = 0; t < kWaves; ++t)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) lds.rows[t][wave * kMine + i][lane] = o[t][i];
     const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
-    if (p.splits > 1 && g == 0 && !low) {
-        float *ml = p.partial_ml + (item * kRows + kMyRows * wave + col) * 2;
-        ml[0] = m;
-        ml[1] = l;
-    }
+    if (p.splits > 1 && g == 0 && !low)
+        p.partial_ml[item * kRows + kMyRows * wave + col] = f32x4_t{m.score, m.value, l.base, l.sum};
     lds_barrier();
     // the rows that the wave has the sums of: a row's dims, four a lane, in as many rows at a time as a wave holds
     constexpr int kLanes = D / 4, kTogether = 64 / kLanes;
@@ -773,14 +810,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 #pragma unroll 1
     for (int k = 0; k < kMyRows; k += kTogether) {
         const int local = k + lane / kLanes, at = row0 + kMyRows * wave + local;
-        const float scale = __shfl(norm, local);
+        const Quotient row_quotient(__shfl(quotient.norm, local), __shfl(quotient.exponent, local));
         if (at >= tile.total) break;
         f32x4_t y = lds.rows[wave][four >> 2][16 * (four & 3) + local];
         if constexpr (SPLIT) y += lds.rows[wave][four >> 2][16 * (four & 3) + local + 8] * (1.0f / kLoScale);
-        y *= scale;
+        y = row_quotient(y);
         const int head = kvh * p.group + at % p.group;
         if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + kMyRows * wave + local) * D + dim) = y;
-        else finish<DT>(p, y, scale != 0.0f, tile.begin + at / p.group, head, head * D + dim, dim);
+        else finish<DT>(p, y, row_quotient.some(), tile.begin + at / p.group, head, head * D + dim, dim);
     }
 }
 
@@ -800,8 +837,7 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     const size_t y_index = static_cast<size_t>(row / tile_rows) * p.cache.kv_heads + kvh;
     const size_t tiles_y = static_cast<size_t>(p.row_tiles) * p.cache.kv_heads;
     const size_t item = (static_cast<size_t>(seq) * tiles_y + y_index) * p.splits;
-    const float *ml = p.partial_ml + (item * tile_rows + row % tile_rows) * 2;
-    const size_t ml_step = static_cast<size_t>(tile_rows) * 2;
+    const f32x4_t *ml = p.partial_ml + item * tile_rows + row % tile_rows;
 
     const int lane = threadIdx.x & 63;
     const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes, dim = 64 * slice + 4 * at;
@@ -814,19 +850,35 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
         early[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         if (group + k * kGroups < active) early[k] = *reinterpret_cast<const f32x4_t *>(from + (group + k * kGroups) * step);
     }
-    float top = -__builtin_inff();
-#pragma unroll 1
-    for (int i = lane; i < active; i += 64) top = fmaxf(top, ml[i * ml_step]);
-    top = wave_max(top);
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    float total = 0.0f;
+    Base top = {-__builtin_inff(), 0.0f};
+    Denominator total;
 #pragma unroll 1
     for (int i = lane; i < active; i += 64) {
-        const float w = exp2_fast(ml[i * ml_step] - base);
-        total += ml[i * ml_step + 1] * w;
-        if (threadIdx.x < 64) weight[i] = w;
+        const f32x4_t join = ml[static_cast<size_t>(i) * tile_rows];
+        const Base other = {join[0], join[1]};
+        if (above(other, top) > 0.0f) top = other;
+        total.add(join[2], join[3]);
     }
-    total = wave_sum(total);
+    top = larger_of_lanes<32>(top);
+    top = larger_of_lanes<16>(top);
+    top = larger_of_lanes<8>(top);
+    top = larger_of_lanes<4>(top);
+    top = larger_of_lanes<2>(top);
+    top = larger_of_lanes<1>(top);
+    total.add_lane<32>();
+    total.add_lane<16>();
+    total.add_lane<8>();
+    total.add_lane<4>();
+    total.add_lane<2>();
+    total.add_lane<1>();
+    if (threadIdx.x < 64) {
+#pragma unroll 1
+        for (int i = lane; i < active; i += 64) {
+            const f32x4_t join = ml[static_cast<size_t>(i) * tile_rows];
+            const Base other = {join[0], join[1]};
+            weight[i] = other.score > -__builtin_inff() ? exp2_fast(above(other, top)) : 0.0f;
+        }
+    }
     lds_barrier();
     f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -840,10 +892,9 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     const int used = min(active, kGroups);
 #pragma unroll 4
     for (int k = 1; k < used; ++k) y += sums[k][at];
-    const float norm = total > 0.0f || total != total ? 1.0f / (total * (kPScale * 127.0f)) : 0.0f;
-    y = y * norm;
+    const Quotient quotient(top, total, kPScale);
     const int head = kvh * p.group + row % p.group;
-    finish<DT>(p, y, norm != 0.0f, tile.begin + row / p.group, head, head * D + dim, dim);
+    finish<DT>(p, quotient(y), quotient.some(), tile.begin + row / p.group, head, head * D + dim, dim);
 }
 
 template <int D, Dtype DT, int ROWS>

@@ -46,7 +46,8 @@ struct Kv8AttentionParams {
     int group = 0;            // query heads of a kv head
     float scale_log2 = 0.0f;  // softmax scale * log2(e) / 127
     bool vec = false;         // q, gate and out allow four-element accesses
-    float *partial = nullptr, *partial_ml = nullptr;  // [kKv8PartialRows][head], [kKv8PartialRows][2]
+    float *partial = nullptr;        // [kKv8PartialRows][head]
+    f32x4_t *partial_ml = nullptr;   // [kKv8PartialRows]
     int splits = 0, row_tiles = 0;  // set by the launcher
 };
 hipError_t launch_kv8_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8Plan &plan, hipStream_t stream);

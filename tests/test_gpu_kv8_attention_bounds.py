@@ -109,3 +109,66 @@ def test_a_row_alone_and_among_others(ctx, dtype):
             c.upload()
             check(c, c.run(max_length=max_length))
             c.cache.free()
+
+
+def towards(c, s, index, factor):
+    """Sequence s's queries lean on its page `index`: every head's kv head's first key there."""
+    group = c.heads // c.kv
+    for h in range(c.heads):
+        code = c.keys[0, c.tables[s, index], h // group, 0].astype(np.float32)
+        c.q[c.starts[s]:c.starts[s + 1], h, 0] = torch.from_numpy(code * (factor / 127)).to(TYPES[c.dtype])
+
+
+# decode (fp32's kernel of 8 rows, four digits), 16 rows a workgroup, 64 (32 with fp32) rows a workgroup
+FORMS = [([1, 2], FEW), ([12, 3], FEW), ([12, 3], MANY)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,max_length", FORMS)
+@pytest.mark.parametrize("magnitude", [1e-2, 1e-9, 1e-12, 1e-30])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pages_of_zeros_beside_quiet_ones(ctx, dtype, magnitude, counts, max_length):
+    """Pages of zeros take part in the softmax, and cost the others' values none of their places: with scores like the
+    others', and (the second sequence) some 20 to 45 bits ahead of them."""
+    c = Case(ctx, 8, 2, 128, 16, counts, [90, 400], dtype, seed=5)
+    c.value_max[:] = magnitude
+    c.value_max[0, c.tables[0, 1:3]] = c.value_max[0, c.tables[1, 4]] = 0.0
+    c.scale *= 0.5
+    towards(c, 1, 4, 3.0)
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,max_length", FORMS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_magnitudes_up_to_the_largest_number(ctx, dtype, counts, max_length):
+    """Pages from 2^90 to 2^127, some beside ordinary ones; quiet pages that are chosen among them."""
+    c = Case(ctx, 8, 2, 64, 16, counts, [150, 300], dtype, seed=6)
+    c.value_max[:] = 2.0 ** np.random.default_rng(3).uniform(90, 127, c.value_max.shape)
+    c.value_max[0, c.tables[0, 3:5]] = 1.5
+    c.value_max[0, c.tables[1, 2]] = 3e-30
+    towards(c, 1, 2, 60.0)
+    c.upload()
+    got = c.run(max_length=max_length)
+    assert np.all(np.isfinite(got))
+    check(c, got)
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,max_length", FORMS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scores_beyond_24_bits(ctx, dtype, counts, max_length):
+    """Queries so large that the scores' own places are whole numbers and more: one key is half of them ahead and wins
+    alone, and its page's magnitude is not mixed up with another's.  Where the weight is one, roundings of the weight are
+    those of one product and one quotient: 2^-18 holds all of them."""
+    c = Case(ctx, 4, 2, 64, 16, counts, [70, 100], dtype, seed=7)
+    c.value_max[0, c.tables[0, :4], 0] = [1e-20, 1e20, 3.0, 1e6]
+    for s in range(2):
+        towards(c, s, 1, 1e9)
+    c.upload()
+    want, _ = tight(c)
+    assert np.all(np.abs(c.run(max_length=max_length) - want) <= np.abs(want) * (2.0 ** -18 + 1.01 * HALF_STEP[dtype]))
+    c.cache.free()
