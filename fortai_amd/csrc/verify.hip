@@ -508,11 +508,12 @@ __global__ __launch_bounds__(THREADS) void verify_finish_kernel(VerifyParams p) 
             double before = below_at;
 #pragma unroll 1
             for (int v = 0; v < wave; ++v) before += waves[v];
-            // a thread's tokens start where the one before it ends, to the bit, and its last one ends where it does
+            // Sums in another order may differ in their last places, also where a thread's tokens weigh
+            // nothing: a thread offers only tokens that do, and every thread that ends past the border
+            // offers one (its last where rounding hides the first), so that the lowest offered is the token.
             const double border = border_at, upto = before + prefix;
             double c = __shfl_up(upto, 1);
             if (lane == 0) c = before;
-            const bool mine = c <= border && upto > border;
             int first = 0x7fffffff, end = -1;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(THREADS) void verify_finish_kernel(VerifyParams p) 
                 end = w[i] > 0.0 ? from + i : end;
                 first = w[i] > 0.0 && c > border ? min(first, from + i) : first;
             }
-            first = mine ? min(first, end) : 0x7fffffff;
+            if (first > end) first = upto > border && end >= 0 ? end : 0x7fffffff;
             // the lowest token found, else the last that weighs anything
             first = wave_least(first);
             end = wave_most(end);
