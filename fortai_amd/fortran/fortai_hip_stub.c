@@ -5,7 +5,8 @@
  * (src/backend/cpu/fortai_cuda_stub.c:13-23) does: a create or upload sets
  * its out-handle to NULL and fails with FORTAI_HIP_RUNTIME_ERROR, every
  * destroy (NULL included) succeeds, every other call fails with
- * FORTAI_HIP_RUNTIME_ERROR and last_error says why.  Linking the real library
+ * FORTAI_HIP_RUNTIME_ERROR and last_error says why; what asks for a number
+ * gives the one that stands for none (0 bytes, a length or count of -1).  Linking the real library
  * overrides all of them. */
 #include "fortai_hip_backend.h"
 
@@ -929,13 +930,13 @@ FORTAI_HIP_WEAK int fortai_hip_kv8_pages_compact(fortai_hip_kv8_pages *pool, int
 FORTAI_HIP_WEAK int64_t fortai_hip_kv8_pages_length(const fortai_hip_kv8_pages *pool, int sequence)
 {
     (void)pool; (void)sequence;
-    return 0;
+    return -1;
 }
 
 FORTAI_HIP_WEAK int fortai_hip_kv8_pages_free_count(const fortai_hip_kv8_pages *pool)
 {
     (void)pool;
-    return FORTAI_HIP_RUNTIME_ERROR;
+    return -1;
 }
 
 FORTAI_HIP_WEAK int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool,

@@ -597,7 +597,7 @@ int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
  * at most `capacity` of them; the moves go through copy_pages before the next
  * append or attention, and tables that were taken before are stale.
  * tables: the pages of count sequences, rows of table_pitch, -1 behind the last.
- * length (-1: no such sequence) and free_count ask. */
+ * length (-1: no such sequence) and free_count (-1: no pool) ask. */
 int fortai_hip_kv8_pages_create(int pages, int page_tokens, int sequences, int table_pitch,
     fortai_hip_kv8_pages **pool);
 int fortai_hip_kv8_pages_destroy(fortai_hip_kv8_pages *pool);

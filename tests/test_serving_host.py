@@ -146,6 +146,18 @@ def test_pages_refusals():
     pool.free()
 
 
+def test_the_stub_counts_no_pages(tmp_path):
+    """Without the library: a length and a count of -1, as the library answers where there is no pool."""
+    so = str(tmp_path / "libstub.so")
+    subprocess.run(["gcc", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"),
+                    os.path.join(ROOT, "fortai_amd", "fortran", "fortai_hip_stub.c"), "-o", so], check=True)
+    for lib in (C.CDLL(so), B.load()):
+        lib.fortai_hip_kv8_pages_length.restype = C.c_int64
+        lib.fortai_hip_kv8_bytes.restype = C.c_size_t
+        assert lib.fortai_hip_kv8_pages_length(None, 0) == -1 and lib.fortai_hip_kv8_pages_free_count(None) == -1
+        assert lib.fortai_hip_kv8_bytes(1, 0, 16, 1, 64) == 0
+
+
 # ------------------------------------------------------------- checks
 def test_rope_checks_and_frequencies(tmp_path):
     lib = compiled(tmp_path, '''
