@@ -172,3 +172,102 @@ def test_scores_beyond_24_bits(ctx, dtype, counts, max_length):
     want, _ = tight(c)
     assert np.all(np.abs(c.run(max_length=max_length) - want) <= np.abs(want) * (2.0 ** -18 + 1.01 * HALF_STEP[dtype]))
     c.cache.free()
+
+
+def odd_pages(ctx, head, dtype):
+    """Pages that are not there, of zeros, loud and quiet ones, in one sequence; ordinary ones in the other."""
+    c = Case(ctx, 8, 2, head, 16, [30, 19], [250, 90], dtype, seed=head)
+    c.tables[0, 2:4] = [-1, c.pages + 5]
+    c.key_max[:, c.tables[0, 5:8]] = 0.0
+    c.value_max[:, c.tables[0, 6:9]] = 0.0
+    c.value_max[:, c.tables[0, 10]] = 1e4
+    c.value_max[:, c.tables[0, 11]] = 1e-30
+    c.key_max[:, c.tables[1, 3]] *= 3.0
+    c.scale = -c.scale
+    return c
+
+
+def unlike_magnitudes(ctx, dtype, count):
+    """Value pages from 1e-6 to 1e6."""
+    c = Case(ctx, 2, 1, 64, 16, [count], [300], dtype, seed=6)
+    c.value_max[0, :, 0] = 10.0 ** np.random.default_rng(1).uniform(-6, 6, c.pages)
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_length", [FEW, MANY])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("head", [64, 128, 256])
+def test_odd_pages(ctx, head, dtype, max_length):
+    c = odd_pages(ctx, head, dtype)
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,max_length", [(1, FEW), (20, FEW), (40, MANY)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_unlike_magnitudes(ctx, dtype, count, max_length):
+    c = unlike_magnitudes(ctx, dtype, count)
+    if dtype == "f16":
+        c.value_max /= 100.0  # results within its range
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,max_length", FORMS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_loud_page_ruled_out_and_a_quiet_one_chosen(ctx, dtype, counts, max_length):
+    c = Case(ctx, 8, 2, 128, 64, counts, [100, 200], dtype, seed=8)
+    c.value_max[0, c.tables[:, 0]] = 1e-3
+    c.value_max[0, c.tables[:, 1]] = 1e3
+    for s in range(2):
+        towards(c, s, 0, 4.0)
+    c.upload()
+    check(c, c.run(max_length=max_length))
+    c.cache.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,counts", [("f32", [1, 1, 1, 1]), ("bf16", [30, 25, 2, 1]), ("bf16", [3, 2, 2, 1])])
+def test_row_starts_that_are_out_of_range(ctx, dtype, counts):
+    """Clipped to the batch's rows and max_rows: those rows as a batch that says so has them, every other row and what
+    lies around the output as they were."""
+    c = Case(ctx, 4, 2, 64, 16, counts, [100, 60, 5, 33], dtype, seed=5)
+    c.upload()
+    rows, most, guard = int(c.starts[-1]), max(counts), 4
+    results = []
+    for starts in ([0, -5, 2 ** 31 - 1, 1, 0], [0, 0, min(rows, most), rows, rows]):
+        around = torch.full((rows + 2 * guard, 4, 64), 77.0, dtype=TYPES[dtype], device="cuda")
+        c.dev[0].copy_(torch.tensor(starts, dtype=torch.int32))
+        lengths = [9, 60, -rows, 7] if starts[1] == 0 else [9, 60, 5, 7]
+        c.dev[1].copy_(torch.tensor(lengths, dtype=torch.int32))
+        c.out = around[guard:guard + rows]
+        torch.cuda.synchronize()
+        c.run()
+        results.append(around.clone())
+    got, want = (r.double().cpu().numpy() for r in results)
+    inside = slice(guard, guard + min(rows, most))
+    assert np.array_equal(got[inside], want[inside]) and not np.any(got[inside] == 77.0)
+    got[inside] = 77.0
+    assert np.all(got == 77.0)
+
+
+def test_the_bounds_turn_wrong_rows_down():
+    """Zeros, the negated result and results without the quieter pages are outside what the checks above allow, in every
+    row and head that has a value."""
+    cases = [odd_pages(None, head, dtype) for head in (64, 128, 256) for dtype in ("f32", "bf16")]
+    cases += [unlike_magnitudes(None, dtype, 20) for dtype in ("f32", "bf16")]
+    for c in cases:
+        want, bound = allowed(c)
+        there = np.abs(want).max(axis=2) > 0
+        for wrong in (np.zeros_like(want), -want):
+            assert np.all((np.abs(wrong - want) > bound).any(axis=2)[there])
+    quiet = unlike_magnitudes(None, "f32", 20)  # half a step of bf16 is more than these pages add
+    want, bound = allowed(quiet)
+    quiet.value_max = np.where(quiet.value_max < 100.0, 0.0, quiet.value_max).astype(np.float32)
+    without, _ = tight(quiet)
+    assert np.mean((np.abs(without - want) > bound).any(axis=2)) > 0.9
