@@ -184,13 +184,18 @@ __device__ __forceinline__ void wait_lds() {
 // Written out because the compiler, which cannot tell one buffer's loads from
 // another's, would have every LDS read wait for all of them; wait_loads() says which
 // have to be there.  There is no destination register.
+// m0 is a register that the compiler keeps for itself and warns about: it holds nothing
+// across a statement that names it, which is all that is asked.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int INST>
 __device__ __forceinline__ void load_to_lds(uint32_t to, uint64_t base, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
                  :
                  : "s"(to), "v"(offset), "s"(base), "n"(INST)
-                 : "memory");  // m0 too, which nothing else here uses
+                 : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)(p)));
