@@ -471,15 +471,17 @@ int fortai_hip_qwen35_batch_set_prefill_mode(fortai_hip_qwen35_batch *batch_deco
 
 /* ============ [extension] serving operators ==========================
  * The operators of a step that runs several tokens of several sequences over a
- * shared cache.  As everywhere, they are enqueued on the context's stream; data
- * that another stream produced has to be complete (or waited for) before the
- * call.  The caller's current device stays current.  Arrays of activations are
- * fp32, fp16 or bf16, computed on in fp32 and rounded once, to nearest even.
- * Pitches count elements, at most 2^31; base addresses are aligned to their
- * element.  Row counts go up to 2^23.  Where nothing else is said, what a call
- * writes overlaps nothing that it reads.  Handles are created while no capture is
- * under way, and destroyed before their context; the page bookkeeping is used by
- * one thread at a time. */
+ * shared cache.  As everywhere, they are enqueued on the context's stream, which
+ * neither waits for another stream nor is waited for: inputs that do not come from
+ * earlier calls of this context have to be complete when a call is made, and its
+ * outputs may be read elsewhere, as its inputs may be written again, once the
+ * context is synchronized (fortai_hip_q8_context_synchronize, or the device).  The
+ * caller's current device stays current.  Arrays of activations are fp32, fp16 or
+ * bf16, computed on in fp32 and rounded once, to nearest even.  Pitches count
+ * elements, at most 2^31; base addresses are aligned to their element.  Row counts
+ * go up to 2^23.  Where nothing else is said, what a call writes overlaps nothing
+ * that it reads.  Handles are created while no capture is under way, and destroyed
+ * before their context; the page bookkeeping is used by one thread at a time. */
 #define FORTAI_HIP_DTYPE_F32 0
 #define FORTAI_HIP_DTYPE_F16 1
 #define FORTAI_HIP_DTYPE_BF16 2
@@ -496,7 +498,7 @@ int fortai_hip_qwen35_batch_set_prefill_mode(fortai_hip_qwen35_batch *batch_deco
  * device: rows x heads vectors of head_size (a multiple of 4, rope_dimension to
  * 256); row r is at device_positions[r] (int32).  device_norm (fp32
  * [head_size], may be NULL): each vector is RMS-normalised over head_size with
- * these weights first.  Dims from rope_dimension on are not rotated.  The
+ * these weights and epsilon (above 0) first.  Dims from rope_dimension on are not rotated.  The
  * output may be the input itself (same pitches), or an array apart from it.  A
  * context that replays the call in a graph keeps the handle. */
 #define FORTAI_HIP_ROPE_PLAIN 0
@@ -527,12 +529,15 @@ int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype, const void *device_
  * tokens; lengths[s] tokens of it precede them, so that its i-th row is token
  * lengths[s] + i, in page tables[s][token / page_tokens].  All three arrays are
  * device memory, read when the call's kernels run.  max_rows: at least the rows
- * of any sequence (rows past it are left out).  Ids outside the pool (-1, say)
+ * of any sequence (rows past it are left out), at most rows.  Ids outside the pool (-1, say)
  * are pages that are not there, as are those past table_pitch.
  *
  * append: rows of keys and values [rows][kv_heads][head_size] at row pitches.
  * The page's magnitude is the largest of its tokens so far; when new tokens
- * raise it, the codes that the page holds are rounded to the new one.  Codes are
+ * raise it, the codes that the page holds are rounded to the new one, which adds up to
+ * half a code of it to their error each time.  A magnitude never falls while the page has
+ * a first token that stands: a draft that is rejected after its append leaves the codes of
+ * the tokens before it as it has rounded them.  Codes are
  * the nearest integers to 127 x / magnitude, ties to even, in exact arithmetic.
  * NaN is stored as zero, an infinity as the page's largest magnitude.  A page
  * whose first token is among the rows starts anew; tokens without a page, and
