@@ -87,14 +87,17 @@ __device__ __forceinline__ float rounded(float product) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+constexpr float kNone = -3e38f;      // a base of nothing; finite, so that differences are
+constexpr float kHuge = 4194304.0f;  // 2^22: a whole score below it, plus an exponent, is exact
+
 // What products p_j A_v are held against: 2^(score + value), with a whole number near a
-// score and the exponent of a magnitude (score -infinity: nothing yet).  The two are
-// kept apart: their sum would lose the exponent beside a large score.
+// score and the exponent of a magnitude.  Beside a huge score the two are kept apart:
+// their sum would lose the exponent.
 struct Base {
     float score, value;
 };
 
-// log2 of a over b; exact wherever it matters, NaN where neither is there
+// log2 of a over b, exact wherever it matters
 __device__ __forceinline__ float above(const Base &a, const Base &b) { return (a.score - b.score) + (a.value - b.value); }
 
 // the larger of this lane's and that of the lane N further on
@@ -104,13 +107,22 @@ __device__ __forceinline__ Base larger_of_lanes(const Base &a) {
     return above(b, a) > 0.0f ? b : a;
 }
 
+// the largest of the four lanes of a row
+__device__ __forceinline__ Base largest_of_row(const Base &a, bool some_huge) {
+    if (some_huge) return larger_of_lanes<32>(larger_of_lanes<16>(a));
+    float sum = a.score + a.value;
+    sum = fmaxf(sum, xor_lane<16>(sum));
+    sum = fmaxf(sum, xor_lane<32>(sum));
+    return Base{sum, 0.0f};
+}
+
 // A softmax's denominator, sum 2^base.
 struct Denominator {
-    float base = -__builtin_inff(), sum = 0.0f;
+    float base = kNone, sum = 0.0f;
     __device__ __forceinline__ void add(float other_base, float other_sum) {
-        const float top = fmaxf(base, other_base), zero = top == -__builtin_inff() ? 0.0f : top;  // not exp(nan)
-        sum = sum * exp2_fast(base - zero) + other_sum * exp2_fast(other_base - zero);
-        base = top;
+        const float d = other_base - base, scale = exp2_fast(-fabsf(d));
+        sum = __builtin_fmaf(d > 0.0f ? sum : other_sum, scale, d > 0.0f ? other_sum : sum);
+        base = fmaxf(base, other_base);
     }
     template <int N>
     __device__ __forceinline__ void add_lane() { add(xor_lane<N>(base), xor_lane<N>(sum)); }
@@ -385,8 +397,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     const float factor = factors[col];  // of S: softmax scale, log2 e, the query's power of two, 1 / 127^2
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kDims];
-    Base m = {-__builtin_inff(), 0.0f};  // of o
-    Denominator l;                       // of this lane's tokens
+    Base m = {kNone, 0.0f};  // of o
+    Denominator l;           // of this lane's tokens
 #pragma unroll
     for (int d = 0; d < kDims; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -465,14 +477,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
             const bool some = top > -__builtin_inff();
             const float whole = some ? __builtin_rintf(top) : 0.0f;
             // a page of zeros counts in the denominator, but has no products
-            const Base own = {some && value_top > 0.0f ? whole : -__builtin_inff(),
-                static_cast<float>(__builtin_amdgcn_frexp_expf(value_top))};
-            const Base now = larger_of_lanes<32>(larger_of_lanes<16>(own));
-            const bool higher = above(now, m) > 0.0f;
-            const float alpha = higher ? exp2_fast(above(m, now)) : 1.0f;
-            if (higher) m = now;
-            const float rest = own.score > -__builtin_inff()
-                ? exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(value_top) * kPScale) : 0.0f;
+            const Base own = {some && value_top > 0.0f ? whole : kNone, static_cast<float>(__builtin_amdgcn_frexp_expf(value_top))};
+            const Base now = largest_of_row(own, __any(fabsf(whole) >= kHuge));
+            const float higher = above(now, m);
+            const float alpha = exp2_fast(-fmaxf(higher, 0.0f));
+            if (higher > 0.0f) m = now;
+            const float rest = exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(value_top) * kPScale);
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -485,7 +495,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
                 else b[2 + (j >> 3)][j & 7] = static_cast<_Float16>(left);
                 b[j >> 3][j & 7] = h;
             }
-            l.add(some ? whole : -__builtin_inff(), sum);
+            l.add(some ? whole : kNone, sum);
             if (n != first && __any(alpha != 1.0f)) {
 #pragma unroll
                 for (int d = 0; d < kDims; ++d)
@@ -519,7 +529,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     l.add_lane<32>();
     if (g == 0 && !low) joins[wave][col] = f32x4_t{m.score, m.value, l.base, l.sum};
     lds_barrier();
-    Base top = {-__builtin_inff(), 0.0f};
+    Base top = {kNone, 0.0f};
     Denominator total;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -528,7 +538,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         if (above(other, top) > 0.0f) top = other;
         total.add(join[2], join[3]);
     }
-    const float scale = m.score > -__builtin_inff() ? exp2_fast(above(m, top)) * share : 0.0f;
+    const float scale = exp2_fast(above(m, top)) * share;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) lds.join[wave][d][lane] = o[d] * scale;
     lds_barrier();
@@ -653,7 +663,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
     const float weight0 = low ? 1.0f / 256.0f : 1.0f;  // of a first digit, where they are four
     const int position = row < tile.total ? tile.length + row / p.group : -1;  // the last token that the row sees
     f32x4_t o[kWaves][kMine];  // of row r of every wave's
-    Base m = {-__builtin_inff(), 0.0f};
+    Base m = {kNone, 0.0f};
     Denominator l;  // of this lane's tokens
 #pragma unroll
     for (int t = 0; t < kWaves; ++t)
@@ -727,21 +737,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         top *= f;
         const bool some = top > -__builtin_inff();
         const float whole = some ? __builtin_rintf(top) : 0.0f;
+        const bool some_huge = __any(fabsf(whole) >= kHuge);
+        float scale = f;
+        if (some_huge) {  // the same rounded products as the largest one: exact ones may lie far above it
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] *= f;
+            scale = 1.0f;
+        }
         // a page of zeros counts in the denominator, but has no products
-        const Base own = {some && v_top > 0.0f ? whole : -__builtin_inff(), static_cast<float>(__builtin_amdgcn_frexp_expf(v_top))};
-        const Base now = larger_of_lanes<32>(larger_of_lanes<16>(own));
+        const Base own = {some && v_top > 0.0f ? whole : kNone, static_cast<float>(__builtin_amdgcn_frexp_expf(v_top))};
+        const Base now = largest_of_row(own, some_huge);
         // a new base only where the old one is left behind by more than 2^4
-        const bool higher = above(now, m) > 4.0f;
-        const float alpha = higher ? exp2_fast(above(m, now)) : 1.0f;
-        if (higher) m = now;
-        const float rest = own.score > -__builtin_inff()
-            ? exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(v_top) * kWideScale) : 0.0f;
+        const float higher = above(now, m);
+        const float alpha = higher > 4.0f ? exp2_fast(-higher) : 1.0f;
+        if (higher > 4.0f) m = now;
+        const float rest = exp2_fast(above(own, m)) * (__builtin_amdgcn_frexp_mantf(v_top) * kWideScale);
         float sum = 0.0f;
         f16x8_t b[kHalves][2];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-            // the same rounded product as the largest one: beyond 2^24 the exact one may lie far above it
-            const float e0 = exp2_fast(y[j] * f - whole), e1 = exp2_fast(y[j + 1] * f - whole);
+            const float e0 = exp2_fast(__builtin_fmaf(y[j], scale, -whole)), e1 = exp2_fast(__builtin_fmaf(y[j + 1], scale, -whole));
             sum += e0 + e1;
             const f32x2_t e = {rounded(e0 * rest), rounded(e1 * rest)};
             f16x2_t h = __builtin_convertvector(e, f16x2_t);
@@ -756,7 +771,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
             b[0][j >> 3][j & 7] = h[0];
             b[0][j >> 3][(j & 7) + 1] = h[1];
         }
-        l.add(some ? whole : -__builtin_inff(), sum);
+        l.add(some ? whole : kNone, sum);
 #pragma unroll
         for (int half = 0; half < kHalves; ++half) {
             lds.tile.weights[half][wave][0][lane] = b[half][0];
@@ -855,7 +870,7 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
         early[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         if (group + k * kGroups < active) early[k] = *reinterpret_cast<const f32x4_t *>(from + (group + k * kGroups) * step);
     }
-    Base top = {-__builtin_inff(), 0.0f};
+    Base top = {kNone, 0.0f};
     Denominator total;
 #pragma unroll 1
     for (int i = lane; i < active; i += 64) {
@@ -881,7 +896,7 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
         for (int i = lane; i < active; i += 64) {
             const f32x4_t join = ml[static_cast<size_t>(i) * tile_rows];
             const Base other = {join[0], join[1]};
-            weight[i] = other.score > -__builtin_inff() ? exp2_fast(above(other, top)) : 0.0f;
+            weight[i] = exp2_fast(above(other, top));
         }
     }
     lds_barrier();
