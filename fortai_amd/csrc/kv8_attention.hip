@@ -38,12 +38,12 @@
 // Few rows (decode steps, drafts): the four waves of a workgroup take tiles in turn, two
 // workgroups a CU; `splits` workgroups share a sequence's head, joined by a second
 // launch (the last workgroup joining instead: every workgroup writes its L2 back for
-// that, 88 us where two launches take 25).  Bound by what a wave has to issue for a
-// tile (about 1,000 instructions, a third of them turning value codes into fp16) and,
-// where a wave has one tile or two, by the way there and back.  Eight sequences of up
-// to 8190 tokens, 16 heads of 256: 26.1 us for 80 MB (values read into registers as they
+// that, 88 us where two launches take 25).  Bound by what a wave has to issue, 560 vector
+// instructions a tile and 1,040 around its tiles (queries, join, quotients; counted at
+// heads of 256), and, where a wave has one tile or two, by the loads that wait for each
+// other on the way there: page word, keys, then values.  Eight sequences of up to 8190 tokens, 16 heads of 256: 25.8 us for 81 MB (values read into registers as they
 // are operands, in pieces of 16 bytes out of rows of 64: 12 % more); five rows over
-// 32,760 tokens 22.9 us for 33.5 MB; 600 tokens 13.2 us.
+// 32,760 tokens 22.8 us for 33.6 MB; 600 tokens 13.2 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"
@@ -574,11 +574,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // Scores: f y with y the digits' sum and f > 0 the same for a lane's 16 tokens (one
 // page), so that only y is masked and searched for its largest.
 //
-// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 382 us, 0.6 PFLOP/s with a
-// product of three digits or two halves counted once.  Where the products had two digits
-// and one half (250 us; the 16-row kernel 409) a version in which every wave read the
-// whole tile's values from LDS took 265, values by loads to LDS, as the keys, 273, and
-// priority for the products was worth 12.
+// 2000 tokens of 16 heads (4 kv heads of 256) behind 6000: 367 to 383 us on three cards, 0.6
+// PFLOP/s with a product of three digits or two halves counted once.  Matrix instructions (112 a wave's
+// tile) are 54 % of a SIMD's time and its 400 vector instructions the rest: two waves a
+// SIMD overlap little.  Where the products had two digits and one half (249 us; the
+// 16-row kernel 409) a version in which every wave read the whole tile's values from LDS
+// took 265, values by loads to LDS, as the keys, 273, and priority for the products was
+// worth 12.
 template <int D, Dtype DT, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
     constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<SPLIT>;

@@ -21,7 +21,7 @@
 // a page is in flight at once (four blocks one after the other: the read back of
 // 2,300 prompt tokens 12.4 us instead of 10.8, an append of them 45 us, 27 KB of code,
 // instead of 16).  A token of each of eight sequences: append 6.4 us, read back 5.6.
-// Page copies: 1.06 GB in 174 us, 6.1 TB/s.
+// Page copies: 1.05 GB in 174 us, 6.0 TB/s.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "serving_kernels.h"

@@ -77,15 +77,18 @@ struct Kv8Plan {
 // fp32 queries always have 8 rows in an instruction's 16 columns (each twice, for the
 // two halves of its numbers), others where 8 are enough.  More than twice as many rows
 // take the kernel with four times as many a workgroup, if the cached tokens are so many
-// that the smaller workgroups would have four tiles of 64 a SIMD (heads of 256: 40 rows
-// of 16 bits over 30,000 tokens, 5.5 tiles a SIMD, 29.8 us against 36.7; 256 rows over
-// 1,000 tokens, one tile a SIMD, 21.5 against 19.6; fp32, 64 rows over 30,000 tokens,
-// 41.3 against 44.4, 8,000 over 7,000 561 against 853).
+// that the smaller workgroups would have four tiles of 64 a SIMD.  Heads of 256, 16 bits:
+// 40 rows over 30,000 tokens, 5.5 tiles a SIMD, 36.4 us against 39.4 (64 rows, which fill
+// the smaller workgroups, 37.6 against 34.8); 256 rows over 1,000 tokens, one tile a SIMD,
+// 26.0 against 22.3; 8,000 behind 7,000 413 against 560.  fp32: 64 rows over 30,000
+// tokens 42.7 against 45.9, 8,000 behind 7,000 661 against 958; where many rows are split
+// over few tokens their join costs more than either (1,000 behind 1,000, split in four,
+// 54.7 against 27.5 unsplit).
 // Tokens are split until there are two workgroups a CU for heads of 256 (more for
 // smaller ones, which take less LDS), as far as every one has a tile for each of its
 // four waves (two tiles where the waves share them) and the partial results fit: one workgroup a CU
-// costs 29.7 us where two cost 25.0 (eight sequences of up to 8190 tokens); one tile a
-// wave costs 13.0 us where three cost 19.4 (600 tokens).
+// costs 30.5 us where two cost 25.9 (eight sequences of up to 8190 tokens); one tile a
+// wave costs 13.2 us where three cost 17.0 (600 tokens).
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
     Kv8Plan p;
     const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
