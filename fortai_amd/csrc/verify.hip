@@ -62,8 +62,11 @@ struct RowExp {
         y = __builtin_fma(y, r, 0x1.000000000003dp+0);
         return __builtin_ldexp(y, static_cast<int>(__builtin_bit_cast(uint2, k).x));
     }
-    // no weight where x is -infinity
-    __device__ __forceinline__ double operator()(float x) const { return x == -__builtin_inff() ? 0.0 : raw(x); }
+    // No weight for what lies lower than 2^-1000, as far as 64 bits tell it from nothing: -infinity, and masks
+    // by the type's lowest number, which a draw at u = 0 would otherwise find.
+    __device__ __forceinline__ double operator()(float x) const {
+        return static_cast<double>(x) - top > least ? raw(x) : 0.0;
+    }
 };
 
 __device__ __forceinline__ void sequence_rows(const VerifyParams &p, int seq, int *begin, int *end) {

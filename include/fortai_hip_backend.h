@@ -635,8 +635,8 @@ int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool, const int *seq
  * Outputs: emitted (int64 [rows]) has for each sequence the drafts that stand, the
  * drawn token, then -1; accepted (int32 [sequences]) how many stand; logprobs
  * (fp32 [rows], may be NULL) log p of each emitted token, 0 behind them (T <= 0:
- * at T = 1).  A logit of -infinity or NaN has no weight, +infinity counts as the
- * largest number; a deciding row without any weight emits -1 with -infinity.  A
+ * at T = 1).  A logit of -infinity or NaN has no weight, nor has one whose weight is
+ * below 2^-1000 of its row's largest; +infinity counts as the largest number; a deciding row without any weight emits -1 with -infinity.  A
  * draft outside the vocabulary does not stand.  Rows of no sequence are left as
  * they were.  Logits are fp32, fp16 or bf16 at row pitches; a verifier is made
  * for at most max_rows rows, max_sequences sequences (both up to 65535) and one

@@ -1,6 +1,7 @@
 """Draft verification where the draw's border falls between two tokens: sums in
 another order may tell the two apart, but nothing else may come out."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -55,3 +56,34 @@ def test_a_draw_at_the_middle_of_what_is_left(ctx, vocab, first, second):
     emitted, accepted, _ = s.run()
     assert not accepted.any()
     assert set(emitted[0::2].tolist()) <= {first[-1], second[0]}, emitted
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("vocab", [40, 5000, 150000])
+def test_masks_of_the_types_lowest_value(ctx, vocab, drafts, dtype):
+    """Tokens masked by the lowest finite number weigh nothing: no u draws them, 0 included, and no draft of them stands."""
+    s = Step(ctx, [1, 3, 2], vocab, dtype, drafts, 3)
+    allowed = torch.zeros(vocab, dtype=torch.bool)
+    allowed[7:vocab - 9:3] = True
+    s.target[:, ~allowed] = torch.finfo(s.target.dtype).min
+    if drafts:
+        s.draft[:, ~allowed] = torch.finfo(s.target.dtype).min
+    s.tokens[:] = 2
+    for u in (0.0, 1.0 - 2.0 ** -24):
+        s.uniforms[:] = u
+        got = s.run()
+        assert not got[1].any() and np.all(allowed.numpy()[got[0][[0, 1, 4]]])
+        if u == 0.0 and not drafts:
+            assert np.all(got[0][[0, 1, 4]] == 7)  # the lowest that weighs anything
+
+
+def test_drafts_that_neither_distribution_gives_any_weight(ctx):
+    """At a temperature so low that both probabilities are below what 64 bits hold: not u q < p."""
+    s = Step(ctx, [4, 4, 4], 4096, "f32", True, 4)
+    s.temperatures[:] = 1e-3
+    worst = torch.stack([(t / 1e-3).log_softmax(0) for t in s.target.double()])
+    s.tokens[1:] = worst[:-1].argmin(dim=1)
+    got = s.run()
+    assert not got[1].any()
+    s.check(got)
