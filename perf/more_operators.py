@@ -1,0 +1,687 @@
+"""The operators that a drafted step of several sequences needs around its products, and their plain forms.
+
+A server that runs several tokens of several sequences a step, over layers of gated delta rules and of
+attention, adds a block's output to the residual stream and takes the norm's result as 8-bit tokens into the
+next product; runs the delta rule's rows (with the causal convolution in front of it) on from each sequence's
+state, which has to survive drafts that are turned down; attends over pages that sequences share since they
+forked; and applies penalties, biases and masks to the logits before drafts are verified.  Each case is one of
+those calls at one size; ``draw`` gives further sizes of the same ranges.  With ``own`` false ``run`` computes
+the same results in elementary torch operations.
+
+Head layouts are those of ``fortai_amd.synth.CONFIGS`` and generic ones; sequences of a batch differ in length.
+"""
+
+import math
+
+import numpy as np
+import torch
+
+if torch.cuda.is_available():
+    DEV = "cuda"
+else:
+    DEV = "cpu"
+
+own = False
+
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+EPS = 1e-6
+CHUNK = 64  # rows that the plain form of the delta rule takes at once
+
+
+# ------------------------------------------------------------------- cases
+def listed():
+    return [
+        # one new token of each of eight sequences, no drafts
+        {"name": "gdn_decode", "kind": "gdn", "key_heads": 16, "value_heads": 16, "head": 128, "kernel": 4, "pending": 0,
+         "sequences": 8, "rows": 1, "dtype": "f32"},
+        # up to four drafts and the token before them, behind a step of which some drafts were turned down
+        {"name": "gdn_drafts", "kind": "gdn", "key_heads": 16, "value_heads": 32, "head": 128, "kernel": 4, "pending": 5,
+         "sequences": 8, "rows": 5, "dtype": "bf16"},
+        # one long document
+        {"name": "gdn_document", "kind": "gdn", "key_heads": 16, "value_heads": 16, "head": 128, "kernel": 4, "pending": 0,
+         "sequences": 1, "rows": 2000, "dtype": "bf16"},
+        # eight prompts of up to 512 tokens
+        {"name": "gdn_prompts", "kind": "gdn", "key_heads": 16, "value_heads": 32, "head": 128, "kernel": 4, "pending": 5,
+         "sequences": 8, "rows": 512, "dtype": "f32"},
+        # the block's output and the residual stream of a decode step of eight sequences
+        {"name": "norm_decode", "kind": "norm", "use": "residual", "rows": 8, "width": 1024, "dtype": "f32"},
+        # the same of a prompt of 4096 tokens
+        {"name": "norm_prompt", "kind": "norm", "use": "residual", "rows": 4096, "width": 2560, "dtype": "f32"},
+        # a prompt's delta rule outputs, normalised by heads and gated, into the output projection
+        {"name": "norm_gated", "kind": "norm", "use": "gated", "rows": 2000, "width": 4096, "dtype": "bf16"},
+        # one sequence with a short history, a small vocabulary
+        {"name": "logits_one", "kind": "logits", "sequences": 1, "rows": 1, "vocab": 16384, "history": 300, "window": 64,
+         "bias": False, "mask": False, "dtype": "f32"},
+        # up to four drafts of each of eight sequences, long histories, some held to a grammar
+        {"name": "logits_batch", "kind": "logits", "sequences": 8, "rows": 5, "vocab": 248320, "history": 8000, "window": 0,
+         "bias": True, "mask": True, "dtype": "f32"},
+        # four answers to one short question
+        {"name": "shared_few", "kind": "shared", "heads": 8, "kv_heads": 2, "head": 256, "page": 32, "groups": 1,
+         "sequences": 4, "rows": 1, "shared": 1000, "tokens": 100, "gate": True, "dtype": "f32"},
+        # a decode step of 32 sequences behind one system prompt of 8000 tokens
+        {"name": "shared_batch", "kind": "shared", "heads": 16, "kv_heads": 4, "head": 256, "page": 64, "groups": 1,
+         "sequences": 32, "rows": 1, "shared": 8000, "tokens": 190, "gate": True, "dtype": "f32"},
+        # drafts of 16 sequences that go on from two long documents
+        {"name": "shared_drafts", "kind": "shared", "heads": 8, "kv_heads": 2, "head": 256, "page": 64, "groups": 2,
+         "sequences": 16, "rows": 5, "shared": 24000, "tokens": 700, "gate": True, "dtype": "bf16"},
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(["gdn", "gdn", "gdn", "norm", "norm", "logits", "shared", "shared"])
+    dtype = rng.choice(["f32", "f16", "bf16"])
+    if kind == "gdn":
+        key_heads, value_heads = rng.choice([(16, 16), (16, 32), (2, 4), (4, 4), (3, 9), (1, 1), (5, 10), (8, 32)])
+        case = {"kind": kind, "key_heads": key_heads, "value_heads": value_heads, "head": rng.choice([64, 128, 128]),
+                "kernel": rng.choice([4, 4, 2, 3, 5, 8]), "pending": rng.choice([0, 0, 5, 9, 16]),
+                "sequences": rng.randint(1, 8), "rows": 1, "dtype": dtype}
+        form = rng.choice(["decode", "drafts", "prompt", "prompt"])
+        if form == "drafts":
+            case["pending"] = rng.choice([5, 9, 16])
+            case["rows"] = rng.randint(2, case["pending"])
+        elif form == "prompt":
+            case["rows"] = _log(rng, 2, 4000 // case["sequences"])
+        return case
+    if kind == "norm":
+        use = rng.choice(["residual", "gated", "product"])
+        width = 64 * rng.randint(1, 72) if use != "residual" else 32 * rng.randint(1, 160)
+        return {"kind": kind, "use": use, "rows": _log(rng, 1, 4096 if width <= 2560 else 2000), "width": width, "dtype": dtype}
+    if kind == "logits":
+        return {"kind": kind, "sequences": rng.randint(1, 8), "rows": rng.randint(1, 5),
+                "vocab": rng.choice([4096, 16384, 248320, _log(rng, 500, 240000)]), "history": _log(rng, 1, 8000),
+                "window": rng.choice([0, 0, 1, 64, 1000]), "bias": rng.random() < 0.5, "mask": rng.random() < 0.5, "dtype": dtype}
+    heads, kv_heads = rng.choice([(8, 2), (16, 4), (4, 2), (6, 6), (12, 1), (5, 5), (24, 3)])
+    sequences = _log(rng, 2, 32)
+    return {"kind": kind, "heads": heads, "kv_heads": kv_heads, "head": rng.choice([64, 128, 256]),
+            "page": rng.choice([16, 32, 64]), "groups": rng.randint(1, max(1, min(3, sequences // 2))), "sequences": sequences,
+            "rows": rng.choice([1, 1, rng.randint(2, 5)]), "shared": _log(rng, 20, 24000), "tokens": _log(rng, 1, 700),
+            "gate": rng.random() < 0.5, "dtype": dtype}
+
+
+def _spread(most, n):
+    """A number of each of n sequences: the first has the most, later ones down to a fifth."""
+    return [max(1, int(round(most * (1.0 - 0.8 * s / max(1, n - 1))))) for s in range(n)]
+
+
+def _rows_of(case):
+    if case["rows"] <= 17:  # a decode step: numbers of drafts differ
+        return [max(1, case["rows"] - s % 3) for s in range(case["sequences"])]
+    return _spread(case["rows"], case["sequences"])
+
+
+# ------------------------------------------------------------------ inputs
+def _generator(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(0x51AB + 7919 * int(seed))
+    return g
+
+
+def _normal(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def _uniform(g, *shape):
+    return torch.rand(*shape, generator=g, device=DEV)
+
+
+def _below(g, high, *shape):
+    return torch.randint(0, high, shape, generator=g, device=DEV)
+
+
+def _int32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _starts(counts):
+    return _int32(np.concatenate([[0], np.cumsum(counts)]).tolist())
+
+
+_CONTEXT = None
+
+
+def _context():
+    """The program's one context: its calls run in order on one stream."""
+    global _CONTEXT
+    if _CONTEXT is None:
+        from fortai_amd import backend
+        _CONTEXT = backend.Context(0)
+    return _CONTEXT
+
+
+class _State:
+    """What a program holds for one case; its handles are given back with it."""
+
+    def __init__(self, case):
+        self.case = case
+        self.handles = []
+
+    def __del__(self):
+        try:
+            for h in self.handles:
+                h.free()
+        except Exception:
+            pass
+
+
+def prepare(case, seed):
+    s = _State(case)
+    globals()["_prepare_" + case["kind"]](s, _generator(seed), case)
+    if own:
+        _hold(s, case)
+    if DEV == "cuda":
+        torch.cuda.synchronize()
+    return s
+
+
+def _hold(s, case):
+    """The framework's handles over these inputs, which a program keeps beside them (the inputs are the same without)."""
+    from fortai_amd import backend
+    ctx = _context()
+    if case["kind"] == "gdn":
+        s.handles.append(backend.GdnCache(
+            ctx, 1, s.slots, case["key_heads"], case["value_heads"], case["head"], case["kernel"], case["pending"], s.total,
+            storage=s.storage.data_ptr(), storage_bytes=4 * s.storage.numel()))
+        s.batch = backend.GdnBatch(case["sequences"], s.total, s.most, s.row_starts.data_ptr(), s.slot.data_ptr(),
+                                   s.standing.data_ptr())
+    elif case["kind"] == "shared":
+        s.handles.append(backend.Kv8Cache(ctx, 1, s.pages, case["page"], case["kv_heads"], case["head"],
+                                          storage=s.storage.data_ptr(), storage_bytes=s.storage.numel()))
+        s.batch = backend.Kv8Batch(case["sequences"], s.total, s.most, s.row_starts.data_ptr(), s.lengths.data_ptr(),
+                                   s.tables.data_ptr(), s.pitch)
+        s.sharing = backend.Kv8Groups(case["groups"], s.group_rows, s.group_starts.data_ptr(), s.group_shared.data_ptr(),
+                                      s.group_of.data_ptr())
+
+
+def _gdn_planes(s, case):
+    """The storage's planes, as views, in order: states [slots][value_heads][head][head], conv inputs
+    [slots][kernel - 1 + pending][channels], pending rows' keys [slots][pending][key_heads][head], updates
+    [slots][pending][value_heads][head] and decays [slots][pending][value_heads], then how many there are."""
+    kh, vh, d, p, n = case["key_heads"], case["value_heads"], case["head"], case["pending"], s.slots
+    shapes = [(n, vh, d, d), (n, case["kernel"] - 1 + p, (2 * kh + vh) * d), (n, p, kh, d), (n, p, vh, d), (n, p, vh), (n,)]
+    sizes = [math.prod(shape) for shape in shapes]
+    planes = [part.view(shape) for part, shape in zip(torch.split(s.storage, sizes), shapes)]
+    return planes[:5] + [planes[5].view(torch.int32)]
+
+
+def _prepare_gdn(s, g, case):
+    kh, vh, d, p, n, dtype = (case["key_heads"], case["value_heads"], case["head"], case["pending"], case["sequences"],
+                              DTYPES[case["dtype"]])
+    counts = _rows_of(case)
+    channels = (2 * kh + vh) * d
+    s.total, s.most, s.slots = sum(counts), max(counts), n + 2
+    s.row_starts = _starts(counts)
+    s.slot = torch.randperm(s.slots, generator=g, device=DEV)[:n].to(torch.int32)
+    # the projections' outputs, the small ones side by side
+    s.qkv = _normal(g, s.total, channels).to(dtype)
+    s.gates = _normal(g, 2, s.total, vh).to(dtype)
+    s.conv = 0.3 * _normal(g, channels, case["kernel"])
+    s.ssm_a = -torch.exp(_normal(g, vh) - 1.5)
+    s.ssm_dt = _normal(g, vh)
+    # a state that a few hundred tokens have left, and a step whose rows have not been judged yet
+    floats = s.slots * (vh * d * d + (case["kernel"] - 1 + p) * channels + p * (kh * d + vh * d + vh) + 1)
+    s.storage = torch.empty(floats, dtype=torch.float32, device=DEV)
+    state, window, keys, updates, decays, count = _gdn_planes(s, case)
+    state.copy_(0.15 * _normal(g, *state.shape))
+    window.copy_(_normal(g, *window.shape))
+    k = _normal(g, *keys.shape)
+    keys.copy_(k / k.square().sum(dim=-1, keepdim=True).sqrt())
+    updates.copy_(0.2 * _normal(g, *updates.shape))
+    decays.copy_(torch.exp(-0.5 * _uniform(g, *decays.shape)))
+    count.copy_(_below(g, p + 1, s.slots).to(torch.int32))
+    # how many of those rows stand; now and then a sequence begins
+    stands = (_uniform(g, n) * (count[s.slot.long()] + 1)).to(torch.int32)
+    s.standing = torch.where(_uniform(g, n) < 0.15, torch.full_like(stands, -1), stands)
+    s.out = torch.empty(s.total, vh, d, dtype=dtype, device=DEV)
+
+
+def _prepare_norm(s, g, case):
+    rows, width, dtype = case["rows"], case["width"], DTYPES[case["dtype"]]
+    s.group = width if case["use"] == "residual" else 128 if width % 128 == 0 else 64
+    # a few channels of a residual stream are far larger than the others
+    loud = torch.exp(0.8 * _normal(g, width))
+    s.x = (_normal(g, rows, width) * (0.3 if case["use"] == "residual" else loud)).to(dtype)
+    s.residual = (_normal(g, rows, width) * loud).to(dtype) if case["use"] == "residual" else None
+    s.gate = None if case["use"] == "residual" else (1.5 * _normal(g, rows, width)).to(dtype)
+    s.weight = None if case["use"] == "product" else 1.0 + 0.1 * _normal(g, s.group)
+    s.sum = torch.empty_like(s.x) if case["use"] == "residual" else None
+    s.ld = -(-rows // 128) * 128
+    s.tokens = torch.empty(s.ld * (-(-width // 128) * 4) * 36, dtype=torch.uint8, device=DEV)
+    s.values = torch.empty(rows, width, dtype=torch.float32, device=DEV)
+
+
+def _prepare_logits(s, g, case):
+    n, vocab, dtype = case["sequences"], case["vocab"], DTYPES[case["dtype"]]
+    counts, lengths = _rows_of(case), _spread(case["history"], case["sequences"])
+    s.total, s.most, s.pitch = sum(counts), max(counts), max(lengths)
+    s.row_starts, s.lengths = _starts(counts), _int32(lengths)
+    s.logits = (3.0 * _normal(g, s.total, vocab)).to(dtype)
+    # text repeats itself: most tokens are among the first of the vocabulary
+    s.history = (_uniform(g, n, s.pitch).pow(4) * vocab).long().clamp_max(vocab - 1)
+    s.tokens = (_uniform(g, s.total).pow(4) * vocab).long().clamp_max(vocab - 1)
+    # repetition, frequency, presence
+    s.penalties = torch.stack([1.0 + 0.3 * _uniform(g, n), 0.3 * _uniform(g, n), 0.5 * _uniform(g, n)], dim=1).contiguous()
+    s.bias = 0.5 * _normal(g, vocab) if case["bias"] else None
+    s.masks = s.mask_of = None
+    if case["mask"]:
+        # few masks serve many rows; words of 32 tokens, the lowest bit first
+        s.masks = _below(g, 1 << 32, 3, -(-vocab // 32)).to(torch.int32)
+        s.mask_of = _below(g, 4, s.total).to(torch.int32) - 1
+    s.out = torch.empty_like(s.logits)
+
+
+def _prepare_shared(s, g, case):
+    n, page, kv, head, dtype = case["sequences"], case["page"], case["kv_heads"], case["head"], DTYPES[case["dtype"]]
+    counts, tokens = _rows_of(case), _spread(case["tokens"], n)
+    groups = case["groups"]
+    bounds = [n * i // groups for i in range(groups + 1)]
+    # whole pages are shared; documents differ in length
+    shared = [max(1, case["shared"] // (i + 1) // page) * page for i in range(groups)]
+    group_of = [i for i in range(groups) for _ in range(bounds[i], bounds[i + 1])]
+    lengths = [shared[group_of[q]] + tokens[q] - 1 for q in range(n)]
+    need = [-(-(l + r) // page) for l, r in zip(lengths, counts)]
+    common = [shared[group_of[q]] // page for q in range(n)]
+    s.pages, s.pitch = sum(k - c for k, c in zip(need, common)) + sum(x // page for x in shared) + 3, max(need)
+    order = torch.randperm(s.pages, generator=g, device=DEV).to(torch.int32)
+    s.tables = torch.full((n, s.pitch), -1, dtype=torch.int32, device=DEV)
+    at, first = 0, []
+    for x in shared:
+        first.append(order[at:at + x // page])
+        at += x // page
+    for q in range(n):
+        s.tables[q, :common[q]] = first[group_of[q]]
+        s.tables[q, common[q]:need[q]] = order[at:at + need[q] - common[q]]
+        at += need[q] - common[q]
+    codes, maxima = s.pages * kv * page * head, s.pages * kv
+    s.storage = torch.empty(2 * codes + 8 * maxima, dtype=torch.uint8, device=DEV)
+    step = 1 << 26
+    for at in range(0, 2 * codes, step):
+        m = min(step, 2 * codes - at)
+        s.storage[at:at + m] = (_normal(g, m) * 36.0).round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
+    s.storage[2 * codes:] = (torch.exp(0.25 * _normal(g, 2 * maxima)) * 3.5).view(torch.uint8)
+    s.total, s.most, s.longest, s.longest_shared = sum(counts), max(counts), max(l + r for l, r in zip(lengths, counts)), max(shared)
+    s.row_starts, s.lengths = _starts(counts), _int32(lengths)
+    s.group_starts, s.group_shared, s.group_of = _int32(bounds), _int32(shared), _int32(group_of)
+    s.group_rows = max(sum(counts[a:b]) for a, b in zip(bounds, bounds[1:]))
+    s.host = (bounds, shared, lengths, counts)
+    heads = case["heads"]
+    q = _normal(g, s.total, heads, 2 if case["gate"] else 1, head)
+    q[:, :, 0] *= 2.0 * torch.exp(0.3 * _normal(g, 1, heads, 1))
+    s.q = q.to(dtype)
+    s.scale = 1.0 / math.sqrt(head)
+    s.out = torch.empty(s.total, heads, head, dtype=dtype, device=DEV)
+
+
+# --------------------------------------------------------------------- run
+def run(state):
+    return globals()[("_own_" if own else "_run_") + state.case["kind"]](state, state.case)
+
+
+def _gdn_outputs(s, case, out):
+    names = ("states", "inputs", "keys", "updates", "decays", "counts")
+    planes = dict(zip(names, _gdn_planes(s, case)))
+    planes["out"] = out
+    return {name: plane for name, plane in planes.items() if plane.numel()}
+
+
+def _own_gdn(s, case):
+    s.handles[0].run(0, s.batch, s.qkv.data_ptr(), s.gates[0].data_ptr(), s.gates[1].data_ptr(), s.conv.data_ptr(),
+                     s.ssm_a.data_ptr(), s.ssm_dt.data_ptr(), s.out.data_ptr(), dtype=case["dtype"], eps=EPS)
+    return _gdn_outputs(s, case, s.out)
+
+
+def _own_norm(s, case):
+    ptr = lambda t: None if t is None else t.data_ptr()
+    ctx = _context()
+    ctx.norm_tokens(s.x.data_ptr(), case["rows"], case["width"], dtype=case["dtype"], residual=ptr(s.residual), sum=ptr(s.sum),
+                    norm=ptr(s.weight), group=s.group, eps=EPS, gate=ptr(s.gate), tokens=s.tokens.data_ptr())
+    # the values that the 8-bit tokens stand for
+    ctx.tokens_read(s.tokens.data_ptr(), case["rows"], case["width"], s.values.data_ptr(), dtype="f32")
+    return {"values": s.values} if s.sum is None else {"values": s.values, "sum": s.sum}
+
+
+def _own_logits(s, case):
+    ptr = lambda t: None if t is None else t.data_ptr()
+    _context().adjust_logits(s.logits.data_ptr(), case["vocab"], s.out.data_ptr(), s.row_starts.data_ptr(), case["sequences"],
+                             s.total, dtype=case["dtype"], tokens=s.tokens.data_ptr(), history=s.history.data_ptr(),
+                             history_pitch=s.pitch, history_lengths=s.lengths.data_ptr(), window=case["window"],
+                             penalties=s.penalties.data_ptr(), bias=ptr(s.bias), masks=ptr(s.masks),
+                             mask_count=0 if s.masks is None else s.masks.shape[0], mask_of=ptr(s.mask_of))
+    return s.out
+
+
+def _own_shared(s, case):
+    parts, head, at = s.q.shape[2], case["head"], s.q.data_ptr()
+    s.handles[0].shared_attention(0, s.batch, s.sharing, at, case["heads"], s.out.data_ptr(), s.scale, s.longest,
+                                  s.longest_shared, dtype=case["dtype"],
+                                  gate=at + head * s.q.element_size() if parts == 2 else None, query_head_pitch=parts * head,
+                                  query_pitch=case["heads"] * parts * head)
+    return s.out
+
+
+# ------------------------------------------------------------- plain forms
+def _padded(starts, most):
+    """Row numbers [sequences][most] of a ragged batch, and which of them are there."""
+    starts = starts.long()
+    rows = starts[:-1, None] + torch.arange(most, device=DEV)
+    there = rows < starts[1:, None]
+    return torch.where(there, rows, torch.zeros_like(rows)), there
+
+
+def _silu(x):
+    return x / (1.0 + torch.exp(-x))
+
+
+def _run_gdn(s, case):
+    kh, vh, d, p, n, taps = (case["key_heads"], case["value_heads"], case["head"], case["pending"], case["sequences"],
+                             case["kernel"])
+    state, window, keys, updates, decays, count = _gdn_planes(s, case)
+    slot = s.slot.long()
+    begins = s.standing < 0
+    stands = torch.minimum(s.standing, count[slot]).clamp_min(0).long()
+    # the rows of every sequence behind the inputs that the convolution still sees
+    rows, there = _padded(s.row_starts, s.most)
+    r = there.sum(dim=1)
+    x = torch.where(there[:, :, None], s.qkv[rows].float(), 0.0)
+    before = torch.gather(window[slot], 1, (stands[:, None] + torch.arange(taps - 1, device=DEV))[:, :, None].expand(-1, -1, x.shape[2]))
+    x = torch.cat([torch.where(begins[:, None, None], 0.0, before), x], dim=1)
+    y = sum(s.conv[:, t] * x[:, t:t + s.most] for t in range(taps))
+    q, k, v = torch.split(_silu(y), [kh * d, kh * d, vh * d], dim=2)
+    unit = lambda t: t / torch.sqrt((t * t).sum(dim=-1, keepdim=True)).clamp_min(EPS)
+    q, k = unit(q.reshape(n, -1, kh, d)) / math.sqrt(d), unit(k.reshape(n, -1, kh, d))
+    v = v.reshape(n, -1, vh, d)
+    a = s.gates[0].float()[rows] + s.ssm_dt
+    decay = s.ssm_a * (torch.clamp_min(a, 0.0) + torch.log1p(torch.exp(-torch.abs(a))))
+    decay = torch.where(there[:, :, None], decay, 0.0)
+    beta = torch.where(there[:, :, None], 1.0 / (1.0 + torch.exp(-s.gates[1].float()[rows])), 0.0)
+    # the pending rows that stand
+    S = torch.where(begins[:, None, None, None], 0.0, state[slot])
+    head_of = torch.arange(vh, device=DEV) // (vh // kh)
+    for i in range(p):
+        on = (i < stands)[:, None]
+        S = torch.where(on, decays[slot, i], 1.0)[:, :, None, None] * S + \
+            torch.where(on[:, :, None], updates[slot, i], 0.0)[..., None] * keys[slot, i][:, head_of][:, :, None, :]
+    settled = S
+    # chunks of rows [n][chunks][heads][C][...]; rows past the last one change nothing
+    C = min(CHUNK, s.most)
+    chunks = -(-s.most // C)
+    cut = lambda t: torch.nn.functional.pad(t, (0, 0) * (t.dim() - 2) + (0, chunks * C - s.most)).unflatten(1, (chunks, C)).transpose(2, 3)
+    qc, kc, vc = cut(q)[:, :, head_of], cut(torch.where(there[:, :, None, None], k, 0.0))[:, :, head_of], cut(v)
+    bc, total = cut(beta), torch.cumsum(cut(decay).double(), dim=-1)
+    gap = total[..., :, None] - total[..., None, :]
+    lower = torch.ones(C, C, dtype=torch.bool, device=DEV).tril()
+    weight = torch.where(lower, torch.exp(torch.where(lower, gap, 0.0)), 0.0).float()
+    kt = kc.transpose(3, 4).contiguous()
+    A = bc[..., None] * weight * torch.matmul(kc, kt)
+    inner = weight * torch.matmul(qc, kt)
+    through = torch.exp(total).float()[..., None]
+    X = torch.cat([bc[..., None] * through * kc, bc[..., None] * vc], dim=-1)
+    for i in range(1, C):
+        X[..., i, :] -= (A[..., i, :i, None] * X[..., :i, :]).sum(dim=-2)
+    W, U = X[..., :d], X[..., d:]
+    rest = torch.exp(total[..., -1:] - total).float()[..., None]
+    out, delta = [], []
+    for c in range(chunks):
+        St = S.transpose(2, 3).contiguous()
+        D = U[:, c] - torch.matmul(W[:, c], St)
+        out.append(through[:, c] * torch.matmul(qc[:, c], St) + torch.matmul(inner[:, c], D))
+        S = through[:, c, :, -1:] * S + torch.matmul((rest[:, c] * D).transpose(2, 3).contiguous(), kc[:, c])
+        delta.append(D)
+    join = lambda t: torch.stack(t, dim=1).transpose(2, 3).flatten(1, 2)[:, :s.most]
+    # what is kept: rows up to `pending` wait for their verdict
+    waits = r <= p
+    state[slot] = torch.where(waits[:, None, None, None], settled, S)
+    at = torch.arange(window.shape[1], device=DEV)
+    take = torch.where(waits[:, None], at, r[:, None] + at)
+    kept = at < torch.where(waits, taps - 1 + r, taps - 1)[:, None]
+    fresh = torch.gather(x, 1, take.clamp_max(x.shape[1] - 1)[:, :, None].expand(-1, -1, x.shape[2]))
+    window[slot] = torch.where(kept[:, :, None], fresh, window[slot])
+    if p:
+        log = torch.arange(p, device=DEV)
+        kept, take = (log < r[:, None]) & waits[:, None], log.clamp_max(s.most - 1)
+        keys[slot] = torch.where(kept[:, :, None, None], k[:, take], keys[slot])
+        updates[slot] = torch.where(kept[:, :, None, None], join(delta)[:, take], updates[slot])
+        decays[slot] = torch.where(kept[:, :, None], torch.exp(decay[:, take]), decays[slot])
+    count[slot] = torch.where(waits, r, 0).to(torch.int32)
+    return _gdn_outputs(s, case, join(out)[there].to(s.out.dtype))
+
+
+def _tokens_of(y):
+    """The values that rows hold in blocks of 32 codes with a 16-bit scale.  y in 64 bits, where a quotient next to
+    a half stays on its side; quotients that are halves but for y's own rounding (gates that are equal) become
+    halves in 32 bits, and go to the even code."""
+    blocks = y.unflatten(1, (-1, 32))
+    top = blocks.abs().amax(dim=-1, keepdim=True)
+    codes = torch.where(top > 0, torch.round((127.0 * blocks / top).float()), 0.0)
+    return (codes * (top / 127.0).float().to(torch.float16).float()).flatten(1)
+
+
+def _run_norm(s, case):
+    h = s.x
+    if s.residual is not None:
+        h = (s.x.float() + s.residual.float()).to(s.x.dtype)
+    y = h.double()
+    if s.weight is not None:
+        y = y.unflatten(1, (-1, s.group))
+        y = (y * s.weight.double() / torch.sqrt((y * y).mean(dim=-1, keepdim=True) + EPS)).flatten(1)
+    if s.gate is not None:
+        y = y * _silu(s.gate.double())
+    values = _tokens_of(y)
+    return {"values": values} if s.residual is None else {"values": values, "sum": h}
+
+
+def _run_logits(s, case):
+    vocab, most = case["vocab"], s.most
+    rows, there = _padded(s.row_starts, most)
+    # for every row the tokens so far: the history, then the step's up to this row
+    step = torch.where(there, s.tokens[rows], 0)
+    text = torch.cat([s.history, step], dim=1)
+    at = torch.arange(text.shape[1], device=DEV)
+    i = torch.arange(most, device=DEV)
+    end = s.lengths.long()[:, None] + i + 1
+    place = torch.where(at < s.pitch, at, s.lengths.long()[:, None] + at - s.pitch)[:, None, :]
+    seen = torch.where(at < s.pitch, at < s.lengths.long()[:, None, None], at - s.pitch <= i[:, None])
+    if case["window"]:
+        seen = seen & (place >= end[:, :, None] - case["window"])
+    counts = torch.zeros(case["sequences"], most, vocab, dtype=torch.float32, device=DEV)
+    counts.scatter_add_(2, text[:, None, :].expand(-1, most, -1), seen.float())
+    counts = counts[there]
+    rep, freq, pres = (t[:, None].expand(-1, most)[there][:, None] for t in s.penalties.unbind(1))
+    x = s.logits.float()
+    y = torch.where(x > 0, x / rep, x * rep) - counts * freq - pres
+    x = torch.where(counts > 0, y, x)
+    if s.bias is not None:
+        x = x + s.bias
+    if s.masks is not None:
+        token = torch.arange(vocab, device=DEV)
+        allowed = (s.masks[:, token // 32] >> (token % 32).to(torch.int32)) & 1
+        x = torch.where((s.mask_of[:, None] < 0) | (allowed[s.mask_of.clamp_min(0).long()] != 0), x, -math.inf)
+    return x.to(s.logits.dtype)
+
+
+def _kv8_planes(s, case):
+    """Key codes [pages][kv_heads][page][head], value codes [pages][kv_heads][head][page], maxima [pages][kv_heads]."""
+    kv, page, head = case["kv_heads"], case["page"], case["head"]
+    codes = s.pages * kv * page * head
+    keys = s.storage[:codes].view(torch.int8).view(s.pages, kv, page, head)
+    values = s.storage[codes:2 * codes].view(torch.int8).view(s.pages, kv, head, page)
+    maxima = s.storage[2 * codes:].view(torch.float32).view(2, s.pages, kv)
+    return keys, values, maxima[0], maxima[1]
+
+
+def _cached(s, case, ids):
+    """Keys and values [...][kv_heads][tokens][head] of the tokens in pages ids [...][pages]."""
+    keys, values, key_max, value_max = _kv8_planes(s, case)
+    k = (keys[ids].float() * (key_max[ids] / 127.0)[..., None, None]).transpose(-4, -3).flatten(-3, -2)
+    v = (values[ids].float() * (value_max[ids] / 127.0)[..., None, None]).transpose(-4, -3).transpose(-2, -1).flatten(-3, -2)
+    return k, v
+
+
+def _run_shared(s, case):
+    page, kv, head, heads, most = case["page"], case["kv_heads"], case["head"], case["heads"], s.most
+    group = heads // kv
+    rows, there = _padded(s.row_starts, most)
+    q = s.q[:, :, 0].float()[rows] * s.scale                        # [n][most][heads][head]
+    q = q.unflatten(2, (kv, group)).permute(0, 2, 3, 1, 4).flatten(2, 3)  # [n][kv][group * most][head]
+    bounds, shared = s.host[0], s.host[1]
+    out = []
+    for a, b, tokens in zip(bounds, bounds[1:], shared):
+        # the shared tokens once, for the rows of every sequence
+        k, v = _cached(s, case, s.tables[a, :tokens // page].long())
+        one = q[a:b].transpose(0, 1).flatten(1, 2).contiguous()
+        first = torch.matmul(one, k.transpose(1, 2).contiguous()).unflatten(1, (b - a, -1)).transpose(0, 1)
+        own_k, own_v = _cached(s, case, s.tables[a:b, tokens // page:].long().clamp_min(0))
+        last = torch.matmul(q[a:b], own_k.transpose(2, 3).contiguous()).unflatten(2, (group, most))
+        position = s.lengths[a:b].long()[:, None] - tokens + torch.arange(most, device=DEV)
+        seen = torch.arange(last.shape[-1], device=DEV) <= position[:, None, None, :, None]
+        last = torch.where(seen, last, -math.inf).flatten(2, 3)
+        top = torch.maximum(first.amax(dim=-1, keepdim=True), last.amax(dim=-1, keepdim=True))
+        first, last = torch.exp(first - top), torch.exp(last - top)
+        total = first.sum(dim=-1, keepdim=True) + last.sum(dim=-1, keepdim=True)
+        y = torch.matmul(first.transpose(0, 1).flatten(1, 2), v).unflatten(1, (b - a, -1)).transpose(0, 1)
+        out.append((y + torch.matmul(last, own_v)) / total)
+    out = torch.cat(out).unflatten(2, (group, most)).permute(0, 3, 1, 2, 4).flatten(2, 3)[there]
+    if case["gate"]:
+        out = out / (1.0 + torch.exp(-s.q[:, :, 1].float()))
+    return out.to(s.q.dtype)
+
+
+# -------------------------------------------------------------------- work
+def work(case):
+    kind, size = case["kind"], {"f32": 4, "f16": 2, "bf16": 2}[case["dtype"]]
+    rows = _rows_of(case) if kind != "norm" else [case["rows"]]
+    total = sum(rows)
+    if kind == "gdn":
+        kh, vh, d, p, taps = case["key_heads"], case["value_heads"], case["head"], case["pending"], case["kernel"]
+        channels = (2 * kh + vh) * d
+        waiting = sum(r for r in rows if r <= p)
+        floats = 2 * case["sequences"] * vh * d * d + channels * (2 * case["sequences"] * (taps - 1) + waiting + taps) + \
+            waiting * ((kh + vh) * d + vh)
+        return {"bytes": total * size * (channels + vh * d + 2 * vh) + 4 * floats, "flops": total * vh * d * d * 7}
+    if kind == "norm":
+        values = total * case["width"]
+        arrays = {"residual": 3, "gated": 2, "product": 2}[case["use"]]
+        # tokens written, read again, their values written
+        return {"bytes": values * (arrays * size + 2 * 1.125 + 4), "flops": 8 * values}
+    if kind == "logits":
+        n = total * case["vocab"]
+        text = 8 * sum(min(l, case["window"] or l) for l in _spread(case["history"], case["sequences"]))
+        return {"bytes": 2 * n * size + text + (4 * case["vocab"] if case["bias"] else 0) + (3 * case["vocab"] // 8 if case["mask"] else 0),
+                "flops": 4 * n}
+    groups, n, page = case["groups"], case["sequences"], case["page"]
+    shared = [max(1, case["shared"] // (i + 1) // page) * page for i in range(groups)]
+    bounds = [n * i // groups for i in range(groups + 1)]
+    tokens = _spread(case["tokens"], n)
+    q, width = case["heads"] * case["head"], case["kv_heads"] * case["head"]
+    pairs = sum(rows[i] * (shared[g] + tokens[i]) for g in range(groups) for i in range(bounds[g], bounds[g + 1]))
+    return {"bytes": 2 * width * (sum(shared) + sum(t + r for t, r in zip(tokens, rows))) + total * q * size * (3 if case["gate"] else 2),
+            "flops": 4 * pairs * q}
+
+
+# ------------------------------------------------------------------- exact
+def exact(case, seed):
+    """The results from the definitions in 64 bits, token by token, row by row or head by head."""
+    return globals()["_exact_" + case["kind"]](prepare(case, seed), case)
+
+
+def _exact_gdn(s, case):
+    kh, vh, d, p, taps = case["key_heads"], case["value_heads"], case["head"], case["pending"], case["kernel"]
+    planes = _gdn_planes(s, case)
+    state, window, keys, updates, decays = (t.double() for t in planes[:5])
+    counts, bounds, standing, slots = planes[5].tolist(), s.row_starts.tolist(), s.standing.tolist(), s.slot.tolist()
+    qkv, alpha, beta, conv = s.qkv.double(), s.gates[0].double(), s.gates[1].double(), s.conv.double()
+    out = torch.empty(s.total, vh, d, dtype=torch.float64, device=DEV)
+    for seq, slot in enumerate(slots):
+        first, end = bounds[seq], bounds[seq + 1]
+        stands = max(0, min(standing[seq], counts[slot]))
+        S, seen = state[slot].clone(), window[slot, stands:stands + taps - 1].clone()
+        if standing[seq] < 0:
+            S, seen = torch.zeros_like(S), torch.zeros_like(seen)
+        for i in range(stands):
+            k = keys[slot, i].repeat_interleave(vh // kh, dim=0)
+            S = decays[slot, i][:, None, None] * S + updates[slot, i][:, :, None] * k[:, None, :]
+        waits = end - first <= p
+        if waits:
+            state[slot] = S
+        inputs = torch.cat([seen, qkv[first:end]])
+        for row in range(first, end):
+            u = (inputs[row - first:row - first + taps] * conv.t()).sum(dim=0)
+            u = u * torch.sigmoid(u)
+            q, k, v = u[:kh * d].view(kh, d), u[kh * d:2 * kh * d].view(kh, d), u[2 * kh * d:].view(vh, d)
+            q, k = ((t / t.norm(dim=1, keepdim=True).clamp_min(EPS)) for t in (q, k))
+            log = torch.exp(s.ssm_a.double() * torch.nn.functional.softplus(alpha[row] + s.ssm_dt.double(), threshold=40.0))
+            if waits:
+                keys[slot, row - first], decays[slot, row - first] = k, log
+            q, k = q.repeat_interleave(vh // kh, dim=0) / math.sqrt(d), k.repeat_interleave(vh // kh, dim=0)
+            S = S * log[:, None, None]
+            delta = torch.sigmoid(beta[row])[:, None] * (v - (S * k[:, None, :]).sum(dim=2))
+            S = S + delta[:, :, None] * k[:, None, :]
+            out[row] = (S * q[:, None, :]).sum(dim=2)
+            if waits:
+                updates[slot, row - first] = delta
+        if waits:
+            window[slot, :taps - 1 + end - first] = inputs
+        else:
+            state[slot], window[slot, :taps - 1] = S, inputs[end - first:]
+    names = ("states", "inputs", "keys", "updates", "decays")
+    found = {name: t for name, t in zip(names, (state, window, keys, updates, decays)) if t.numel()}
+    return {**found, "counts": None, "out": out}
+
+
+def _exact_norm(s, case):
+    h = s.x if s.residual is None else (s.x.double() + s.residual.double()).to(s.x.dtype)
+    y = h.double()
+    if s.weight is not None:
+        parts = y.view(-1, s.group)
+        y = (parts / parts.square().mean(dim=1, keepdim=True).add(EPS).sqrt() * s.weight.double()).view(y.shape)
+    if s.gate is not None:
+        y = y * s.gate.double() * torch.sigmoid(s.gate.double())
+    b = y.view(-1, 32)
+    top = b.abs().max(dim=1, keepdim=True).values
+    codes = torch.round((b * 127.0 / top.clamp_min(1e-300)).float()).double()
+    values = (codes * (top / 127.0).float().half().double()).view(y.shape)
+    return {"values": values} if s.residual is None else {"values": values, "sum": s.x.double() + s.residual.double()}
+
+
+def _exact_logits(s, case):
+    vocab, bounds, lengths = case["vocab"], s.row_starts.tolist(), s.lengths.tolist()
+    out = s.logits.double()
+    for seq in range(case["sequences"]):
+        rep, freq, pres = (float(x) for x in s.penalties[seq])
+        for row in range(bounds[seq], bounds[seq + 1]):
+            text = torch.cat([s.history[seq, :lengths[seq]], s.tokens[bounds[seq]:row + 1]])
+            text = text[-case["window"]:] if case["window"] else text
+            n = torch.bincount(text, minlength=vocab).double()
+            x = out[row]
+            x = torch.where(n > 0, torch.where(x > 0, x / rep, x * rep) - freq * n - pres * (n > 0), x)
+            if s.bias is not None:
+                x = x + s.bias.double()
+            if s.masks is not None and int(s.mask_of[row]) >= 0:
+                bits = s.masks[int(s.mask_of[row])].long()[:, None] >> torch.arange(32, device=DEV)
+                x = x.masked_fill((bits & 1).view(-1)[:vocab] == 0, -math.inf)
+            out[row] = x
+    return out
+
+
+def _exact_shared(s, case):
+    page, kv, head, heads = case["page"], case["kv_heads"], case["head"], case["heads"]
+    keys, values, key_max, value_max = _kv8_planes(s, case)
+    out = torch.empty(s.total, heads, head, dtype=torch.float64, device=DEV)
+    start = 0
+    for seq, (length, rows) in enumerate(zip(s.host[2], s.host[3])):
+        ids = s.tables[seq, :-(-(length + rows) // page)].long()
+        mask = torch.arange(length + rows, device=DEV) <= length + torch.arange(rows, device=DEV)[:, None]
+        for g in range(kv):
+            k = (keys[ids, g].double() * key_max[ids, g].double()[:, None, None] / 127.0).reshape(-1, head)[:length + rows]
+            v = (values[ids, g].double() * value_max[ids, g].double()[:, None, None] / 127.0).transpose(1, 2)
+            v = v.reshape(-1, head)[:length + rows]
+            for h in range(g * (heads // kv), (g + 1) * (heads // kv)):
+                scores = (s.q[start:start + rows, h, 0].double() @ k.t().contiguous()) * s.scale
+                out[start:start + rows, h] = torch.softmax(scores.masked_fill(~mask, -math.inf), dim=-1) @ v
+        start += rows
+    if case["gate"]:
+        out = out * torch.sigmoid(s.q[:, :, 1].double())
+    return out
