@@ -144,10 +144,19 @@ _SIGNATURES = {
     "fortai_hip_kv8_pages_length": [_vp, _i],
     "fortai_hip_kv8_pages_free_count": [_vp],
     "fortai_hip_kv8_pages_tables": [_vp, _vp, _i, _vp, _i],
+    "fortai_hip_norm_tokens_device": [_vp, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _f, _vp, _i64, _i, _i, _vp, _i64,
+                                      _vp],
+    "fortai_hip_q8_tokens_read_device": [_vp, _i, _vp, _i, _i, _vp, _i64],
+    "fortai_hip_logits_adjust_device": [_vp, _i, _vp, _i64, _i, _i, _i, _vp, _vp, _vp, _i64],
+    "fortai_hip_gdn_bytes": [_i, _i, _i, _i, _i, _i, _i],
+    "fortai_hip_gdn_create": [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vpp],
+    "fortai_hip_gdn_destroy": [_vp],
+    "fortai_hip_gdn_run_device": [_vp, _i, _vp, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _vp, _i64],
+    "fortai_hip_gdn_copy_slots": [_vp, _vp, _vp, _i],
 }
 _RESTYPE = {"fortai_hip_q8_last_error": C.c_char_p, "fortai_hip_q8_tokens_bytes": C.c_size_t,
             "fortai_hip_q8_pack_bytes": C.c_size_t, "fortai_hip_kv8_bytes": C.c_size_t,
-            "fortai_hip_kv8_pages_length": C.c_int64}
+            "fortai_hip_kv8_pages_length": C.c_int64, "fortai_hip_gdn_bytes": C.c_size_t}
 
 _lib: Optional[C.CDLL] = None
 
@@ -204,6 +213,14 @@ def _ptr(a: np.ndarray) -> C.c_void_p:
     return C.c_void_p(a.ctypes.data)
 
 
+class LogitRules(C.Structure):
+    """fortai_hip_logit_rules: what Context.adjust_logits applies."""
+
+    _fields_ = [("window", _i), ("mask_count", _i), ("penalties", _vp), ("tokens", _vp), ("history", _vp),
+                ("history_lengths", _vp), ("bias", _vp), ("masks", _vp), ("mask_of", _vp), ("history_pitch", _i64),
+                ("bias_pitch", _i64), ("mask_pitch", _i64)]
+
+
 class Context:
     """A device context: stream, device position/token, scratch (fortai_cuda_q8_context)."""
 
@@ -256,6 +273,37 @@ class Context:
 
     def graph_launch(self) -> None:
         self.call("fortai_hip_q8_context_graph_launch", self.h)
+
+    # ---- around a step's products (device arrays as addresses or DeviceBuffers; dense unless pitches are given)
+    def norm_tokens(self, x, rows: int, width: int, dtype: str = "f32", residual=None, sum=None, norm=None,
+                    group: Optional[int] = None, eps: float = 1e-6, gate=None, output=None, tokens=None,
+                    x_pitch: Optional[int] = None, residual_pitch: Optional[int] = None, sum_pitch: Optional[int] = None,
+                    gate_pitch: Optional[int] = None, output_pitch: Optional[int] = None) -> None:
+        """x [rows][width] (+ residual -> sum), RMS norm over groups, gate -> output and 8-bit tokens
+        (fortai_hip_norm_tokens_device)."""
+        pitch = lambda p: width if p is None else p
+        self.check(self.lib.fortai_hip_norm_tokens_device(
+            self.h, DTYPES[dtype], _dev(x), pitch(x_pitch), _dev(residual), pitch(residual_pitch), _dev(sum), pitch(sum_pitch),
+            _dev(norm), width if group is None else group, eps, _dev(gate), pitch(gate_pitch), rows, width, _dev(output),
+            pitch(output_pitch), _dev(tokens)), "fortai_hip_norm_tokens_device")
+
+    def tokens_read(self, tokens, rows: int, width: int, out, dtype: str = "f32", out_pitch: Optional[int] = None) -> None:
+        """The values of a buffer of 8-bit tokens as rows."""
+        self.check(self.lib.fortai_hip_q8_tokens_read_device(self.h, DTYPES[dtype], _dev(tokens), rows, width, _dev(out),
+                                                             width if out_pitch is None else out_pitch),
+                   "fortai_hip_q8_tokens_read_device")
+
+    def adjust_logits(self, logits, vocab: int, out, row_starts, sequences: int, rows: int, dtype: str = "f32", tokens=None,
+                      history=None, history_pitch: int = 0, history_lengths=None, window: int = 0, penalties=None, bias=None,
+                      bias_pitch: int = 0, masks=None, mask_count: int = 0, mask_pitch: Optional[int] = None, mask_of=None,
+                      pitch: Optional[int] = None, out_pitch: Optional[int] = None) -> None:
+        """Penalties for repeated tokens, biases and masks on logits [rows][vocab] (fortai_hip_logits_adjust_device)."""
+        rules = LogitRules(window, mask_count, _dev(penalties), _dev(tokens), _dev(history), _dev(history_lengths), _dev(bias),
+                           _dev(masks), _dev(mask_of), history_pitch, bias_pitch,
+                           (vocab + 31) // 32 if mask_pitch is None else mask_pitch)
+        self.check(self.lib.fortai_hip_logits_adjust_device(
+            self.h, DTYPES[dtype], _dev(logits), vocab if pitch is None else pitch, rows, vocab, sequences, _dev(row_starts),
+            C.addressof(rules), _dev(out), vocab if out_pitch is None else out_pitch), "fortai_hip_logits_adjust_device")
 
     # ---- device buffers
     def alloc(self, nbytes: int) -> "DeviceBuffer":
@@ -792,4 +840,58 @@ class Verifier:
     def free(self) -> None:
         if self.h:
             self.ctx.lib.fortai_hip_verifier_destroy(self.h)
+            self.h = None
+
+
+class GdnBatch(C.Structure):
+    """Which rows of a call belong to which sequence, and where its state is (fortai_hip_gdn_batch): device int32
+    row_starts [sequences + 1], slots [sequences] and standing [sequences] (None: every pending row stands)."""
+
+    _fields_ = [("sequences", _i), ("rows", _i), ("max_rows", _i), ("row_starts", _vp), ("slots", _vp), ("standing", _vp)]
+
+    def __init__(self, sequences: int, rows: int, max_rows: int, row_starts, slots, standing=None):
+        super().__init__(sequences, rows, max_rows, _dev(row_starts), _dev(slots), _dev(standing))
+
+
+class GdnCache:
+    """States of the gated delta rule (fortai_hip_gdn_cache), over the caller's device storage of GdnCache.bytes()
+    bytes or over its own, for calls of up to max_rows rows."""
+
+    def __init__(self, ctx: Context, layers: int, slots: int, key_heads: int, value_heads: int, head_size: int,
+                 conv_kernel: int, pending: int, max_rows: int, storage=None, storage_bytes: int = 0):
+        self.ctx, self.slots = ctx, slots
+        self.channels, self.value_heads, self.width = (2 * key_heads + value_heads) * head_size, value_heads, value_heads * head_size
+        h = C.c_void_p()
+        ctx.call("fortai_hip_gdn_create", ctx.h, layers, slots, key_heads, value_heads, head_size, conv_kernel, pending, max_rows,
+                 _dev(storage), storage_bytes, C.byref(h))
+        self.h = h
+
+    @staticmethod
+    def bytes(layers: int, slots: int, key_heads: int, value_heads: int, head_size: int, conv_kernel: int, pending: int) -> int:
+        """Bytes of the storage (0: no such cache)."""
+        return load().fortai_hip_gdn_bytes(layers, slots, key_heads, value_heads, head_size, conv_kernel, pending)
+
+    def run(self, layer: int, batch: GdnBatch, qkv, alpha, beta, conv, ssm_a, ssm_dt, out, dtype: str = "f32",
+            eps: float = 1e-6, qkv_pitch: Optional[int] = None, alpha_pitch: Optional[int] = None,
+            beta_pitch: Optional[int] = None, out_pitch: Optional[int] = None) -> None:
+        """The batch's rows: qkv [rows][channels], alpha and beta [rows][value_heads] (dense unless pitches are given),
+        fp32 conv [channels][conv_kernel], ssm_a and ssm_dt [value_heads] -> out [rows][value_heads][head_size]."""
+        self.ctx.check(self.ctx.lib.fortai_hip_gdn_run_device(
+            self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(qkv), self.channels if qkv_pitch is None else qkv_pitch,
+            _dev(alpha), self.value_heads if alpha_pitch is None else alpha_pitch, _dev(beta),
+            self.value_heads if beta_pitch is None else beta_pitch, _dev(conv), _dev(ssm_a), _dev(ssm_dt), eps, _dev(out),
+            self.width if out_pitch is None else out_pitch), "fortai_hip_gdn_run_device")
+
+    def copy_slots(self, source, target) -> None:
+        """Slot target[i] becomes a copy of slot source[i], in every layer (host int32 arrays)."""
+        f = np.ascontiguousarray(source, dtype=np.int32)
+        t = np.ascontiguousarray(target, dtype=np.int32)
+        if f.shape != t.shape or f.ndim != 1:
+            raise ValueError("need as many source as target slots")
+        self.ctx.check(self.ctx.lib.fortai_hip_gdn_copy_slots(self.h, f.ctypes.data, t.ctypes.data, len(f)),
+                       "fortai_hip_gdn_copy_slots")
+
+    def free(self) -> None:
+        if self.h:
+            self.ctx.lib.fortai_hip_gdn_destroy(self.h)
             self.h = None

@@ -5,34 +5,12 @@
 #include "fortai_hip_context.h"
 #include "serving_checks.h"
 #include "serving_kernels.h"
+#include "serving_scope.h"
 
 #include <mutex>
 #include <new>
 
 using namespace fortai_hip;
-
-namespace {
-
-// The context's device for the length of a call; the caller's own device is
-// current again after it.
-class DeviceScope {
-public:
-    explicit DeviceScope(int device) {
-        if (hipGetDevice(&before_) != hipSuccess) before_ = device;
-        if (before_ != device) (void)hipSetDevice(device);
-        device_ = device;
-    }
-    ~DeviceScope() {
-        if (before_ != device_) (void)hipSetDevice(before_);
-    }
-    DeviceScope(const DeviceScope &) = delete;
-    DeviceScope &operator=(const DeviceScope &) = delete;
-
-private:
-    int before_ = 0, device_ = 0;
-};
-
-}  // namespace
 
 struct fortai_hip_rope {
     fortai_hip_q8_context *context = nullptr;
@@ -99,13 +77,6 @@ const char *check_batch(const fortai_hip_kv8_batch *b) {
     if (!b) return "kv8: no batch";
     return check_kv8_batch(b->sequences, b->rows, b->max_rows, b->table_pitch, b->device_row_starts, b->device_lengths,
         b->device_tables);
-}
-
-// Making a handle is no work of a graph: its copy or clearing would wait for a replay.
-const char *check_no_capture(fortai_hip_q8_context *c) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c->stream, &status) == hipSuccess && status == hipStreamCaptureStatusNone) return nullptr;
-    return "handles are created before a capture begins";
 }
 
 bool empty(const fortai_hip_kv8_batch *b) { return b->sequences == 0 || b->rows == 0 || b->max_rows == 0; }

@@ -1,0 +1,69 @@
+// What the kernels of the delta rule over rows share (gdn_rows.hip, gdn_chunks.hip).
+// Every number that comes from device memory (row starts, slots, counts) is brought
+// into range before it is used.
+#pragma once
+
+#include "fortai_hip_internal.h"
+#include "kv8_device.h"
+#include "step_kernels.h"
+
+namespace fortai_hip {
+
+// A sequence's rows [begin, begin + count), its slot (-1: none of the cache's), how
+// many of the slot's pending rows stand, and whether it begins anew.
+struct GdnSequence {
+    int begin, count, slot, stands;
+    bool begins;
+};
+
+__device__ __forceinline__ GdnSequence gdn_sequence(const GdnRowsParams &p, int seq) {
+    GdnSequence s;
+    const int32_t *starts = p.batch.starts;
+    int b = read_only(starts + seq), e = read_only(starts + seq + 1);
+    b = min(max(b, 0), p.batch.rows);
+    e = min(max(e, b), p.batch.rows);
+    s.begin = b;
+    s.count = min(e - b, p.batch.max_rows);
+    s.slot = read_only(p.batch.slots + seq);
+    if (s.slot < 0 || s.slot >= p.cache.slots) s.slot = -1;
+    const int standing = p.batch.standing ? read_only(p.batch.standing + seq) : kGdnMaxPending;
+    s.begins = standing < 0;
+    s.stands = standing;  // to be brought into [0, pending rows] by the reader of the slot's count
+    return s;
+}
+
+__device__ __forceinline__ int gdn_stands(const GdnRowsParams &p, const GdnSequence &s) {
+    const int pending = min(max(p.cache.counts[s.slot], 0), p.cache.pending);
+    return min(max(s.stands, 0), pending);
+}
+
+__device__ __forceinline__ float gdn_silu(float x) { return x / (1.0f + expf(-x)); }
+
+// ssm_a softplus(alpha + ssm_dt): the logarithm of a row's decay
+__device__ __forceinline__ float gdn_log_decay(float a, float alpha, float dt) {
+    const float x = alpha + dt;
+    return a * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+}
+
+__device__ __forceinline__ float gdn_sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// The inputs of a channel that a slot keeps, written by one thread: behind a sequence
+// of rows that wait, the taps - 1 inputs before them and theirs; otherwise the last
+// taps - 1.  In place, in ascending order: what is read lies at or behind what is written.
+template <typename E>
+__device__ __forceinline__ void gdn_keep_inputs(const GdnRowsParams &p, const GdnSequence &s, bool waits, int channel) {
+    const int channels = p.cache.channels(), before = p.cache.taps - 1;
+    float *window = p.cache.inputs + static_cast<int64_t>(s.slot) * (before + p.cache.pending) * channels + channel;
+    const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
+    const int from = waits ? 0 : s.count, kept = before + (waits ? s.count : 0);
+#pragma unroll 1
+    for (int j = 0; j < kept; ++j) {
+        const int at = from + j;
+        float v = 0.0f;
+        if (at >= before) v = static_cast<float>(x[static_cast<int64_t>(at - before) * p.qkv_row]);
+        else if (!s.begins) v = window[static_cast<int64_t>(s.stands + at) * channels];
+        window[static_cast<int64_t>(j) * channels] = v;
+    }
+}
+
+}  // namespace fortai_hip

@@ -1,0 +1,280 @@
+// The gated delta rule over a batch's rows, for sequences of few rows (decode steps
+// and drafts), and the slots' copies.
+//
+//   u = sum_i w_i x_{t - taps + 1 + i}, y = u / (1 + exp(-u))        per channel: q, k, v
+//   q = y_q / max(|y_q|, eps) / sqrt(head), k = y_k / max(|y_k|, eps)
+//   a = exp(ssm_a softplus(alpha + ssm_dt)), b = 1 / (1 + exp(-beta))
+//   d = b (v - a S k),  S = a S + d k^T,  o = S q
+//
+// Rows that wait: S is stored as it stands before them, their k, d and a beside it.
+// The next call applies those that stand while S is in registers: one read and one
+// write of S a step, whether drafts stand or not.
+//
+// Bound by memory: a step reads and writes S, 128 KiB a head of 128, for 7 operations a
+// value.  A workgroup has ROWS rows of one head's S, eight lanes a row, a lane four
+// columns of every 32: the products with k and q are sums over a lane's columns and three
+// exchanges between neighbours, and nothing of S goes through LDS.  The convolution of
+// the head's q and k, 2 head channels, is done by every workgroup of the head again
+// instead of a launch of its own.
+//
+// Who may overwrite what others read: the inputs and keys of a key head are read by all
+// its workgroups.  Each counts itself in once its reads are done, and the last one
+// writes; the slot's count likewise for the whole sequence.  Nothing that one workgroup
+// writes is read by another, so a plain count is enough.
+#include "gdn_device.h"
+
+namespace fortai_hip {
+
+namespace {
+
+template <Dtype DT, int D, int ROWS>
+__global__ __launch_bounds__(ROWS * 8) void gdn_few_kernel(const GdnRowsParams p) {
+    typedef typename Element<DT>::type E;
+    constexpr int kThreads = ROWS * 8, kWaves = kThreads / 64, kFours = D / 32, kBlocks = D / ROWS;
+    constexpr int kChannels = 2 * D + ROWS, kTurns = (kChannels + kThreads - 1) / kThreads;
+    __shared__ __align__(16) float qs[kGdnFewRows][D], ks[kGdnFewRows][D], log_k[kGdnMaxPending][D];
+    __shared__ float vs[kGdnFewRows][ROWS], log_d[kGdnMaxPending][ROWS], os[kGdnFewRows][ROWS], ds[kGdnFewRows][ROWS];
+    __shared__ float rates[kGdnFewRows], decays[kGdnFewRows], log_a[kGdnMaxPending];
+    __shared__ int last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const GdnView &c = p.cache;
+    GdnSequence s = gdn_sequence(p, blockIdx.y);
+    if (s.count == 0 || s.count > kGdnFewRows || s.slot < 0) return;
+    const int r = s.count, h = blockIdx.x / kBlocks, block = blockIdx.x % kBlocks, r0 = block * ROWS;
+    const int group = c.value_heads / c.key_heads, kh = h / group, channels = c.channels(), before = c.taps - 1;
+    const bool waits = r <= c.pending;
+
+    // this thread's row of S
+    const int local = tid >> 3, l = tid & 7;
+    f32x4_t S[kFours];
+    float *state = c.states + ((static_cast<int64_t>(s.slot) * c.value_heads + h) * D + r0 + local) * D + 4 * l;
+#pragma unroll
+    for (int f = 0; f < kFours; ++f) S[f] = *reinterpret_cast<const f32x4_t *>(state + 32 * f);
+    s.stands = gdn_stands(p, s);
+    const int stands = s.begins ? 0 : s.stands;
+
+    // the pending rows that stand
+    for (int i = 0; i < stands; ++i) {
+        const int64_t row = static_cast<int64_t>(s.slot) * c.pending + i;
+        for (int at = tid; at < D; at += kThreads) log_k[i][at] = c.keys[(row * c.key_heads + kh) * D + at];
+        if (tid < ROWS) log_d[i][tid] = c.updates[(row * c.value_heads + h) * D + r0 + tid];
+        if (tid == 0) log_a[i] = c.decays[row * c.value_heads + h];
+    }
+    // the rows' gates
+    if (tid < r) {
+        const int64_t row = s.begin + tid;
+        const float alpha = static_cast<float>(static_cast<const E *>(p.alpha)[row * p.alpha_row + h]);
+        const float beta = static_cast<float>(static_cast<const E *>(p.beta)[row * p.beta_row + h]);
+        rates[tid] = gdn_sigmoid(beta);
+        decays[tid] = expf(gdn_log_decay(p.ssm_a[h], alpha, p.ssm_dt[h]));
+    }
+    // the convolution of this workgroup's channels
+    const auto channel_of = [&](int at) {
+        return at < D ? kh * D + at : at < 2 * D ? (c.key_heads + kh) * D + at - D : (2 * c.key_heads + h) * D + r0 + at - 2 * D;
+    };
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+        const int at = turn * kThreads + tid;
+        if (at >= kChannels) break;
+        const int channel = channel_of(at);
+        const float *window = c.inputs + static_cast<int64_t>(s.slot) * (before + c.pending) * channels + channel;
+        const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
+        // aligned to the newest: seen[kGdnMaxTaps - 1] is the row's own
+        float seen[kGdnMaxTaps], w[kGdnMaxTaps];
+        const int first = kGdnMaxTaps - c.taps;
+#pragma unroll
+        for (int j = 0; j < kGdnMaxTaps; ++j) {
+            seen[j] = w[j] = 0.0f;
+            if (j >= first) {
+                w[j] = p.conv[static_cast<int64_t>(channel) * c.taps + j - first];
+                if (j < kGdnMaxTaps - 1 && !s.begins) seen[j] = window[static_cast<int64_t>(stands + j - first) * channels];
+            }
+        }
+        float *to = at < D ? &qs[0][at] : at < 2 * D ? &ks[0][at - D] : &vs[0][at - 2 * D];
+        const int pitch = at < 2 * D ? D : ROWS;
+#pragma unroll 1
+        for (int i = 0; i < r; ++i) {
+            seen[kGdnMaxTaps - 1] = static_cast<float>(x[i * p.qkv_row]);
+            float u = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kGdnMaxTaps; ++j)
+                if (j >= first) u = __builtin_fmaf(w[j], seen[j], u);
+            to[i * pitch] = gdn_silu(u);
+#pragma unroll
+            for (int j = 0; j + 1 < kGdnMaxTaps; ++j) seen[j] = seen[j + 1];
+        }
+    }
+    __syncthreads();
+    // every read of what others may overwrite has its data
+    int arrived = 0;
+    int *arrivals = p.arrivals + static_cast<int64_t>(blockIdx.y) * (c.key_heads + 1);
+    if (tid == 0) arrived = __hip_atomic_fetch_add(arrivals + kh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // norms, a row's q or k a wave at a time
+    for (int i = wave; i < 2 * r; i += kWaves) {
+        float *v = i < r ? qs[i] : ks[i - r];
+        float x[D / 64], sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            x[k] = v[64 * k + lane];
+            sum += x[k] * x[k];
+        }
+        sum = wave_sum(sum);
+        float inverse = 1.0f / fmaxf(sqrtf(sum), p.eps);
+        if (i < r) inverse *= 1.0f / sqrtf(static_cast<float>(D));
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) v[64 * k + lane] = x[k] * inverse;
+    }
+    __syncthreads();
+
+    if (s.begins) {
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) S[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll 1
+    for (int i = 0; i < stands; ++i) {
+        const float a = log_a[i], d = log_d[i][local];
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const f32x4_t k = *reinterpret_cast<const f32x4_t *>(&log_k[i][32 * f + 4 * l]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[f][e] = __builtin_fmaf(d, k[e], S[f][e] * a);
+        }
+    }
+    if (waits && (stands > 0 || s.begins)) {
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) *reinterpret_cast<f32x4_t *>(state + 32 * f) = S[f];
+    }
+#pragma unroll 1
+    for (int i = 0; i < r; ++i) {
+        const float a = decays[i];
+        f32x4_t k[kFours];
+        float asked = 0.0f;
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            k[f] = *reinterpret_cast<const f32x4_t *>(&ks[i][32 * f + 4 * l]);
+            S[f] *= a;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asked = __builtin_fmaf(S[f][e], k[f][e], asked);
+        }
+        asked = group_sum_up(asked, 8);
+        const float d = rates[i] * (vs[i][local] - asked);
+        float o = 0.0f;
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const f32x4_t q = *reinterpret_cast<const f32x4_t *>(&qs[i][32 * f + 4 * l]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                S[f][e] = __builtin_fmaf(d, k[f][e], S[f][e]);
+                o = __builtin_fmaf(S[f][e], q[e], o);
+            }
+        }
+        o = group_sum_up(o, 8);
+        if (l == 0) {
+            os[i][local] = o;
+            ds[i][local] = d;
+        }
+    }
+    if (!waits) {
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) *reinterpret_cast<f32x4_t *>(state + 32 * f) = S[f];
+    }
+    if (tid == 0) {
+        last = arrived == group * kBlocks - 1;
+        if (last) __hip_atomic_store(arrivals + kh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    for (int at = tid; at < r * ROWS; at += kThreads) {
+        const int i = at / ROWS, local_row = at % ROWS;
+        static_cast<E *>(p.out)[(s.begin + i) * p.out_row + h * D + r0 + local_row] = static_cast<E>(os[i][local_row]);
+        if (waits)
+            c.updates[((static_cast<int64_t>(s.slot) * c.pending + i) * c.value_heads + h) * D + r0 + local_row] = ds[i][local_row];
+    }
+    // this workgroup's own channels, and as the last of its key head the ones it shares
+    if (tid < ROWS) gdn_keep_inputs<E>(p, s, waits, channel_of(2 * D + tid));
+    if (!last) return;
+    for (int at = tid; at < 2 * D; at += kThreads) gdn_keep_inputs<E>(p, s, waits, channel_of(at));
+    if (waits) {
+        for (int at = tid; at < r * D; at += kThreads)
+            c.keys[((static_cast<int64_t>(s.slot) * c.pending + at / D) * c.key_heads + kh) * D + at % D] = ks[at / D][at % D];
+        for (int at = tid; at < r * group; at += kThreads) {
+            const int i = at / group, head = kh * group + at % group;
+            const float alpha = static_cast<float>(static_cast<const E *>(p.alpha)[(s.begin + i) * p.alpha_row + head]);
+            c.decays[(static_cast<int64_t>(s.slot) * c.pending + i) * c.value_heads + head] =
+                expf(gdn_log_decay(p.ssm_a[head], alpha, p.ssm_dt[head]));
+        }
+    }
+    if (tid == 0) {
+        int *heads = arrivals + c.key_heads;
+        if (__hip_atomic_fetch_add(heads, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == c.key_heads - 1) {
+            __hip_atomic_store(heads, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            c.counts[s.slot] = waits ? r : 0;
+        }
+    }
+}
+
+struct SlotPairs {
+    int32_t from[kKv8PairsPerLaunch], to[kKv8PairsPerLaunch];
+};
+
+// planes of `count` floats a slot, one behind the other, [layers][slots][count] each
+__global__ __launch_bounds__(256) void gdn_copy_slots_kernel(float *plane, int64_t count, int slots, SlotPairs pairs) {
+    const int64_t layer = static_cast<int64_t>(blockIdx.z) * slots;
+    const float *from = plane + (layer + pairs.from[blockIdx.y]) * count;
+    float *to = plane + (layer + pairs.to[blockIdx.y]) * count;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) to[i] = from[i];
+}
+
+template <Dtype DT, int D>
+hipError_t few_typed(const GdnRowsParams &p, hipStream_t stream) {
+    const GdnView &c = p.cache;
+    // 32 rows of S a workgroup where that leaves two workgroups a CU: fewer of them do
+    // the same convolution
+    if (static_cast<int64_t>(p.batch.sequences) * c.value_heads * (D / 32) >= 512)
+        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 32>), dim3(c.value_heads * (D / 32), p.batch.sequences), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 16>), dim3(c.value_heads * (D / 16), p.batch.sequences), dim3(128), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <Dtype DT>
+hipError_t few_head(const GdnRowsParams &p, hipStream_t stream) {
+    return p.cache.head == 64 ? few_typed<DT, 64>(p, stream) : few_typed<DT, 128>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_gdn_few(const GdnRowsParams &p, Dtype dtype, hipStream_t stream) {
+    if (dtype == Dtype::F32) return few_head<Dtype::F32>(p, stream);
+    if (dtype == Dtype::F16) return few_head<Dtype::F16>(p, stream);
+    return few_head<Dtype::BF16>(p, stream);
+}
+
+hipError_t launch_gdn_copy_slots(const GdnView &c, int layers, const int32_t *from, const int32_t *to, int count, hipStream_t stream) {
+    const int64_t d = c.head;
+    struct Plane {
+        float *at;
+        int64_t count;
+    } planes[6] = {{c.states, c.value_heads * d * d}, {c.inputs, static_cast<int64_t>(c.taps - 1 + c.pending) * c.channels()},
+        {c.keys, c.pending * c.key_heads * d}, {c.updates, c.pending * c.value_heads * d},
+        {c.decays, static_cast<int64_t>(c.pending) * c.value_heads}, {reinterpret_cast<float *>(c.counts), 1}};
+    for (int at = 0; at < count; at += kKv8PairsPerLaunch) {
+        const int n = count - at < kKv8PairsPerLaunch ? count - at : kKv8PairsPerLaunch;
+        SlotPairs pairs = {};
+        for (int i = 0; i < n; ++i) {
+            pairs.from[i] = from[at + i];
+            pairs.to[i] = to[at + i];
+        }
+        for (const Plane &plane : planes) {
+            if (plane.count == 0) continue;
+            const int64_t wanted = (plane.count + 1023) / 1024;
+            const dim3 grid(static_cast<unsigned>(wanted < 1024 ? wanted : 1024), n, layers);
+            hipLaunchKernelGGL(gdn_copy_slots_kernel, grid, dim3(256), 0, stream, plane.at, plane.count, c.slots, pairs);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
+}
+
+}  // namespace fortai_hip

@@ -1,0 +1,156 @@
+// Rules on the logits of a step's rows, before they are verified or drawn from.
+//
+//   n = how often the token is among the text's last `window` tokens
+//   n > 0:  x = x > 0 ? x / repetition : x * repetition;  x -= n frequency + presence
+//   x += bias;  tokens that the row's mask leaves out: -infinity
+//
+// The text of a row is its sequence's history and the step's tokens up to the row.
+// A workgroup has a chunk of the vocabulary and a run of one sequence's rows: it
+// counts the chunk's tokens in the text once, in LDS by their place in the chunk (no
+// hashing, and integer sums, whose order does not matter), and from row to row adds
+// the one token that comes and takes away the one that leaves the window, while the
+// next row's logits are on their way.
+#include "fortai_hip_internal.h"
+#include "kv8_device.h"
+#include "step_kernels.h"
+
+namespace fortai_hip {
+
+namespace {
+
+constexpr int kRuleThreads = 256;
+
+template <Dtype DT, bool VEC, int CHUNK>
+__global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p) {
+    typedef typename Element<DT>::type E;
+    constexpr int kFours = CHUNK / (4 * kRuleThreads);
+    __shared__ __align__(16) int counts[CHUNK];
+    const int seq = blockIdx.y, first = blockIdx.x * CHUNK, thread = threadIdx.x;
+    int begin = read_only(p.row_starts + seq), end = read_only(p.row_starts + seq + 1);
+    begin = min(max(begin, 0), p.rows);
+    end = min(max(end, begin), p.rows);
+    // this workgroup's share of the rows
+    const int parts = gridDim.z, part = blockIdx.z, share = (end - begin + parts - 1) / parts;
+    const int row0 = begin + part * share, row1 = min(row0 + share, end);
+    if (row0 >= row1) return;
+
+    f32x4_t x[kFours];
+    const auto load_row = [&](int row) {
+        const E *at = static_cast<const E *>(p.logits) + static_cast<int64_t>(row) * p.logits_row + first;
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const int i = 4 * (f * kRuleThreads + thread);
+            if (VEC ? first + i < p.vocab : first + i + 3 < p.vocab) {
+                x[f] = load4<DT, VEC>(at + i);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[f][k] = first + i + k < p.vocab ? static_cast<float>(at[i + k]) : 0.0f;
+            }
+        }
+    };
+    load_row(row0);
+
+    const bool counting = p.penalties != nullptr;
+    float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
+    int64_t length = 0;  // of the history
+    const int64_t *history = nullptr;
+    const auto token_at = [&](int64_t place) { return place < length ? history[place] : p.tokens[begin + (place - length)]; };
+    const auto count = [&](int64_t token, int by) {
+        const int64_t at = token - first;
+        if (at >= 0 && at < CHUNK && token < p.vocab) atomicAdd(&counts[at], by);
+    };
+    const auto text_end = [&](int row) { return length + (p.tokens ? row - begin + 1 : 0); };
+    if (counting) {
+        repetition = p.penalties[3 * seq];
+        frequency = p.penalties[3 * seq + 1];
+        presence = p.penalties[3 * seq + 2];
+        if (p.history) {
+            length = min(max(static_cast<int64_t>(p.history_lengths[seq]), static_cast<int64_t>(0)), p.history_pitch);
+            history = p.history + seq * p.history_pitch;
+        }
+        for (int i = thread; i < CHUNK; i += kRuleThreads) counts[i] = 0;
+        lds_barrier();
+        const int64_t last = text_end(row0), from = p.window > 0 && last > p.window ? last - p.window : 0;
+        for (int64_t place = from + thread; place < last; place += kRuleThreads) count(token_at(place), 1);
+        lds_barrier();
+    }
+
+#pragma unroll 1
+    for (int row = row0; row < row1; ++row) {
+        f32x4_t y[kFours];
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) y[f] = x[f];
+        if (row + 1 < row1) load_row(row + 1);
+        const int mask = p.masks ? p.mask_of[row] : -1;
+        const uint32_t *allowed = mask >= 0 && mask < p.mask_count ? p.masks + mask * p.mask_pitch : nullptr;
+        const float *bias = p.bias ? p.bias + seq * p.bias_pitch + first : nullptr;
+        E *to = static_cast<E *>(p.out) + static_cast<int64_t>(row) * p.out_row + first;
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const int i = 4 * (f * kRuleThreads + thread);
+            if (first + i >= p.vocab) continue;
+            if (counting) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int n = counts[i + k];
+                    const float seen = (y[f][k] > 0.0f ? y[f][k] / repetition : y[f][k] * repetition) - static_cast<float>(n) * frequency - presence;
+                    y[f][k] = n > 0 ? seen : y[f][k];
+                }
+            }
+            const bool four = VEC || first + i + 3 < p.vocab;
+            if (bias) {
+                if (VEC) {
+                    y[f] += *reinterpret_cast<const f32x4_t *>(bias + i);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (first + i + k < p.vocab) y[f][k] += bias[i + k];
+                }
+            }
+            if (allowed) {
+                const uint32_t bits = allowed[(first + i) >> 5] >> ((first + i) & 31);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (!(bits >> k & 1u)) y[f][k] = -__builtin_inff();
+            }
+            if (four) {
+                store4<DT, VEC>(to + i, y[f]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (first + i + k < p.vocab) to[i + k] = static_cast<E>(y[f][k]);
+            }
+        }
+        if (counting && p.tokens && row + 1 < row1) {
+            lds_barrier();
+            if (thread == 0) {
+                const int64_t last = text_end(row + 1);
+                count(token_at(last - 1), 1);
+                if (p.window > 0 && last > p.window) count(token_at(last - 1 - p.window), -1);
+            }
+            lds_barrier();
+        }
+    }
+}
+
+template <Dtype DT, bool VEC>
+hipError_t rules_typed(const LogitRulesParams &p, hipStream_t stream) {
+    // rows of a sequence stay together up to eight: the text is counted once for them
+    const int average = (p.rows + p.sequences - 1) / p.sequences, parts = (average + 7) / 8;
+    const int64_t groups = static_cast<int64_t>(p.sequences) * parts;
+    if (groups * ((p.vocab + 4095) / 4096) >= 256)
+        hipLaunchKernelGGL((logit_rules_kernel<DT, VEC, 4096>), dim3((p.vocab + 4095) / 4096, p.sequences, parts), dim3(kRuleThreads), 0, stream, p);
+    else
+        hipLaunchKernelGGL((logit_rules_kernel<DT, VEC, 1024>), dim3((p.vocab + 1023) / 1024, p.sequences, parts), dim3(kRuleThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_logit_rules(const LogitRulesParams &p, Dtype dtype, bool vec, hipStream_t stream) {
+    if (dtype == Dtype::F32) return vec ? rules_typed<Dtype::F32, true>(p, stream) : rules_typed<Dtype::F32, false>(p, stream);
+    if (dtype == Dtype::F16) return vec ? rules_typed<Dtype::F16, true>(p, stream) : rules_typed<Dtype::F16, false>(p, stream);
+    return vec ? rules_typed<Dtype::BF16, true>(p, stream) : rules_typed<Dtype::BF16, false>(p, stream);
+}
+
+}  // namespace fortai_hip

@@ -41,6 +41,7 @@ typedef struct fortai_hip_rope fortai_hip_rope;                        /* [exten
 typedef struct fortai_hip_kv8_cache fortai_hip_kv8_cache;              /* [extension] */
 typedef struct fortai_hip_kv8_pages fortai_hip_kv8_pages;              /* [extension] */
 typedef struct fortai_hip_verifier fortai_hip_verifier;                /* [extension] */
+typedef struct fortai_hip_gdn_cache fortai_hip_gdn_cache;              /* [extension] */
 
 enum {
     FORTAI_HIP_OK = 0,
@@ -649,6 +650,120 @@ int fortai_hip_verify_drafts_device(fortai_hip_verifier *verifier, int dtype,
     int64_t draft_pitch, const void *device_tokens, const void *device_uniforms,
     const void *device_temperatures, int sequences, const void *device_row_starts, int rows,
     void *device_emitted, void *device_accepted, void *device_logprobs);
+
+/* ---- around a step's products: 8-bit tokens, the delta rule's rows, logits ----
+ *
+ * Norm into 8-bit tokens, what fortai_hip_q8_mmq_device and _exact_device take.
+ *   h = x + residual (NULL: x), rounded to dtype; stored at device_sum (may be NULL)
+ *   y = h w / sqrt(mean(h^2) + epsilon) over groups of `group` values (the whole
+ *       width, or 32, 64, 128 or 256 that divide it), weights fp32 [group];
+ *       device_norm NULL: y = h
+ *   y *= z / (1 + exp(-z)) with z of device_gate (NULL: no gate), at its own pitch:
+ *       with a norm of heads, a delta rule's gated output; without, gate and up
+ * to device_output (y in dtype, may be NULL) and device_tokens (may be NULL, not
+ * both): fortai_hip_q8_tokens_bytes(rows, width) bytes, aligned to 16, laid out as
+ * fortai_hip_q8_quantize_tokens_device does.  For a block of 32 values with m their
+ * largest magnitude the scale is m / 127 rounded to fp32, then to fp16, the codes are
+ * 127 y / m rounded to fp32, then to the nearest integer, ties to even; all in 64 bits up to
+ * there.  A block with a NaN or an infinity has a scale of NaN.  The buffer's rows
+ * past `rows` are not written (no product's output depends on them).  device_sum may be x or the
+ * residual itself (same pitch).  width: a multiple of 32, up to 2^20.
+ * tokens_read: the values code * scale of such a buffer as rows of dtype. */
+int fortai_hip_norm_tokens_device(fortai_hip_q8_context *context, int dtype, const void *device_x,
+    int64_t x_pitch, const void *device_residual, int64_t residual_pitch, void *device_sum,
+    int64_t sum_pitch, const void *device_norm, int group, float epsilon, const void *device_gate,
+    int64_t gate_pitch, int rows, int width, void *device_output, int64_t output_pitch,
+    void *device_tokens);
+int fortai_hip_q8_tokens_read_device(fortai_hip_q8_context *context, int dtype,
+    const void *device_tokens, int rows, int width, void *device_output, int64_t output_pitch);
+
+/* Rules on the logits of a step's rows, in the order
+ *   n = occurrences of the token among the last `window` tokens (0: all) of the
+ *       row's text: its sequence's history, then the step's tokens up to this row
+ *   n > 0: x = x > 0 ? x / repetition : x * repetition;
+ *          x = x - n * frequency - presence
+ *   x += bias;  tokens that the row's mask does not allow: -infinity
+ * device_row_starts (int32 [sequences + 1]) and device_tokens (int64 [rows], may be
+ * NULL) are those of fortai_hip_verify_drafts_device.  device_history: int64
+ * [sequences] at history_pitch, of which device_history_lengths[s] (int32) count, or
+ * NULL.  device_penalties: fp32 [sequences][repetition above 0, frequency, presence],
+ * or NULL for none.  device_bias: fp32 [vocab] a sequence at bias_pitch (0: one for
+ * all), or NULL.  device_masks: mask_count masks at mask_pitch words of 32 bits, a
+ * bit a token, the lowest first, set where it is allowed; device_mask_of (int32
+ * [rows]) says which one a row has, -1 or another that there is not: none.
+ * Tokens outside the vocabulary are not counted.  The output may be the logits
+ * themselves (same pitch).  Rows of no sequence are left as they were.  Rows and
+ * sequences up to 65535, the vocabulary to 2^28. */
+typedef struct fortai_hip_logit_rules {
+    int window, mask_count;
+    const void *device_penalties, *device_tokens, *device_history, *device_history_lengths;
+    const void *device_bias, *device_masks, *device_mask_of;
+    int64_t history_pitch, bias_pitch, mask_pitch;
+} fortai_hip_logit_rules;
+int fortai_hip_logits_adjust_device(fortai_hip_q8_context *context, int dtype,
+    const void *device_logits, int64_t logits_pitch, int rows, int vocab, int sequences,
+    const void *device_row_starts, const fortai_hip_logit_rules *rules, void *device_output,
+    int64_t output_pitch);
+
+/* The gated delta rule (fortai_qwen35_cpu.f90:856-906) over a batch's rows, with the
+ * causal convolution in front of it:
+ *   u_t = sum_i conv[channel][i] x_{t - conv_kernel + 1 + i},  y = u / (1 + exp(-u))
+ *   of the channels [key_heads][head] queries, as many keys, [value_heads][head] values;
+ *   q, k = y / max(|y|, epsilon) over the head, q also over sqrt(head); value head h goes
+ *   with key head h / (value_heads / key_heads)
+ *   a = exp(ssm_a softplus(alpha + ssm_dt)),  b = 1 / (1 + exp(-beta))
+ *   d = b (v - a S k),  S = a S + d k^T,  output = S q
+ * A cache has `layers` layers of `slots` slots, each a sequence's state, and keeps
+ * between calls what the next one needs.  Its storage is fortai_hip_gdn_bytes bytes
+ * (0: no such cache), aligned to 16, in this order, all fp32 but the last:
+ *   S       [layers][slots][value_heads][head: value dim][head: key dim]
+ *   inputs  [layers][slots][conv_kernel - 1 + pending][channels], oldest first
+ *   keys    [layers][slots][pending][key_heads][head]
+ *   updates [layers][slots][pending][value_heads][head]
+ *   decays  [layers][slots][pending][value_heads]
+ *   counts  int32 [layers][slots], of pending rows
+ * create: over the caller's device storage, which is taken as it is and stays the
+ * caller's, or with NULL over storage of its own, cleared (states of sequences that
+ * begin).  head_size 64 or 128; conv_kernel 2 to 8; pending 0 to 16; a call's rows up
+ * to max_rows (to 2^19), for which workspaces are made.
+ *
+ * Rows row_starts[s] .. row_starts[s + 1] - 1 of a batch are sequence s's next tokens,
+ * slots[s] is its state; two sequences of a batch must not have the same.  Up to
+ * `pending` rows of a sequence wait for their verdict: S is kept as it stands before
+ * them, and k, d, a and x beside it.  standing[s] says how many of the rows that the
+ * slot's last call left waiting stand (the verifier's accepted + 1; above their number: all); the others never
+ * were.  -1: the sequence begins, with a state and inputs of zeros.  device_standing
+ * NULL: all stand.  More rows than `pending` stand at once.  All three arrays are
+ * device int32, read when the kernels run.  max_rows: at least the rows of any
+ * sequence (rows past it are left out), at most rows.  A sequence without rows keeps
+ * its slot as it is; the rows of one whose slot is not in the cache are left as they
+ * were.  Rows of qkv (channels), alpha and beta (value_heads) and of the output
+ * [value_heads][head] at their pitches in dtype; conv [channels][conv_kernel], ssm_a
+ * and ssm_dt [value_heads] in fp32.  Up to 16 rows of a sequence go one by one, more in
+ * chunks of 64 with the same result up to rounding.  Sequences up to 16384.
+ * copy_slots: slot to[i] becomes a copy of slot from[i] in every layer, pending rows
+ * too; host arrays, used before the call returns.  No slot may be written twice, or
+ * be both read and written. */
+typedef struct fortai_hip_gdn_batch {
+    int sequences, rows, max_rows;
+    const void *device_row_starts; /* int32 [sequences + 1] */
+    const void *device_slots;      /* int32 [sequences] */
+    const void *device_standing;   /* int32 [sequences], or NULL */
+} fortai_hip_gdn_batch;
+
+size_t fortai_hip_gdn_bytes(int layers, int slots, int key_heads, int value_heads, int head_size,
+    int conv_kernel, int pending);
+int fortai_hip_gdn_create(fortai_hip_q8_context *context, int layers, int slots, int key_heads,
+    int value_heads, int head_size, int conv_kernel, int pending, int max_rows, void *device_storage,
+    size_t storage_bytes, fortai_hip_gdn_cache **cache);
+int fortai_hip_gdn_destroy(fortai_hip_gdn_cache *cache);
+int fortai_hip_gdn_run_device(fortai_hip_gdn_cache *cache, int layer,
+    const fortai_hip_gdn_batch *batch, int dtype, const void *device_qkv, int64_t qkv_pitch,
+    const void *device_alpha, int64_t alpha_pitch, const void *device_beta, int64_t beta_pitch,
+    const void *device_conv, const void *device_ssm_a, const void *device_ssm_dt, float epsilon,
+    void *device_output, int64_t output_pitch);
+int fortai_hip_gdn_copy_slots(fortai_hip_gdn_cache *cache, const int32_t *from, const int32_t *to,
+    int count);
 
 #ifdef __cplusplus
 }
