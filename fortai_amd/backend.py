@@ -144,6 +144,8 @@ _SIGNATURES = {
     "fortai_hip_kv8_pages_length": [_vp, _i],
     "fortai_hip_kv8_pages_free_count": [_vp],
     "fortai_hip_kv8_pages_tables": [_vp, _vp, _i, _vp, _i],
+    "fortai_hip_kv8_shared_attention_device": [_vp, _i, _vp, _vp, _i, _vp, _i64, _i64, _vp, _i, _f, _i, _i, _vp, _i64],
+    "fortai_hip_kv8_pages_groups": [_vp, _vp, _i, _vp, _vp, _vp, _vp],
     "fortai_hip_norm_tokens_device": [_vp, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _f, _vp, _i64, _i, _i, _vp, _i64,
                                       _vp],
     "fortai_hip_q8_tokens_read_device": [_vp, _i, _vp, _i, _i, _vp, _i64],
@@ -695,6 +697,16 @@ class Kv8Batch(C.Structure):
         super().__init__(sequences, rows, max_rows, table_pitch, _dev(row_starts), _dev(lengths), _dev(tables))
 
 
+class Kv8Groups(C.Structure):
+    """Which sequences of a batch share their first tokens' pages (fortai_hip_kv8_groups): device int32 starts
+    [groups + 1], shared [groups] tokens and group_of [sequences]; max_rows: the most rows of a group."""
+
+    _fields_ = [("groups", _i), ("max_rows", _i), ("starts", _vp), ("shared", _vp), ("group_of", _vp)]
+
+    def __init__(self, groups: int, max_rows: int, starts, shared, group_of):
+        super().__init__(groups, max_rows, _dev(starts), _dev(shared), _dev(group_of))
+
+
 class Kv8Cache:
     """8-bit paged key/value cache (fortai_hip_kv8_cache), over the caller's
     device storage of Kv8Cache.bytes() bytes or over its own."""
@@ -741,6 +753,17 @@ class Kv8Cache:
             self.h, layer, C.addressof(batch), DTYPES[dtype], _dev(query), heads * hp if query_pitch is None else query_pitch,
             hp, _dev(gate), heads, scale, max_length, _dev(out), heads * self.head_size if out_pitch is None else out_pitch),
             "fortai_hip_kv8_attention_device")
+
+    def shared_attention(self, layer: int, batch: Kv8Batch, sharing: Kv8Groups, query, heads: int, out, scale: float,
+                         max_length: int, max_shared: int, dtype: str = "f32", gate=None, query_pitch: Optional[int] = None,
+                         query_head_pitch: Optional[int] = None, out_pitch: Optional[int] = None) -> None:
+        """attention() with the tokens that groups of sequences share read once for all their rows; max_shared: about
+        the most of them."""
+        hp = self.head_size if query_head_pitch is None else query_head_pitch
+        self.ctx.check(self.ctx.lib.fortai_hip_kv8_shared_attention_device(
+            self.h, layer, C.addressof(batch), C.addressof(sharing), DTYPES[dtype], _dev(query),
+            heads * hp if query_pitch is None else query_pitch, hp, _dev(gate), heads, scale, max_length, max_shared, _dev(out),
+            heads * self.head_size if out_pitch is None else out_pitch), "fortai_hip_kv8_shared_attention_device")
 
     def copy_pages(self, source, target) -> None:
         """Page target[i] becomes a copy of page source[i], in every layer (host int32 arrays)."""
@@ -807,6 +830,16 @@ class Kv8Pages:
         self._check(self.lib.fortai_hip_kv8_pages_tables(self.h, _ptr(s), len(s), _ptr(out), self.table_pitch),
                     "fortai_hip_kv8_pages_tables")
         return out
+
+    def groups(self, sequences):
+        """Which of these sequences share leading pages with the ones before them: int32 arrays starts [groups + 1],
+        shared [groups] and group_of [len(sequences)], for Kv8Groups."""
+        s = np.ascontiguousarray(sequences, dtype=np.int32)
+        starts, shared, group_of = (np.zeros(len(s) + 1, dtype=np.int32) for _ in range(3))
+        n = C.c_int()
+        self._check(self.lib.fortai_hip_kv8_pages_groups(self.h, _ptr(s), len(s), _ptr(starts), _ptr(shared), _ptr(group_of),
+                                                         C.byref(n)), "fortai_hip_kv8_pages_groups")
+        return starts[:n.value + 1].copy(), shared[:n.value].copy(), group_of[:len(s)].copy()
 
     def free(self) -> None:
         if self.h:

@@ -81,6 +81,56 @@ const char *check_batch(const fortai_hip_kv8_batch *b) {
 
 bool empty(const fortai_hip_kv8_batch *b) { return b->sequences == 0 || b->rows == 0 || b->max_rows == 0; }
 
+// Attention of a batch's rows, over tokens that sequences share (sharing: may be null) and their own.
+int attend(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch, const fortai_hip_kv8_groups *sharing, int dtype,
+    const void *query, int64_t query_pitch, int64_t query_head_pitch, const void *gate, int heads, float scale, int max_length,
+    int max_shared, void *output, int64_t output_pitch) {
+    fortai_hip_q8_context *c = h->context;
+    if (const char *wrong = check_batch(batch)) return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (sharing)
+        if (const char *wrong = check_kv8_groups(sharing->groups, sharing->max_rows, batch->rows, batch->sequences, max_shared,
+                sharing->device_starts, sharing->device_shared, sharing->device_group_of))
+            return fail(c, FORTAI_HIP_INVALID, wrong);
+    if (empty(batch)) return FORTAI_HIP_OK;
+    if (const char *wrong = check_kv8_attention(h->shape, layer, dtype, batch->rows, batch->max_rows, query, query_pitch,
+            query_head_pitch, gate, heads, scale, max_length, output, output_pitch))
+        return fail(c, FORTAI_HIP_INVALID, wrong);
+    Kv8AttentionParams p;
+    p.cache = h->layer(layer);
+    p.batch = batch_rows(batch);
+    p.q = query;
+    p.gate = gate;
+    p.out = output;
+    p.q_row = query_pitch;
+    p.q_head = query_head_pitch;
+    p.out_row = output_pitch;
+    p.group = heads / h->shape.kv_heads;
+    p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074 / 127.0);
+    p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0) &&
+        vector4_ok(gate, dtype, 0, 0);
+    p.partial = h->partial;
+    p.partial_ml = reinterpret_cast<f32x4_t *>(h->partial + static_cast<size_t>(kKv8PartialRows) * h->shape.head);
+    const bool fp32 = dtype == FORTAI_HIP_DTYPE_F32;
+    const int head = h->shape.head, kv_heads = h->shape.kv_heads;
+    const int64_t rows = static_cast<int64_t>(batch->max_rows) * p.group;
+    const DeviceScope scope(c->device);
+    const std::lock_guard<std::mutex> lock(h->launches);
+    if (sharing && sharing->groups > 0 && sharing->max_rows > 0) {
+        const Kv8SharedPlan plan = kv8_shared_plan(fp32, head, batch->sequences, sharing->groups, kv_heads, rows,
+            static_cast<int64_t>(sharing->max_rows) * p.group, max_length > max_shared ? max_length - max_shared : 1, max_shared);
+        if (plan.shares) {
+            p.sharing.starts = static_cast<const int32_t *>(sharing->device_starts);
+            p.sharing.shared = static_cast<const int32_t *>(sharing->device_shared);
+            p.sharing.group_of = static_cast<const int32_t *>(sharing->device_group_of);
+            p.sharing.groups = sharing->groups;
+            p.sharing.max_rows = sharing->max_rows;
+            return done(c, launch_kv8_shared_attention(p, static_cast<Dtype>(dtype), plan, c->stream), "kv8 shared attention");
+        }
+    }
+    const Kv8Plan plan = kv8_plan(fp32, head, batch->sequences, kv_heads, rows, max_length);
+    return done(c, launch_kv8_attention(p, static_cast<Dtype>(dtype), plan, c->stream), "kv8 attention");
+}
+
 }  // namespace
 
 extern "C" {
@@ -251,32 +301,17 @@ int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *h, int layer, const fo
     const void *query, int64_t query_pitch, int64_t query_head_pitch, const void *gate, int heads, float scale,
     int max_length, void *output, int64_t output_pitch) {
     if (!h) return FORTAI_HIP_INVALID;
-    fortai_hip_q8_context *c = h->context;
-    if (const char *wrong = check_batch(batch)) return fail(c, FORTAI_HIP_INVALID, wrong);
-    if (empty(batch)) return FORTAI_HIP_OK;
-    if (const char *wrong = check_kv8_attention(h->shape, layer, dtype, batch->rows, batch->max_rows, query, query_pitch,
-            query_head_pitch, gate, heads, scale, max_length, output, output_pitch))
-        return fail(c, FORTAI_HIP_INVALID, wrong);
-    Kv8AttentionParams p;
-    p.cache = h->layer(layer);
-    p.batch = batch_rows(batch);
-    p.q = query;
-    p.gate = gate;
-    p.out = output;
-    p.q_row = query_pitch;
-    p.q_head = query_head_pitch;
-    p.out_row = output_pitch;
-    p.group = heads / h->shape.kv_heads;
-    p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634074 / 127.0);
-    p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0) &&
-        vector4_ok(gate, dtype, 0, 0);
-    p.partial = h->partial;
-    p.partial_ml = reinterpret_cast<f32x4_t *>(h->partial + static_cast<size_t>(kKv8PartialRows) * h->shape.head);
-    const Kv8Plan plan = kv8_plan(dtype == FORTAI_HIP_DTYPE_F32, h->shape.head, batch->sequences, h->shape.kv_heads,
-        static_cast<int64_t>(batch->max_rows) * p.group, max_length);
-    const DeviceScope scope(c->device);
-    const std::lock_guard<std::mutex> lock(h->launches);
-    return done(c, launch_kv8_attention(p, static_cast<Dtype>(dtype), plan, c->stream), "kv8 attention");
+    return attend(h, layer, batch, nullptr, dtype, query, query_pitch, query_head_pitch, gate, heads, scale, max_length, 0, output,
+        output_pitch);
+}
+
+int fortai_hip_kv8_shared_attention_device(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch,
+    const fortai_hip_kv8_groups *sharing, int dtype, const void *query, int64_t query_pitch, int64_t query_head_pitch,
+    const void *gate, int heads, float scale, int max_length, int max_shared, void *output, int64_t output_pitch) {
+    if (!h) return FORTAI_HIP_INVALID;
+    if (!sharing) return fail(h->context, FORTAI_HIP_INVALID, "kv8: no groups");
+    return attend(h, layer, batch, sharing, dtype, query, query_pitch, query_head_pitch, gate, heads, scale, max_length, max_shared,
+        output, output_pitch);
 }
 
 int fortai_hip_kv8_copy_pages(fortai_hip_kv8_cache *h, const int32_t *from, const int32_t *to, int count) {

@@ -177,6 +177,89 @@ __device__ __forceinline__ RowTile row_tile(const Kv8AttentionParams &p, int seq
     return t;
 }
 
+// What a workgroup does: rows row0 .. of a kv head, as `split` of `splits` over the tiles
+// from first_tile on, with the table of sequence seq; `item` is its place among the partial
+// results.
+struct Work {
+    int seq, kvh, row0, split, splits, first_tile;
+    RowTile tile;
+    size_t item;
+};
+
+// Rows and shared tokens of a group: whole tiles, 0 where its rows are more than the call
+// was cut for or its numbers name no sequences.
+struct Group {
+    int first, begin, rows, shared;
+};
+
+__device__ __forceinline__ Group group_at(const Kv8AttentionParams &p, int index) {
+    Group g;
+    const int s0 = read_only(p.sharing.starts + index), s1 = read_only(p.sharing.starts + index + 1);
+    const int tokens = min(read_only(p.sharing.shared + index), p.batch.pitch * p.cache.page_tokens);
+    g.first = g.begin = g.rows = g.shared = 0;
+    if (s0 < 0 || s1 <= s0 || s1 > p.batch.sequences) return g;
+    int last, count;
+    p.batch.range(s0, &g.begin, &count);
+    p.batch.range(s1 - 1, &last, &count);
+    g.first = s0;
+    g.rows = max(last + count - g.begin, 0);
+    g.shared = g.rows <= p.sharing.max_rows && tokens > 0 ? tokens / kTileTokens * kTileTokens : 0;
+    return g;
+}
+
+// What sequence seq leaves to its group (*index): every row of it, all among the group's, sees
+// all of these tokens.
+__device__ __forceinline__ Group shared_by(const Kv8AttentionParams &p, int seq, const RowTile &tile, int *index) {
+    Group g = {0, 0, 0, 0};
+    *index = read_only(p.sharing.group_of + seq);
+    if (*index < 0 || *index >= p.sharing.groups) return g;
+    g = group_at(p, *index);
+    const int end = read_only(p.sharing.starts + *index + 1), rows = tile.total / p.group;
+    if (seq < g.first || seq >= end || tile.length < g.shared || tile.begin < g.begin || tile.begin - g.begin + rows > g.rows) g.shared = 0;
+    return g;
+}
+
+template <bool SHARING, int ROWS>
+__device__ __forceinline__ Work work_of(const Kv8AttentionParams &p) {
+    Work w;
+    if constexpr (!SHARING) {
+        w.seq = blockIdx.z;
+        w.kvh = blockIdx.y % p.cache.kv_heads;
+        w.row0 = (blockIdx.y / p.cache.kv_heads) * ROWS;
+        w.split = blockIdx.x;
+        w.splits = p.splits;
+        w.first_tile = 0;
+        w.tile = row_tile(p, w.seq, w.row0, ROWS);
+        w.item = ((static_cast<size_t>(w.seq) * gridDim.y + blockIdx.y) * p.splits) + w.split;
+    } else {
+        // first the groups' blocks, then the sequences'
+        const int block = blockIdx.x + p.first_block;
+        const int of_groups = p.sharing.groups * p.shared_row_tiles * p.cache.kv_heads * p.shared_splits;
+        const bool group = block < of_groups;
+        const int at = group ? block : block - of_groups, tiles = group ? p.shared_row_tiles : p.row_tiles;
+        w.splits = group ? p.shared_splits : p.splits;
+        w.split = at % w.splits;
+        const int rest = at / w.splits, rows = rest / p.cache.kv_heads, who = rows / tiles;
+        w.kvh = rest % p.cache.kv_heads;
+        w.row0 = (rows % tiles) * ROWS;
+        // partial results: the groups' rows, then the sequences'
+        w.item = static_cast<size_t>(at) + (group ? 0 : static_cast<size_t>(p.own_at) / ROWS);
+        if (group) {
+            const Group g = group_at(p, who);
+            w.seq = g.first;
+            w.first_tile = 0;
+            // every row sees all of the tokens
+            w.tile = RowTile{g.begin, g.shared > 0 ? g.rows * p.group : 0, g.shared, g.shared, g.shared / kTileTokens};
+        } else {
+            w.seq = who;
+            w.tile = row_tile(p, who, w.row0, ROWS);
+            int index;
+            w.first_tile = shared_by(p, who, w.tile, &index).shared / kTileTokens;
+        }
+    }
+    return w;
+}
+
 // Until at most N of this wave's loads from memory are on their way (gfx9 s_waitcnt:
 // vmcnt in bits 3:0 and 15:14, the other counters left alone), with no LDS access
 // moved across it.
@@ -312,7 +395,7 @@ __device__ __forceinline__ int key_turn(int r) {
     return D == 256 ? r : D == 128 ? r >> 1 : 3 * (r >> 3);
 }
 
-template <int D, Dtype DT, bool SPLIT>
+template <int D, Dtype DT, bool SPLIT, bool SHARING>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8AttentionParams p) {
     typedef typename Element<DT>::type E;
     constexpr int kRows = SPLIT ? 8 : 16;           // in an instruction's 16 columns
@@ -329,8 +412,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kRows;
-    const int split = blockIdx.x, step = p.splits * kWaves, first = split * kWaves + wave;
+    Work work;
+    if constexpr (SHARING) work = work_of<true, kRows>(p);
+    const int seq = SHARING ? work.seq : blockIdx.z;
+    const int split = SHARING ? work.split : blockIdx.x, step = (SHARING ? work.splits : p.splits) * kWaves;
+    const int first = (SHARING ? work.first_tile : 0) + split * kWaves + wave;
     const int P = p.cache.page_tokens, shift_p = 31 - __builtin_clz(P), row_shift = shift_p - 4;
     // the pages of a tile's four groups of 16 tokens
     int page0, page1, page2, page3;
@@ -343,10 +429,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         page2 = find_page(n * kTileTokens + 32);
         page3 = find_page(n * kTileTokens + 48);
     };
-    find_pages(first);
-    const RowTile tile = row_tile(p, seq, row0, kRows);
+    find_pages(first);  // on its way beside the sequence's own numbers
+    if constexpr (!SHARING) work = work_of<false, kRows>(p);
+    const int kvh = work.kvh, row0 = work.row0;
+    const RowTile tile = work.tile;
     if (row0 >= tile.total) return;
-    if (split > 0 && split * kWaves >= tile.tiles) return;  // the join does not look at it
+    if (split > 0 && work.first_tile + split * kWaves >= tile.tiles) return;  // the join does not look at it
+    const bool whole = !SHARING && p.splits == 1;
 
     const size_t page_stride = static_cast<size_t>(p.cache.kv_heads) * P * D;
     const uint64_t keys = reinterpret_cast<uint64_t>(p.cache.keys) + static_cast<size_t>(kvh) * P * D;
@@ -543,7 +632,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
     for (int d = 0; d < kDims; ++d) lds.join[wave][d][lane] = o[d] * scale;
     lds_barrier();
     if (low || row >= tile.total) return;
-    const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
+    const size_t item = work.item;
     const int head = kvh * p.group + row % p.group;
     const int64_t at = tile.begin + row / p.group;
     const Quotient quotient(top, total, kPScale);
@@ -557,10 +646,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
             for (int w = 0; w < kWaves; ++w) y += lds.join[w][d][lane + 8];
         }
         const int dim = 16 * d + 4 * g;
-        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + col) * D + dim) = y;
+        if (!whole) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + col) * D + dim) = y;
         else finish<DT>(p, quotient(y), quotient.some(), at, head, head * D + dim, dim);
     }
-    if (p.splits > 1 && wave == 0 && g == 0)
+    if (!whole && wave == 0 && g == 0)
         p.partial_ml[item * kRows + col] = f32x4_t{top.score, top.value, total.base, total.sum};
 }
 
@@ -581,7 +670,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // 16-row kernel 409) a version in which every wave read the whole tile's values from LDS
 // took 265, values by loads to LDS, as the keys, 273, and priority for the products was
 // worth 12.
-template <int D, Dtype DT, bool SPLIT>
+template <int D, Dtype DT, bool SPLIT, bool SHARING>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
     constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<SPLIT>;
     constexpr int kMyRows = SPLIT ? 8 : 16, kRows = kWaves * kMyRows;
@@ -604,12 +693,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int seq = blockIdx.z, kvh = blockIdx.y % p.cache.kv_heads, row0 = (blockIdx.y / p.cache.kv_heads) * kRows;
-    const int split = blockIdx.x, step = p.splits;
+    const Work work = work_of<SHARING, kRows>(p);
+    const int seq = work.seq, kvh = work.kvh, row0 = work.row0, split = work.split, step = work.splits;
+    const int first = work.first_tile + split;
     const int P = p.cache.page_tokens, shift_p = 31 - __builtin_clz(P);
-    const RowTile tile = row_tile(p, seq, row0, kRows);
+    const RowTile tile = work.tile;
     if (row0 >= tile.total) return;
-    if (split > 0 && split >= tile.tiles) return;  // the join does not look at it
+    if (split > 0 && first >= tile.tiles) return;  // the join does not look at it
+    const bool whole_rows = !SHARING && p.splits == 1;
 
     const size_t page_stride = static_cast<size_t>(p.cache.kv_heads) * P * D;
     const uint64_t keys = reinterpret_cast<uint64_t>(p.cache.keys) + static_cast<size_t>(kvh) * P * D;
@@ -644,11 +735,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         key_top = p.cache.key_max[at];
         value_top = p.cache.value_max[at];
     };
-    int page = checked(page_id(split)), next_id = -1;  // the page of this tile, and the word that says the next one's
-    if (split < tile.tiles) {
+    int page = checked(page_id(first)), next_id = -1;  // the page of this tile, and the word that says the next one's
+    if (first < tile.tiles) {
         load_keys(page, 0);
         load_tops(page);
-        next_id = page_id(split + step);
+        next_id = page_id(first + step);
         load_values(page);
     }
     stage_queries<D, DT, SPLIT, 64>(p, tile, row0 + kMyRows * wave, kvh, lane, reinterpret_cast<uint32_t *>(lds.start.operands[wave]),
@@ -675,7 +766,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 
     int buffer = 0;
 #pragma unroll 1
-    for (int n = split; n < tile.tiles; n += step) {
+    for (int n = first; n < tile.tiles; n += step) {
         const bool more = n + step < tile.tiles;
         wait_loads<kMine>();  // all but the values, which were asked for last
         lds_barrier();  // every wave's keys are there, and its products with the tile before done
@@ -816,14 +907,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 
     l.add_lane<16>();
     l.add_lane<32>();
-    const Quotient quotient = p.splits > 1 ? Quotient(kPScale / kWideScale, 0) : Quotient(m, l, kWideScale);
+    const Quotient quotient = !whole_rows ? Quotient(kPScale / kWideScale, 0) : Quotient(m, l, kWideScale);
     lds_barrier();  // the last tile's products are done
 #pragma unroll
     for (int t = 0; t < kWaves; ++t)
 #pragma unroll
         for (int i = 0; i < kMine; ++i) lds.rows[t][wave * kMine + i][lane] = o[t][i];
-    const size_t item = ((static_cast<size_t>(seq) * gridDim.y + blockIdx.y) * p.splits) + split;
-    if (p.splits > 1 && g == 0 && !low)
+    const size_t item = work.item;
+    if (!whole_rows && g == 0 && !low)
         p.partial_ml[item * kRows + kMyRows * wave + col] = f32x4_t{m.score, m.value, l.base, l.sum};
     lds_barrier();
     // the rows that the wave has the sums of: a row's dims, four a lane, in as many rows at a time as a wave holds
@@ -838,7 +929,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         if constexpr (SPLIT) y += lds.rows[wave][four >> 2][16 * (four & 3) + local + 8] * (1.0f / kLoScale);
         y = row_quotient(y);
         const int head = kvh * p.group + at % p.group;
-        if (p.splits > 1) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + kMyRows * wave + local) * D + dim) = y;
+        if (!whole_rows) *reinterpret_cast<f32x4_t *>(p.partial + (item * kRows + kMyRows * wave + local) * D + dim) = y;
         else finish<DT>(p, y, row_quotient.some(), tile.begin + at / p.group, head, head * D + dim, dim);
     }
 }
@@ -919,14 +1010,139 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
     finish<DT>(p, quotient(y), quotient.some(), tile.begin + row / p.group, head, head * D + dim, dim);
 }
 
+// The same where a row's tokens are its group's, then its own: the partial results of
+// both.
+template <int D, Dtype DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionParams p) {
+    constexpr int kLanes = 16, kGroups = THREADS / kLanes;
+    __shared__ float weight[2 * kKv8MaxSplits];
+    __shared__ f32x4_t sums[kGroups][kLanes];
+    const int seq = blockIdx.z, kvh = blockIdx.y / (D / 64), slice = blockIdx.y % (D / 64), row = blockIdx.x;
+    const RowTile tile = row_tile(p, seq, row / p.own_rows * p.own_rows, p.own_rows);
+    if (row >= tile.total) return;
+    int index;
+    const Group g = shared_by(p, seq, tile, &index);
+    const auto active = [](int tiles, int splits, int rows) {
+        const int together = rows > 16 ? 1 : kWaves;  // tiles that a workgroup's waves take at once
+        return min(splits, max((tiles + together - 1) / together, 1));
+    };
+    const int own = active(tile.tiles - g.shared / kTileTokens, p.splits, p.own_rows);
+    const int all = own + (g.shared > 0 ? active(g.shared / kTileTokens, p.shared_splits, p.shared_rows) : 0);
+    // place of this row in the first split of either
+    const int group_row = (tile.begin - g.begin) * p.group + row;
+    const auto place = [&](int who, int tiles, int at, int rows, int splits) {
+        return (((static_cast<int64_t>(who) * tiles + at / rows) * p.cache.kv_heads + kvh) * splits) * rows + at % rows;
+    };
+    const int64_t own_at = p.own_at + place(seq, p.row_tiles, row, p.own_rows, p.splits);
+    const int64_t group_at = place(max(index, 0), p.shared_row_tiles, group_row, p.shared_rows, p.shared_splits);
+    const auto partial_row = [&](int i) {
+        return i < own ? own_at + static_cast<int64_t>(i) * p.own_rows : group_at + static_cast<int64_t>(i - own) * p.shared_rows;
+    };
+
+    const int lane = threadIdx.x & 63;
+    Base top = {kNone, 0.0f};
+    Denominator total;
+#pragma unroll 1
+    for (int i = lane; i < all; i += 64) {
+        const f32x4_t join = p.partial_ml[partial_row(i)];
+        const Base other = {join[0], join[1]};
+        if (above(other, top) > 0.0f) top = other;
+        total.add(join[2], join[3]);
+    }
+    top = larger_of_lanes<32>(top);
+    top = larger_of_lanes<16>(top);
+    top = larger_of_lanes<8>(top);
+    top = larger_of_lanes<4>(top);
+    top = larger_of_lanes<2>(top);
+    top = larger_of_lanes<1>(top);
+    total.add_lane<32>();
+    total.add_lane<16>();
+    total.add_lane<8>();
+    total.add_lane<4>();
+    total.add_lane<2>();
+    total.add_lane<1>();
+    if (threadIdx.x < 64) {
+#pragma unroll 1
+        for (int i = lane; i < all; i += 64) {
+            const f32x4_t join = p.partial_ml[partial_row(i)];
+            const Base other = {join[0], join[1]};
+            weight[i] = exp2_fast(above(other, top));
+        }
+    }
+    lds_barrier();
+    const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes, dim = 64 * slice + 4 * at;
+    f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = group; i < all; i += kGroups) y += *reinterpret_cast<const f32x4_t *>(p.partial + partial_row(i) * D + dim) * weight[i];
+    sums[group][at] = y;
+    lds_barrier();
+    if (threadIdx.x >= kLanes) return;
+    const int used = min(all, kGroups);
+#pragma unroll 4
+    for (int k = 1; k < used; ++k) y += sums[k][at];
+    const Quotient quotient(top, total, kPScale);
+    const int head = kvh * p.group + row % p.group;
+    finish<DT>(p, quotient(y), quotient.some(), tile.begin + row / p.group, head, head * D + dim, dim);
+}
+
+// `blocks` blocks from first_block on, of the groups' and the sequences' one after the other
+template <int D, Dtype DT, int ROWS>
+hipError_t launch_shared_rows(Kv8AttentionParams p, int first_block, int blocks, hipStream_t stream) {
+    p.first_block = first_block;
+    constexpr bool kSplit = ROWS == 8 || ROWS == 32;
+    if constexpr (ROWS > 16) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT, kSplit, true>), dim3(blocks), dim3(kWaves * 64), 0, stream, p);
+    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, kSplit, true>), dim3(blocks), dim3(kWaves * 64), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <int D, Dtype DT>
+hipError_t launch_shared_typed(Kv8AttentionParams p, const Kv8SharedPlan &cut, hipStream_t stream) {
+    const Kv8Plan &plan = cut.own, &shared = cut.group;
+    p.own_at = static_cast<int>(cut.own_at);
+    p.splits = plan.splits;
+    p.row_tiles = plan.row_tiles;
+    p.own_rows = plan.rows;
+    p.shared_splits = shared.splits;
+    p.shared_row_tiles = shared.row_tiles;
+    p.shared_rows = shared.rows;
+    const int heads = p.cache.kv_heads;
+    const int of_groups = p.sharing.groups * shared.row_tiles * heads * shared.splits, own = p.batch.sequences * plan.row_tiles * heads * plan.splits;
+    const auto launch = [&](int rows, int first_block, int blocks) {
+        if constexpr (DT == Dtype::F32)
+            return rows == 8 ? launch_shared_rows<D, DT, 8>(p, first_block, blocks, stream) : launch_shared_rows<D, DT, 32>(p, first_block, blocks, stream);
+        else
+            return rows == 8 ? launch_shared_rows<D, DT, 8>(p, first_block, blocks, stream)
+                : rows == 16 ? launch_shared_rows<D, DT, 16>(p, first_block, blocks, stream)
+                             : launch_shared_rows<D, DT, 64>(p, first_block, blocks, stream);
+    };
+    hipError_t e;
+    if (plan.rows == shared.rows) {
+        e = launch(plan.rows, 0, of_groups + own);
+    } else {
+        e = launch(shared.rows, 0, of_groups);
+        if (e == hipSuccess) e = launch(plan.rows, of_groups, own);
+    }
+    if (e != hipSuccess) return e;
+    const dim3 rows(p.batch.max_rows * p.group, heads * (D / 64), p.batch.sequences);
+    hipLaunchKernelGGL((kv8_shared_join_kernel<D, DT, 256>), rows, dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <Dtype DT>
+hipError_t launch_shared_head(const Kv8AttentionParams &p, const Kv8SharedPlan &plan, hipStream_t stream) {
+    if (p.cache.head == 64) return launch_shared_typed<64, DT>(p, plan, stream);
+    if (p.cache.head == 128) return launch_shared_typed<128, DT>(p, plan, stream);
+    return launch_shared_typed<256, DT>(p, plan, stream);
+}
+
 template <int D, Dtype DT, int ROWS>
 hipError_t launch_rows(Kv8AttentionParams p, const Kv8Plan &plan, hipStream_t stream) {
     const dim3 grid(plan.splits, plan.row_tiles * p.cache.kv_heads, p.batch.sequences);
     p.splits = plan.splits;
     p.row_tiles = plan.row_tiles;
     constexpr bool kSplit = ROWS == 8 || ROWS == 32;
-    if constexpr (ROWS > 16) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT, kSplit>), grid, dim3(kWaves * 64), 0, stream, p);
-    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, kSplit>), grid, dim3(kWaves * 64), 0, stream, p);
+    if constexpr (ROWS > 16) hipLaunchKernelGGL((kv8_attention_wide_kernel<D, DT, kSplit, false>), grid, dim3(kWaves * 64), 0, stream, p);
+    else hipLaunchKernelGGL((kv8_attention_kernel<D, DT, kSplit, false>), grid, dim3(kWaves * 64), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && plan.splits > 1) {
         const dim3 rows(p.batch.max_rows * p.group, p.cache.kv_heads * (D / 64), p.batch.sequences);
@@ -961,6 +1177,12 @@ hipError_t launch_kv8_attention(const Kv8AttentionParams &p, Dtype dtype, const 
     if (dtype == Dtype::F32) return launch_head<Dtype::F32>(p, plan, stream);
     if (dtype == Dtype::F16) return launch_head<Dtype::F16>(p, plan, stream);
     return launch_head<Dtype::BF16>(p, plan, stream);
+}
+
+hipError_t launch_kv8_shared_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8SharedPlan &plan, hipStream_t stream) {
+    if (dtype == Dtype::F32) return launch_shared_head<Dtype::F32>(p, plan, stream);
+    if (dtype == Dtype::F16) return launch_shared_head<Dtype::F16>(p, plan, stream);
+    return launch_shared_head<Dtype::BF16>(p, plan, stream);
 }
 
 }  // namespace fortai_hip

@@ -89,7 +89,8 @@ struct Kv8Plan {
 // four waves (two tiles where the waves share them) and the partial results fit: one workgroup a CU
 // costs 30.5 us where two cost 25.9 (eight sequences of up to 8190 tokens); one tile a
 // wave costs 13.2 us where three cost 17.0 (600 tokens).
-inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length) {
+inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length,
+    int64_t partial_rows = kKv8PartialRows) {
     Kv8Plan p;
     const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
     const int few = fp32 || rows <= 8 ? 8 : 16;
@@ -98,11 +99,35 @@ inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
     const int64_t base = p.row_tiles * heads, fill = 512 * (256 / head), least = much ? 128 : 256;
     const int64_t wanted = (fill + base - 1) / base, useful = (max_length + least - 1) / least;
-    const int64_t room = kKv8PartialRows / (base * p.rows);
+    const int64_t room = partial_rows / (base * p.rows);
     int64_t s = wanted < useful ? wanted : useful;
     s = s < room ? s : room;
     s = s < kKv8MaxSplits ? s : kKv8MaxSplits;
     p.splits = s < 1 ? 1 : static_cast<int>(s);
+    return p;
+}
+
+// How a call is cut whose sequences share tokens: the groups' tokens and the sequences'
+// own, which have their partial results behind the groups' from row own_at on.  shares
+// is false where these do not fit.
+struct Kv8SharedPlan {
+    Kv8Plan own, group;
+    int64_t own_at = 0;
+    bool shares = false;
+};
+
+inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int groups, int kv_heads, int64_t rows, int64_t group_rows,
+    int64_t max_own, int64_t max_shared) {
+    Kv8SharedPlan p;
+    const auto partial = [&](const Kv8Plan &plan, int who) {
+        return static_cast<int64_t>(who) * plan.row_tiles * kv_heads * plan.rows * plan.splits;
+    };
+    // the sequences' own tokens are few: what they leave of the workspace is the groups'
+    p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8PartialRows / 2);
+    const int64_t own = partial(p.own, sequences);
+    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, own < kKv8PartialRows ? kKv8PartialRows - own - 63 : 0);
+    p.own_at = (partial(p.group, groups) + 63) / 64 * 64;
+    p.shares = max_shared >= 64 && p.own_at + own <= kKv8PartialRows;
     return p;
 }
 

@@ -183,4 +183,45 @@ int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *p, const int *sequen
     return FORTAI_HIP_OK;
 }
 
+// The tokens of `count` sequences in a row are compared with those of a group's first one;
+// a sequence joins while that leaves more tokens that need not be read again.
+int fortai_hip_kv8_pages_groups(const fortai_hip_kv8_pages *p, const int *sequences, int count, int32_t *starts, int32_t *shared,
+    int32_t *group_of, int *groups) {
+    if (!p || !groups || count < 0 || !starts || (count > 0 && (!sequences || !shared || !group_of))) return FORTAI_HIP_INVALID;
+    *groups = 0;
+    for (int i = 0; i < count; ++i)
+        if (!p->has(sequences[i])) return FORTAI_HIP_INVALID;
+    constexpr int64_t kLeast = 64;  // tokens: what attention shares is whole tiles of 64
+    int n = 0, first = 0;
+    while (first < count) {
+        const std::vector<int32_t> &table = p->tables[sequences[first]];
+        int64_t common = p->lengths[sequences[first]];
+        int end = first + 1;
+        while (end < count) {
+            const std::vector<int32_t> &other = p->tables[sequences[end]];
+            size_t same = 0;
+            while (same < table.size() && same < other.size() && table[same] == other[same]) ++same;
+            int64_t tokens = static_cast<int64_t>(same) * p->page_tokens;
+            if (tokens > p->lengths[sequences[end]]) tokens = p->lengths[sequences[end]];
+            if (tokens > common) tokens = common;
+            const int64_t members = end - first;
+            if (tokens < kLeast || (members > 1 && tokens * members < common * (members - 1))) break;
+            common = tokens;
+            ++end;
+        }
+        const bool alone = end == first + 1;
+        // sequences that share nothing lie together in groups of no shared tokens
+        if (!alone || n == 0 || shared[n - 1] != 0) {
+            starts[n] = first;
+            shared[n] = alone ? 0 : static_cast<int32_t>(common);
+            ++n;
+        }
+        for (int i = first; i < end; ++i) group_of[i] = n - 1;
+        first = end;
+    }
+    starts[n] = count;
+    *groups = n;
+    return FORTAI_HIP_OK;
+}
+
 }  // extern "C"

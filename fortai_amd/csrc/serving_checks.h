@@ -160,6 +160,17 @@ inline const char *check_kv8_attention(const Kv8Shape &s, int layer, int dtype, 
     return nullptr;
 }
 
+inline const char *check_kv8_groups(int groups, int max_rows, int rows, int sequences, int max_shared, const void *starts,
+    const void *shared, const void *group_of) {
+    if (groups < 0 || groups > sequences) return "kv8: groups 0 to the sequences";
+    if (max_rows < 0 || max_rows > rows) return "kv8: a group's rows 0 to the batch's";
+    if (max_shared < 0) return "kv8: max_shared below 0";
+    if (groups == 0) return nullptr;
+    if (!starts || !shared || !group_of) return "kv8: null array";
+    if (!aligned(starts, 4) || !aligned(shared, 4) || !aligned(group_of, 4)) return "kv8: misaligned array";
+    return nullptr;
+}
+
 // Pairs that can be copied in any order: ids within the pool, no page written
 // twice, none both read and written.  May throw std::bad_alloc.
 inline const char *check_page_pairs(const int32_t *from, const int32_t *to, int count, int pages) {

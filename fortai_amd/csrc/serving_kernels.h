@@ -37,9 +37,18 @@ hipError_t launch_kv8_read(const Kv8View &cache, const Kv8Rows &batch, Dtype dty
 hipError_t launch_kv8_copy_pages(const Kv8View &cache, size_t layer_codes, size_t layer_tops, int layers,
     const int32_t *from, const int32_t *to, int count, hipStream_t stream);
 
+// Sequences that share their first tokens' pages.
+struct Kv8Sharing {
+    const int32_t *starts = nullptr;    // [groups + 1], sequences
+    const int32_t *shared = nullptr;    // [groups], tokens
+    const int32_t *group_of = nullptr;  // [sequences]
+    int groups = 0, max_rows = 0;       // rows of a group
+};
+
 struct Kv8AttentionParams {
     Kv8View cache;
     Kv8Rows batch;
+    Kv8Sharing sharing;  // of calls that share
     const void *q = nullptr, *gate = nullptr;  // gate: null, or at q's pitches
     void *out = nullptr;
     int64_t q_row = 0, q_head = 0, out_row = 0;
@@ -48,8 +57,10 @@ struct Kv8AttentionParams {
     bool vec = false;         // q, gate and out allow four-element accesses
     float *partial = nullptr;        // [kKv8PartialRows][head]
     f32x4_t *partial_ml = nullptr;   // [kKv8PartialRows]
-    int splits = 0, row_tiles = 0;  // set by the launcher
+    int splits = 0, row_tiles = 0;  // set by the launcher; of a call that shares, for each sequence's own tokens
+    int shared_splits = 0, shared_row_tiles = 0, shared_rows = 0, own_rows = 0, own_at = 0, first_block = 0;
 };
+hipError_t launch_kv8_shared_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8SharedPlan &plan, hipStream_t stream);
 hipError_t launch_kv8_attention(const Kv8AttentionParams &p, Dtype dtype, const Kv8Plan &plan, hipStream_t stream);
 hipError_t launch_kv8_clear(void *storage, size_t bytes, hipStream_t stream);
 

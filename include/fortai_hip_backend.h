@@ -589,6 +589,29 @@ int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
     int64_t query_head_pitch, const void *device_gate, int heads, float scale, int max_length,
     void *device_output, int64_t output_pitch);
 
+/* The same for sequences that share their first tokens' pages, as forks do: the shared
+ * tokens are read once for all rows of a group.  Group g is the sequences group_starts[g]
+ * .. group_starts[g + 1] - 1 of the batch (so their rows lie together); the first
+ * shared[g] tokens of all of them are in the same pages, and are read through the table
+ * of the first.  group_of[s] names the group of a sequence, -1: none.  Whole tiles of 64
+ * tokens are shared; a sequence whose lengths[s] is less than them shares nothing, and so
+ * does a group of more than max_rows rows.  All three arrays are device int32.  max_shared:
+ * about the largest shared[g], for cutting the work, as max_length.  Results are as
+ * accurate as fortai_hip_kv8_attention_device's, summed in another order.  Where the
+ * partial results of the rows exceed the cache's workspace, or there are no groups, the
+ * call is that one. */
+typedef struct fortai_hip_kv8_groups {
+    int groups, max_rows;
+    const void *device_starts;   /* int32 [groups + 1] */
+    const void *device_shared;   /* int32 [groups] */
+    const void *device_group_of; /* int32 [sequences] */
+} fortai_hip_kv8_groups;
+int fortai_hip_kv8_shared_attention_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, const fortai_hip_kv8_groups *sharing, int dtype,
+    const void *device_query, int64_t query_pitch, int64_t query_head_pitch, const void *device_gate,
+    int heads, float scale, int max_length, int max_shared, void *device_output,
+    int64_t output_pitch);
+
 /* Which pages whose tokens lie in: host bookkeeping for one pool and up to
  * `sequences` sequences of at most table_pitch pages; no GPU is needed, and a
  * refused call (INVALID) changes nothing.
@@ -603,6 +626,9 @@ int fortai_hip_kv8_attention_device(fortai_hip_kv8_cache *cache, int layer,
  * at most `capacity` of them; the moves go through copy_pages before the next
  * append or attention, and tables that were taken before are stale.
  * tables: the pages of count sequences, rows of table_pitch, -1 behind the last.
+ * groups: which of count sequences, in this order, share leading pages with the ones
+ * before them, as fortai_hip_kv8_groups wants it (host arrays starts [count + 1], shared
+ * and group_of [count]); groups of no shared tokens hold the others.
  * length (-1: no such sequence) and free_count (-1: no pool) ask. */
 int fortai_hip_kv8_pages_create(int pages, int page_tokens, int sequences, int table_pitch,
     fortai_hip_kv8_pages **pool);
@@ -617,6 +643,8 @@ int64_t fortai_hip_kv8_pages_length(const fortai_hip_kv8_pages *pool, int sequen
 int fortai_hip_kv8_pages_free_count(const fortai_hip_kv8_pages *pool);
 int fortai_hip_kv8_pages_tables(const fortai_hip_kv8_pages *pool, const int *sequences, int count,
     int32_t *tables, int table_pitch);
+int fortai_hip_kv8_pages_groups(const fortai_hip_kv8_pages *pool, const int *sequences, int count,
+    int32_t *starts, int32_t *shared, int32_t *group_of, int *groups);
 
 /* Verification of drafted tokens.  Rows row_starts[s] .. row_starts[s + 1] - 1
  * (device int32 [sequences + 1]) are the step of sequence s: its first row ran
