@@ -187,6 +187,7 @@ def _hold(s, case):
             storage=s.storage.data_ptr(), storage_bytes=4 * s.storage.numel()))
         s.batch = backend.GdnBatch(case["sequences"], s.total, s.most, s.row_starts.data_ptr(), s.slot.data_ptr(),
                                    s.standing.data_ptr())
+        s.views = _gdn_outputs(s, case, s.out)
     elif case["kind"] == "shared":
         s.handles.append(backend.Kv8Cache(ctx, 1, s.pages, case["page"], case["kv_heads"], case["head"],
                                           storage=s.storage.data_ptr(), storage_bytes=s.storage.numel()))
@@ -330,7 +331,7 @@ def _gdn_outputs(s, case, out):
 def _own_gdn(s, case):
     s.handles[0].run(0, s.batch, s.qkv.data_ptr(), s.gates[0].data_ptr(), s.gates[1].data_ptr(), s.conv.data_ptr(),
                      s.ssm_a.data_ptr(), s.ssm_dt.data_ptr(), s.out.data_ptr(), dtype=case["dtype"], eps=EPS)
-    return _gdn_outputs(s, case, s.out)
+    return s.views
 
 
 def _own_norm(s, case):
