@@ -22,7 +22,8 @@ struct fortai_hip_gdn_cache {
     bool owned = false;
     // made with the cache and never again, so that a captured call keeps their addresses
     int *arrivals = nullptr, *stands = nullptr;
-    float *rows = nullptr, *through = nullptr, *inner = nullptr, *decay = nullptr, *rate = nullptr;
+    _Float16 *asks = nullptr, *keys_by_dim = nullptr, *through = nullptr, *inner = nullptr;
+    float *values = nullptr, *decay = nullptr, *rate = nullptr;
     std::mutex launches;  // a call's launches follow each other on the stream
 
     GdnView layer(int index) const {
@@ -51,9 +52,11 @@ struct fortai_hip_gdn_cache {
         if (owned) release(storage);
         release(arrivals);
         release(stands);
-        release(rows);
+        release(asks);
+        release(keys_by_dim);
         release(through);
         release(inner);
+        release(values);
         release(decay);
         release(rate);
     }
@@ -200,9 +203,11 @@ int fortai_hip_gdn_create(fortai_hip_q8_context *c, int layers, int slots, int k
     if (e == hipSuccess) e = launch_kv8_clear(h->arrivals, counters * sizeof(int), c->stream);
     if (max_rows > kGdnFewRows) {
         if (e == hipSuccess) e = alloc(&h->stands, static_cast<size_t>(kGdnMaxSequences));
-        if (e == hipSuccess) e = alloc(&h->rows, rows * s.channels());
-        if (e == hipSuccess) e = alloc(&h->through, rows * value_heads * head_size);
-        if (e == hipSuccess) e = alloc(&h->inner, rows * value_heads * kGdnChunk);
+        if (e == hipSuccess) e = alloc(&h->asks, rows * 2 * key_heads * 2 * head_size);
+        if (e == hipSuccess) e = alloc(&h->keys_by_dim, gdn_runs(rows) * key_heads * head_size * 2 * kGdnRun);
+        if (e == hipSuccess) e = alloc(&h->through, rows * value_heads * 2 * head_size);
+        if (e == hipSuccess) e = alloc(&h->inner, rows * value_heads * 2 * kGdnChunk);
+        if (e == hipSuccess) e = alloc(&h->values, rows * value_heads * head_size);
         if (e == hipSuccess) e = alloc(&h->decay, rows * value_heads);
         if (e == hipSuccess) e = alloc(&h->rate, rows * value_heads);
     }
@@ -257,9 +262,12 @@ int fortai_hip_gdn_run_device(fortai_hip_gdn_cache *h, int layer, const fortai_h
     p.out_row = output_pitch;
     p.eps = epsilon;
     p.arrivals = h->arrivals;
-    p.rows = h->rows;
+    p.pairs = aligned(qkv, 2 * dtype_bytes(dtype)) && qkv_pitch % 2 == 0;
+    p.asks = h->asks;
+    p.keys_by_dim = h->keys_by_dim;
     p.through = h->through;
     p.inner = h->inner;
+    p.values = h->values;
     p.decay = h->decay;
     p.rate = h->rate;
     p.stands = h->stands;

@@ -3,46 +3,129 @@
 //
 // With c_i the sum of the chunk's logarithmic decays up to row i, S the state before the
 // chunk and d_i the updates (gdn_rows.hip has the recurrence):
-//   A_ij = b_i exp(c_i - c_j) k_i.k_j  (j < i)
-//   (I + A) W = diag(b exp(c)) K,  (I + A) U = diag(b) V
+//   A_ij = b_i exp(c_i - c_j) k_i.k_j  (j < i),  T = (I + A)^-1
+//   W = T diag(b exp(c)) K,  U = T diag(b) V
 //   D = U - W S^T,  O = diag(exp(c)) Q S^T + tril(exp(c_i - c_j) q_i.k_j) D
 //   S <- exp(c_n) S + sum_j exp(c_n - c_j) d_j k_j^T
 // Only the last two lines go from chunk to chunk.  Three launches: convolution, norms and
 // gates of all rows; W, U and the weights of every chunk and head at once; then the
-// states through their chunks, a workgroup 16 value dims of a head, whose part of S stays
-// in registers.
+// states through their chunks, a workgroup 16 or 32 value dims of a head, whose part of S
+// stays in registers.
+//
+// Products run in fp16 matrix instructions with fp32 sums: an operand is two numbers,
+// x 2^10 = h + l, and h h + h l + l h keeps 22 bits of either (three instructions of a
+// sixteenth of the fp32 one's time each).  That is as exact as the sums' own fp32
+// rounding, if x is not far below the largest of its kind: q, k, W, T and the weights are
+// at most 1 (a row's update answers any value at most its own size: the rule is a
+// contraction); V, S and D have any size, and are held against a power of two of their
+// column's largest, for every 32 (16, heads of 64) key dims of S and every 16 rows of D,
+// which are a wave's own.  S itself, the updates and all sums are fp32.
 //
 // The sums c are taken in 64 bits: far into a decay they are large, and their differences
-// are not.  Products are in fp32 matrix instructions.
+// are not.
 #include "gdn_device.h"
+
+#include <type_traits>
 
 namespace fortai_hip {
 
 namespace {
 
-constexpr int kRun = 16;  // rows that a wave of the first launch takes
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ f32x4_t mfma4(f32x4_t a, f32x4_t b, f32x4_t c) {
-    // the four elements are the four k indexes of lane group g, the same ones on both sides
+constexpr int kRun = kGdnRun;       // rows that a wave of the first launch takes
+constexpr float kOne = 1024.0f;     // 2^10
+constexpr float kProduct = 1.0f / (kOne * kOne);
+
+template <typename V>
+struct Pair {
+    V h, l;
+};
+typedef Pair<f16x4_t> Pair4;
+typedef Pair<f16x8_t> Pair8;
+
+// scaled: x times what brings it to 2^10 at most.  It is rounded to fp32 before anything is
+// done with it: the compiler folds a multiplication into a conversion to fp16 (one
+// rounding), but not into every use of it, and a lower half that is left over from
+// another upper half is off by a whole step.
+__device__ __forceinline__ void split(float scaled, _Float16 &h, _Float16 &l) {
+    asm("" : "+v"(scaled));
+    h = static_cast<_Float16>(scaled);
+    l = static_cast<_Float16>(scaled - static_cast<float>(h));
+}
+
+__device__ __forceinline__ Pair4 split4(f32x4_t scaled) {
+    Pair4 p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 h, l;
+        split(scaled[e], h, l);
+        p.h[e] = h;
+        p.l[e] = l;
+    }
+    return p;
+}
+
+__device__ __forceinline__ f32x4_t product(const Pair4 &a, const Pair4 &b, f32x4_t c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, b.l, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a.h, b.h, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t product(const Pair8 &a, const Pair8 &b, f32x4_t c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.l, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
+}
+
+// the four elements are the four k indexes of lane group g, the same ones on both sides
+__device__ __forceinline__ f32x4_t product32(f32x4_t a, f32x4_t b, f32x4_t c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
 }
 
+template <typename V>
+__device__ __forceinline__ Pair<V> load_pair(const _Float16 *at, int apart) {
+    return Pair<V>{*reinterpret_cast<const V *>(at), *reinterpret_cast<const V *>(at + apart)};
+}
+
+// The power of two that brings numbers up to `top` to 2^10 at most, and back (1 for nothing).
+struct Scale {
+    float to, from;
+    __device__ __forceinline__ explicit Scale(float top) {
+        const int e = top > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 128) : 0;
+        to = __builtin_ldexpf(kOne, -e);
+        from = __builtin_ldexpf(kProduct, e);
+    }
+};
+
+__device__ __forceinline__ float largest(f32x4_t x) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); }
+// over the four lane groups that share a column
+__device__ __forceinline__ float largest_of_column(float x) {
+    x = fmaxf(x, xor_lane<16>(x));
+    return fmaxf(x, xor_lane<32>(x));
+}
+
 __device__ __forceinline__ bool gdn_is_many(const GdnSequence &s) { return s.count > kGdnFewRows && s.slot >= 0; }
 
-// Convolution, norms and gates: a wave has one head of q, k or v, or every gate, of a run.
+// Where the transposed keys of the 16 rows from `row` on are kept.  Sequences of more than
+// 16 rows begin at least 17 apart, so no two runs have the same place.
+__device__ __forceinline__ int64_t run_place(const GdnSequence &s, int64_t row) { return row / kRun + s.begin / (kRun + 1); }
+
+// Convolution, norms and gates: a wave has 128 channels (two a lane) of a run, or every gate.
 template <Dtype DT, int D>
 __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
-    constexpr int kMine = D / 64;
-    const int lane = threadIdx.x & 63, head = blockIdx.x * 4 + (threadIdx.x >> 6), seq = blockIdx.z;
+    typedef E E2 __attribute__((ext_vector_type(2)));
+    const int lane = threadIdx.x & 63, part = blockIdx.x * 4 + (threadIdx.x >> 6), seq = blockIdx.z;
     const GdnView &c = p.cache;
     GdnSequence s = gdn_sequence(p, seq);
     if (!gdn_is_many(s)) return;
-    const int i0 = blockIdx.y * kRun, rows = min(s.count - i0, kRun), heads = 2 * c.key_heads + c.value_heads;
-    if (rows <= 0 || head > heads) return;
-    if (head == heads) {
+    const int i0 = blockIdx.y * kRun, rows = min(s.count - i0, kRun), channels = c.channels(), parts = (channels + 127) / 128;
+    if (rows <= 0 || part > parts) return;
+    if (part == parts) {
         for (int at = lane; at < rows * c.value_heads; at += 64) {
             const int64_t row = s.begin + i0 + at / c.value_heads;
             const int h = at % c.value_heads;
@@ -53,93 +136,111 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
         }
         return;
     }
-    const int channels = c.channels(), before = c.taps - 1, first = kGdnMaxTaps - c.taps;
+    const int before = c.taps - 1, first = kGdnMaxTaps - c.taps;
     if (i0 == 0) s.stands = gdn_stands(p, s);
-    float x[kGdnMaxTaps - 1 + kRun][kMine], w[kGdnMaxTaps][kMine];
+    // heads of 64: the last wave may have one head only (its other lanes repeat it and store nothing)
+    const bool mine = part * 128 + 2 * lane < channels;
+    const int channel = mine ? part * 128 + 2 * lane : channels - D + (2 * lane) % D;
+    f32x2_t x[kGdnMaxTaps - 1 + kRun], w[kGdnMaxTaps];
+    const E *rows_at = static_cast<const E *>(p.qkv) + channel;
 #pragma unroll
     for (int j = 0; j < kGdnMaxTaps - 1 + kRun; ++j) {
         const int row = i0 + j - (kGdnMaxTaps - 1);
-#pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            const int channel = head * D + 64 * k + lane;
-            x[j][k] = 0.0f;
-            if (row >= 0) {
-                x[j][k] = static_cast<float>(static_cast<const E *>(p.qkv)[(s.begin + min(row, s.count - 1)) * p.qkv_row + channel]);
-            } else if (row >= -before && !s.begins) {
-                x[j][k] = c.inputs[(static_cast<int64_t>(s.slot) * (before + c.pending) + s.stands + before + row) * channels + channel];
+        x[j] = f32x2_t{0.0f, 0.0f};
+        if (row >= 0) {
+            const E *at = rows_at + (s.begin + min(row, s.count - 1)) * p.qkv_row;
+            if (p.pairs) {
+                const E2 v = *reinterpret_cast<const E2 *>(at);
+                x[j] = f32x2_t{static_cast<float>(v[0]), static_cast<float>(v[1])};
+            } else {
+                x[j] = f32x2_t{static_cast<float>(at[0]), static_cast<float>(at[1])};
             }
+        } else if (row >= -before && !s.begins) {
+            const float *at = c.inputs + (static_cast<int64_t>(s.slot) * (before + c.pending) + s.stands + before + row) * channels + channel;
+            x[j] = f32x2_t{at[0], at[1]};
         }
     }
 #pragma unroll
-    for (int j = 0; j < kGdnMaxTaps; ++j)
-#pragma unroll
-        for (int k = 0; k < kMine; ++k)
-            w[j][k] = j >= first ? p.conv[static_cast<int64_t>(head * D + 64 * k + lane) * c.taps + j - first] : 0.0f;
+    for (int j = 0; j < kGdnMaxTaps; ++j) {
+        const float *at = p.conv + static_cast<int64_t>(channel) * c.taps + j - first;
+        w[j] = j >= first ? f32x2_t{at[0], at[c.taps]} : f32x2_t{0.0f, 0.0f};
+    }
+    const int head = channel / D, dim = channel % D;
+    const bool is_value = head >= 2 * c.key_heads, is_key = !is_value && head >= c.key_heads;
+    const int64_t row0 = s.begin + i0;
+    f16x2_t th[kRun], tl[kRun];  // the keys' halves
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-        if (i >= rows) break;
-        float y[kMine], sum = 0.0f;
+        f32x2_t y = {0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            float u = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kGdnMaxTaps; ++j)
-                if (j >= first) u = __builtin_fmaf(w[j][k], x[i + j][k], u);
-            y[k] = gdn_silu(u);
-            sum += y[k] * y[k];
+        for (int j = 0; j < kGdnMaxTaps; ++j)
+            if (j >= first) y = f32x2_t{__builtin_fmaf(w[j][0], x[i + j][0], y[0]), __builtin_fmaf(w[j][1], x[i + j][1], y[1])};
+        y = f32x2_t{gdn_silu(y[0]), gdn_silu(y[1])};
+        if (is_value) {
+            if (mine && i < rows)
+                *reinterpret_cast<f32x2_t *>(p.values + (row0 + i) * (c.value_heads * D) + channel - 2 * c.key_heads * D) = y;
         }
-        if (head < 2 * c.key_heads) {
-            float inverse = 1.0f / fmaxf(sqrtf(wave_sum(sum)), p.eps);
-            if (head < c.key_heads) inverse *= 1.0f / sqrtf(static_cast<float>(D));
+        const float sum = group_sum_up(y[0] * y[0] + y[1] * y[1], D / 2);
+        float inverse = kOne / fmaxf(sqrtf(sum), p.eps);
+        if (!is_key) inverse *= 1.0f / sqrtf(static_cast<float>(D));
+        const f32x2_t k = {y[0] * inverse, y[1] * inverse};
 #pragma unroll
-            for (int k = 0; k < kMine; ++k) y[k] *= inverse;
+        for (int k2 = 0; k2 < 2; ++k2) {
+            _Float16 high, low;
+            split(k[k2], high, low);
+            th[i][k2] = high;
+            tl[i][k2] = low;
         }
+        if (!is_value && mine && i < rows) {
+            _Float16 *to = p.asks + ((row0 + i) * 2 * c.key_heads + head) * (2 * D) + dim;
+            *reinterpret_cast<f16x2_t *>(to) = th[i];
+            *reinterpret_cast<f16x2_t *>(to + D) = tl[i];
+        }
+    }
+    if (is_key && mine) {  // rows past the last are never used: their updates are zero, these are finite
+        _Float16 *to = p.keys_by_dim + ((run_place(s, row0) * c.key_heads + head - c.key_heads) * D + dim) * (2 * kRun);
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) p.rows[static_cast<int64_t>(s.begin + i0 + i) * channels + head * D + 64 * k + lane] = y[k];
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int part8 = 0; part8 < 2; ++part8) {
+                f16x8_t h, l;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h[e] = th[8 * part8 + e][k];
+                    l[e] = tl[8 * part8 + e][k];
+                }
+                *reinterpret_cast<f16x8_t *>(to + k * 2 * kRun + 8 * part8) = h;
+                *reinterpret_cast<f16x8_t *>(to + k * 2 * kRun + kRun + 8 * part8) = l;
+            }
     }
     if (i0 != 0) return;
     // its own channels' reads of the slot's inputs are done
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) gdn_keep_inputs<E>(p, s, false, head * D + 64 * k + lane);
-    if (head == 0 && lane == 0) p.stands[seq] = s.begins ? -1 : s.stands;
+    if (mine) {
+        gdn_keep_inputs<E>(p, s, false, channel);
+        gdn_keep_inputs<E>(p, s, false, channel + 1);
+    }
+    if (channel == 0 && lane == 0) p.stands[seq] = s.begins ? -1 : s.stands;
 }
 
 // W, U and the weights of one chunk and value head.
 template <int D>
 __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
-    constexpr int kPitch = D + 4, kPitchA = kGdnChunk + 4;
-    __shared__ __align__(16) float ks[kGdnChunk * kPitch], qs[kGdnChunk * kPitch], as[kGdnChunk * kPitchA];
+    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 8, kSteps = D / 32, kTiles = D / 64;
+    // A, then T in place of its blocks' ends; T with b exp(c) and with b, in halves
+    __shared__ __align__(16) float as[kGdnChunk * kPitch], ts[kGdnChunk * kPitch];
+    __shared__ __align__(16) _Float16 halves[2][2][kGdnChunk * kPitchT];
     __shared__ double sums[kGdnChunk];
     __shared__ float rates[kGdnChunk];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
     const GdnSequence s = gdn_sequence(p, blockIdx.z);
     if (!gdn_is_many(s)) return;
     const int n = min(s.count - static_cast<int>(blockIdx.x) * kGdnChunk, kGdnChunk), h = blockIdx.y;
     if (n <= 0) return;
     const int64_t row0 = s.begin + static_cast<int64_t>(blockIdx.x) * kGdnChunk;
-    const int kh = h / (c.value_heads / c.key_heads), channels = c.channels();
-    const float *base = p.rows + row0 * channels;
+    const int kh = h / (c.value_heads / c.key_heads);
 
-    // the solution's columns: one a thread, W's, then U's
-    const int column = tid % (2 * D);
-    const bool of_u = column >= D;
-    float x[kGdnChunk];
-    if (tid < 2 * D && of_u) {
-        const float *v = base + (2 * c.key_heads + h) * D + column - D;
-#pragma unroll
-        for (int i = 0; i < kGdnChunk; ++i) x[i] = v[static_cast<int64_t>(min(i, n - 1)) * channels];
-    }
-    for (int at = 4 * tid; at < kGdnChunk * D; at += 1024) {
-        const int i = at / D, d = at % D;
-        f32x4_t q = {0.0f, 0.0f, 0.0f, 0.0f}, k = q;
-        if (i < n) {
-            q = *reinterpret_cast<const f32x4_t *>(base + static_cast<int64_t>(i) * channels + kh * D + d);
-            k = *reinterpret_cast<const f32x4_t *>(base + static_cast<int64_t>(i) * channels + (c.key_heads + kh) * D + d);
-        }
-        *reinterpret_cast<f32x4_t *>(qs + i * kPitch + d) = q;
-        *reinterpret_cast<f32x4_t *>(ks + i * kPitch + d) = k;
-    }
     if (wave == 0) {
         const int64_t at = (row0 + min(lane, n - 1)) * c.value_heads + h;
         double sum = lane < n ? static_cast<double>(p.decay[at]) : 0.0;
@@ -157,180 +258,355 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
             p.rate[at] = expf(static_cast<float>(all - sum));
         }
     }
-    __syncthreads();
-
-    // k_i.k_j and q_i.k_j of 16 rows i a wave, 16 columns j at a time
-    const int i_of = 16 * wave + 4 * g;
-#pragma unroll 1
-    for (int tile = 0; tile <= wave; ++tile) {
-        f32x4_t kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
+    // k_i.k_j (waves 0 and 1) and q_i.k_j (2 and 3) in tiles of 16 rows i and 16 j: rows 0 and 3, or 1 and 2, five tiles
+    const bool of_queries = wave >= 2;
+    const int row_tiles[2] = {wave & 1, 3 - (wave & 1)};
+    const int64_t row_pitch = 2 * c.key_heads * 2 * D;
+    const auto row_at = [&](int i, bool query) {
+        return p.asks + (row0 + min(i, n - 1)) * row_pitch + (query ? kh : c.key_heads + kh) * (2 * D) + 8 * g;
+    };
+    Pair8 a[2][kSteps];
 #pragma unroll
-        for (int d = 0; d < D; d += 16) {
-            const f32x4_t b = *reinterpret_cast<const f32x4_t *>(ks + (16 * tile + m) * kPitch + d + 4 * g);
-            kk = mfma4(*reinterpret_cast<const f32x4_t *>(ks + (16 * wave + m) * kPitch + d + 4 * g), b, kk);
-            qk = mfma4(*reinterpret_cast<const f32x4_t *>(qs + (16 * wave + m) * kPitch + d + 4 * g), b, qk);
-        }
-        const int j = 16 * tile + m;
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = i_of + e;
-            const float weight = j <= i ? expf(static_cast<float>(sums[i] - sums[j])) : 0.0f;
-            as[i * kPitchA + j] = j < i ? rates[i] * weight * kk[e] : 0.0f;
-            if (i < n) p.inner[((row0 + i) * c.value_heads + h) * kGdnChunk + j] = weight * qk[e];
+        for (int k = 0; k < kSteps; ++k) a[r][k] = load_pair<f16x8_t>(row_at(16 * row_tiles[r] + m, of_queries) + 32 * k, D);
+    f32x4_t dots[2][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        dots[0][t] = dots[1][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (t > row_tiles[1]) continue;
+        Pair8 b[kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) b[k] = load_pair<f16x8_t>(row_at(16 * t + m, false) + 32 * k, D);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (t > row_tiles[r]) continue;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) dots[r][t] = product(a[r][k], b[k], dots[r][t]);
         }
     }
-    __syncthreads();
-
-    if (tid >= 2 * D) return;
+    // this wave's columns of V, on their way
+    const int column = 16 * kTiles * wave + m;
+    float *values = p.values + (row0 * c.value_heads + h) * D + column;
+    f32x4_t v[kTiles][4];
 #pragma unroll
-    for (int i = 0; i < kGdnChunk; ++i) {
-        if (!of_u) x[i] = ks[i * kPitch + column] * expf(static_cast<float>(sums[i]));
-        x[i] *= rates[i];
-    }
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int i = 1; i < kGdnChunk; ++i) {
-#pragma unroll
-        for (int j = 0; j < i; j += 4) {
-            const f32x4_t a = *reinterpret_cast<const f32x4_t *>(as + i * kPitchA + j);
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (j + e < i) x[i] = __builtin_fmaf(-a[e], x[j + e], x[i]);
+                v[t][b][e] = values[static_cast<int64_t>(min(16 * b + 4 * g + e, n - 1)) * (c.value_heads * D) + 16 * t];
+    __syncthreads();  // sums and rates
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (t > row_tiles[r]) continue;
+            const int j = 16 * t + m;
+            const double at_j = sums[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 16 * row_tiles[r] + 4 * g + e;
+                const float weight = (j <= i ? expf(static_cast<float>(sums[i] - at_j)) : 0.0f) * dots[r][t][e];
+                if (!of_queries) {
+                    as[i * kPitch + j] = j < i ? rates[i] * weight * kProduct : 0.0f;
+                } else if (i < n) {
+                    _Float16 *to = p.inner + ((row0 + i) * c.value_heads + h) * (2 * kGdnChunk) + j, high, low;
+                    split(weight * (kProduct * kOne), high, low);
+                    to[0] = high;
+                    to[kGdnChunk] = low;
+                }
+            }
+        }
+    __syncthreads();  // A
+
+    // the inverse of a wave's block on the diagonal, a column a lane
+    {
+        const float *block = as + 16 * wave * kPitch + 16 * wave;
+        float x[16];
+        f32x4_t rows4[16][4];
+#pragma unroll
+        for (int i = 1; i < 16; ++i)
+#pragma unroll
+            for (int q = 0; q < (i + 3) / 4; ++q) rows4[i][q] = *reinterpret_cast<const f32x4_t *>(block + i * kPitch + 4 * q);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = i == m ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+#pragma unroll
+            for (int i = j + 1; i < 16; ++i) x[i] = __builtin_fmaf(-rows4[i][j / 4][j % 4], x[j], x[i]);
+        float *to = ts + 16 * wave * kPitch + 16 * wave + m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i / 4 == g) to[i * kPitch] = x[i];
+    }
+    // below it: T_ij = -T_ii sum_k A_ik T_kj, a distance from the diagonal at a time
+    const auto column_of = [&](int block_row, int block_column) {  // [k = 4 g + e][m]
+        const float *at = ts + (16 * block_row + 4 * g) * kPitch + 16 * block_column + m;
+        return f32x4_t{at[0], at[kPitch], at[2 * kPitch], at[3 * kPitch]};
+    };
+    const auto row_of = [&](const float *matrix, int block_row, int block_column) {  // [m][k = 4 g + e]
+        return *reinterpret_cast<const f32x4_t *>(matrix + (16 * block_row + m) * kPitch + 16 * block_column + 4 * g);
+    };
+#pragma unroll
+    for (int distance = 1; distance < 4; ++distance) {
+        __syncthreads();
+        if (wave + distance < 4) {
+            const int i = wave + distance, j = wave;
+            f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < distance; ++k) sum = product32(row_of(as, i, j + k), column_of(j + k, j), sum);
+            const f32x4_t block = product32(row_of(ts, i, i), sum, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ts[(16 * i + 4 * g + e) * kPitch + 16 * j + m] = -block[e];
         }
     }
-    if (of_u) {
-        float *v = p.rows + row0 * channels + (2 * c.key_heads + h) * D + column - D;
+    __syncthreads();  // T
+    // the columns' factors go into T
+    for (int at = 4 * tid; at < kGdnChunk * kGdnChunk; at += 1024) {
+        const int i = at / kGdnChunk, j = at % kGdnChunk;
+        if (j / 16 > i / 16) continue;
+        const f32x4_t t = *reinterpret_cast<const f32x4_t *>(ts + i * kPitch + j);
+        f32x4_t of_w, of_u;
 #pragma unroll
-        for (int i = 0; i < kGdnChunk; ++i)
-            if (i < n) v[static_cast<int64_t>(i) * channels] = x[i];
-    } else {
-        float *w = p.through + (row0 * c.value_heads + h) * D + column;
+        for (int e = 0; e < 4; ++e) {
+            of_u[e] = t[e] * rates[j + e] * kOne;
+            of_w[e] = of_u[e] * expf(static_cast<float>(sums[j + e]));
+        }
+        const Pair4 w = split4(of_w), u = split4(of_u);
+        *reinterpret_cast<f16x4_t *>(&halves[0][0][i * kPitchT + j]) = w.h;
+        *reinterpret_cast<f16x4_t *>(&halves[0][1][i * kPitchT + j]) = w.l;
+        *reinterpret_cast<f16x4_t *>(&halves[1][0][i * kPitchT + j]) = u.h;
+        *reinterpret_cast<f16x4_t *>(&halves[1][1][i * kPitchT + j]) = u.l;
+    }
+    // this wave's columns of V as operands, and of K
+    float from[kTiles];
+    Pair4 vs[kTiles][4], ks[kTiles][4];
 #pragma unroll
-        for (int i = 0; i < kGdnChunk; ++i)
-            if (i < n) w[static_cast<int64_t>(i) * c.value_heads * D] = x[i];
+    for (int t = 0; t < kTiles; ++t) {
+        const Scale scale(largest_of_column(fmaxf(fmaxf(largest(v[t][0]), largest(v[t][1])), fmaxf(largest(v[t][2]), largest(v[t][3])))));
+        from[t] = scale.from;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            vs[t][b] = split4(v[t][b] * scale.to);
+            const int64_t run = run_place(s, row0 + min(16 * b, (n - 1) / 16 * 16));
+            ks[t][b] = load_pair<f16x4_t>(p.keys_by_dim + ((run * c.key_heads + kh) * D + column + 16 * t) * (2 * kRun) + 4 * g, kRun);
+        }
+    }
+    __syncthreads();
+    const auto half_at = [&](int which, int i, int b) {
+        const int at = (16 * i + m) * kPitchT + 16 * b + 4 * g;
+        return Pair4{*reinterpret_cast<const f16x4_t *>(&halves[which][0][at]), *reinterpret_cast<const f16x4_t *>(&halves[which][1][at])};
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f32x4_t w[kTiles], u[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) w[t] = u[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b <= i; ++b) {
+            const Pair4 of_w = half_at(0, i, b), of_u = half_at(1, i, b);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                w[t] = product(of_w, ks[t][b], w[t]);
+                u[t] = product(of_u, vs[t][b], u[t]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * i + 4 * g + e;
+            if (row >= n) continue;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                values[static_cast<int64_t>(row) * (c.value_heads * D) + 16 * t] = u[t][e] * from[t];
+                _Float16 *to = p.through + ((row0 + row) * c.value_heads + h) * (2 * D) + column + 16 * t, high, low;
+                split(w[t][e] * (kProduct * kOne), high, low);
+                to[0] = high;
+                to[D] = low;
+            }
+        }
     }
 }
 
-// The state of 16 value dims of a head through a sequence's chunks.  In the matrix
-// instructions' results a lane has value dim m and four key dims (of S) or rows (of D and O).
-template <Dtype DT, int D>
+// The state of 16 NT value dims of a head through a sequence's chunks.  In the matrix
+// instructions' results a lane has value dim m and four key dims (of S) or rows (of D and
+// O).  A wave has 16 rows of the chunk and a quarter of the key dims.
+template <Dtype DT, int D, int NT>
 __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
-    constexpr int kSlices = D / 16, kTiles = D / 64, kPitch = D + 4, kPitchD = kGdnChunk + 4;
-    __shared__ __align__(16) float ss[16 * kPitch], ds[16 * kPitchD], rest[16 * kPitchD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+    constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8;
+    // an operand takes a wave's key dims at once: 32, or 16 of heads of 64
+    typedef std::conditional_t<D == 128, f16x8_t, f16x4_t> Ask;
+    constexpr int kAsk = D == 128 ? 8 : 4;
+    __shared__ __align__(16) _Float16 sh[2][16 * NT * kPitch], dh[2][16 * NT * kPitchD], rh[2][16 * NT * kPitchD];
+    __shared__ float s_from[4][16 * NT], d_from[4][16 * NT], r_from[4][16 * NT];
+    const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
     const GdnSequence s = gdn_sequence(p, blockIdx.y);
     if (!gdn_is_many(s)) return;
+    // a head's slices on one die, whose L2 then serves them all
     const int blocks = gridDim.x, block = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-    const int h = block / kSlices, r0 = (block % kSlices) * 16;
-    const int kh = h / (c.value_heads / c.key_heads), channels = c.channels();
+    const int h = block / kSlices, r0 = (block % kSlices) * 16 * NT;
+    const int kh = h / (c.value_heads / c.key_heads);
     const int stands = p.stands[blockIdx.y];
 
-    f32x4_t S[kTiles];
+    f32x4_t S[NT][kTiles];
     float *state = c.states + ((static_cast<int64_t>(s.slot) * c.value_heads + h) * D + r0 + m) * D + 16 * kTiles * wave + 4 * g;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-        S[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (stands >= 0) S[t] = *reinterpret_cast<const f32x4_t *>(state + 16 * t);
-    }
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            S[u][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (stands >= 0) S[u][t] = *reinterpret_cast<const f32x4_t *>(state + 16 * u * D + 16 * t);
+        }
 #pragma unroll 1
     for (int i = 0; i < stands; ++i) {  // the pending rows that stand
         const int64_t row = static_cast<int64_t>(s.slot) * c.pending + i;
-        const float a = c.decays[row * c.value_heads + h], d = c.updates[(row * c.value_heads + h) * D + r0 + m];
+        const float a = c.decays[row * c.value_heads + h];
+        const float *d = c.updates + (row * c.value_heads + h) * D + r0 + m;
         const float *k = c.keys + (row * c.key_heads + kh) * D + 16 * kTiles * wave + 4 * g;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) S[t] = S[t] * a + d * *reinterpret_cast<const f32x4_t *>(k + 16 * t);
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) S[u][t] = S[u][t] * a + d[16 * u] * *reinterpret_cast<const f32x4_t *>(k + 16 * t);
     }
     if (h == 0 && r0 == 0 && tid == 0) c.counts[s.slot] = 0;
 
-    f32x4_t w[D / 16], q[D / 16];
-    const auto load_asked = [&](int64_t row0, int n) {
-        const int64_t row = row0 + min(16 * wave + m, n - 1);
-        const float *w_at = p.through + (row * c.value_heads + h) * D + 4 * g;
-        const float *q_at = p.rows + row * channels + kh * D + 4 * g;
+    // a chunk's operands are asked for as soon as the one before has used its own
+    Pair<Ask> w[4], q[4];
+    const auto load_asks = [&](int i0) {
+        const int64_t row = s.begin + min(i0 + 16 * wave + m, s.count - 1);
+        const _Float16 *w_at = p.through + (row * c.value_heads + h) * (2 * D) + kAsk * g;
+        const _Float16 *q_at = p.asks + (row * 2 * c.key_heads + kh) * (2 * D) + kAsk * g;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-            w[d] = *reinterpret_cast<const f32x4_t *>(w_at + 16 * d);
-            q[d] = *reinterpret_cast<const f32x4_t *>(q_at + 16 * d);
+        for (int k = 0; k < 4; ++k) {
+            w[k] = load_pair<Ask>(w_at + 4 * kAsk * k, D);
+            q[k] = load_pair<Ask>(q_at + 4 * kAsk * k, D);
         }
     };
-    load_asked(s.begin, min(s.count, kGdnChunk));
+    Pair4 inner[4], keys[kTiles][4];
+    float u[NT][4], through[4], left[4], whole;
+    const auto load_rest = [&](int i0) {
+        const int n = min(s.count - i0, kGdnChunk);
+        const int64_t row0 = s.begin + i0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t row = row0 + min(16 * wave + 4 * g + e, n - 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) u[t][e] = p.values[(row * c.value_heads + h) * D + r0 + 16 * t + m];
+            through[e] = p.decay[row * c.value_heads + h];
+            left[e] = p.rate[row * c.value_heads + h];
+        }
+        whole = p.decay[(row0 + n - 1) * c.value_heads + h];
+        const _Float16 *inner_at = p.inner + ((row0 + min(16 * wave + m, n - 1)) * c.value_heads + h) * (2 * kGdnChunk) + 4 * g;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            inner[b] = load_pair<f16x4_t>(inner_at + 16 * min(b, wave), kGdnChunk);
+            const int64_t run = run_place(s, row0 + min(16 * b, (n - 1) / 16 * 16));
+            const _Float16 *k = p.keys_by_dim + ((run * c.key_heads + kh) * D + 16 * kTiles * wave + m) * (2 * kRun) + 4 * g;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) keys[t][b] = load_pair<f16x4_t>(k + 16 * t * (2 * kRun), kRun);
+        }
+    };
+    load_asks(0);
+    load_rest(0);
 #pragma unroll 1
     for (int i0 = 0; i0 < s.count; i0 += kGdnChunk) {
         const int n = min(s.count - i0, kGdnChunk);
         const int64_t row0 = s.begin + i0;
+        const bool more = i0 + kGdnChunk < s.count;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4_t *>(ss + m * kPitch + 16 * (kTiles * wave + t) + 4 * g) = S[t];
-        // what the chunk needs later on
-        float u[4], through[4], left[4];
+        for (int t = 0; t < NT; ++t) {
+            float top = largest(S[t][0]);
+            if constexpr (kTiles > 1) top = fmaxf(top, largest(S[t][1]));
+            const Scale scale(largest_of_column(top));
+            if (g == 0) s_from[wave][16 * t + m] = scale.from;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t row = row0 + min(16 * wave + 4 * g + e, n - 1);
-            u[e] = p.rows[row * channels + (2 * c.key_heads + h) * D + r0 + m];
-            through[e] = p.decay[row * c.value_heads + h];
-            left[e] = p.rate[row * c.value_heads + h];
+            for (int k = 0; k < kTiles; ++k) {
+                const Pair4 x = split4(S[t][k] * scale.to);
+                const int at = (16 * t + m) * kPitch + 16 * (kTiles * wave + k) + 4 * g;
+                *reinterpret_cast<f16x4_t *>(&sh[0][at]) = x.h;
+                *reinterpret_cast<f16x4_t *>(&sh[1][at]) = x.l;
+            }
         }
-        const float whole = p.decay[(row0 + n - 1) * c.value_heads + h];
-        f32x4_t inner[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            inner[t] = *reinterpret_cast<const f32x4_t *>(p.inner + ((row0 + min(16 * wave + m, n - 1)) * c.value_heads + h) * kGdnChunk +
-                16 * min(t, wave) + 4 * g);
-        f32x4_t k[kTiles][4];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    k[t][b][e] = p.rows[(row0 + min(16 * b + 4 * g + e, n - 1)) * channels + (c.key_heads + kh) * D +
-                        16 * (kTiles * wave + t) + m];
-        __syncthreads();  // every wave's part of S is there
+        lds_barrier();  // every wave's part of S is there
 
-        f32x4_t asked = {0.0f, 0.0f, 0.0f, 0.0f}, o = asked;
+        f32x4_t asked[NT], o[NT];
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-            const f32x4_t b = *reinterpret_cast<const f32x4_t *>(ss + m * kPitch + 16 * d + 4 * g);
-            asked = mfma4(w[d], b, asked);
-            o = mfma4(q[d], b, o);
+        for (int t = 0; t < NT; ++t) {
+            asked[t] = o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
+                const Pair<Ask> b = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
+                const float from = s_from[k][16 * t + m];
+                const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                asked[t] += product(w[k], b, zero) * from;
+                o[t] += product(q[k], b, zero) * from;
+            }
         }
-        if (i0 + kGdnChunk < s.count) load_asked(row0 + kGdnChunk, min(s.count - i0 - kGdnChunk, kGdnChunk));
-        f32x4_t d, d_left;
+        if (more) load_asks(i0 + kGdnChunk);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            d[e] = 16 * wave + 4 * g + e < n ? u[e] - asked[e] : 0.0f;
-            d_left[e] = d[e] * left[e];
-            o[e] *= through[e];
+        for (int t = 0; t < NT; ++t) {
+            f32x4_t d, d_left;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                d[e] = 16 * wave + 4 * g + e < n ? u[t][e] - asked[t][e] : 0.0f;
+                d_left[e] = d[e] * left[e];
+                o[t][e] *= through[e];
+            }
+            const Scale ds(largest_of_column(largest(d))), rs(largest_of_column(largest(d_left)));
+            const Pair4 x = split4(d * ds.to), y = split4(d_left * rs.to);
+            const int at = (16 * t + m) * kPitchD + 16 * wave + 4 * g;
+            *reinterpret_cast<f16x4_t *>(&dh[0][at]) = x.h;
+            *reinterpret_cast<f16x4_t *>(&dh[1][at]) = x.l;
+            *reinterpret_cast<f16x4_t *>(&rh[0][at]) = y.h;
+            *reinterpret_cast<f16x4_t *>(&rh[1][at]) = y.l;
+            if (g == 0) {
+                d_from[wave][16 * t + m] = ds.from;
+                r_from[wave][16 * t + m] = rs.from;
+            }
         }
-        *reinterpret_cast<f32x4_t *>(ds + m * kPitchD + 16 * wave + 4 * g) = d;
-        *reinterpret_cast<f32x4_t *>(rest + m * kPitchD + 16 * wave + 4 * g) = d_left;
-        __syncthreads();  // every wave's updates are there, and its reads of S done
+        lds_barrier();  // every wave's updates are there, and its reads of S done
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (t <= wave) o = mfma4(inner[t], *reinterpret_cast<const f32x4_t *>(ds + m * kPitchD + 16 * t + 4 * g), o);
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) S[t] *= whole;
+            for (int k = 0; k < kTiles; ++k) S[t][k] *= whole;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const f32x4_t updates = *reinterpret_cast<const f32x4_t *>(rest + m * kPitchD + 16 * b + 4 * g);
+            for (int b = 0; b < 4; ++b) {
+                const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
+                const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                const Pair4 r = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) S[t] = mfma4(k[t][b], updates, S[t]);
+                for (int k = 0; k < kTiles; ++k) S[t][k] += product(keys[k][b], r, zero) * r_from[b][16 * t + m];
+                if (b <= wave) {
+                    const Pair4 d = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
+                    o[t] += product(inner[b], d, zero) * d_from[b][16 * t + m];
+                }
+            }
         }
+        if (more) load_rest(i0 + kGdnChunk);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = 16 * wave + 4 * g + e;
-            if (i < n) static_cast<E *>(p.out)[(row0 + i) * p.out_row + h * D + r0 + m] = static_cast<E>(o[e]);
+            if (i >= n) continue;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                static_cast<E *>(p.out)[(row0 + i) * p.out_row + h * D + r0 + 16 * t + m] = static_cast<E>(o[t][e]);
         }
     }
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4_t *>(state + 16 * t) = S[t];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < kTiles; ++k) *reinterpret_cast<f32x4_t *>(state + 16 * t * D + 16 * k) = S[t][k];
 }
 
 template <Dtype DT, int D>
 hipError_t many_typed(const GdnRowsParams &p, hipStream_t stream) {
     const GdnView &c = p.cache;
-    const int heads = 2 * c.key_heads + c.value_heads + 1;  // one more for the gates
-    hipLaunchKernelGGL((gdn_inputs_kernel<DT, D>), dim3((heads + 3) / 4, (p.batch.max_rows + kRun - 1) / kRun, p.batch.sequences),
+    const int parts = (c.channels() + 127) / 128 + 1;  // one more for the gates
+    hipLaunchKernelGGL((gdn_inputs_kernel<DT, D>), dim3((parts + 3) / 4, (p.batch.max_rows + kRun - 1) / kRun, p.batch.sequences),
         dim3(256), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -338,7 +614,11 @@ hipError_t many_typed(const GdnRowsParams &p, hipStream_t stream) {
         dim3(256), 0, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((gdn_states_kernel<DT, D>), dim3(c.value_heads * (D / 16), p.batch.sequences), dim3(256), 0, stream, p);
+    // 32 value dims a workgroup where that leaves two workgroups a CU: they read a chunk's operands half as often
+    if (static_cast<int64_t>(p.batch.sequences) * c.value_heads * (D / 32) >= 512)
+        hipLaunchKernelGGL((gdn_states_kernel<DT, D, 2>), dim3(c.value_heads * (D / 32), p.batch.sequences), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((gdn_states_kernel<DT, D, 1>), dim3(c.value_heads * (D / 16), p.batch.sequences), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

@@ -48,6 +48,7 @@ hipError_t launch_logit_rules(const LogitRulesParams &p, Dtype dtype, bool vec, 
 constexpr int kGdnMaxPending = 16;      // rows that may wait for their verdict
 constexpr int kGdnFewRows = 16;         // a sequence's rows up to which the recurrent kernel takes them
 constexpr int kGdnChunk = 64;           // rows of a chunk otherwise
+constexpr int kGdnRun = 16;             // rows whose keys are kept by dims
 constexpr int kGdnMaxSequences = 16384;
 constexpr int kGdnMaxTaps = 8;
 
@@ -79,14 +80,19 @@ struct GdnRowsParams {
     int64_t qkv_row = 0, alpha_row = 0, beta_row = 0, out_row = 0;
     float eps = 0.0f;
     int *arrivals = nullptr;  // [kGdnMaxSequences][key_heads + 1], zeros between calls
-    // of many rows:
-    float *rows = nullptr;    // [rows][channels]: queries (over sqrt(head)), keys, values; then updates without the state
-    float *through = nullptr; // [rows][value_heads][head]: keys that the state is asked with
-    float *inner = nullptr;   // [rows][value_heads][kGdnChunk]: weights of the chunk's updates
+    bool pairs = false;       // qkv allows two-element accesses
+    // of many rows; numbers as two fp16 halves of x 2^10, first all upper ones:
+    _Float16 *asks = nullptr;         // [rows][queries over sqrt(head), keys][key_heads][2][head]
+    _Float16 *keys_by_dim = nullptr;  // [runs][key_heads][head][2][kGdnRun]
+    _Float16 *through = nullptr;      // [rows][value_heads][2][head]: W
+    _Float16 *inner = nullptr;        // [rows][value_heads][2][kGdnChunk]: weights of the chunk's updates
+    float *values = nullptr;          // [rows][value_heads][head]: V, then U
     float *decay = nullptr;   // [rows][value_heads]: logarithms; then summed from the chunk's start
     float *rate = nullptr;    // [rows][value_heads]: beta
     int *stands = nullptr;    // [kGdnMaxSequences]
 };
+// runs of up to `rows` rows (their places: gdn_chunks.hip)
+inline size_t gdn_runs(size_t rows) { return rows / kGdnRun + rows / (kGdnRun + 1) + 1; }
 // few rows of every sequence that has few
 hipError_t launch_gdn_few(const GdnRowsParams &p, Dtype dtype, hipStream_t stream);
 // the others: convolution, norms and gates; products within chunks; the states through them
