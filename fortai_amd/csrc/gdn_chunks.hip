@@ -86,11 +86,6 @@ __device__ __forceinline__ f32x4_t product32(f32x4_t a, f32x4_t b, f32x4_t c) {
     return c;
 }
 
-template <typename V>
-__device__ __forceinline__ Pair<V> load_pair(const _Float16 *at, int apart) {
-    return Pair<V>{*reinterpret_cast<const V *>(at), *reinterpret_cast<const V *>(at + apart)};
-}
-
 // The power of two that brings numbers up to `top` to 2^10 at most, and back (1 for nothing).
 struct Scale {
     float to, from;
@@ -108,21 +103,47 @@ __device__ __forceinline__ float largest_of_column(float x) {
     return fmaxf(x, xor_lane<32>(x));
 }
 
-__device__ __forceinline__ bool gdn_is_many(const GdnSequence &s) { return s.count > kGdnFewRows && s.slot >= 0; }
+__device__ __forceinline__ bool gdn_is_many(const GdnRowsParams &p, const GdnSequence &s) { return s.count > p.few && s.slot >= 0; }
 
-// Where the transposed keys of the 16 rows from `row` on are kept.  Sequences of more than
-// 16 rows begin at least 17 apart, so no two runs have the same place.
+// Operands are kept as the matrix instructions take them, a run (16 rows) of a head at a
+// time, lane after lane, so that a wave's load is one piece of memory: a lane has row or
+// dim m = lane & 15 and, of the index that is summed over, four or eight numbers from lane
+// group g = lane >> 4.  Sequences of more than 16 rows begin at least 17 apart, so that no two
+// runs have the same place.  (One sequence by itself may have fewer.)
 __device__ __forceinline__ int64_t run_place(const GdnSequence &s, int64_t row) { return row / kRun + s.begin / (kRun + 1); }
 
-// Convolution, norms and gates: a wave has 128 channels (two a lane) of a run, or every gate.
-template <Dtype DT, int D>
+template <int D>
+struct Runs {
+    // numbers of a row that a lane has at once, of D key dims in four steps
+    static constexpr int kAsk = D / 16;
+    typedef std::conditional_t<D == 128, f16x8_t, f16x4_t> Ask;
+    static constexpr int kHead = kRun * D * 2;  // halves of a run of a head
+    // queries, keys (rows m) and W: [step][upper, lower][lane][kAsk]
+    static __device__ __forceinline__ Pair<Ask> row_step(const _Float16 *run, int step, int lane) {
+        const _Float16 *at = run + (step * 2 * 64 + lane) * kAsk;
+        return Pair<Ask>{*reinterpret_cast<const Ask *>(at), *reinterpret_cast<const Ask *>(at + 64 * kAsk)};
+    }
+};
+// keys (dims m of a tile) and the weights (rows m, of 16 updates): [lane][upper four, lower four]
+__device__ __forceinline__ Pair4 four_step(const _Float16 *tile, int lane) {
+    const f16x8_t v = *reinterpret_cast<const f16x8_t *>(tile + lane * 8);
+    return Pair4{f16x4_t{v[0], v[1], v[2], v[3]}, f16x4_t{v[4], v[5], v[6], v[7]}};
+}
+__device__ __forceinline__ void store_four_step(_Float16 *tile, int lane, const Pair4 &x) {
+    *reinterpret_cast<f16x8_t *>(tile + lane * 8) = f16x8_t{x.h[0], x.h[1], x.h[2], x.h[3], x.l[0], x.l[1], x.l[2], x.l[3]};
+}
+
+// Convolution, norms and gates: a wave has 128 channels (two a lane) of a run, or every
+// gate.  TAPS: of the convolution, 0: as many as there are.
+template <Dtype DT, int D, int TAPS>
 __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
     typedef E E2 __attribute__((ext_vector_type(2)));
+    constexpr int kTaps = TAPS ? TAPS : kGdnMaxTaps;
     const int lane = threadIdx.x & 63, part = blockIdx.x * 4 + (threadIdx.x >> 6), seq = blockIdx.z;
     const GdnView &c = p.cache;
     GdnSequence s = gdn_sequence(p, seq);
-    if (!gdn_is_many(s)) return;
+    if (!gdn_is_many(p, s)) return;
     const int i0 = blockIdx.y * kRun, rows = min(s.count - i0, kRun), channels = c.channels(), parts = (channels + 127) / 128;
     if (rows <= 0 || part > parts) return;
     if (part == parts) {
@@ -136,16 +157,16 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
         }
         return;
     }
-    const int before = c.taps - 1, first = kGdnMaxTaps - c.taps;
+    const int taps = TAPS ? TAPS : c.taps, before = taps - 1, first = kTaps - taps;
     if (i0 == 0) s.stands = gdn_stands(p, s);
     // heads of 64: the last wave may have one head only (its other lanes repeat it and store nothing)
     const bool mine = part * 128 + 2 * lane < channels;
     const int channel = mine ? part * 128 + 2 * lane : channels - D + (2 * lane) % D;
-    f32x2_t x[kGdnMaxTaps - 1 + kRun], w[kGdnMaxTaps];
+    f32x2_t x[kTaps - 1 + kRun], w[kTaps];
     const E *rows_at = static_cast<const E *>(p.qkv) + channel;
 #pragma unroll
-    for (int j = 0; j < kGdnMaxTaps - 1 + kRun; ++j) {
-        const int row = i0 + j - (kGdnMaxTaps - 1);
+    for (int j = 0; j < kTaps - 1 + kRun; ++j) {
+        const int row = i0 + j - (kTaps - 1);
         x[j] = f32x2_t{0.0f, 0.0f};
         if (row >= 0) {
             const E *at = rows_at + (s.begin + min(row, s.count - 1)) * p.qkv_row;
@@ -161,57 +182,61 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
         }
     }
 #pragma unroll
-    for (int j = 0; j < kGdnMaxTaps; ++j) {
-        const float *at = p.conv + static_cast<int64_t>(channel) * c.taps + j - first;
-        w[j] = j >= first ? f32x2_t{at[0], at[c.taps]} : f32x2_t{0.0f, 0.0f};
+    for (int j = 0; j < kTaps; ++j) {
+        const float *at = p.conv + static_cast<int64_t>(channel) * taps + j - first;
+        w[j] = j >= first ? f32x2_t{at[0], at[taps]} : f32x2_t{0.0f, 0.0f};
     }
     const int head = channel / D, dim = channel % D;
     const bool is_value = head >= 2 * c.key_heads, is_key = !is_value && head >= c.key_heads;
-    const int64_t row0 = s.begin + i0;
-    f16x2_t th[kRun], tl[kRun];  // the keys' halves
+    const int64_t run = run_place(s, s.begin + i0);
+    const float root = kOne / sqrtf(static_cast<float>(D));
+    _Float16 *asks = p.asks + (run * 2 * c.key_heads + (is_value ? 0 : head)) * Runs<D>::kHead;
+    // step, lane group and place of this lane's dims
+    constexpr int kAsk = Runs<D>::kAsk;
+    asks += (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16) * kAsk + dim % kAsk;
+    const int tile_at = (dim >> 4) * 64 + (dim & 15);  // the first of its tile's lanes that have this dim
+    _Float16 *by_dim = p.keys_by_dim + (run * c.key_heads + (is_key ? head - c.key_heads : 0)) * Runs<D>::kHead + tile_at * 8;
+    float *values = p.values + (run * c.value_heads + (is_value ? head - 2 * c.key_heads : 0)) * (kRun * D) + tile_at * 4;
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        f32x2_t y = {0.0f, 0.0f};
+    for (int four = 0; four < kRun / 4; ++four) {
+        f32x4_t y[2];  // this lane's dims, four rows
 #pragma unroll
-        for (int j = 0; j < kGdnMaxTaps; ++j)
-            if (j >= first) y = f32x2_t{__builtin_fmaf(w[j][0], x[i + j][0], y[0]), __builtin_fmaf(w[j][1], x[i + j][1], y[1])};
-        y = f32x2_t{gdn_silu(y[0]), gdn_silu(y[1])};
-        if (is_value) {
-            if (mine && i < rows)
-                *reinterpret_cast<f32x2_t *>(p.values + (row0 + i) * (c.value_heads * D) + channel - 2 * c.key_heads * D) = y;
-        }
-        const float sum = group_sum_up(y[0] * y[0] + y[1] * y[1], D / 2);
-        float inverse = kOne / fmaxf(sqrtf(sum), p.eps);
-        if (!is_key) inverse *= 1.0f / sqrtf(static_cast<float>(D));
-        const f32x2_t k = {y[0] * inverse, y[1] * inverse};
+        for (int e = 0; e < 4; ++e) {
+            const int i = 4 * four + e;
+            float u0 = 0.0f, u1 = 0.0f;
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-            _Float16 high, low;
-            split(k[k2], high, low);
-            th[i][k2] = high;
-            tl[i][k2] = low;
-        }
-        if (!is_value && mine && i < rows) {
-            _Float16 *to = p.asks + ((row0 + i) * 2 * c.key_heads + head) * (2 * D) + dim;
-            *reinterpret_cast<f16x2_t *>(to) = th[i];
-            *reinterpret_cast<f16x2_t *>(to + D) = tl[i];
-        }
-    }
-    if (is_key && mine) {  // rows past the last are never used: their updates are zero, these are finite
-        _Float16 *to = p.keys_by_dim + ((run_place(s, row0) * c.key_heads + head - c.key_heads) * D + dim) * (2 * kRun);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int part8 = 0; part8 < 2; ++part8) {
-                f16x8_t h, l;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = th[8 * part8 + e][k];
-                    l[e] = tl[8 * part8 + e][k];
+            for (int j = 0; j < kTaps; ++j)
+                if (j >= first) {
+                    u0 = __builtin_fmaf(w[j][0], x[i + j][0], u0);
+                    u1 = __builtin_fmaf(w[j][1], x[i + j][1], u1);
                 }
-                *reinterpret_cast<f16x8_t *>(to + k * 2 * kRun + 8 * part8) = h;
-                *reinterpret_cast<f16x8_t *>(to + k * 2 * kRun + kRun + 8 * part8) = l;
+            u0 = gdn_silu(u0);
+            u1 = gdn_silu(u1);
+            float inverse = 1.0f;
+            if (!is_value) {
+                const float sum = group_sum_up(u0 * u0 + u1 * u1, D / 2);
+                inverse = (is_key ? kOne : root) / fmaxf(sqrtf(sum), p.eps);
             }
+            y[0][e] = u0 * inverse;
+            y[1][e] = u1 * inverse;
+        }
+        if (!mine) continue;
+        // rows past the last are those of the last inputs again: finite, and their updates are zero
+        if (is_value) {
+            *reinterpret_cast<f32x4_t *>(values + 16 * four * 4) = y[0];
+            *reinterpret_cast<f32x4_t *>(values + 16 * four * 4 + 4) = y[1];
+            continue;
+        }
+        const Pair4 a = split4(y[0]), b = split4(y[1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            *reinterpret_cast<f16x2_t *>(asks + (4 * four + e) * kAsk) = f16x2_t{a.h[e], b.h[e]};
+            *reinterpret_cast<f16x2_t *>(asks + (64 + 4 * four + e) * kAsk) = f16x2_t{a.l[e], b.l[e]};
+        }
+        if (is_key) {
+            store_four_step(by_dim + 16 * four * 8, 0, a);
+            store_four_step(by_dim + 16 * four * 8, 1, b);
+        }
     }
     if (i0 != 0) return;
     // its own channels' reads of the slot's inputs are done
@@ -225,25 +250,26 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
 // W, U and the weights of one chunk and value head.
 template <int D>
 __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
-    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 8, kSteps = D / 32, kTiles = D / 64;
-    // A, then T in place of its blocks' ends; T with b exp(c) and with b, in halves
+    typedef typename Runs<D>::Ask Ask;
+    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 8, kTiles = D / 64, kHead = Runs<D>::kHead;
+    // A, and T; T with b exp(c) and with b, in halves
     __shared__ __align__(16) float as[kGdnChunk * kPitch], ts[kGdnChunk * kPitch];
     __shared__ __align__(16) _Float16 halves[2][2][kGdnChunk * kPitchT];
-    __shared__ double sums[kGdnChunk];
+    __shared__ double sums[kGdnChunk];  // binary logarithms
     __shared__ float rates[kGdnChunk];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
     const GdnSequence s = gdn_sequence(p, blockIdx.z);
-    if (!gdn_is_many(s)) return;
+    if (!gdn_is_many(p, s)) return;
     const int n = min(s.count - static_cast<int>(blockIdx.x) * kGdnChunk, kGdnChunk), h = blockIdx.y;
     if (n <= 0) return;
-    const int64_t row0 = s.begin + static_cast<int64_t>(blockIdx.x) * kGdnChunk;
-    const int kh = h / (c.value_heads / c.key_heads);
+    const int64_t row0 = s.begin + static_cast<int64_t>(blockIdx.x) * kGdnChunk, run0 = run_place(s, row0);
+    const int kh = h / (c.value_heads / c.key_heads), last_run = (n - 1) / kRun;
 
     if (wave == 0) {
         const int64_t at = (row0 + min(lane, n - 1)) * c.value_heads + h;
-        double sum = lane < n ? static_cast<double>(p.decay[at]) : 0.0;
+        double sum = lane < n ? static_cast<double>(p.decay[at]) * 1.4426950408889634 : 0.0;
         const float rate = lane < n ? p.rate[at] : 0.0f;
 #pragma unroll
         for (int step = 1; step < 64; step *= 2) {
@@ -253,71 +279,61 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
         sums[lane] = sum;
         rates[lane] = rate;
         const double all = __shfl(sum, 63);
-        if (lane < n) {  // for the launch that follows
-            p.decay[at] = expf(static_cast<float>(sum));
-            p.rate[at] = expf(static_cast<float>(all - sum));
+        if (lane / kRun <= last_run) {  // for the launch that follows
+            float *to = p.chunk_gates + ((run0 + lane / kRun) * c.value_heads + h) * (2 * kRun) + lane % kRun;
+            to[0] = __builtin_amdgcn_exp2f(static_cast<float>(sum));
+            to[kRun] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum));
         }
     }
-    // k_i.k_j (waves 0 and 1) and q_i.k_j (2 and 3) in tiles of 16 rows i and 16 j: rows 0 and 3, or 1 and 2, five tiles
+    // k_j.k_i (waves 0 and 1) and k_j.q_i (2 and 3) in tiles of 16 j and 16 rows i: rows 0 and 3, or 1 and 2, five tiles
     const bool of_queries = wave >= 2;
-    const int row_tiles[2] = {wave & 1, 3 - (wave & 1)};
-    const int64_t row_pitch = 2 * c.key_heads * 2 * D;
-    const auto row_at = [&](int i, bool query) {
-        return p.asks + (row0 + min(i, n - 1)) * row_pitch + (query ? kh : c.key_heads + kh) * (2 * D) + 8 * g;
-    };
-    Pair8 a[2][kSteps];
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) a[r][k] = load_pair<f16x8_t>(row_at(16 * row_tiles[r] + m, of_queries) + 32 * k, D);
+    const auto run_of = [&](int tile, int head) { return p.asks + ((run0 + min(tile, last_run)) * 2 * c.key_heads + head) * kHead; };
     f32x4_t dots[2][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        dots[0][t] = dots[1][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (t > row_tiles[1]) continue;
-        Pair8 b[kSteps];
+    for (int r = 0; r < 2; ++r) {
+        const int row_tile = r ? 3 - (wave & 1) : wave & 1;
+        Pair<Ask> a[4];
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) b[k] = load_pair<f16x8_t>(row_at(16 * t + m, false) + 32 * k, D);
+        for (int k = 0; k < 4; ++k) a[k] = Runs<D>::row_step(run_of(row_tile, of_queries ? kh : c.key_heads + kh), k, lane);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (t > row_tiles[r]) continue;
+        for (int t = 0; t < 4; ++t) {
+            dots[r][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (t > row_tile || t > r + 2) continue;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) dots[r][t] = product(a[r][k], b[k], dots[r][t]);
+            for (int k = 0; k < 4; ++k)
+                dots[r][t] = product(Runs<D>::row_step(run_of(t, c.key_heads + kh), k, lane), a[k], dots[r][t]);
         }
     }
     // this wave's columns of V, on their way
-    const int column = 16 * kTiles * wave + m;
-    float *values = p.values + (row0 * c.value_heads + h) * D + column;
+    float *values = p.values + (run0 * c.value_heads + h) * (kRun * D) + (kTiles * wave * 64 + lane) * 4;
+    const int64_t run_values = static_cast<int64_t>(c.value_heads) * (kRun * D);
     f32x4_t v[kTiles][4];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[t][b][e] = values[static_cast<int64_t>(min(16 * b + 4 * g + e, n - 1)) * (c.value_heads * D) + 16 * t];
+        for (int b = 0; b < 4; ++b) v[t][b] = *reinterpret_cast<const f32x4_t *>(values + min(b, last_run) * run_values + t * 256);
     __syncthreads();  // sums and rates
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < 2; ++r) {
+        const int row_tile = r ? 3 - (wave & 1) : wave & 1, i = 16 * row_tile + m;
+        const double at_i = sums[i];
+        const float rate = rates[i] * kProduct;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            if (t > row_tiles[r]) continue;
-            const int j = 16 * t + m;
-            const double at_j = sums[j];
+            if (t > row_tile || t > r + 2) continue;
+            f32x4_t x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = 16 * row_tiles[r] + 4 * g + e;
-                const float weight = (j <= i ? expf(static_cast<float>(sums[i] - at_j)) : 0.0f) * dots[r][t][e];
-                if (!of_queries) {
-                    as[i * kPitch + j] = j < i ? rates[i] * weight * kProduct : 0.0f;
-                } else if (i < n) {
-                    _Float16 *to = p.inner + ((row0 + i) * c.value_heads + h) * (2 * kGdnChunk) + j, high, low;
-                    split(weight * (kProduct * kOne), high, low);
-                    to[0] = high;
-                    to[kGdnChunk] = low;
-                }
+                const int j = 16 * t + 4 * g + e;
+                const bool counts = of_queries ? j <= i : j < i;
+                const float weight = __builtin_amdgcn_exp2f(static_cast<float>(at_i - sums[j]));
+                x[e] = counts ? weight * dots[r][t][e] * (of_queries ? kProduct * kOne : rate) : 0.0f;
             }
+            if (!of_queries) *reinterpret_cast<f32x4_t *>(as + i * kPitch + 16 * t + 4 * g) = x;
+            else if (row_tile <= last_run)
+                store_four_step(p.inner + (((run0 + row_tile) * c.value_heads + h) * 4 + t) * (kRun * 32), lane, split4(x));
         }
+    }
     __syncthreads();  // A
 
     // the inverse of a wave's block on the diagonal, a column a lane
@@ -348,13 +364,13 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
     const auto row_of = [&](const float *matrix, int block_row, int block_column) {  // [m][k = 4 g + e]
         return *reinterpret_cast<const f32x4_t *>(matrix + (16 * block_row + m) * kPitch + 16 * block_column + 4 * g);
     };
-#pragma unroll
+#pragma unroll 1
     for (int distance = 1; distance < 4; ++distance) {
         __syncthreads();
         if (wave + distance < 4) {
             const int i = wave + distance, j = wave;
             f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < distance; ++k) sum = product32(row_of(as, i, j + k), column_of(j + k, j), sum);
             const f32x4_t block = product32(row_of(ts, i, i), sum, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
@@ -371,7 +387,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             of_u[e] = t[e] * rates[j + e] * kOne;
-            of_w[e] = of_u[e] * expf(static_cast<float>(sums[j + e]));
+            of_w[e] = of_u[e] * __builtin_amdgcn_exp2f(static_cast<float>(sums[j + e]));
         }
         const Pair4 w = split4(of_w), u = split4(of_u);
         *reinterpret_cast<f16x4_t *>(&halves[0][0][i * kPitchT + j]) = w.h;
@@ -389,8 +405,7 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             vs[t][b] = split4(v[t][b] * scale.to);
-            const int64_t run = run_place(s, row0 + min(16 * b, (n - 1) / 16 * 16));
-            ks[t][b] = load_pair<f16x4_t>(p.keys_by_dim + ((run * c.key_heads + kh) * D + column + 16 * t) * (2 * kRun) + 4 * g, kRun);
+            ks[t][b] = four_step(p.keys_by_dim + ((run0 + min(b, last_run)) * c.key_heads + kh) * kHead + (kTiles * wave + t) * (kRun * 32), lane);
         }
     }
     __syncthreads();
@@ -398,8 +413,11 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
         const int at = (16 * i + m) * kPitchT + 16 * b + 4 * g;
         return Pair4{*reinterpret_cast<const f16x4_t *>(&halves[which][0][at]), *reinterpret_cast<const f16x4_t *>(&halves[which][1][at])};
     };
+    // of W a lane has four key dims of row m, of U four rows of value dim m
+    const int lane_dim = 16 * kTiles * wave + 4 * g, kAsk = Runs<D>::kAsk;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        if (i > last_run) break;
         f32x4_t w[kTiles], u[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) w[t] = u[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -408,22 +426,19 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
             const Pair4 of_w = half_at(0, i, b), of_u = half_at(1, i, b);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
-                w[t] = product(of_w, ks[t][b], w[t]);
+                w[t] = product(ks[t][b], of_w, w[t]);
                 u[t] = product(of_u, vs[t][b], u[t]);
             }
         }
+        _Float16 *through = p.through + ((run0 + i) * c.value_heads + h) * kHead;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * i + 4 * g + e;
-            if (row >= n) continue;
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                values[static_cast<int64_t>(row) * (c.value_heads * D) + 16 * t] = u[t][e] * from[t];
-                _Float16 *to = p.through + ((row0 + row) * c.value_heads + h) * (2 * D) + column + 16 * t, high, low;
-                split(w[t][e] * (kProduct * kOne), high, low);
-                to[0] = high;
-                to[D] = low;
-            }
+        for (int t = 0; t < kTiles; ++t) {
+            *reinterpret_cast<f32x4_t *>(values + i * run_values + t * 256) = u[t] * from[t];
+            const Pair4 x = split4(w[t] * (kProduct * kOne));
+            const int dim = lane_dim + 16 * t;
+            _Float16 *to = through + (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16 + m) * kAsk + dim % kAsk;
+            *reinterpret_cast<f16x4_t *>(to) = x.h;
+            *reinterpret_cast<f16x4_t *>(to + 64 * kAsk) = x.l;
         }
     }
 }
@@ -434,17 +449,16 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
 template <Dtype DT, int D, int NT>
 __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
-    constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8;
-    // an operand takes a wave's key dims at once: 32, or 16 of heads of 64
-    typedef std::conditional_t<D == 128, f16x8_t, f16x4_t> Ask;
-    constexpr int kAsk = D == 128 ? 8 : 4;
+    typedef typename Runs<D>::Ask Ask;
+    constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8, kAsk = Runs<D>::kAsk;
+    constexpr int kHead = Runs<D>::kHead;
     __shared__ __align__(16) _Float16 sh[2][16 * NT * kPitch], dh[2][16 * NT * kPitchD], rh[2][16 * NT * kPitchD];
     __shared__ float s_from[4][16 * NT], d_from[4][16 * NT], r_from[4][16 * NT];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
     const GdnSequence s = gdn_sequence(p, blockIdx.y);
-    if (!gdn_is_many(s)) return;
+    if (!gdn_is_many(p, s)) return;
     // a head's slices on one die, whose L2 then serves them all
     const int blocks = gridDim.x, block = blocks % 8 == 0 ? (blockIdx.x % 8) * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
     const int h = block / kSlices, r0 = (block % kSlices) * 16 * NT;
@@ -474,48 +488,50 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
     if (h == 0 && r0 == 0 && tid == 0) c.counts[s.slot] = 0;
 
     // a chunk's operands are asked for as soon as the one before has used its own
+    const int64_t run_first = run_place(s, s.begin);
+    const int last_run = (s.count - 1) / kRun;
+    const auto run_at = [&](int run) { return run_first + min(run, last_run); };
     Pair<Ask> w[4], q[4];
-    const auto load_asks = [&](int i0) {
-        const int64_t row = s.begin + min(i0 + 16 * wave + m, s.count - 1);
-        const _Float16 *w_at = p.through + (row * c.value_heads + h) * (2 * D) + kAsk * g;
-        const _Float16 *q_at = p.asks + (row * 2 * c.key_heads + kh) * (2 * D) + kAsk * g;
+    const auto load_asks = [&](int run0) {
+        const int64_t run = run_at(run0 + wave);
+        const _Float16 *w_at = p.through + (run * c.value_heads + h) * kHead, *q_at = p.asks + (run * 2 * c.key_heads + kh) * kHead;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            w[k] = load_pair<Ask>(w_at + 4 * kAsk * k, D);
-            q[k] = load_pair<Ask>(q_at + 4 * kAsk * k, D);
+            w[k] = Runs<D>::row_step(w_at, k, lane);
+            q[k] = Runs<D>::row_step(q_at, k, lane);
         }
     };
+    f32x4_t u[NT], through, left;
+    float whole;
+    const auto load_updates = [&](int run0) {
+        const int64_t at = run_at(run0 + wave) * c.value_heads + h;
+        through = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + 4 * g);
+        left = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + kRun + 4 * g);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) u[t] = *reinterpret_cast<const f32x4_t *>(p.values + at * (kRun * D) + ((r0 / 16 + t) * 64 + lane) * 4);
+    };
     Pair4 inner[4], keys[kTiles][4];
-    float u[NT][4], through[4], left[4], whole;
-    const auto load_rest = [&](int i0) {
-        const int n = min(s.count - i0, kGdnChunk);
-        const int64_t row0 = s.begin + i0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t row = row0 + min(16 * wave + 4 * g + e, n - 1);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) u[t][e] = p.values[(row * c.value_heads + h) * D + r0 + 16 * t + m];
-            through[e] = p.decay[row * c.value_heads + h];
-            left[e] = p.rate[row * c.value_heads + h];
-        }
-        whole = p.decay[(row0 + n - 1) * c.value_heads + h];
-        const _Float16 *inner_at = p.inner + ((row0 + min(16 * wave + m, n - 1)) * c.value_heads + h) * (2 * kGdnChunk) + 4 * g;
+    const auto load_rest = [&](int run0) {
+        const int row = min(s.count - 1, run0 * kRun + kGdnChunk - 1);
+        whole = p.chunk_gates[((run_first + row / kRun) * c.value_heads + h) * (2 * kRun) + row % kRun];
+        const _Float16 *inner_at = p.inner + (run_at(run0 + wave) * c.value_heads + h) * (4 * kRun * 32);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            inner[b] = load_pair<f16x4_t>(inner_at + 16 * min(b, wave), kGdnChunk);
-            const int64_t run = run_place(s, row0 + min(16 * b, (n - 1) / 16 * 16));
-            const _Float16 *k = p.keys_by_dim + ((run * c.key_heads + kh) * D + 16 * kTiles * wave + m) * (2 * kRun) + 4 * g;
+            inner[b] = four_step(inner_at + min(b, wave) * (kRun * 32), lane);
+            const _Float16 *k = p.keys_by_dim + (run_at(run0 + b) * c.key_heads + kh) * kHead + kTiles * wave * (kRun * 32);
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) keys[t][b] = load_pair<f16x4_t>(k + 16 * t * (2 * kRun), kRun);
+            for (int t = 0; t < kTiles; ++t) keys[t][b] = four_step(k + t * (kRun * 32), lane);
         }
     };
     load_asks(0);
+    load_updates(0);
     load_rest(0);
+    E *out = static_cast<E *>(p.out) + (s.begin + static_cast<int64_t>(16 * wave + 4 * g)) * p.out_row + h * D + r0 + m;
 #pragma unroll 1
     for (int i0 = 0; i0 < s.count; i0 += kGdnChunk) {
-        const int n = min(s.count - i0, kGdnChunk);
-        const int64_t row0 = s.begin + i0;
+        const int mine = s.count - i0 - 16 * wave - 4 * g;  // this lane's rows that are there
         const bool more = i0 + kGdnChunk < s.count;
+        const int next = i0 / kRun + 4;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float top = largest(S[t][0]);
@@ -546,13 +562,13 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                 o[t] += product(q[k], b, zero) * from;
             }
         }
-        if (more) load_asks(i0 + kGdnChunk);
+        if (more) load_asks(next);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             f32x4_t d, d_left;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                d[e] = 16 * wave + 4 * g + e < n ? u[t][e] - asked[t][e] : 0.0f;
+                d[e] = e < mine ? u[t][e] - asked[t][e] : 0.0f;
                 d_left[e] = d[e] * left[e];
                 o[t][e] *= through[e];
             }
@@ -568,6 +584,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                 r_from[wave][16 * t + m] = rs.from;
             }
         }
+        if (more) load_updates(next);
         lds_barrier();  // every wave's updates are there, and its reads of S done
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -586,14 +603,13 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                 }
             }
         }
-        if (more) load_rest(i0 + kGdnChunk);
+        if (more) load_rest(next);
+        E *to = out + i0 * p.out_row;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = 16 * wave + 4 * g + e;
-            if (i >= n) continue;
+            if (e >= mine) continue;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                static_cast<E *>(p.out)[(row0 + i) * p.out_row + h * D + r0 + 16 * t + m] = static_cast<E>(o[t][e]);
+            for (int t = 0; t < NT; ++t) to[e * p.out_row + 16 * t] = static_cast<E>(o[t][e]);
         }
     }
 #pragma unroll
@@ -606,8 +622,9 @@ template <Dtype DT, int D>
 hipError_t many_typed(const GdnRowsParams &p, hipStream_t stream) {
     const GdnView &c = p.cache;
     const int parts = (c.channels() + 127) / 128 + 1;  // one more for the gates
-    hipLaunchKernelGGL((gdn_inputs_kernel<DT, D>), dim3((parts + 3) / 4, (p.batch.max_rows + kRun - 1) / kRun, p.batch.sequences),
-        dim3(256), 0, stream, p);
+    const dim3 runs((parts + 3) / 4, (p.batch.max_rows + kRun - 1) / kRun, p.batch.sequences);
+    if (c.taps == 4) hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 4>), runs, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 0>), runs, dim3(256), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((gdn_chunk_kernel<D>), dim3((p.batch.max_rows + kGdnChunk - 1) / kGdnChunk, c.value_heads, p.batch.sequences),

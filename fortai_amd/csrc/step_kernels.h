@@ -81,14 +81,17 @@ struct GdnRowsParams {
     float eps = 0.0f;
     int *arrivals = nullptr;  // [kGdnMaxSequences][key_heads + 1], zeros between calls
     bool pairs = false;       // qkv allows two-element accesses
-    // of many rows; numbers as two fp16 halves of x 2^10, first all upper ones:
-    _Float16 *asks = nullptr;         // [rows][queries over sqrt(head), keys][key_heads][2][head]
-    _Float16 *keys_by_dim = nullptr;  // [runs][key_heads][head][2][kGdnRun]
-    _Float16 *through = nullptr;      // [rows][value_heads][2][head]: W
-    _Float16 *inner = nullptr;        // [rows][value_heads][2][kGdnChunk]: weights of the chunk's updates
-    float *values = nullptr;          // [rows][value_heads][head]: V, then U
-    float *decay = nullptr;   // [rows][value_heads]: logarithms; then summed from the chunk's start
-    float *rate = nullptr;    // [rows][value_heads]: beta
+    int few = kGdnFewRows;    // sequences of more rows go through chunks
+    // of these, a run of 16 rows and a head at a time (gdn_chunks.hip); numbers as two fp16
+    // halves of x 2^10:
+    _Float16 *asks = nullptr;         // [runs][queries over sqrt(head), keys][key_heads], by rows
+    _Float16 *keys_by_dim = nullptr;  // [runs][key_heads], by dims
+    _Float16 *through = nullptr;      // [runs][value_heads]: W, by rows
+    _Float16 *inner = nullptr;        // [runs][value_heads][4]: weights of the chunk's updates, by rows
+    float *values = nullptr;          // [runs][value_heads]: V, then U, by dims
+    float *chunk_gates = nullptr;     // [runs][value_heads][2][kGdnRun]: decays since the chunk's start, and to its end
+    float *decay = nullptr;           // [rows][value_heads]: logarithms
+    float *rate = nullptr;            // [rows][value_heads]: beta
     int *stands = nullptr;    // [kGdnMaxSequences]
 };
 // runs of up to `rows` rows (their places: gdn_chunks.hip)

@@ -72,9 +72,26 @@ class Layer:
         chunked = len(x) > 16 if chunked is None else chunked
         S, eS, inputs = slot.S, slot.eS, slot.inputs
         out, bound, waiting, recent = [], [], [], np.zeros((self.vh, d))
+        rows, least = [], np.zeros((len(x), self.vh, d))
         for i in range(len(x)):
             seen = np.concatenate([inputs, x[i][None]])
-            q, eq, k, ek, v, ev, a, ea, b, eb, key = self.row(seen, alpha[i], beta[i])
+            rows.append(self.row(seen, alpha[i], beta[i]))
+            inputs = seen[1:]
+        if chunked and len(x):
+            # a chunk's values and updates are pairs of fp16 of at most 2^10, their columns' largest: the lower half's
+            # smallest step is 2^-24, so that each is off by 2^-25 of 2^10 at least, 2^-35 of the largest
+            T, values, updates = S, [], []
+            for q, eq, k, ek, v, ev, a, ea, b, eb, key in rows:
+                dv = b[:, None] * (v - a[:, None] * np.einsum("hrc,hc->hr", T, k))
+                T = a[:, None, None] * T + dv[:, :, None] * k[:, None, :]
+                values.append(np.abs(v))
+                updates.append(np.abs(dv))
+            for i in range(0, len(x), 64):
+                least[i:i + 64] = 2.0 ** -35 * (np.max(values[i:i + 64], axis=0) + np.max(updates[i:i + 64], axis=0))
+        inputs = slot.inputs
+        for i in range(len(x)):
+            seen = np.concatenate([inputs, x[i][None]])
+            q, eq, k, ek, v, ev, a, ea, b, eb, key = rows[i]
             size = np.linalg.norm(S, axis=2)
             asked = a[:, None] * np.einsum("hrc,hc->hr", S, k)
             dv = b[:, None] * (v - asked)
@@ -82,7 +99,7 @@ class Layer:
             # rows' updates (each at most its own size) beside them, through the triangle (64 more) and back
             n = d / 8 + 8 if not chunked else d + 16
             among = np.zeros((self.vh, d)) if not chunked else 4 * 64 * U * recent
-            ed = b[:, None] * (ev + a[:, None] * size * (ek[:, None] + n * U) + ea[:, None] * size + among) + \
+            ed = b[:, None] * (ev + a[:, None] * size * (ek[:, None] + n * U) + ea[:, None] * size + among) + least[i] + \
                 np.abs(dv) * (4 * U) + np.abs(v - asked) * eb[:, None]
             # an error of S goes through a (1 - b k k^T), which makes nothing larger
             S = a[:, None, None] * S + dv[:, :, None] * k[:, None, :]

@@ -202,6 +202,51 @@ def test_far_and_equal_keys(ctx):
     run.close()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_that_are_the_keys(ctx, d):
+    """A chunk's rows ask for what they have just stored: an error of any operand's lower half shows in the outputs."""
+    for seed in range(4):
+        run = Run(ctx, 40 + seed, 2, 4, d, 4, 0, 2, 400)
+        c = run.layer
+        n = c.kh * d
+        c.conv[n:2 * n] = c.conv[:n]
+        run.weights[0].copy_(torch.from_numpy(c.conv))
+        real = run.rng.standard_normal
+
+        class Draw:
+            @staticmethod
+            def standard_normal(shape):
+                x = real(shape)
+                if shape[1] == c.channels:
+                    x[:, n:2 * n] = x[:, :n]
+                return x
+
+        run.rng = Draw
+        run.step([200, 70], [0, 1], [-1, -1])
+        run.step([65, 130], [0, 1], [0, 0])
+        run.check_storage()
+        run.close()
+
+
+def test_one_sequence_that_may_have_many_rows(ctx):
+    """Alone and without pending rows a sequence goes through chunks however few its rows are."""
+    run = Run(ctx, 53, 2, 4, 64, 4, 0, 2, 100)
+    c = run.layer
+    for count, standing in ((1, -1), (2, 0), (40, 0), (5, 0), (1, 0), (16, -1)):
+        x, alpha, beta = (run.rng.standard_normal((40, w)).astype(np.float32) for w in (c.channels, c.vh, c.vh))
+        dev = [torch.from_numpy(a).cuda() for a in (x, alpha, beta)]
+        out = torch.full((40, c.vh * c.d), 9.0, device="cuda")
+        numbers = [torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([0, count], [1], [standing])]
+        torch.cuda.synchronize()
+        run.cache.run(1, B.GdnBatch(1, 40, 40, *(a.data_ptr() for a in numbers)), *(a.data_ptr() for a in dev), *(w.data_ptr() for w in run.weights), out.data_ptr())
+        ctx.synchronize()
+        want, bound = c.run(run.model[1], standing, *(a[:count].astype(np.float64) for a in (x, alpha, beta)), chunked=True)
+        got = out.double().cpu().numpy()
+        assert (np.abs(got[:count].reshape(want.shape) - want) <= bound + 2.0 ** -24 * np.abs(want)).all() and (got[count:] == 9.0).all()
+        run.check_storage()
+    run.close()
+
+
 def test_slots_that_are_not_there(ctx):
     """Rows of a slot outside the cache, and row starts outside the arrays, reach nothing else."""
     run = Run(ctx, 17, 2, 4, 64, 4, 3, 2, 40)
