@@ -13,13 +13,17 @@
 // stays in registers.
 //
 // Products run in fp16 matrix instructions with fp32 sums: an operand is two numbers,
-// x 2^10 = h + l, and h h + h l + l h keeps 22 bits of either (three instructions of a
+// x scale = h + l, and h h + h l + l h keeps 22 bits of either (three instructions of a
 // sixteenth of the fp32 one's time each).  That is as exact as the sums' own fp32
-// rounding, if x is not far below the largest of its kind: q, k, W, T and the weights are
-// at most 1 (a row's update answers any value at most its own size: the rule is a
-// contraction); V, S and D have any size, and are held against a power of two of their
-// column's largest, for every 32 (16, heads of 64) key dims of S and every 16 rows of D,
-// which are a wave's own.  S itself, the updates and all sums are fp32.
+// rounding, if x is not far below the largest of its kind.  q, k, W, T and the weights are
+// at most 1 (decays are at most 1, and a row's update answers any value at most its own
+// size: the rule is a contraction) and scaled by 2^10.  V, S and D have any size: a column (one value
+// dim) is scaled by a power of two, V by its largest in the chunk, S and D by bounds: with
+// s the largest of S before the chunk and u that of U,
+//   |D| <= u + sqrt(head) s,  |S after it| <= exp(c_n) s + 64 max |D|,
+// which no wave has to wait for another's numbers for.  They exceed the largest by 2^10 or
+// so; halves that are scaled to 2^15 lose bits below 2^-3, 2^-18 of the bound.  S itself, the
+// updates and all sums are fp32.
 //
 // The sums c are taken in 64 bits: far into a decay they are large, and their differences
 // are not.
@@ -86,13 +90,14 @@ __device__ __forceinline__ f32x4_t product32(f32x4_t a, f32x4_t b, f32x4_t c) {
     return c;
 }
 
-// The power of two that brings numbers up to `top` to 2^10 at most, and back (1 for nothing).
+// The power of two that brings numbers up to `top` below 2^15, and back from a product with
+// a number times 2^10 (1 for nothing).
 struct Scale {
     float to, from;
     __device__ __forceinline__ explicit Scale(float top) {
         const int e = top > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 128) : 0;
-        to = __builtin_ldexpf(kOne, -e);
-        from = __builtin_ldexpf(kProduct, e);
+        to = __builtin_ldexpf(32768.0f, -e);
+        from = __builtin_ldexpf(1.0f / (32768.0f * kOne), e);
     }
 };
 
@@ -140,6 +145,8 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     typedef typename Element<DT>::type E;
     typedef E E2 __attribute__((ext_vector_type(2)));
     constexpr int kTaps = TAPS ? TAPS : kGdnMaxTaps;
+    // a wave's results as they lie in memory, 16 bytes a unit: written from here a piece at a time
+    __shared__ u32x4_t images[4][512];
     const int lane = threadIdx.x & 63, part = blockIdx.x * 4 + (threadIdx.x >> 6), seq = blockIdx.z;
     const GdnView &c = p.cache;
     GdnSequence s = gdn_sequence(p, seq);
@@ -147,13 +154,23 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     const int i0 = blockIdx.y * kRun, rows = min(s.count - i0, kRun), channels = c.channels(), parts = (channels + 127) / 128;
     if (rows <= 0 || part > parts) return;
     if (part == parts) {
-        for (int at = lane; at < rows * c.value_heads; at += 64) {
-            const int64_t row = s.begin + i0 + at / c.value_heads;
-            const int h = at % c.value_heads;
-            const float alpha = static_cast<float>(static_cast<const E *>(p.alpha)[row * p.alpha_row + h]);
-            const float beta = static_cast<float>(static_cast<const E *>(p.beta)[row * p.beta_row + h]);
-            p.decay[row * c.value_heads + h] = gdn_log_decay(p.ssm_a[h], alpha, p.ssm_dt[h]);
-            p.rate[row * c.value_heads + h] = gdn_sigmoid(beta);
+        const int all = rows * c.value_heads;
+        for (int at0 = lane; at0 < all; at0 += 256) {
+            float alpha[4], beta[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = min(at0 + 64 * k, all - 1), h = at % c.value_heads;
+                const int64_t row = s.begin + i0 + at / c.value_heads;
+                alpha[k] = static_cast<float>(static_cast<const E *>(p.alpha)[row * p.alpha_row + h]);
+                beta[k] = static_cast<float>(static_cast<const E *>(p.beta)[row * p.beta_row + h]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = min(at0 + 64 * k, all - 1), h = at % c.value_heads;
+                const int64_t to = (s.begin + i0) * static_cast<int64_t>(c.value_heads) + at;
+                p.decay[to] = gdn_log_decay(p.ssm_a[h], alpha[k], p.ssm_dt[h]);
+                p.rate[to] = gdn_sigmoid(beta[k]);
+            }
         }
         return;
     }
@@ -162,25 +179,29 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     // heads of 64: the last wave may have one head only (its other lanes repeat it and store nothing)
     const bool mine = part * 128 + 2 * lane < channels;
     const int channel = mine ? part * 128 + 2 * lane : channels - D + (2 * lane) % D;
-    f32x2_t x[kTaps - 1 + kRun], w[kTaps];
+    f32x2_t x[kTaps - 1 + 4], ahead[4], w[kTaps];
     const E *rows_at = static_cast<const E *>(p.qkv) + channel;
+    const auto input = [&](int row) {
+        const E *at = rows_at + (s.begin + min(row, s.count - 1)) * p.qkv_row;
+        if (p.pairs) {
+            const E2 v = *reinterpret_cast<const E2 *>(at);
+            return f32x2_t{static_cast<float>(v[0]), static_cast<float>(v[1])};
+        }
+        return f32x2_t{static_cast<float>(at[0]), static_cast<float>(at[1])};
+    };
 #pragma unroll
-    for (int j = 0; j < kTaps - 1 + kRun; ++j) {
+    for (int j = 0; j < kTaps - 1; ++j) {
         const int row = i0 + j - (kTaps - 1);
         x[j] = f32x2_t{0.0f, 0.0f};
         if (row >= 0) {
-            const E *at = rows_at + (s.begin + min(row, s.count - 1)) * p.qkv_row;
-            if (p.pairs) {
-                const E2 v = *reinterpret_cast<const E2 *>(at);
-                x[j] = f32x2_t{static_cast<float>(v[0]), static_cast<float>(v[1])};
-            } else {
-                x[j] = f32x2_t{static_cast<float>(at[0]), static_cast<float>(at[1])};
-            }
+            x[j] = input(row);
         } else if (row >= -before && !s.begins) {
             const float *at = c.inputs + (static_cast<int64_t>(s.slot) * (before + c.pending) + s.stands + before + row) * channels + channel;
             x[j] = f32x2_t{at[0], at[1]};
         }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) ahead[k] = input(i0 + k);
 #pragma unroll
     for (int j = 0; j < kTaps; ++j) {
         const float *at = p.conv + static_cast<int64_t>(channel) * taps + j - first;
@@ -189,20 +210,30 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     const int head = channel / D, dim = channel % D;
     const bool is_value = head >= 2 * c.key_heads, is_key = !is_value && head >= c.key_heads;
     const int64_t run = run_place(s, s.begin + i0);
-    const float root = kOne / sqrtf(static_cast<float>(D));
-    _Float16 *asks = p.asks + (run * 2 * c.key_heads + (is_value ? 0 : head)) * Runs<D>::kHead;
-    // step, lane group and place of this lane's dims
-    constexpr int kAsk = Runs<D>::kAsk;
-    asks += (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16) * kAsk + dim % kAsk;
+    // 2^10 over the length, but no more than over epsilon; queries also over sqrt(head)
+    const float one = is_key ? kOne : kOne / sqrtf(static_cast<float>(D)), most = fminf(one / p.eps, 3e38f);
+    // the head's part of the image, D * 4 units (heads of 64: two heads a wave, half its lanes each)
+    constexpr int kAsk = Runs<D>::kAsk, kUnits = D * 4, kHeadLanes = D / 2;
+    u32x4_t *image = images[threadIdx.x >> 6] + (lane / kHeadLanes) * kUnits;
+    // lanes that write together have the same row, or four rows, of different steps or tiles: their units are turned so
+    // that they meet different banks
+    const int turn_shift = is_value ? 6 : 4, turn_low = is_value ? 1 : 3, turn_high = is_value ? 0 : 12;
+    const auto turned = [&](int unit) { return unit ^ (unit >> turn_shift & turn_low) ^ (unit >> 5 & turn_high); };
     const int tile_at = (dim >> 4) * 64 + (dim & 15);  // the first of its tile's lanes that have this dim
+    const int ask_at = (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16) * kAsk + dim % kAsk;  // in halves, of row 0
     _Float16 *by_dim = p.keys_by_dim + (run * c.key_heads + (is_key ? head - c.key_heads : 0)) * Runs<D>::kHead + tile_at * 8;
-    float *values = p.values + (run * c.value_heads + (is_value ? head - 2 * c.key_heads : 0)) * (kRun * D) + tile_at * 4;
-#pragma unroll
+    // rows past the last are those of the last inputs again: finite, and their updates are zero
+#pragma unroll 1
     for (int four = 0; four < kRun / 4; ++four) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[kTaps - 1 + k] = ahead[k];
+        if (four + 1 < kRun / 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ahead[k] = input(i0 + 4 * four + 4 + k);
+        }
         f32x4_t y[2];  // this lane's dims, four rows
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = 4 * four + e;
+        for (int i = 0; i < 4; ++i) {
             float u0 = 0.0f, u1 = 0.0f;
 #pragma unroll
             for (int j = 0; j < kTaps; ++j)
@@ -212,31 +243,38 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
                 }
             u0 = gdn_silu(u0);
             u1 = gdn_silu(u1);
-            float inverse = 1.0f;
-            if (!is_value) {
-                const float sum = group_sum_up(u0 * u0 + u1 * u1, D / 2);
-                inverse = (is_key ? kOne : root) / fmaxf(sqrtf(sum), p.eps);
-            }
-            y[0][e] = u0 * inverse;
-            y[1][e] = u1 * inverse;
+            const float sum = group_sum_up(u0 * u0 + u1 * u1, kHeadLanes);
+            const float inverse = is_value ? 1.0f : fminf(__builtin_amdgcn_rsqf(sum) * one, most);
+            y[0][i] = u0 * inverse;
+            y[1][i] = u1 * inverse;
         }
-        if (!mine) continue;
-        // rows past the last are those of the last inputs again: finite, and their updates are zero
+#pragma unroll
+        for (int j = 0; j + 1 < kTaps; ++j) x[j] = x[j + 4];
         if (is_value) {
-            *reinterpret_cast<f32x4_t *>(values + 16 * four * 4) = y[0];
-            *reinterpret_cast<f32x4_t *>(values + 16 * four * 4 + 4) = y[1];
+            reinterpret_cast<f32x4_t *>(image)[turned(tile_at + 16 * four)] = y[0];
+            reinterpret_cast<f32x4_t *>(image)[turned(tile_at + 16 * four + 1)] = y[1];
             continue;
         }
         const Pair4 a = split4(y[0]), b = split4(y[1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            *reinterpret_cast<f16x2_t *>(asks + (4 * four + e) * kAsk) = f16x2_t{a.h[e], b.h[e]};
-            *reinterpret_cast<f16x2_t *>(asks + (64 + 4 * four + e) * kAsk) = f16x2_t{a.l[e], b.l[e]};
+        for (int i = 0; i < 4; ++i) {
+            const int at = ask_at + (4 * four + i) * kAsk;
+            reinterpret_cast<f16x2_t *>(image + turned(at / 8))[at % 8 / 2] = f16x2_t{a.h[i], b.h[i]};
+            reinterpret_cast<f16x2_t *>(image + turned((at + 64 * kAsk) / 8))[at % 8 / 2] = f16x2_t{a.l[i], b.l[i]};
         }
-        if (is_key) {
+        if (is_key && mine) {
             store_four_step(by_dim + 16 * four * 8, 0, a);
             store_four_step(by_dim + 16 * four * 8, 1, b);
         }
+    }
+    wave_lds_fence();
+    u32x4_t *to = is_value ? reinterpret_cast<u32x4_t *>(p.values + (run * c.value_heads + head - 2 * c.key_heads) * (kRun * D))
+                           : reinterpret_cast<u32x4_t *>(p.asks + (run * 2 * c.key_heads + head) * Runs<D>::kHead);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int unit = k * kHeadLanes + lane % kHeadLanes;
+        const u32x4_t v = image[turned(unit)];
+        if (mine) to[unit] = v;
     }
     if (i0 != 0) return;
     // its own channels' reads of the slot's inputs are done
@@ -248,13 +286,15 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
 }
 
 // W, U and the weights of one chunk and value head.
+// Three workgroups a CU: each goes through a chain of small steps with barriers between
+// them, and waits most of the time.
 template <int D>
-__global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
+__global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p) {
     typedef typename Runs<D>::Ask Ask;
-    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 8, kTiles = D / 64, kHead = Runs<D>::kHead;
-    // A, and T; T with b exp(c) and with b, in halves
-    __shared__ __align__(16) float as[kGdnChunk * kPitch], ts[kGdnChunk * kPitch];
-    __shared__ __align__(16) _Float16 halves[2][2][kGdnChunk * kPitchT];
+    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 4, kTiles = D / 64, kHead = Runs<D>::kHead;
+    // A, and T; then T with b exp(c) (where A was) and with b, in halves
+    __shared__ __align__(16) float as[2 * kGdnChunk * kPitch], ts[kGdnChunk * kPitch];
+    _Float16(*halves)[2][kGdnChunk * kPitchT] = reinterpret_cast<_Float16(*)[2][kGdnChunk * kPitchT]>(as);
     __shared__ double sums[kGdnChunk];  // binary logarithms
     __shared__ float rates[kGdnChunk];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
@@ -340,17 +380,20 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
     {
         const float *block = as + 16 * wave * kPitch + 16 * wave;
         float x[16];
-        f32x4_t rows4[16][4];
-#pragma unroll
-        for (int i = 1; i < 16; ++i)
-#pragma unroll
-            for (int q = 0; q < (i + 3) / 4; ++q) rows4[i][q] = *reinterpret_cast<const f32x4_t *>(block + i * kPitch + 4 * q);
+        f32x4_t four[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = i == m ? 1.0f : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 15; ++j)
+        for (int j = 0; j < 15; ++j) {
+            if (j % 4 == 0) {  // four columns of A
 #pragma unroll
-            for (int i = j + 1; i < 16; ++i) x[i] = __builtin_fmaf(-rows4[i][j / 4][j % 4], x[j], x[i]);
+                for (int i = 1; i < 16; ++i)
+                    if (i > j) four[i] = *reinterpret_cast<const f32x4_t *>(block + i * kPitch + j);
+            }
+#pragma unroll
+            for (int i = 1; i < 16; ++i)
+                if (i > j) x[i] = __builtin_fmaf(-four[i][j % 4], x[j], x[i]);
+        }
         float *to = ts + 16 * wave * kPitch + 16 * wave + m;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -415,6 +458,9 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
     };
     // of W a lane has four key dims of row m, of U four rows of value dim m
     const int lane_dim = 16 * kTiles * wave + 4 * g, kAsk = Runs<D>::kAsk;
+    float top[kTiles];  // of U's columns
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) top[t] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i > last_run) break;
@@ -433,13 +479,20 @@ __global__ __launch_bounds__(256) void gdn_chunk_kernel(const GdnRowsParams p) {
         _Float16 *through = p.through + ((run0 + i) * c.value_heads + h) * kHead;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-            *reinterpret_cast<f32x4_t *>(values + i * run_values + t * 256) = u[t] * from[t];
+            u[t] *= from[t];
+            top[t] = fmaxf(top[t], largest(u[t]));
+            *reinterpret_cast<f32x4_t *>(values + i * run_values + t * 256) = u[t];
             const Pair4 x = split4(w[t] * (kProduct * kOne));
             const int dim = lane_dim + 16 * t;
             _Float16 *to = through + (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16 + m) * kAsk + dim % kAsk;
             *reinterpret_cast<f16x4_t *>(to) = x.h;
             *reinterpret_cast<f16x4_t *>(to + 64 * kAsk) = x.l;
         }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        top[t] = largest_of_column(top[t]);
+        if (g == 0) p.tops[(run0 * c.value_heads + h) * D + 16 * (kTiles * wave + t) + m] = top[t];
     }
 }
 
@@ -453,7 +506,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
     constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8, kAsk = Runs<D>::kAsk;
     constexpr int kHead = Runs<D>::kHead;
     __shared__ __align__(16) _Float16 sh[2][16 * NT * kPitch], dh[2][16 * NT * kPitchD], rh[2][16 * NT * kPitchD];
-    __shared__ float s_from[4][16 * NT], d_from[4][16 * NT], r_from[4][16 * NT];
+    __shared__ float tops[4][16 * NT];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
@@ -502,13 +555,16 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
         }
     };
     f32x4_t u[NT], through, left;
-    float whole;
+    float u_top[NT], whole;
     const auto load_updates = [&](int run0) {
         const int64_t at = run_at(run0 + wave) * c.value_heads + h;
         through = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + 4 * g);
         left = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + kRun + 4 * g);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) u[t] = *reinterpret_cast<const f32x4_t *>(p.values + at * (kRun * D) + ((r0 / 16 + t) * 64 + lane) * 4);
+        for (int t = 0; t < NT; ++t) {
+            u[t] = *reinterpret_cast<const f32x4_t *>(p.values + at * (kRun * D) + ((r0 / 16 + t) * 64 + lane) * 4);
+            u_top[t] = p.tops[(run_at(run0) * c.value_heads + h) * D + r0 + 16 * t + m];
+        }
     };
     Pair4 inner[4], keys[kTiles][4];
     const auto load_rest = [&](int run0) {
@@ -527,6 +583,30 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
     load_updates(0);
     load_rest(0);
     E *out = static_cast<E *>(p.out) + (s.begin + static_cast<int64_t>(16 * wave + 4 * g)) * p.out_row + h * D + r0 + m;
+    // a column's largest number of this wave's part of S
+    const auto top_of = [&](int t) {
+        float top = largest(S[t][0]);
+        if constexpr (kTiles > 1) top = fmaxf(top, largest(S[t][1]));
+        return largest_of_column(top);
+    };
+    const auto column_top = [&](int t) {
+        return fmaxf(fmaxf(tops[0][16 * t + m], tops[1][16 * t + m]), fmaxf(tops[2][16 * t + m], tops[3][16 * t + m]));
+    };
+    float s_to[NT], s_from[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float top = top_of(t);
+        if (g == 0) tops[wave][16 * t + m] = top;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const Scale scale(column_top(t));
+        s_to[t] = scale.to;
+        s_from[t] = scale.from;
+    }
+    lds_barrier();
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int i0 = 0; i0 < s.count; i0 += kGdnChunk) {
         const int mine = s.count - i0 - 16 * wave - 4 * g;  // this lane's rows that are there
@@ -534,13 +614,11 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
         const int next = i0 / kRun + 4;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float top = largest(S[t][0]);
-            if constexpr (kTiles > 1) top = fmaxf(top, largest(S[t][1]));
-            const Scale scale(largest_of_column(top));
-            if (g == 0) s_from[wave][16 * t + m] = scale.from;
+            const float top = top_of(t);
+            if (g == 0) tops[wave][16 * t + m] = top;
 #pragma unroll
             for (int k = 0; k < kTiles; ++k) {
-                const Pair4 x = split4(S[t][k] * scale.to);
+                const Pair4 x = split4(S[t][k] * s_to[t]);
                 const int at = (16 * t + m) * kPitch + 16 * (kTiles * wave + k) + 4 * g;
                 *reinterpret_cast<f16x4_t *>(&sh[0][at]) = x.h;
                 *reinterpret_cast<f16x4_t *>(&sh[1][at]) = x.l;
@@ -550,59 +628,69 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
 
         f32x4_t asked[NT], o[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            asked[t] = o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < NT; ++t) asked[t] = o[t] = zero;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
                 const Pair<Ask> b = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
-                const float from = s_from[k][16 * t + m];
-                const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                asked[t] += product(w[k], b, zero) * from;
-                o[t] += product(q[k], b, zero) * from;
+                asked[t] = product(w[k], b, asked[t]);
+                o[t] = product(q[k], b, o[t]);
             }
-        }
         if (more) load_asks(next);
+        float d_from[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            const float top = column_top(t), most = __builtin_fmaf(top, D == 128 ? 11.32f : 8.01f, u_top[t]) * 1.001f;
+            const Scale scale(most), after(__builtin_fmaf(top, whole, 64.0f * most));
             f32x4_t d, d_left;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                d[e] = e < mine ? u[t][e] - asked[t][e] : 0.0f;
+                d[e] = e < mine ? __builtin_fmaf(asked[t][e], -s_from[t], u[t][e]) : 0.0f;
                 d_left[e] = d[e] * left[e];
-                o[t][e] *= through[e];
+                o[t][e] *= through[e] * s_from[t];
             }
-            const Scale ds(largest_of_column(largest(d))), rs(largest_of_column(largest(d_left)));
-            const Pair4 x = split4(d * ds.to), y = split4(d_left * rs.to);
+            d_from[t] = scale.from;
+            s_to[t] = after.to;
+            s_from[t] = after.from;
+            const Pair4 x = split4(d * scale.to), y = split4(d_left * scale.to);
             const int at = (16 * t + m) * kPitchD + 16 * wave + 4 * g;
             *reinterpret_cast<f16x4_t *>(&dh[0][at]) = x.h;
             *reinterpret_cast<f16x4_t *>(&dh[1][at]) = x.l;
             *reinterpret_cast<f16x4_t *>(&rh[0][at]) = y.h;
             *reinterpret_cast<f16x4_t *>(&rh[1][at]) = y.l;
-            if (g == 0) {
-                d_from[wave][16 * t + m] = ds.from;
-                r_from[wave][16 * t + m] = rs.from;
-            }
         }
         if (more) load_updates(next);
         lds_barrier();  // every wave's updates are there, and its reads of S done
+        f32x4_t added[NT][kTiles], among[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            among[t] = zero;
 #pragma unroll
-            for (int k = 0; k < kTiles; ++k) S[t][k] *= whole;
+            for (int k = 0; k < kTiles; ++k) added[t][k] = zero;
+        }
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
-                const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
                 const Pair4 r = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
 #pragma unroll
-                for (int k = 0; k < kTiles; ++k) S[t][k] += product(keys[k][b], r, zero) * r_from[b][16 * t + m];
+                for (int k = 0; k < kTiles; ++k) added[t][k] = product(keys[k][b], r, added[t][k]);
                 if (b <= wave) {
                     const Pair4 d = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
-                    o[t] += product(inner[b], d, zero) * d_from[b][16 * t + m];
+                    among[t] = product(inner[b], d, among[t]);
                 }
             }
-        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int k = 0; k < kTiles; ++k) S[t][k][e] = __builtin_fmaf(added[t][k][e], d_from[t], S[t][k][e] * whole);
+                o[t][e] = __builtin_fmaf(among[t][e], d_from[t], o[t][e]);
+            }
         if (more) load_rest(next);
         E *to = out + i0 * p.out_row;
 #pragma unroll

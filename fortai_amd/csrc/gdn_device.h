@@ -53,7 +53,8 @@ __device__ __forceinline__ float gdn_sigmoid(float x) { return 1.0f / (1.0f + ex
 
 // The inputs of a channel that a slot keeps, written by one thread: behind a sequence
 // of rows that wait, the taps - 1 inputs before them and theirs; otherwise the last
-// taps - 1.  In place, in ascending order: what is read lies at or behind what is written.
+// taps - 1.  In place, in ascending order, four at a time: what is read lies at or behind
+// what is written.
 template <typename E>
 __device__ __forceinline__ void gdn_keep_inputs(const GdnRowsParams &p, const GdnSequence &s, bool waits, int channel) {
     const int channels = p.cache.channels(), before = p.cache.taps - 1;
@@ -61,12 +62,18 @@ __device__ __forceinline__ void gdn_keep_inputs(const GdnRowsParams &p, const Gd
     const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
     const int from = waits ? 0 : s.count, kept = before + (waits ? s.count : 0);
 #pragma unroll 1
-    for (int j = 0; j < kept; ++j) {
-        const int at = from + j;
-        float v = 0.0f;
-        if (at >= before) v = static_cast<float>(x[static_cast<int64_t>(at - before) * p.qkv_row]);
-        else if (!s.begins) v = window[static_cast<int64_t>(s.stands + at) * channels];
-        window[static_cast<int64_t>(j) * channels] = v;
+    for (int j = 0; j < kept; j += 4) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = from + min(j + k, kept - 1);
+            v[k] = 0.0f;
+            if (at >= before) v[k] = static_cast<float>(x[static_cast<int64_t>(at - before) * p.qkv_row]);
+            else if (!s.begins) v[k] = window[static_cast<int64_t>(s.stands + at) * channels];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (j + k < kept) window[static_cast<int64_t>(j + k) * channels] = v[k];
     }
 }
 

@@ -90,6 +90,7 @@ struct GdnRowsParams {
     _Float16 *inner = nullptr;        // [runs][value_heads][4]: weights of the chunk's updates, by rows
     float *values = nullptr;          // [runs][value_heads]: V, then U, by dims
     float *chunk_gates = nullptr;     // [runs][value_heads][2][kGdnRun]: decays since the chunk's start, and to its end
+    float *tops = nullptr;            // [runs][value_heads][head]: a chunk's largest |U| of each value dim, at its first run
     float *decay = nullptr;           // [rows][value_heads]: logarithms
     float *rate = nullptr;            // [rows][value_heads]: beta
     int *stands = nullptr;    // [kGdnMaxSequences]
