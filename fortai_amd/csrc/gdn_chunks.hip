@@ -139,8 +139,8 @@ __device__ __forceinline__ void store_four_step(_Float16 *tile, int lane, const 
 }
 
 // Convolution, norms and gates: a wave has 128 channels (two a lane) of a run, or every
-// gate.  TAPS: of the convolution, 0: as many as there are.
-template <Dtype DT, int D, int TAPS>
+// gate.  TAPS: of the convolution, 0: as many as there are.  PAIRS: two elements at once.
+template <Dtype DT, int D, int TAPS, bool PAIRS>
 __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
     typedef E E2 __attribute__((ext_vector_type(2)));
@@ -183,11 +183,11 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     const E *rows_at = static_cast<const E *>(p.qkv) + channel;
     const auto input = [&](int row) {
         const E *at = rows_at + (s.begin + min(row, s.count - 1)) * p.qkv_row;
-        if (p.pairs) {
+        if constexpr (PAIRS) {
             const E2 v = *reinterpret_cast<const E2 *>(at);
             return f32x2_t{static_cast<float>(v[0]), static_cast<float>(v[1])};
         }
-        return f32x2_t{static_cast<float>(at[0]), static_cast<float>(at[1])};
+        else return f32x2_t{static_cast<float>(at[0]), static_cast<float>(at[1])};
     };
 #pragma unroll
     for (int j = 0; j < kTaps - 1; ++j) {
@@ -227,10 +227,8 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     for (int four = 0; four < kRun / 4; ++four) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[kTaps - 1 + k] = ahead[k];
-        if (four + 1 < kRun / 4) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ahead[k] = input(i0 + 4 * four + 4 + k);
-        }
+        for (int k = 0; k < 4; ++k) ahead[k] = input(i0 + min(4 * four + 4, kRun - 4) + k);
         f32x4_t y[2];  // this lane's dims, four rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -287,94 +285,109 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
 
 // W, U and the weights of one chunk and value head.
 // Three workgroups a CU: each goes through a chain of small steps with barriers between
-// them, and waits most of the time.
+// them, and waits most of the time.  Everything that comes from memory is asked for before
+// the first of them, without conditions, so that no wait is for more than it needs.
 template <int D>
 __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p) {
     typedef typename Runs<D>::Ask Ask;
-    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 4, kTiles = D / 64, kHead = Runs<D>::kHead;
-    // A, and T; then T with b exp(c) (where A was) and with b, in halves
+    constexpr int kPitch = kGdnChunk + 4, kPitchT = kGdnChunk + 4, kTiles = D / 64, kHead = Runs<D>::kHead, kAsk = Runs<D>::kAsk;
+    // first the keys by rows; then A, and T beside it; then T with b exp(c) (where A was) and with b, in halves
     __shared__ __align__(16) float as[2 * kGdnChunk * kPitch], ts[kGdnChunk * kPitch];
+    static_assert(sizeof(as) >= 4 * kHead * sizeof(_Float16), "the keys of four runs");
     _Float16(*halves)[2][kGdnChunk * kPitchT] = reinterpret_cast<_Float16(*)[2][kGdnChunk * kPitchT]>(as);
     __shared__ double sums[kGdnChunk];  // binary logarithms
-    __shared__ float rates[kGdnChunk];
+    __shared__ __align__(16) float rates[kGdnChunk], asked_rates[kGdnChunk];  // b, and with exp(c)
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
     const GdnSequence s = gdn_sequence(p, blockIdx.z);
     if (!gdn_is_many(p, s)) return;
-    const int n = min(s.count - static_cast<int>(blockIdx.x) * kGdnChunk, kGdnChunk), h = blockIdx.y;
+    const int n = min(s.count - static_cast<int>(blockIdx.y) * kGdnChunk, kGdnChunk), h = blockIdx.x;
     if (n <= 0) return;
-    const int64_t row0 = s.begin + static_cast<int64_t>(blockIdx.x) * kGdnChunk, run0 = run_place(s, row0);
+    const int64_t row0 = s.begin + static_cast<int64_t>(blockIdx.y) * kGdnChunk, run0 = run_place(s, row0);
     const int kh = h / (c.value_heads / c.key_heads), last_run = (n - 1) / kRun;
 
-    if (wave == 0) {
-        const int64_t at = (row0 + min(lane, n - 1)) * c.value_heads + h;
-        double sum = lane < n ? static_cast<double>(p.decay[at]) * 1.4426950408889634 : 0.0;
-        const float rate = lane < n ? p.rate[at] : 0.0f;
+    // gates (of lane's row), a run of keys a wave, and the rows whose products with keys this wave has: of keys
+    // (waves 0 and 1) or queries (2 and 3), runs 0 and 3, or 1 and 2
+    const int64_t gate_at = (row0 + min(lane, n - 1)) * c.value_heads + h;
+    const float my_decay = p.decay[gate_at], my_rate = p.rate[gate_at];
+    const auto run_of = [&](int run, int head) { return p.asks + ((run0 + min(run, last_run)) * 2 * c.key_heads + head) * kHead; };
+    const bool of_queries = wave >= 2;
+    const int odd = wave & 1;
+    Pair<Ask> own[4], a0[4], a1[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) own[k] = Runs<D>::row_step(run_of(wave, c.key_heads + kh), k, lane);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        a0[k] = Runs<D>::row_step(run_of(odd, of_queries ? kh : c.key_heads + kh), k, lane);
+        a1[k] = Runs<D>::row_step(run_of(3 - odd, of_queries ? kh : c.key_heads + kh), k, lane);
+    }
+    {
+        double sum = lane < n ? static_cast<double>(my_decay) * 1.4426950408889634 : 0.0;
+        const float rate = lane < n ? my_rate : 0.0f;
 #pragma unroll
         for (int step = 1; step < 64; step *= 2) {
             const double other = __shfl_up(sum, step);
             if (lane >= step) sum += other;
         }
-        sums[lane] = sum;
-        rates[lane] = rate;
         const double all = __shfl(sum, 63);
-        if (lane / kRun <= last_run) {  // for the launch that follows
-            float *to = p.chunk_gates + ((run0 + lane / kRun) * c.value_heads + h) * (2 * kRun) + lane % kRun;
-            to[0] = __builtin_amdgcn_exp2f(static_cast<float>(sum));
-            to[kRun] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum));
-        }
-    }
-    // k_j.k_i (waves 0 and 1) and k_j.q_i (2 and 3) in tiles of 16 j and 16 rows i: rows 0 and 3, or 1 and 2, five tiles
-    const bool of_queries = wave >= 2;
-    const auto run_of = [&](int tile, int head) { return p.asks + ((run0 + min(tile, last_run)) * 2 * c.key_heads + head) * kHead; };
-    f32x4_t dots[2][4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row_tile = r ? 3 - (wave & 1) : wave & 1;
-        Pair<Ask> a[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a[k] = Runs<D>::row_step(run_of(row_tile, of_queries ? kh : c.key_heads + kh), k, lane);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            dots[r][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (t > row_tile || t > r + 2) continue;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                dots[r][t] = product(Runs<D>::row_step(run_of(t, c.key_heads + kh), k, lane), a[k], dots[r][t]);
-        }
-    }
-    // this wave's columns of V, on their way
-    float *values = p.values + (run0 * c.value_heads + h) * (kRun * D) + (kTiles * wave * 64 + lane) * 4;
-    const int64_t run_values = static_cast<int64_t>(c.value_heads) * (kRun * D);
-    f32x4_t v[kTiles][4];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) v[t][b] = *reinterpret_cast<const f32x4_t *>(values + min(b, last_run) * run_values + t * 256);
-    __syncthreads();  // sums and rates
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row_tile = r ? 3 - (wave & 1) : wave & 1, i = 16 * row_tile + m;
-        const double at_i = sums[i];
-        const float rate = rates[i] * kProduct;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t > row_tile || t > r + 2) continue;
-            f32x4_t x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = 16 * t + 4 * g + e;
-                const bool counts = of_queries ? j <= i : j < i;
-                const float weight = __builtin_amdgcn_exp2f(static_cast<float>(at_i - sums[j]));
-                x[e] = counts ? weight * dots[r][t][e] * (of_queries ? kProduct * kOne : rate) : 0.0f;
+        if (wave == 0) {
+            const float decay = __builtin_amdgcn_exp2f(static_cast<float>(sum));
+            sums[lane] = sum;
+            rates[lane] = rate;
+            asked_rates[lane] = rate * decay;
+            if (lane / kRun <= last_run) {  // for the launch that follows
+                float *to = p.chunk_gates + ((run0 + lane / kRun) * c.value_heads + h) * (2 * kRun) + lane % kRun;
+                to[0] = decay;
+                to[kRun] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum));
             }
-            if (!of_queries) *reinterpret_cast<f32x4_t *>(as + i * kPitch + 16 * t + 4 * g) = x;
-            else if (row_tile <= last_run)
-                store_four_step(p.inner + (((run0 + row_tile) * c.value_heads + h) * 4 + t) * (kRun * 32), lane, split4(x));
         }
     }
-    __syncthreads();  // A
+    _Float16 *keys = reinterpret_cast<_Float16 *>(as);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        _Float16 *to = keys + wave * kHead + (k * 2 * 64 + lane) * kAsk;
+        *reinterpret_cast<Ask *>(to) = own[k].h;
+        *reinterpret_cast<Ask *>(to + 64 * kAsk) = own[k].l;
+    }
+    lds_barrier();  // keys, sums and rates
+    // five products of 16 keys j and 16 rows i: run `odd` with runs 0 (and 1), run 3 - odd with the others up to its own
+    f32x4_t dots[5];
+    int row_run[5], key_run[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+        const bool first = k <= odd;
+        row_run[k] = first ? odd : 3 - odd;
+        key_run[k] = first ? k : k - 1 - odd;
+        dots[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+            const Pair<Ask> b = Runs<D>::row_step(keys + key_run[k] * kHead, step, lane);
+            // only the second product may be of either
+            Pair<Ask> a = k == 0 ? a0[step] : a1[step];
+            if (k == 1) a = odd ? a0[step] : a1[step];
+            dots[k] = product(b, a, dots[k]);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // five products' operands at once are more registers than there are
+    }
+    lds_barrier();  // the keys' place is A's now
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+        const int i = 16 * row_run[k] + m, j0 = 16 * key_run[k] + 4 * g;
+        const double at_i = sums[i];
+        const float factor = of_queries ? kProduct * kOne : rates[i] * kProduct;
+        const int past = of_queries ? i : i - 1;  // the last j that counts
+        f32x4_t x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float weight = __builtin_amdgcn_exp2f(static_cast<float>(at_i - sums[j0 + e]));
+            x[e] = j0 + e <= past ? weight * dots[k][e] * factor : 0.0f;
+        }
+        if (!of_queries) *reinterpret_cast<f32x4_t *>(as + i * kPitch + j0) = x;
+        else if (row_run[k] <= last_run)
+            store_four_step(p.inner + (((run0 + row_run[k]) * c.value_heads + h) * 4 + key_run[k]) * (kRun * 32), lane, split4(x));
+    }
+    lds_barrier();  // A
 
     // the inverse of a wave's block on the diagonal, a column a lane
     {
@@ -386,6 +399,7 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
 #pragma unroll
         for (int j = 0; j < 15; ++j) {
             if (j % 4 == 0) {  // four columns of A
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 1; i < 16; ++i)
                     if (i > j) four[i] = *reinterpret_cast<const f32x4_t *>(block + i * kPitch + j);
@@ -399,6 +413,21 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
         for (int i = 0; i < 16; ++i)
             if (i / 4 == g) to[i * kPitch] = x[i];
     }
+    // this wave's columns of V, on their way
+    float *values = p.values + (run0 * c.value_heads + h) * (kRun * D) + (kTiles * wave * 64 + lane) * 4;
+    const int64_t run_values = static_cast<int64_t>(c.value_heads) * (kRun * D);
+    f32x4_t v[kTiles][4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[t][b] = *reinterpret_cast<const f32x4_t *>(values + min(b, last_run) * run_values + t * 256);
+    // and its key dims
+    Pair4 ks[kTiles][4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            ks[t][b] = four_step(p.keys_by_dim + ((run0 + min(b, last_run)) * c.key_heads + kh) * kHead + (kTiles * wave + t) * (kRun * 32), lane);
     // below it: T_ij = -T_ii sum_k A_ik T_kj, a distance from the diagonal at a time
     const auto column_of = [&](int block_row, int block_column) {  // [k = 4 g + e][m]
         const float *at = ts + (16 * block_row + 4 * g) * kPitch + 16 * block_column + m;
@@ -409,7 +438,7 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
     };
 #pragma unroll 1
     for (int distance = 1; distance < 4; ++distance) {
-        __syncthreads();
+        lds_barrier();
         if (wave + distance < 4) {
             const int i = wave + distance, j = wave;
             f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -420,44 +449,36 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
             for (int e = 0; e < 4; ++e) ts[(16 * i + 4 * g + e) * kPitch + 16 * j + m] = -block[e];
         }
     }
-    __syncthreads();  // T
+    lds_barrier();  // T
     // the columns' factors go into T
     for (int at = 4 * tid; at < kGdnChunk * kGdnChunk; at += 1024) {
         const int i = at / kGdnChunk, j = at % kGdnChunk;
         if (j / 16 > i / 16) continue;
-        const f32x4_t t = *reinterpret_cast<const f32x4_t *>(ts + i * kPitch + j);
-        f32x4_t of_w, of_u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            of_u[e] = t[e] * rates[j + e] * kOne;
-            of_w[e] = of_u[e] * __builtin_amdgcn_exp2f(static_cast<float>(sums[j + e]));
-        }
+        const f32x4_t t = *reinterpret_cast<const f32x4_t *>(ts + i * kPitch + j) * kOne;
+        const f32x4_t of_w = t * *reinterpret_cast<const f32x4_t *>(asked_rates + j), of_u = t * *reinterpret_cast<const f32x4_t *>(rates + j);
         const Pair4 w = split4(of_w), u = split4(of_u);
         *reinterpret_cast<f16x4_t *>(&halves[0][0][i * kPitchT + j]) = w.h;
         *reinterpret_cast<f16x4_t *>(&halves[0][1][i * kPitchT + j]) = w.l;
         *reinterpret_cast<f16x4_t *>(&halves[1][0][i * kPitchT + j]) = u.h;
         *reinterpret_cast<f16x4_t *>(&halves[1][1][i * kPitchT + j]) = u.l;
     }
-    // this wave's columns of V as operands, and of K
+    // this wave's columns of V as operands
     float from[kTiles];
-    Pair4 vs[kTiles][4], ks[kTiles][4];
+    Pair4 vs[kTiles][4];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
         const Scale scale(largest_of_column(fmaxf(fmaxf(largest(v[t][0]), largest(v[t][1])), fmaxf(largest(v[t][2]), largest(v[t][3])))));
         from[t] = scale.from;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            vs[t][b] = split4(v[t][b] * scale.to);
-            ks[t][b] = four_step(p.keys_by_dim + ((run0 + min(b, last_run)) * c.key_heads + kh) * kHead + (kTiles * wave + t) * (kRun * 32), lane);
-        }
+        for (int b = 0; b < 4; ++b) vs[t][b] = split4(v[t][b] * scale.to);
     }
-    __syncthreads();
+    lds_barrier();
     const auto half_at = [&](int which, int i, int b) {
         const int at = (16 * i + m) * kPitchT + 16 * b + 4 * g;
         return Pair4{*reinterpret_cast<const f16x4_t *>(&halves[which][0][at]), *reinterpret_cast<const f16x4_t *>(&halves[which][1][at])};
     };
     // of W a lane has four key dims of row m, of U four rows of value dim m
-    const int lane_dim = 16 * kTiles * wave + 4 * g, kAsk = Runs<D>::kAsk;
+    const int lane_dim = 16 * kTiles * wave + 4 * g;
     float top[kTiles];  // of U's columns
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) top[t] = 0.0f;
@@ -500,7 +521,7 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
 // instructions' results a lane has value dim m and four key dims (of S) or rows (of D and
 // O).  A wave has 16 rows of the chunk and a quarter of the key dims.
 template <Dtype DT, int D, int NT>
-__global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) {
+__global__ __launch_bounds__(256, 2) void gdn_states_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
     typedef typename Runs<D>::Ask Ask;
     constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8, kAsk = Runs<D>::kAsk;
@@ -540,48 +561,55 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
     }
     if (h == 0 && r0 == 0 && tid == 0) c.counts[s.slot] = 0;
 
-    // a chunk's operands are asked for as soon as the one before has used its own
+    // A chunk's operands are asked for as soon as the one before has used its own, without
+    // conditions (the last chunk asks for its own again), so that no wait is for more than it
+    // needs.  A wave whose rows are none asks for whatever lies behind (there is room, and nothing comes of it).
     const int64_t run_first = run_place(s, s.begin);
-    const int last_run = (s.count - 1) / kRun;
-    const auto run_at = [&](int run) { return run_first + min(run, last_run); };
+    const int chunks = (s.count + kGdnChunk - 1) / kGdnChunk, last_run = (s.count - 1) / kRun;
+    const _Float16 *w_at = p.through + ((run_first + wave) * c.value_heads + h) * kHead;
+    const _Float16 *q_at = p.asks + ((run_first + wave) * 2 * c.key_heads + kh) * kHead;
+    const _Float16 *inner_at = p.inner + ((run_first + wave) * c.value_heads + h) * (4 * kRun * 32);
+    const float *u_at = p.values + ((run_first + wave) * c.value_heads + h) * (kRun * D) + (r0 / 16 * 64 + lane) * 4;
+    const float *gates_at = p.chunk_gates + ((run_first + wave) * c.value_heads + h) * (2 * kRun) + 4 * g;
+    const float *tops_at = p.tops + (run_first * c.value_heads + h) * D + r0 + m;
+    const _Float16 *keys_at = p.keys_by_dim + (run_first * c.key_heads + kh) * kHead + kTiles * wave * (kRun * 32);
+    const float *whole_at = p.chunk_gates + (run_first * c.value_heads + h) * (2 * kRun);
+    const int64_t w_step = static_cast<int64_t>(4) * c.value_heads * kHead, q_step = static_cast<int64_t>(8) * c.key_heads * kHead;
+    const int64_t inner_step = static_cast<int64_t>(4) * c.value_heads * (4 * kRun * 32), u_step = static_cast<int64_t>(4) * c.value_heads * (kRun * D);
+    const int64_t gates_step = static_cast<int64_t>(4) * c.value_heads * (2 * kRun), tops_step = static_cast<int64_t>(4) * c.value_heads * D;
     Pair<Ask> w[4], q[4];
-    const auto load_asks = [&](int run0) {
-        const int64_t run = run_at(run0 + wave);
-        const _Float16 *w_at = p.through + (run * c.value_heads + h) * kHead, *q_at = p.asks + (run * 2 * c.key_heads + kh) * kHead;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            w[k] = Runs<D>::row_step(w_at, k, lane);
-            q[k] = Runs<D>::row_step(q_at, k, lane);
-        }
-    };
     f32x4_t u[NT], through, left;
     float u_top[NT], whole;
-    const auto load_updates = [&](int run0) {
-        const int64_t at = run_at(run0 + wave) * c.value_heads + h;
-        through = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + 4 * g);
-        left = *reinterpret_cast<const f32x4_t *>(p.chunk_gates + at * (2 * kRun) + kRun + 4 * g);
+    Pair4 inner[4], keys[kTiles][4];
+    const auto load_ask = [&](int chunk, int k) {
+        w[k] = Runs<D>::row_step(w_at + chunk * w_step, k, lane);
+        q[k] = Runs<D>::row_step(q_at + chunk * q_step, k, lane);
+    };
+    const auto load_updates = [&](int chunk) {
+        through = *reinterpret_cast<const f32x4_t *>(gates_at + chunk * gates_step);
+        left = *reinterpret_cast<const f32x4_t *>(gates_at + chunk * gates_step + kRun);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            u[t] = *reinterpret_cast<const f32x4_t *>(p.values + at * (kRun * D) + ((r0 / 16 + t) * 64 + lane) * 4);
-            u_top[t] = p.tops[(run_at(run0) * c.value_heads + h) * D + r0 + 16 * t + m];
+            u[t] = *reinterpret_cast<const f32x4_t *>(u_at + chunk * u_step + t * 256);
+            u_top[t] = tops_at[chunk * tops_step + 16 * t];
         }
     };
-    Pair4 inner[4], keys[kTiles][4];
-    const auto load_rest = [&](int run0) {
-        const int row = min(s.count - 1, run0 * kRun + kGdnChunk - 1);
-        whole = p.chunk_gates[((run_first + row / kRun) * c.value_heads + h) * (2 * kRun) + row % kRun];
-        const _Float16 *inner_at = p.inner + (run_at(run0 + wave) * c.value_heads + h) * (4 * kRun * 32);
+    const auto load_run = [&](int chunk, int b) {
+        inner[b] = four_step(inner_at + chunk * inner_step + min(b, wave) * (kRun * 32), lane);
+        const int64_t run = min(4 * chunk + b, last_run);  // past it keys may be anything, and count
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            inner[b] = four_step(inner_at + min(b, wave) * (kRun * 32), lane);
-            const _Float16 *k = p.keys_by_dim + (run_at(run0 + b) * c.key_heads + kh) * kHead + kTiles * wave * (kRun * 32);
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) keys[t][b] = four_step(k + t * (kRun * 32), lane);
-        }
+        for (int t = 0; t < kTiles; ++t) keys[t][b] = four_step(keys_at + run * c.key_heads * kHead + t * (kRun * 32), lane);
     };
-    load_asks(0);
+    const auto load_whole = [&](int chunk) {
+        const int row = min(s.count - 1, chunk * kGdnChunk + kGdnChunk - 1);
+        whole = whole_at[static_cast<int64_t>(row / kRun) * c.value_heads * (2 * kRun) + row % kRun];
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) load_ask(0, k);
     load_updates(0);
-    load_rest(0);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) load_run(0, b);
+    load_whole(0);
     E *out = static_cast<E *>(p.out) + (s.begin + static_cast<int64_t>(16 * wave + 4 * g)) * p.out_row + h * D + r0 + m;
     // a column's largest number of this wave's part of S
     const auto top_of = [&](int t) {
@@ -608,10 +636,9 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
     lds_barrier();
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int i0 = 0; i0 < s.count; i0 += kGdnChunk) {
-        const int mine = s.count - i0 - 16 * wave - 4 * g;  // this lane's rows that are there
-        const bool more = i0 + kGdnChunk < s.count;
-        const int next = i0 / kRun + 4;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        const int mine = s.count - chunk * kGdnChunk - 16 * wave - 4 * g;  // this lane's rows that are there
+        const int next = min(chunk + 1, chunks - 1);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float top = top_of(t);
@@ -630,7 +657,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
 #pragma unroll
         for (int t = 0; t < NT; ++t) asked[t] = o[t] = zero;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
@@ -638,7 +665,8 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                 asked[t] = product(w[k], b, asked[t]);
                 o[t] = product(q[k], b, o[t]);
             }
-        if (more) load_asks(next);
+            load_ask(next, k);
+        }
         float d_from[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -648,7 +676,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 d[e] = e < mine ? __builtin_fmaf(asked[t][e], -s_from[t], u[t][e]) : 0.0f;
-                d_left[e] = d[e] * left[e];
+                d_left[e] = e < mine ? d[e] * left[e] : 0.0f;
                 o[t][e] *= through[e] * s_from[t];
             }
             d_from[t] = scale.from;
@@ -661,7 +689,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
             *reinterpret_cast<f16x4_t *>(&rh[0][at]) = y.h;
             *reinterpret_cast<f16x4_t *>(&rh[1][at]) = y.l;
         }
-        if (more) load_updates(next);
+        load_updates(next);
         lds_barrier();  // every wave's updates are there, and its reads of S done
         f32x4_t added[NT][kTiles], among[NT];
 #pragma unroll
@@ -671,7 +699,7 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
             for (int k = 0; k < kTiles; ++k) added[t][k] = zero;
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
@@ -683,6 +711,8 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                     among[t] = product(inner[b], d, among[t]);
                 }
             }
+            load_run(next, b);
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -691,8 +721,8 @@ __global__ __launch_bounds__(256) void gdn_states_kernel(const GdnRowsParams p) 
                 for (int k = 0; k < kTiles; ++k) S[t][k][e] = __builtin_fmaf(added[t][k][e], d_from[t], S[t][k][e] * whole);
                 o[t][e] = __builtin_fmaf(among[t][e], d_from[t], o[t][e]);
             }
-        if (more) load_rest(next);
-        E *to = out + i0 * p.out_row;
+        load_whole(next);
+        E *to = out + static_cast<int64_t>(chunk) * kGdnChunk * p.out_row;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (e >= mine) continue;
@@ -711,11 +741,13 @@ hipError_t many_typed(const GdnRowsParams &p, hipStream_t stream) {
     const GdnView &c = p.cache;
     const int parts = (c.channels() + 127) / 128 + 1;  // one more for the gates
     const dim3 runs((parts + 3) / 4, (p.batch.max_rows + kRun - 1) / kRun, p.batch.sequences);
-    if (c.taps == 4) hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 4>), runs, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 0>), runs, dim3(256), 0, stream, p);
+    if (c.taps == 4 && p.pairs) hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 4, true>), runs, dim3(256), 0, stream, p);
+    else if (p.pairs) hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 0, true>), runs, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((gdn_inputs_kernel<DT, D, 0, false>), runs, dim3(256), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((gdn_chunk_kernel<D>), dim3((p.batch.max_rows + kGdnChunk - 1) / kGdnChunk, c.value_heads, p.batch.sequences),
+    // heads first: they go round the dies, of which each then has as many chunks
+    hipLaunchKernelGGL((gdn_chunk_kernel<D>), dim3(c.value_heads, (p.batch.max_rows + kGdnChunk - 1) / kGdnChunk, p.batch.sequences),
         dim3(256), 0, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -95,8 +95,8 @@ struct GdnRowsParams {
     float *rate = nullptr;            // [rows][value_heads]: beta
     int *stands = nullptr;    // [kGdnMaxSequences]
 };
-// runs of up to `rows` rows (their places: gdn_chunks.hip)
-inline size_t gdn_runs(size_t rows) { return rows / kGdnRun + rows / (kGdnRun + 1) + 1; }
+// runs of up to `rows` rows (their places: gdn_chunks.hip), and of the rest of the last chunk
+inline size_t gdn_runs(size_t rows) { return rows / kGdnRun + rows / (kGdnRun + 1) + 4; }
 // few rows of every sequence that has few
 hipError_t launch_gdn_few(const GdnRowsParams &p, Dtype dtype, hipStream_t stream);
 // the others: convolution, norms and gates; products within chunks; the states through them
