@@ -128,6 +128,40 @@ def test_quotients_that_are_halves(ctx):
         assert torch.equal(codes, torch.round(127.0 * x / top))  # round() takes ties to even
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width,group", [(7, 2048, 128), (1027, 1024, 256), (1500, 4096, 128), (1026, 2560, 2560), (3, 5120, 64)])
+def test_codes_of_gated_rows_alone(ctx, rows, width, group, dtype):
+    g = torch.Generator().manual_seed(rows + width + group)
+    x = torch.randn(rows, width, generator=g).to(TYPES[dtype]).cuda()
+    z = torch.randn(rows, width, generator=g).mul(4).to(TYPES[dtype]).cuda()
+    w = (1.0 + 0.2 * torch.randn(group, generator=g)).cuda()
+    want = definition(x, None, w, group, z, dtype)
+    check(run(ctx, x, None, w, group, z, dtype, want_sum=False, want_output=False), want, dtype, False, False)
+
+
+def test_gated_rows_near_the_ends_of_their_type(ctx):
+    """Large and small gates, weights and rows, one in each block or all of one: the codes are still the nearest."""
+    g = torch.Generator().manual_seed(3)
+    width, gates = 256, (-1e4, -103.0, -89.0, -86.0, -79.0, 79.0, 3e5, 1e20)
+    x = torch.randn(64, width, generator=g)
+    z = torch.randn(64, width, generator=g)
+    w = torch.ones(width)
+    for k, gate in enumerate(gates):
+        z[k, ::32] = gate
+        z[8 + k] = gate
+        z[16 + k] = gate * (1.0 + 0.1 * torch.rand(width, generator=g))
+    x[24:32] *= 1e18
+    x[32:40] *= 1e-22
+    x[40:48, 32:64] *= 1e-20
+    x[48:56] = 0.0
+    for scale in (1.0, 1e-12, 1e12):
+        want = definition(x.cuda(), None, (w * scale).cuda(), width, z.cuda(), "f32")
+        got = run(ctx, x.cuda(), None, (w * scale).cuda(), width, z.cuda(), "f32", want_sum=False, want_output=False)
+        fits = want[3] < 65504  # a scale beyond fp16 is infinite, and its block's values are none
+        codes, scales = planes(got[2], 64, width)[:2]
+        assert torch.equal(codes, want[2]) and torch.equal(scales[fits], want[3][fits]) and not torch.isfinite(scales[~fits]).any()
+
+
 def test_rows_that_are_not_finite(ctx):
     x = torch.randn(4, 128)
     x[1, 40] = float("nan")
