@@ -23,8 +23,10 @@ constexpr int kRuleThreads = 256;
 template <Dtype DT, bool VEC, int CHUNK>
 __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p) {
     typedef typename Element<DT>::type E;
-    constexpr int kFours = CHUNK / (4 * kRuleThreads);
+    constexpr int kFours = CHUNK / (4 * kRuleThreads), kAtOnce = 8;
     __shared__ __align__(16) int counts[CHUNK];
+    // the tokens that come and go with a row, from row0 + 1 on, as places in the chunk (-1: elsewhere)
+    __shared__ int comes[kRuleThreads], goes[kRuleThreads];
     const int seq = blockIdx.y, first = blockIdx.x * CHUNK, thread = threadIdx.x;
     int begin = read_only(p.row_starts + seq), end = read_only(p.row_starts + seq + 1);
     begin = min(max(begin, 0), p.rows);
@@ -55,11 +57,20 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
     int64_t length = 0;  // of the history
     const int64_t *history = nullptr;
     const auto token_at = [&](int64_t place) { return place < length ? history[place] : p.tokens[begin + (place - length)]; };
-    const auto count = [&](int64_t token, int by) {
+    const auto place_of = [&](int64_t token) {
         const int64_t at = token - first;
-        if (at >= 0 && at < CHUNK && token < p.vocab) atomicAdd(&counts[at], by);
+        return at >= 0 && at < CHUNK && token < p.vocab ? static_cast<int>(at) : -1;
     };
     const auto text_end = [&](int row) { return length + (p.tokens ? row - begin + 1 : 0); };
+    // a thread's row of the next kRuleThreads
+    const auto note_tokens = [&](int from_row) {
+        const int row = from_row + thread;
+        comes[thread] = goes[thread] = -1;
+        if (!p.tokens || row >= row1) return;
+        const int64_t last = text_end(row);
+        comes[thread] = place_of(token_at(last - 1));
+        if (p.window > 0 && last > p.window) goes[thread] = place_of(token_at(last - 1 - p.window));
+    };
     if (counting) {
         repetition = p.penalties[3 * seq];
         frequency = p.penalties[3 * seq + 1];
@@ -68,10 +79,25 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
             length = min(max(static_cast<int64_t>(p.history_lengths[seq]), static_cast<int64_t>(0)), p.history_pitch);
             history = p.history + seq * p.history_pitch;
         }
+        const int64_t last = text_end(row0), from = p.window > 0 && last > p.window ? last - p.window : 0;
+        int64_t token[kAtOnce];
+        const auto load_tokens = [&](int64_t place) {
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) token[k] = place + k * kRuleThreads < last ? token_at(place + k * kRuleThreads) : -1;
+        };
+        load_tokens(from + thread);
+        note_tokens(row0 + 1);
         for (int i = thread; i < CHUNK; i += kRuleThreads) counts[i] = 0;
         lds_barrier();
-        const int64_t last = text_end(row0), from = p.window > 0 && last > p.window ? last - p.window : 0;
-        for (int64_t place = from + thread; place < last; place += kRuleThreads) count(token_at(place), 1);
+        for (int64_t place = from + thread; place < last; place += kAtOnce * kRuleThreads) {
+            int at[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) at[k] = place_of(token[k]);
+            load_tokens(place + kAtOnce * kRuleThreads);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k)
+                if (at[k] >= 0) atomicAdd(&counts[at[k]], 1);
+        }
         lds_barrier();
     }
 
@@ -122,13 +148,17 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
             }
         }
         if (counting && p.tokens && row + 1 < row1) {
+            const int ahead = (row - row0) % kRuleThreads;
             lds_barrier();
             if (thread == 0) {
-                const int64_t last = text_end(row + 1);
-                count(token_at(last - 1), 1);
-                if (p.window > 0 && last > p.window) count(token_at(last - 1 - p.window), -1);
+                if (comes[ahead] >= 0) ++counts[comes[ahead]];
+                if (goes[ahead] >= 0) --counts[goes[ahead]];
             }
             lds_barrier();
+            if (ahead == kRuleThreads - 1) {
+                note_tokens(row + 2);
+                lds_barrier();
+            }
         }
     }
 }
