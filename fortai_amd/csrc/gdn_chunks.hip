@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
 // instructions' results a lane has value dim m and four key dims (of S) or rows (of D and
 // O).  A wave has 16 rows of the chunk and a quarter of the key dims.
 template <Dtype DT, int D, int NT>
-__global__ __launch_bounds__(256, 2) void gdn_states_kernel(const GdnRowsParams p) {
+__global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
     typedef typename Runs<D>::Ask Ask;
     constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8, kAsk = Runs<D>::kAsk;
