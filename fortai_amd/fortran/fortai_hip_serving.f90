@@ -1,6 +1,7 @@
 ! fortai_hip_serving.f90 -- the serving operators of libfortai_hip.so from
 ! Fortran: rotary positions, the 8-bit paged key/value cache with its attention,
-! its page bookkeeping, and the verification of drafted tokens.
+! its page bookkeeping, the verification of drafted tokens, the gated delta rule
+! over rows, norms into 8-bit tokens and rules on logits.
 !
 ! The reference runs one token of one sequence at a time and has none of these;
 ! the module keeps the manner of fortai_backend_hip: derived types that hold a
@@ -30,6 +31,35 @@ module fortai_hip_serving
         type(c_ptr) :: tables = c_null_ptr
     end type hip_kv8_batch_t
 
+    ! fortai_hip_kv8_groups: which sequences of a batch share their first pages
+    type, bind(C), public :: hip_kv8_groups_t
+        integer(c_int) :: groups = 0, max_rows = 0
+        type(c_ptr) :: starts = c_null_ptr
+        type(c_ptr) :: shared = c_null_ptr
+        type(c_ptr) :: group_of = c_null_ptr
+    end type hip_kv8_groups_t
+
+    ! fortai_hip_gdn_batch: the rows of a call, whose they are and how many of the last ones stand
+    type, bind(C), public :: hip_gdn_batch_t
+        integer(c_int) :: sequences = 0, rows = 0, max_rows = 0
+        type(c_ptr) :: row_starts = c_null_ptr
+        type(c_ptr) :: slots = c_null_ptr
+        type(c_ptr) :: standing = c_null_ptr
+    end type hip_gdn_batch_t
+
+    ! fortai_hip_logit_rules
+    type, bind(C), public :: hip_logit_rules_t
+        integer(c_int) :: window = 0, mask_count = 0
+        type(c_ptr) :: penalties = c_null_ptr
+        type(c_ptr) :: tokens = c_null_ptr
+        type(c_ptr) :: history = c_null_ptr
+        type(c_ptr) :: history_lengths = c_null_ptr
+        type(c_ptr) :: bias = c_null_ptr
+        type(c_ptr) :: masks = c_null_ptr
+        type(c_ptr) :: mask_of = c_null_ptr
+        integer(c_int64_t) :: history_pitch = 0, bias_pitch = 0, mask_pitch = 0
+    end type hip_logit_rules_t
+
     type, public :: hip_rope_t
         type(c_ptr) :: handle = c_null_ptr
         type(hip_q8_context_t) :: context
@@ -48,6 +78,7 @@ module fortai_hip_serving
         procedure :: append => cache_append
         procedure :: read => cache_read
         procedure :: attention => cache_attention
+        procedure :: shared_attention => cache_shared_attention
         procedure :: copy_pages => cache_copy_pages
     end type hip_kv8_cache_t
 
@@ -63,6 +94,7 @@ module fortai_hip_serving
         procedure :: length => pages_length
         procedure :: free_count => pages_free_count
         procedure :: tables => pages_tables
+        procedure :: groups => pages_groups
     end type hip_kv8_pages_t
 
     type, public :: hip_verifier_t
@@ -74,7 +106,17 @@ module fortai_hip_serving
         procedure :: run => verifier_run
     end type hip_verifier_t
 
-    public :: hip_kv8_bytes
+    type, public :: hip_gdn_cache_t
+        type(c_ptr) :: handle = c_null_ptr
+        type(hip_q8_context_t) :: context
+    contains
+        procedure :: create => gdn_create
+        procedure :: destroy => gdn_destroy
+        procedure :: run => gdn_run
+        procedure :: copy_slots => gdn_copy_slots
+    end type hip_gdn_cache_t
+
+    public :: hip_kv8_bytes, hip_gdn_bytes, hip_norm_tokens, hip_tokens_read, hip_logits_adjust
 
     interface
         integer(c_int) function fh_rope_create(context, rope_dimension, interleaved, base, scaling, factor, &
@@ -139,6 +181,82 @@ module fortai_hip_serving
             integer(c_int64_t), value :: query_pitch, query_head_pitch, output_pitch
             real(c_float), value :: scale
         end function fh_kv8_attention
+        integer(c_int) function fh_kv8_shared_attention(cache, layer, batch, sharing, dtype, query, query_pitch, &
+            query_head_pitch, gate, heads, scale, max_length, max_shared, output, output_pitch) &
+            bind(C, name='fortai_hip_kv8_shared_attention_device')
+            import :: c_float, c_int, c_int64_t, c_ptr, hip_kv8_batch_t, hip_kv8_groups_t
+            type(c_ptr), value :: cache, query, gate, output
+            type(hip_kv8_batch_t), intent(in) :: batch
+            type(hip_kv8_groups_t), intent(in) :: sharing
+            integer(c_int), value :: layer, dtype, heads, max_length, max_shared
+            integer(c_int64_t), value :: query_pitch, query_head_pitch, output_pitch
+            real(c_float), value :: scale
+        end function fh_kv8_shared_attention
+        integer(c_int) function fh_pages_groups(pool, sequences, count, starts, shared, group_of, groups) &
+            bind(C, name='fortai_hip_kv8_pages_groups')
+            import :: c_int, c_int32_t, c_ptr
+            type(c_ptr), value :: pool
+            integer(c_int), intent(in) :: sequences(*)
+            integer(c_int), value :: count
+            integer(c_int32_t), intent(inout) :: starts(*), shared(*), group_of(*)
+            integer(c_int32_t), intent(out) :: groups
+        end function fh_pages_groups
+        integer(c_int) function fh_norm_tokens(context, dtype, x, x_pitch, residual, residual_pitch, total, sum_pitch, norm, &
+            group, epsilon, gate, gate_pitch, rows, width, output, output_pitch, tokens) &
+            bind(C, name='fortai_hip_norm_tokens_device')
+            import :: c_float, c_int, c_int64_t, c_ptr
+            type(c_ptr), value :: context, x, residual, total, norm, gate, output, tokens
+            integer(c_int), value :: dtype, group, rows, width
+            integer(c_int64_t), value :: x_pitch, residual_pitch, sum_pitch, gate_pitch, output_pitch
+            real(c_float), value :: epsilon
+        end function fh_norm_tokens
+        integer(c_int) function fh_tokens_read(context, dtype, tokens, rows, width, output, output_pitch) &
+            bind(C, name='fortai_hip_q8_tokens_read_device')
+            import :: c_int, c_int64_t, c_ptr
+            type(c_ptr), value :: context, tokens, output
+            integer(c_int), value :: dtype, rows, width
+            integer(c_int64_t), value :: output_pitch
+        end function fh_tokens_read
+        integer(c_int) function fh_logits_adjust(context, dtype, logits, logits_pitch, rows, vocab, sequences, row_starts, &
+            rules, output, output_pitch) bind(C, name='fortai_hip_logits_adjust_device')
+            import :: c_int, c_int64_t, c_ptr, hip_logit_rules_t
+            type(c_ptr), value :: context, logits, row_starts, output
+            type(hip_logit_rules_t), intent(in) :: rules
+            integer(c_int), value :: dtype, rows, vocab, sequences
+            integer(c_int64_t), value :: logits_pitch, output_pitch
+        end function fh_logits_adjust
+        integer(c_size_t) function fh_gdn_bytes(layers, slots, key_heads, value_heads, head_size, conv_kernel, pending) &
+            bind(C, name='fortai_hip_gdn_bytes')
+            import :: c_int, c_size_t
+            integer(c_int), value :: layers, slots, key_heads, value_heads, head_size, conv_kernel, pending
+        end function fh_gdn_bytes
+        integer(c_int) function fh_gdn_create(context, layers, slots, key_heads, value_heads, head_size, conv_kernel, pending, &
+            max_rows, storage, storage_bytes, cache) bind(C, name='fortai_hip_gdn_create')
+            import :: c_int, c_ptr, c_size_t
+            type(c_ptr), value :: context, storage
+            integer(c_int), value :: layers, slots, key_heads, value_heads, head_size, conv_kernel, pending, max_rows
+            integer(c_size_t), value :: storage_bytes
+            type(c_ptr), intent(out) :: cache
+        end function fh_gdn_create
+        integer(c_int) function fh_gdn_destroy(cache) bind(C, name='fortai_hip_gdn_destroy')
+            import :: c_int, c_ptr
+            type(c_ptr), value :: cache
+        end function fh_gdn_destroy
+        integer(c_int) function fh_gdn_run(cache, layer, batch, dtype, qkv, qkv_pitch, alpha, alpha_pitch, beta, beta_pitch, &
+            conv, ssm_a, ssm_dt, epsilon, output, output_pitch) bind(C, name='fortai_hip_gdn_run_device')
+            import :: c_float, c_int, c_int64_t, c_ptr, hip_gdn_batch_t
+            type(c_ptr), value :: cache, qkv, alpha, beta, conv, ssm_a, ssm_dt, output
+            type(hip_gdn_batch_t), intent(in) :: batch
+            integer(c_int), value :: layer, dtype
+            integer(c_int64_t), value :: qkv_pitch, alpha_pitch, beta_pitch, output_pitch
+            real(c_float), value :: epsilon
+        end function fh_gdn_run
+        integer(c_int) function fh_gdn_copy_slots(cache, from, to, count) bind(C, name='fortai_hip_gdn_copy_slots')
+            import :: c_int, c_int32_t, c_ptr
+            type(c_ptr), value :: cache
+            integer(c_int32_t), intent(in) :: from(*), to(*)
+            integer(c_int), value :: count
+        end function fh_gdn_copy_slots
         integer(c_int) function fh_kv8_copy_pages(cache, from, to, count) bind(C, name='fortai_hip_kv8_copy_pages')
             import :: c_int, c_int32_t, c_ptr
             type(c_ptr), value :: cache
@@ -404,6 +522,24 @@ contains
             '8-bit cache attention', stat)
     end subroutine cache_attention
 
+    ! the tokens of sequences that share their first pages are read once for a group
+    subroutine cache_shared_attention(self, layer, batch, sharing, dtype, query, query_pitch, query_head_pitch, gate, heads, &
+        scale, max_length, max_shared, output, output_pitch, stat)
+        class(hip_kv8_cache_t), intent(in) :: self
+        integer, intent(in) :: layer, dtype, heads, max_length, max_shared
+        type(hip_kv8_batch_t), intent(in) :: batch
+        type(hip_kv8_groups_t), intent(in) :: sharing
+        type(c_ptr), intent(in) :: query, gate, output
+        integer(c_int64_t), intent(in) :: query_pitch, query_head_pitch, output_pitch
+        real(c_float), intent(in) :: scale
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(self%handle, '8-bit cache', stat)) return
+        call settle(fh_kv8_shared_attention(self%handle, int(layer, c_int), batch, sharing, int(dtype, c_int), query, &
+            query_pitch, query_head_pitch, gate, int(heads, c_int), scale, int(max_length, c_int), int(max_shared, c_int), &
+            output, output_pitch), self%context, '8-bit cache shared attention', stat)
+    end subroutine cache_shared_attention
+
     subroutine cache_copy_pages(self, from, to, stat)
         class(hip_kv8_cache_t), intent(in) :: self
         integer(c_int32_t), intent(in) :: from(:), to(:)
@@ -527,6 +663,26 @@ contains
             int(size(tables, 1), c_int)), nowhere(), 'page tables', stat)
     end subroutine pages_tables
 
+    ! the groups 0 .. groups - 1 of these sequences, in this order; starts has one more than sequences
+    subroutine pages_groups(self, sequences, starts, shared, group_of, groups, stat)
+        class(hip_kv8_pages_t), intent(in) :: self
+        integer(c_int), intent(in) :: sequences(:)
+        integer(c_int32_t), intent(inout) :: starts(:), shared(:), group_of(:)
+        integer, intent(out) :: groups
+        type(status_t), intent(out) :: stat
+        integer(c_int32_t) :: count
+
+        groups = 0
+        if (.not. usable(self%handle, 'page pool', stat)) return
+        if (size(starts) <= size(sequences) .or. size(shared) < size(sequences) .or. size(group_of) < size(sequences)) then
+            call stat%set(FORTAI_INVALID, 'HIP page groups: a place for every sequence, and one more start')
+            return
+        end if
+        call settle(fh_pages_groups(self%handle, sequences, int(size(sequences), c_int), starts, shared, group_of, count), &
+            nowhere(), 'page groups', stat)
+        if (stat%is_ok()) groups = int(count)
+    end subroutine pages_groups
+
     ! ---- draft verification ----
 
     subroutine verifier_create(self, context, max_rows, max_sequences, vocab, stat)
@@ -566,5 +722,124 @@ contains
             temperatures, int(sequences, c_int), row_starts, int(rows, c_int), emitted, accepted, logprobs), self%context, &
             'draft verification', stat)
     end subroutine verifier_run
+
+    ! ---- norms into 8-bit tokens ----
+
+    ! residual, total (the sum), norm, gate, output and tokens may be c_null_ptr
+    subroutine hip_norm_tokens(context, dtype, x, x_pitch, residual, residual_pitch, total, sum_pitch, norm, group, epsilon, &
+        gate, gate_pitch, rows, width, output, output_pitch, tokens, stat)
+        type(hip_q8_context_t), intent(in) :: context
+        integer, intent(in) :: dtype, group, rows, width
+        type(c_ptr), intent(in) :: x, residual, total, norm, gate, output, tokens
+        integer(c_int64_t), intent(in) :: x_pitch, residual_pitch, sum_pitch, gate_pitch, output_pitch
+        real(c_float), intent(in) :: epsilon
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(context%handle, 'context', stat)) return
+        call settle(fh_norm_tokens(context%handle, int(dtype, c_int), x, x_pitch, residual, residual_pitch, total, sum_pitch, &
+            norm, int(group, c_int), epsilon, gate, gate_pitch, int(rows, c_int), int(width, c_int), output, output_pitch, &
+            tokens), context, 'norm into tokens', stat)
+    end subroutine hip_norm_tokens
+
+    subroutine hip_tokens_read(context, dtype, tokens, rows, width, output, output_pitch, stat)
+        type(hip_q8_context_t), intent(in) :: context
+        integer, intent(in) :: dtype, rows, width
+        type(c_ptr), intent(in) :: tokens, output
+        integer(c_int64_t), intent(in) :: output_pitch
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(context%handle, 'context', stat)) return
+        call settle(fh_tokens_read(context%handle, int(dtype, c_int), tokens, int(rows, c_int), int(width, c_int), output, &
+            output_pitch), context, 'reading tokens', stat)
+    end subroutine hip_tokens_read
+
+    ! ---- rules on logits ----
+
+    subroutine hip_logits_adjust(context, dtype, logits, logits_pitch, rows, vocab, sequences, row_starts, rules, output, &
+        output_pitch, stat)
+        type(hip_q8_context_t), intent(in) :: context
+        integer, intent(in) :: dtype, rows, vocab, sequences
+        type(c_ptr), intent(in) :: logits, row_starts, output
+        integer(c_int64_t), intent(in) :: logits_pitch, output_pitch
+        type(hip_logit_rules_t), intent(in) :: rules
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(context%handle, 'context', stat)) return
+        call settle(fh_logits_adjust(context%handle, int(dtype, c_int), logits, logits_pitch, int(rows, c_int), &
+            int(vocab, c_int), int(sequences, c_int), row_starts, rules, output, output_pitch), context, 'rules on logits', &
+            stat)
+    end subroutine hip_logits_adjust
+
+    ! ---- the gated delta rule over rows ----
+
+    ! 0: no such cache
+    integer(c_size_t) function hip_gdn_bytes(layers, slots, key_heads, value_heads, head_size, conv_kernel, pending)
+        integer, intent(in) :: layers, slots, key_heads, value_heads, head_size, conv_kernel, pending
+
+        hip_gdn_bytes = fh_gdn_bytes(int(layers, c_int), int(slots, c_int), int(key_heads, c_int), int(value_heads, c_int), &
+            int(head_size, c_int), int(conv_kernel, c_int), int(pending, c_int))
+    end function hip_gdn_bytes
+
+    ! without storage the cache has its own, cleared
+    subroutine gdn_create(self, context, layers, slots, key_heads, value_heads, head_size, conv_kernel, pending, max_rows, &
+        stat, storage, storage_bytes)
+        class(hip_gdn_cache_t), intent(inout) :: self
+        type(hip_q8_context_t), intent(in) :: context
+        integer, intent(in) :: layers, slots, key_heads, value_heads, head_size, conv_kernel, pending, max_rows
+        type(status_t), intent(out) :: stat
+        type(c_ptr), intent(in), optional :: storage
+        integer(c_size_t), intent(in), optional :: storage_bytes
+        type(c_ptr) :: memory
+        integer(c_size_t) :: bytes
+
+        memory = c_null_ptr
+        bytes = 0
+        if (present(storage)) memory = storage
+        if (present(storage_bytes)) bytes = storage_bytes
+        if (.not. usable(context%handle, 'context', stat)) return
+        call self%destroy(stat)
+        self%context = context
+        call settle(fh_gdn_create(context%handle, int(layers, c_int), int(slots, c_int), int(key_heads, c_int), &
+            int(value_heads, c_int), int(head_size, c_int), int(conv_kernel, c_int), int(pending, c_int), &
+            int(max_rows, c_int), memory, bytes, self%handle), context, 'delta rule cache creation', stat)
+    end subroutine gdn_create
+
+    subroutine gdn_destroy(self, stat)
+        class(hip_gdn_cache_t), intent(inout) :: self
+        type(status_t), intent(out) :: stat
+
+        call stat%clear()
+        if (.not. c_associated(self%handle)) return
+        call settle(fh_gdn_destroy(self%handle), self%context, 'delta rule cache destruction', stat)
+        self%handle = c_null_ptr
+    end subroutine gdn_destroy
+
+    subroutine gdn_run(self, layer, batch, dtype, qkv, qkv_pitch, alpha, alpha_pitch, beta, beta_pitch, conv, ssm_a, ssm_dt, &
+        epsilon, output, output_pitch, stat)
+        class(hip_gdn_cache_t), intent(in) :: self
+        integer, intent(in) :: layer, dtype
+        type(hip_gdn_batch_t), intent(in) :: batch
+        type(c_ptr), intent(in) :: qkv, alpha, beta, conv, ssm_a, ssm_dt, output
+        integer(c_int64_t), intent(in) :: qkv_pitch, alpha_pitch, beta_pitch, output_pitch
+        real(c_float), intent(in) :: epsilon
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(self%handle, 'delta rule cache', stat)) return
+        call settle(fh_gdn_run(self%handle, int(layer, c_int), batch, int(dtype, c_int), qkv, qkv_pitch, alpha, alpha_pitch, &
+            beta, beta_pitch, conv, ssm_a, ssm_dt, epsilon, output, output_pitch), self%context, 'delta rule', stat)
+    end subroutine gdn_run
+
+    subroutine gdn_copy_slots(self, from, to, stat)
+        class(hip_gdn_cache_t), intent(in) :: self
+        integer(c_int32_t), intent(in) :: from(:), to(:)
+        type(status_t), intent(out) :: stat
+
+        if (.not. usable(self%handle, 'delta rule cache', stat)) return
+        if (size(from) /= size(to)) then
+            call stat%set(FORTAI_INVALID, 'HIP slot copy: as many slots to as from')
+            return
+        end if
+        call settle(fh_gdn_copy_slots(self%handle, from, to, int(size(from), c_int)), self%context, 'slot copy', stat)
+    end subroutine gdn_copy_slots
 
 end module fortai_hip_serving

@@ -983,3 +983,100 @@ FORTAI_HIP_WEAK int fortai_hip_verify_drafts_device(fortai_hip_verifier *verifie
     (void)device_emitted; (void)device_accepted; (void)device_logprobs;
     return FORTAI_HIP_RUNTIME_ERROR;
 }
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_shared_attention_device(fortai_hip_kv8_cache *cache, int layer,
+    const fortai_hip_kv8_batch *batch, const fortai_hip_kv8_groups *sharing, int dtype,
+    const void *device_query, int64_t query_pitch, int64_t query_head_pitch, const void *device_gate,
+    int heads, float scale, int max_length, int max_shared, void *device_output,
+    int64_t output_pitch)
+{
+    (void)cache; (void)layer; (void)batch; (void)sharing; (void)dtype; (void)device_query;
+    (void)query_pitch; (void)query_head_pitch; (void)device_gate; (void)heads; (void)scale;
+    (void)max_length; (void)max_shared; (void)device_output; (void)output_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_kv8_pages_groups(const fortai_hip_kv8_pages *pool, const int *sequences, int count,
+    int32_t *starts, int32_t *shared, int32_t *group_of, int *groups)
+{
+    (void)pool; (void)sequences; (void)count; (void)starts; (void)shared; (void)group_of;
+    if (groups) *groups = 0;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_norm_tokens_device(fortai_hip_q8_context *context, int dtype, const void *device_x,
+    int64_t x_pitch, const void *device_residual, int64_t residual_pitch, void *device_sum,
+    int64_t sum_pitch, const void *device_norm, int group, float epsilon, const void *device_gate,
+    int64_t gate_pitch, int rows, int width, void *device_output, int64_t output_pitch,
+    void *device_tokens)
+{
+    (void)context; (void)dtype; (void)device_x; (void)x_pitch; (void)device_residual;
+    (void)residual_pitch; (void)device_sum; (void)sum_pitch; (void)device_norm; (void)group;
+    (void)epsilon; (void)device_gate; (void)gate_pitch; (void)rows; (void)width;
+    (void)device_output; (void)output_pitch; (void)device_tokens;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_q8_tokens_read_device(fortai_hip_q8_context *context, int dtype,
+    const void *device_tokens, int rows, int width, void *device_output, int64_t output_pitch)
+{
+    (void)context; (void)dtype; (void)device_tokens; (void)rows; (void)width;
+    (void)device_output; (void)output_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_logits_adjust_device(fortai_hip_q8_context *context, int dtype,
+    const void *device_logits, int64_t logits_pitch, int rows, int vocab, int sequences,
+    const void *device_row_starts, const fortai_hip_logit_rules *rules, void *device_output,
+    int64_t output_pitch)
+{
+    (void)context; (void)dtype; (void)device_logits; (void)logits_pitch; (void)rows;
+    (void)vocab; (void)sequences; (void)device_row_starts; (void)rules; (void)device_output;
+    (void)output_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK size_t fortai_hip_gdn_bytes(int layers, int slots, int key_heads, int value_heads, int head_size,
+    int conv_kernel, int pending)
+{
+    (void)layers; (void)slots; (void)key_heads; (void)value_heads; (void)head_size;
+    (void)conv_kernel; (void)pending;
+    return 0;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_gdn_create(fortai_hip_q8_context *context, int layers, int slots, int key_heads,
+    int value_heads, int head_size, int conv_kernel, int pending, int max_rows, void *device_storage,
+    size_t storage_bytes, fortai_hip_gdn_cache **cache)
+{
+    (void)context; (void)layers; (void)slots; (void)key_heads; (void)value_heads;
+    (void)head_size; (void)conv_kernel; (void)pending; (void)max_rows; (void)device_storage;
+    (void)storage_bytes;
+    if (cache) *cache = NULL;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_gdn_destroy(fortai_hip_gdn_cache *cache)
+{
+    (void)cache;
+    return FORTAI_HIP_OK;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_gdn_run_device(fortai_hip_gdn_cache *cache, int layer,
+    const fortai_hip_gdn_batch *batch, int dtype, const void *device_qkv, int64_t qkv_pitch,
+    const void *device_alpha, int64_t alpha_pitch, const void *device_beta, int64_t beta_pitch,
+    const void *device_conv, const void *device_ssm_a, const void *device_ssm_dt, float epsilon,
+    void *device_output, int64_t output_pitch)
+{
+    (void)cache; (void)layer; (void)batch; (void)dtype; (void)device_qkv; (void)qkv_pitch;
+    (void)device_alpha; (void)alpha_pitch; (void)device_beta; (void)beta_pitch;
+    (void)device_conv; (void)device_ssm_a; (void)device_ssm_dt; (void)epsilon;
+    (void)device_output; (void)output_pitch;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}
+
+FORTAI_HIP_WEAK int fortai_hip_gdn_copy_slots(fortai_hip_gdn_cache *cache, const int32_t *from, const int32_t *to,
+    int count)
+{
+    (void)cache; (void)from; (void)to; (void)count;
+    return FORTAI_HIP_RUNTIME_ERROR;
+}

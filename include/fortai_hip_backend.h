@@ -626,9 +626,9 @@ int fortai_hip_kv8_shared_attention_device(fortai_hip_kv8_cache *cache, int laye
  * at most `capacity` of them; the moves go through copy_pages before the next
  * append or attention, and tables that were taken before are stale.
  * tables: the pages of count sequences, rows of table_pitch, -1 behind the last.
- * groups: which of count sequences, in this order, share leading pages with the ones
- * before them, as fortai_hip_kv8_groups wants it (host arrays starts [count + 1], shared
- * and group_of [count]); groups of no shared tokens hold the others.
+ * groups: which of count sequences, in this order, share leading pages of 64 tokens or more
+ * with the ones before them, as fortai_hip_kv8_groups wants it (host arrays starts
+ * [count + 1], shared and group_of [count]); groups of no shared tokens hold the others.
  * length (-1: no such sequence) and free_count (-1: no pool) ask. */
 int fortai_hip_kv8_pages_create(int pages, int page_tokens, int sequences, int table_pitch,
     fortai_hip_kv8_pages **pool);
