@@ -27,7 +27,7 @@ struct fortai_hip_kv8_cache {
     Kv8Shape shape;
     uint8_t *storage = nullptr;
     bool owned = false;
-    // partial results of split attention calls, [kKv8PartialRows][head + 4]: made
+    // partial results of split attention calls, [kKv8SharedRows][head + 4]: made
     // with the cache and never again, so that a captured call keeps its address
     float *partial = nullptr;
     std::mutex launches;  // a call's two launches follow each other on the stream
@@ -109,7 +109,7 @@ int attend(fortai_hip_kv8_cache *h, int layer, const fortai_hip_kv8_batch *batch
     p.vec = vector4_ok(query, dtype, query_pitch, query_head_pitch) && vector4_ok(output, dtype, output_pitch, 0) &&
         vector4_ok(gate, dtype, 0, 0);
     p.partial = h->partial;
-    p.partial_ml = reinterpret_cast<f32x4_t *>(h->partial + static_cast<size_t>(kKv8PartialRows) * h->shape.head);
+    p.partial_ml = reinterpret_cast<f32x4_t *>(h->partial + static_cast<size_t>(kKv8SharedRows) * h->shape.head);
     const bool fp32 = dtype == FORTAI_HIP_DTYPE_F32;
     const int head = h->shape.head, kv_heads = h->shape.kv_heads;
     const int64_t rows = static_cast<int64_t>(batch->max_rows) * p.group;
@@ -249,7 +249,7 @@ int fortai_hip_kv8_create(fortai_hip_q8_context *c, int layers, int pages, int p
         h->owned = e == hipSuccess;
         if (e == hipSuccess) e = launch_kv8_clear(h->storage, bytes, c->stream);
     }
-    if (e == hipSuccess) e = alloc(&h->partial, static_cast<size_t>(kKv8PartialRows) * (head_size + 4));
+    if (e == hipSuccess) e = alloc(&h->partial, static_cast<size_t>(kKv8SharedRows) * (head_size + 4));
     if (e != hipSuccess) {
         if (h->owned) release(h->storage);
         release(h->partial);

@@ -144,13 +144,21 @@ struct Quotient {
     __device__ __forceinline__ bool some() const { return norm != 0.0f; }
 };
 
-// Four dims of one row and head, gated and stored.  some: the row saw a token.
 template <Dtype DT>
-__device__ __forceinline__ void finish(const Kv8AttentionParams &p, f32x4_t y, bool some, int64_t row, int head, int out, int dim) {
+__device__ __forceinline__ f32x4_t load_gate(const Kv8AttentionParams &p, int64_t row, int head, int dim) {
+    typedef typename Element<DT>::type E;
+    const E *at = static_cast<const E *>(p.gate) + row * p.q_row + static_cast<int64_t>(head) * p.q_head + dim;
+    return p.vec ? load4<DT, true>(at) : load4<DT, false>(at);
+}
+
+// Four dims of one row and head, gated and stored.  some: the row saw a token; GATE: what
+// load_gate() gave is in *early.
+template <Dtype DT, bool GATE = false>
+__device__ __forceinline__ void finish(const Kv8AttentionParams &p, f32x4_t y, bool some, int64_t row, int head, int out, int dim,
+    const f32x4_t *early = nullptr) {
     typedef typename Element<DT>::type E;
     if (p.gate && some) {
-        const E *at = static_cast<const E *>(p.gate) + row * p.q_row + static_cast<int64_t>(head) * p.q_head + dim;
-        const f32x4_t g = p.vec ? load4<DT, true>(at) : load4<DT, false>(at);
+        const f32x4_t g = GATE ? *early : load_gate<DT>(p, row, head, dim);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = y[i] / (1.0f + expf(-g[i]));
     }
@@ -395,20 +403,28 @@ __device__ __forceinline__ int key_turn(int r) {
     return D == 256 ? r : D == 128 ? r >> 1 : 3 * (r >> 3);
 }
 
+template <int D, bool SPLIT>
+struct FewLds {
+    static constexpr int kRows = SPLIT ? 8 : 16;  // in an instruction's 16 columns
+    union {
+        u32x4_t codes[kWaves][kTileTokens * (D / 16)];  // a tile's keys, then its values
+        f32x4_t join[kWaves][D / 16][64];               // a wave's results for 16 columns
+    } tiles;
+    i32x4_t operands[kSets<SPLIT>][D / 64][64];
+    float factors[kRows];
+    f32x4_t joins[kWaves][kRows];  // a wave's base (score, value) and denominator (base, sum)
+};
+
 template <int D, Dtype DT, bool SPLIT, bool SHARING>
-__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8AttentionParams p) {
+__device__ __forceinline__ void attend_few(const Kv8AttentionParams &p, FewLds<D, SPLIT> &memory) {
     typedef typename Element<DT>::type E;
-    constexpr int kRows = SPLIT ? 8 : 16;           // in an instruction's 16 columns
+    constexpr int kRows = FewLds<D, SPLIT>::kRows, kS = kSets<SPLIT>;
     constexpr int kChunks = D / 64, kDims = D / 16;
     constexpr int kUnits = D / 16;                  // of a key row
-    __shared__ union {
-        u32x4_t codes[kWaves][kTileTokens * kUnits];  // a tile's keys, then its values
-        f32x4_t join[kWaves][kDims][64];              // a wave's results for 16 columns
-    } lds;
-    constexpr int kS = kSets<SPLIT>;
-    __shared__ i32x4_t operands[kS][kChunks][64];
-    __shared__ float factors[kRows];
-    __shared__ f32x4_t joins[kWaves][kRows];  // a wave's base (score, value) and denominator (base, sum)
+    auto &lds = memory.tiles;
+    auto &operands = memory.operands;
+    auto &factors = memory.factors;
+    auto &joins = memory.joins;
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -653,6 +669,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
         p.partial_ml[item * kRows + col] = f32x4_t{top.score, top.value, total.base, total.sum};
 }
 
+template <int D, Dtype DT, bool SPLIT, bool SHARING>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8AttentionParams p) {
+    __shared__ FewLds<D, SPLIT> lds;
+    attend_few<D, DT, SPLIT, SHARING>(p, lds);
+}
+
 // Many rows (a prompt's chunk): 64 rows a workgroup (32 with SPLIT), which share every
 // tile.  For the scores and their weights a wave has 16 (8) of the rows and the whole tile: its queries
 // stay in registers, the keys come from LDS (double buffered).  The weights go to the
@@ -670,14 +692,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_kernel(Kv8Attent
 // 16-row kernel 409) a version in which every wave read the whole tile's values from LDS
 // took 265, values by loads to LDS, as the keys, 273, and priority for the products was
 // worth 12.
-template <int D, Dtype DT, bool SPLIT, bool SHARING>
-__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
-    constexpr int kChunks = D / 64, kDims = D / 16, kUnits = D / 16, kS = kSets<SPLIT>;
-    constexpr int kMyRows = SPLIT ? 8 : 16, kRows = kWaves * kMyRows;
-    constexpr int kKeyUnits = kTileTokens * kUnits;
-    constexpr int kMine = D / 64;  // a wave's 16s of dims
-    constexpr int kHalves = SPLIT ? 1 : 2;  // of a weight, in a column
-    __shared__ union {
+template <int D, bool SPLIT>
+struct WideLds {
+    static constexpr int kKeyUnits = kTileTokens * (D / 16);
+    static constexpr int kHalves = SPLIT ? 1 : 2;  // of a weight, in a column
+    union {
         struct {
             u32x4_t keys[2][kKeyUnits];
             f16x8_t weights[kHalves][kWaves][2][64];  // of a wave's rows
@@ -685,11 +704,21 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
         } tile;
         struct {
             u32x4_t first_keys[kKeyUnits];  // loaded meanwhile
-            i32x4_t operands[kWaves][kS][kChunks][64];
+            i32x4_t operands[kWaves][kSets<SPLIT>][D / 64][64];
         } start;
-        f32x4_t rows[kWaves][kDims][64];
-    } lds;
-    __shared__ float factors[kWaves][16];
+        f32x4_t rows[kWaves][D / 16][64];
+    } tiles;
+    float factors[kWaves][16];
+};
+
+template <int D, Dtype DT, bool SPLIT, bool SHARING>
+__device__ __forceinline__ void attend_wide(const Kv8AttentionParams &p, WideLds<D, SPLIT> &memory) {
+    constexpr int kChunks = D / 64, kUnits = D / 16, kS = kSets<SPLIT>;
+    constexpr int kMyRows = SPLIT ? 8 : 16, kRows = kWaves * kMyRows;
+    constexpr int kKeyUnits = WideLds<D, SPLIT>::kKeyUnits, kHalves = WideLds<D, SPLIT>::kHalves;
+    constexpr int kMine = D / 64;  // a wave's 16s of dims
+    auto &lds = memory.tiles;
+    auto &factors = memory.factors;
 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -934,6 +963,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
     }
 }
 
+template <int D, Dtype DT, bool SPLIT, bool SHARING>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8AttentionParams p) {
+    __shared__ WideLds<D, SPLIT> lds;
+    attend_wide<D, DT, SPLIT, SHARING>(p, lds);
+}
+
+// Many rows of groups, few of each sequence's: both in one launch, so that the second
+// fills what the first leaves.  32 sequences (16 heads, 4 kv heads of 256, fp32) with up to 190
+// tokens of their own behind 8000 shared ones: 31 us, where two launches took 28 and 10.
+template <int D, Dtype DT, bool FEW_SPLIT, bool WIDE_SPLIT>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_both_kernel(Kv8AttentionParams p) {
+    __shared__ union {
+        FewLds<D, FEW_SPLIT> few;
+        WideLds<D, WIDE_SPLIT> wide;
+    } lds;
+    if (static_cast<int>(blockIdx.x) < p.sharing.groups * p.shared_row_tiles * p.cache.kv_heads * p.shared_splits)
+        attend_wide<D, DT, WIDE_SPLIT, true>(p, lds.wide);
+    else
+        attend_few<D, DT, FEW_SPLIT, true>(p, lds.few);
+}
+
 // The splits of one row and head, 64 dims a workgroup: four dims a lane, 16 or 32
 // splits side by side, so that up to 128 are on their way at once.
 template <int D, Dtype DT, int THREADS>
@@ -1011,10 +1061,12 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
 }
 
 // The same where a row's tokens are its group's, then its own: the partial results of
-// both.
+// both.  One wave does 64 dims where it can have a quarter of the partial results on their
+// way at once: four waves of fewer each fill the chip's places twice (32 sequences of 4 kv
+// heads, 33 partial results a row: 8.3 us against 10.0).
 template <int D, Dtype DT, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionParams p) {
-    constexpr int kLanes = 16, kGroups = THREADS / kLanes;
+    constexpr int kLanes = 16, kGroups = THREADS / kLanes, kEarly = THREADS == 64 ? 8 : 4;
     __shared__ float weight[2 * kKv8MaxSplits];
     __shared__ f32x4_t sums[kGroups][kLanes];
     const int seq = blockIdx.z, kvh = blockIdx.y / (D / 64), slice = blockIdx.y % (D / 64), row = blockIdx.x;
@@ -1039,7 +1091,15 @@ __global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionPa
         return i < own ? own_at + static_cast<int64_t>(i) * p.own_rows : group_at + static_cast<int64_t>(i - own) * p.shared_rows;
     };
 
+    // the first partial results of a group and the row's gates, before the weights are known
     const int lane = threadIdx.x & 63;
+    const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes, dim = 64 * slice + 4 * at;
+    const int head = kvh * p.group + row % p.group;
+    f32x4_t early[kEarly], gates = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+        early[k] = *reinterpret_cast<const f32x4_t *>(p.partial + partial_row(min(group + k * kGroups, all - 1)) * D + dim);
+    if (p.gate) gates = load_gate<DT>(p, tile.begin + row / p.group, head, dim);
     Base top = {kNone, 0.0f};
     Denominator total;
 #pragma unroll 1
@@ -1070,10 +1130,12 @@ __global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionPa
         }
     }
     lds_barrier();
-    const int group = threadIdx.x / kLanes, at = threadIdx.x % kLanes, dim = 64 * slice + 4 * at;
     f32x4_t y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+        if (group + k * kGroups < all) y += early[k] * weight[group + k * kGroups];
 #pragma unroll 4
-    for (int i = group; i < all; i += kGroups) y += *reinterpret_cast<const f32x4_t *>(p.partial + partial_row(i) * D + dim) * weight[i];
+    for (int i = group + kEarly * kGroups; i < all; i += kGroups) y += *reinterpret_cast<const f32x4_t *>(p.partial + partial_row(i) * D + dim) * weight[i];
     sums[group][at] = y;
     lds_barrier();
     if (threadIdx.x >= kLanes) return;
@@ -1081,8 +1143,7 @@ __global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionPa
 #pragma unroll 4
     for (int k = 1; k < used; ++k) y += sums[k][at];
     const Quotient quotient(top, total, kPScale);
-    const int head = kvh * p.group + row % p.group;
-    finish<DT>(p, quotient(y), quotient.some(), tile.begin + row / p.group, head, head * D + dim, dim);
+    finish<DT, true>(p, quotient(y), quotient.some(), tile.begin + row / p.group, head, head * D + dim, dim, &gates);
 }
 
 // `blocks` blocks from first_block on, of the groups' and the sequences' one after the other
@@ -1115,16 +1176,26 @@ hipError_t launch_shared_typed(Kv8AttentionParams p, const Kv8SharedPlan &cut, h
                 : rows == 16 ? launch_shared_rows<D, DT, 16>(p, first_block, blocks, stream)
                              : launch_shared_rows<D, DT, 64>(p, first_block, blocks, stream);
     };
+    const auto launch_both = [&](auto kernel) {
+        p.first_block = 0;
+        hipLaunchKernelGGL(kernel, dim3(of_groups + own), dim3(kWaves * 64), 0, stream, p);
+        return hipGetLastError();
+    };
     hipError_t e;
     if (plan.rows == shared.rows) {
         e = launch(plan.rows, 0, of_groups + own);
+    } else if (plan.rows <= 16 && shared.rows > 16) {
+        if constexpr (DT == Dtype::F32) e = launch_both(kv8_attention_both_kernel<D, DT, true, true>);
+        else if (plan.rows == 8) e = launch_both(kv8_attention_both_kernel<D, DT, true, false>);
+        else e = launch_both(kv8_attention_both_kernel<D, DT, false, false>);
     } else {
         e = launch(shared.rows, 0, of_groups);
         if (e == hipSuccess) e = launch(plan.rows, of_groups, own);
     }
     if (e != hipSuccess) return e;
     const dim3 rows(p.batch.max_rows * p.group, heads * (D / 64), p.batch.sequences);
-    hipLaunchKernelGGL((kv8_shared_join_kernel<D, DT, 256>), rows, dim3(256), 0, stream, p);
+    if (plan.splits + shared.splits <= 64) hipLaunchKernelGGL((kv8_shared_join_kernel<D, DT, 64>), rows, dim3(64), 0, stream, p);
+    else hipLaunchKernelGGL((kv8_shared_join_kernel<D, DT, 256>), rows, dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 

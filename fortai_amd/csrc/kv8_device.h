@@ -19,7 +19,10 @@ constexpr int kKv8MaxTokens = 1 << 30;  // the longest table: 2^24 pages of 64 t
 constexpr int kKv8PairsPerLaunch = 448;  // page pairs that fit a launch's arguments beside the rest
 
 constexpr int kKv8MaxSplits = 256;       // workgroups that may share a sequence's head
-constexpr int kKv8PartialRows = 16384;   // rows of partial results that a cache has room for
+constexpr int kKv8PartialRows = 16384;   // rows of partial results that a call may have
+constexpr int kKv8SharedRows = 32768;    // that one with shared tokens may have: what a cache has room for (with as
+                                         // many as the other, 160 rows over 24,000 tokens in two groups had 204
+                                         // workgroups, not 456, and took 61 us, not 41)
 
 
 struct Kv8View {
@@ -123,11 +126,11 @@ inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int gro
         return static_cast<int64_t>(who) * plan.row_tiles * kv_heads * plan.rows * plan.splits;
     };
     // the sequences' own tokens are few: what they leave of the workspace is the groups'
-    p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8PartialRows / 2);
+    p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8SharedRows / 4);
     const int64_t own = partial(p.own, sequences);
-    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, own < kKv8PartialRows ? kKv8PartialRows - own - 63 : 0);
+    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0);
     p.own_at = (partial(p.group, groups) + 63) / 64 * 64;
-    p.shares = max_shared >= 64 && p.own_at + own <= kKv8PartialRows;
+    p.shares = max_shared >= 64 && p.own_at + own <= kKv8SharedRows;
     return p;
 }
 

@@ -55,8 +55,8 @@ struct Kv8AttentionParams {
     int group = 0;            // query heads of a kv head
     float scale_log2 = 0.0f;  // softmax scale * log2(e) / 127
     bool vec = false;         // q, gate and out allow four-element accesses
-    float *partial = nullptr;        // [kKv8PartialRows][head]
-    f32x4_t *partial_ml = nullptr;   // [kKv8PartialRows]
+    float *partial = nullptr;        // [kKv8SharedRows][head]
+    f32x4_t *partial_ml = nullptr;   // [kKv8SharedRows]
     int splits = 0, row_tiles = 0;  // set by the launcher; of a call that shares, for each sequence's own tokens
     int shared_splits = 0, shared_row_tiles = 0, shared_rows = 0, own_rows = 0, own_at = 0, first_block = 0;
 };

@@ -161,7 +161,7 @@ const char *check(int groups, int most, int rows, int sequences, int shared, con
 void plan(int fp32, int head, int sequences, int groups, int kv, int64_t rows, int64_t group_rows, int64_t own, int64_t shared, int64_t *out) {
     const Kv8SharedPlan p = kv8_shared_plan(fp32 != 0, head, sequences, groups, kv, rows, group_rows, own, shared);
     const int64_t all[] = {p.shares, p.own_at, p.own.rows, p.own.row_tiles, p.own.splits, p.group.rows, p.group.row_tiles, p.group.splits,
-        kKv8PartialRows, kKv8MaxSplits};
+        kKv8SharedRows, kKv8MaxSplits};
     for (int i = 0; i < 10; ++i) out[i] = all[i]; }
 }''')
     lib.check.restype = C.c_char_p
