@@ -53,28 +53,35 @@ __device__ __forceinline__ float gdn_sigmoid(float x) { return 1.0f / (1.0f + ex
 
 // The inputs of a channel that a slot keeps, written by one thread: behind a sequence
 // of rows that wait, the taps - 1 inputs before them and theirs; otherwise the last
-// taps - 1.  In place, in ascending order, four at a time: what is read lies at or behind
+// taps - 1.  In place, in ascending order, four or eight at a time: what is read lies at or behind
 // what is written.
-template <typename E>
-__device__ __forceinline__ void gdn_keep_inputs(const GdnRowsParams &p, const GdnSequence &s, bool waits, int channel) {
+template <typename E, int AT_ONCE>
+__device__ __forceinline__ void gdn_keep_some(const GdnRowsParams &p, const GdnSequence &s, float *window, const E *x, int from, int kept) {
     const int channels = p.cache.channels(), before = p.cache.taps - 1;
-    float *window = p.cache.inputs + static_cast<int64_t>(s.slot) * (before + p.cache.pending) * channels + channel;
-    const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
-    const int from = waits ? 0 : s.count, kept = before + (waits ? s.count : 0);
 #pragma unroll 1
-    for (int j = 0; j < kept; j += 4) {
-        float v[4];
+    for (int j = 0; j < kept; j += AT_ONCE) {
+        float v[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < AT_ONCE; ++k) {
             const int at = from + min(j + k, kept - 1);
             v[k] = 0.0f;
             if (at >= before) v[k] = static_cast<float>(x[static_cast<int64_t>(at - before) * p.qkv_row]);
             else if (!s.begins) v[k] = window[static_cast<int64_t>(s.stands + at) * channels];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < AT_ONCE; ++k)
             if (j + k < kept) window[static_cast<int64_t>(j + k) * channels] = v[k];
     }
+}
+
+template <typename E>
+__device__ __forceinline__ void gdn_keep_inputs(const GdnRowsParams &p, const GdnSequence &s, bool waits, int channel) {
+    const int before = p.cache.taps - 1;
+    float *window = p.cache.inputs + static_cast<int64_t>(s.slot) * (before + p.cache.pending) * p.cache.channels() + channel;
+    const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
+    const int from = waits ? 0 : s.count, kept = before + (waits ? s.count : 0);
+    if (kept <= 4) gdn_keep_some<E, 4>(p, s, window, x, from, kept);
+    else gdn_keep_some<E, 8>(p, s, window, x, from, kept);
 }
 
 }  // namespace fortai_hip

@@ -15,7 +15,10 @@
 // columns of every 32: the products with k and q are sums over a lane's columns and three
 // exchanges between neighbours, and nothing of S goes through LDS.  The convolution of
 // the head's q and k, 2 head channels, is done by every workgroup of the head again
-// instead of a launch of its own.
+// instead of a launch of its own.  What bounds it in fact is the chain of dependent loads (row starts, slot,
+// count, pending rows) in front of the arithmetic: all loads of a stage are asked for before the first
+// is waited for.  Eight sequences of one row, 16 heads of 128: 8.7 us for 17 MB; of up to five rows and five
+// pending ones, 32 heads, bf16: 16.6 us for 34 MB (21 where rows were loaded one by one).
 //
 // Who may overwrite what others read: the inputs and keys of a key head are read by all
 // its workgroups.  Each counts itself in once its reads are done, and the last one
@@ -27,11 +30,13 @@ namespace fortai_hip {
 
 namespace {
 
-template <Dtype DT, int D, int ROWS>
+// TAPS: 4 or, 0, as many as the cache says.
+template <Dtype DT, int D, int ROWS, int TAPS>
 __global__ __launch_bounds__(ROWS * 8) void gdn_few_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
     constexpr int kThreads = ROWS * 8, kWaves = kThreads / 64, kFours = D / 32, kBlocks = D / ROWS;
     constexpr int kChannels = 2 * D + ROWS, kTurns = (kChannels + kThreads - 1) / kThreads;
+    constexpr int kAtOnce = 4;  // a thread's rows of a channel on their way at once
     __shared__ __align__(16) float qs[kGdnFewRows][D], ks[kGdnFewRows][D], log_k[kGdnMaxPending][D];
     __shared__ float vs[kGdnFewRows][ROWS], log_d[kGdnMaxPending][ROWS], os[kGdnFewRows][ROWS], ds[kGdnFewRows][ROWS];
     __shared__ float rates[kGdnFewRows], decays[kGdnFewRows], log_a[kGdnMaxPending];
@@ -44,7 +49,32 @@ __global__ __launch_bounds__(ROWS * 8) void gdn_few_kernel(const GdnRowsParams p
     const int group = c.value_heads / c.key_heads, kh = h / group, channels = c.channels(), before = c.taps - 1;
     const bool waits = r <= c.pending;
 
-    // this thread's row of S
+    // Everything is asked for before anything is waited for: the rows' inputs and weights of this workgroup's
+    // channels, a thread's row of S, then what needs the number of pending rows that stand.
+    const auto channel_of = [&](int at) {
+        return at < D ? kh * D + at : at < 2 * D ? (c.key_heads + kh) * D + at - D : (2 * c.key_heads + h) * D + r0 + at - 2 * D;
+    };
+    constexpr int kTaps = TAPS > 0 ? TAPS : kGdnMaxTaps;
+    const int first = TAPS > 0 ? 0 : kGdnMaxTaps - c.taps;  // aligned to the newest: seen[kTaps - 1] is the row's own
+    const E *x[kTurns];
+    float seen[kTurns][kTaps], w[kTurns][kTaps], next[kTurns][kAtOnce];
+    const auto load_rows = [&](int row) {
+#pragma unroll
+        for (int turn = 0; turn < kTurns; ++turn)
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) next[turn][k] = static_cast<float>(x[turn][min(row + k, r - 1) * p.qkv_row]);
+    };
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+        const int channel = channel_of(min(turn * kThreads + tid, kChannels - 1));
+        x[turn] = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
+#pragma unroll
+        for (int j = 0; j < kTaps; ++j) w[turn][j] = p.conv[static_cast<int64_t>(channel) * c.taps + max(j - first, 0)];
+    }
+    load_rows(0);
+    const int gate_row = s.begin + min(tid, r - 1);
+    const E alpha = static_cast<const E *>(p.alpha)[static_cast<int64_t>(gate_row) * p.alpha_row + h];
+    const E beta = static_cast<const E *>(p.beta)[static_cast<int64_t>(gate_row) * p.beta_row + h];
     const int local = tid >> 3, l = tid & 7;
     f32x4_t S[kFours];
     float *state = c.states + ((static_cast<int64_t>(s.slot) * c.value_heads + h) * D + r0 + local) * D + 4 * l;
@@ -52,56 +82,76 @@ __global__ __launch_bounds__(ROWS * 8) void gdn_few_kernel(const GdnRowsParams p
     for (int f = 0; f < kFours; ++f) S[f] = *reinterpret_cast<const f32x4_t *>(state + 32 * f);
     s.stands = gdn_stands(p, s);
     const int stands = s.begins ? 0 : s.stands;
-
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+        const int channel = channel_of(min(turn * kThreads + tid, kChannels - 1));
+        const float *window = c.inputs + static_cast<int64_t>(s.slot) * (before + c.pending) * channels + channel;
+#pragma unroll
+        for (int j = 0; j + 1 < kTaps; ++j) seen[turn][j] = window[static_cast<int64_t>(stands + max(j - first, 0)) * channels];
+    }
     // the pending rows that stand
-    for (int i = 0; i < stands; ++i) {
-        const int64_t row = static_cast<int64_t>(s.slot) * c.pending + i;
-        for (int at = tid; at < D; at += kThreads) log_k[i][at] = c.keys[(row * c.key_heads + kh) * D + at];
-        if (tid < ROWS) log_d[i][tid] = c.updates[(row * c.value_heads + h) * D + r0 + tid];
-        if (tid == 0) log_a[i] = c.decays[row * c.value_heads + h];
+    if (stands > 0) {
+        const int64_t row0 = static_cast<int64_t>(s.slot) * c.pending;
+        const float *keys = c.keys + (row0 * c.key_heads + kh) * D, *updates = c.updates + (row0 * c.value_heads + h) * D + r0;
+        const int64_t key_row = static_cast<int64_t>(c.key_heads) * D, update_row = static_cast<int64_t>(c.value_heads) * D;
+        const int all = stands * D, few = stands * ROWS;
+        const int at_d = min(tid, few - 1);
+        const float d = updates[at_d / ROWS * update_row + at_d % ROWS];
+        const float a = c.decays[(row0 + min(tid, stands - 1)) * c.value_heads + h];
+#pragma unroll 1
+        for (int base = tid; base < all; base += 4 * kThreads) {
+            float k[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = min(base + i * kThreads, all - 1);
+                k[i] = keys[at / D * key_row + at % D];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (base + i * kThreads < all) log_k[0][base + i * kThreads] = k[i];
+        }
+        if (tid < few) log_d[0][tid] = d;
+        for (int at = tid + kThreads; at < few; at += kThreads) log_d[0][at] = updates[at / ROWS * update_row + at % ROWS];
+        if (tid < stands) log_a[tid] = a;
     }
     // the rows' gates
     if (tid < r) {
-        const int64_t row = s.begin + tid;
-        const float alpha = static_cast<float>(static_cast<const E *>(p.alpha)[row * p.alpha_row + h]);
-        const float beta = static_cast<float>(static_cast<const E *>(p.beta)[row * p.beta_row + h]);
-        rates[tid] = gdn_sigmoid(beta);
-        decays[tid] = expf(gdn_log_decay(p.ssm_a[h], alpha, p.ssm_dt[h]));
+        rates[tid] = gdn_sigmoid(static_cast<float>(beta));
+        decays[tid] = expf(gdn_log_decay(p.ssm_a[h], static_cast<float>(alpha), p.ssm_dt[h]));
     }
-    // the convolution of this workgroup's channels
-    const auto channel_of = [&](int at) {
-        return at < D ? kh * D + at : at < 2 * D ? (c.key_heads + kh) * D + at - D : (2 * c.key_heads + h) * D + r0 + at - 2 * D;
-    };
+    // the convolution
 #pragma unroll
-    for (int turn = 0; turn < kTurns; ++turn) {
-        const int at = turn * kThreads + tid;
-        if (at >= kChannels) break;
-        const int channel = channel_of(at);
-        const float *window = c.inputs + static_cast<int64_t>(s.slot) * (before + c.pending) * channels + channel;
-        const E *x = static_cast<const E *>(p.qkv) + static_cast<int64_t>(s.begin) * p.qkv_row + channel;
-        // aligned to the newest: seen[kGdnMaxTaps - 1] is the row's own
-        float seen[kGdnMaxTaps], w[kGdnMaxTaps];
-        const int first = kGdnMaxTaps - c.taps;
+    for (int turn = 0; turn < kTurns; ++turn)
 #pragma unroll
-        for (int j = 0; j < kGdnMaxTaps; ++j) {
-            seen[j] = w[j] = 0.0f;
-            if (j >= first) {
-                w[j] = p.conv[static_cast<int64_t>(channel) * c.taps + j - first];
-                if (j < kGdnMaxTaps - 1 && !s.begins) seen[j] = window[static_cast<int64_t>(stands + j - first) * channels];
-            }
+        for (int j = 0; j + 1 < kTaps; ++j) {
+            if (s.begins || j < first) seen[turn][j] = 0.0f;
+            if (j < first) w[turn][j] = 0.0f;
         }
-        float *to = at < D ? &qs[0][at] : at < 2 * D ? &ks[0][at - D] : &vs[0][at - 2 * D];
-        const int pitch = at < 2 * D ? D : ROWS;
 #pragma unroll 1
-        for (int i = 0; i < r; ++i) {
-            seen[kGdnMaxTaps - 1] = static_cast<float>(x[i * p.qkv_row]);
-            float u = 0.0f;
+    for (int i = 0; i < r; i += kAtOnce) {
+        float now[kTurns][kAtOnce];
 #pragma unroll
-            for (int j = 0; j < kGdnMaxTaps; ++j)
-                if (j >= first) u = __builtin_fmaf(w[j], seen[j], u);
-            to[i * pitch] = gdn_silu(u);
+        for (int turn = 0; turn < kTurns; ++turn)
 #pragma unroll
-            for (int j = 0; j + 1 < kGdnMaxTaps; ++j) seen[j] = seen[j + 1];
+            for (int k = 0; k < kAtOnce; ++k) now[turn][k] = next[turn][k];
+        if (i + kAtOnce < r) load_rows(i + kAtOnce);
+#pragma unroll
+        for (int turn = 0; turn < kTurns; ++turn) {
+            const int at = turn * kThreads + tid;
+            if (at >= kChannels) break;
+            float *to = at < D ? &qs[0][at] : at < 2 * D ? &ks[0][at - D] : &vs[0][at - 2 * D];
+            const int pitch = at < 2 * D ? D : ROWS;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (i + k >= r) break;
+                seen[turn][kTaps - 1] = now[turn][k];
+                float u = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kTaps; ++j) u = __builtin_fmaf(w[turn][j], seen[turn][j], u);
+                to[(i + k) * pitch] = gdn_silu(u);
+#pragma unroll
+                for (int j = 0; j + 1 < kTaps; ++j) seen[turn][j] = seen[turn][j + 1];
+            }
         }
     }
     __syncthreads();
@@ -225,21 +275,22 @@ __global__ __launch_bounds__(256) void gdn_copy_slots_kernel(float *plane, int64
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) to[i] = from[i];
 }
 
-template <Dtype DT, int D>
+template <Dtype DT, int D, int TAPS>
 hipError_t few_typed(const GdnRowsParams &p, hipStream_t stream) {
     const GdnView &c = p.cache;
     // 32 rows of S a workgroup where that leaves two workgroups a CU: fewer of them do
     // the same convolution
     if (static_cast<int64_t>(p.batch.sequences) * c.value_heads * (D / 32) >= 512)
-        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 32>), dim3(c.value_heads * (D / 32), p.batch.sequences), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 32, TAPS>), dim3(c.value_heads * (D / 32), p.batch.sequences), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 16>), dim3(c.value_heads * (D / 16), p.batch.sequences), dim3(128), 0, stream, p);
+        hipLaunchKernelGGL((gdn_few_kernel<DT, D, 16, TAPS>), dim3(c.value_heads * (D / 16), p.batch.sequences), dim3(128), 0, stream, p);
     return hipGetLastError();
 }
 
 template <Dtype DT>
 hipError_t few_head(const GdnRowsParams &p, hipStream_t stream) {
-    return p.cache.head == 64 ? few_typed<DT, 64>(p, stream) : few_typed<DT, 128>(p, stream);
+    if (p.cache.taps == 4) return p.cache.head == 64 ? few_typed<DT, 64, 4>(p, stream) : few_typed<DT, 128, 4>(p, stream);
+    return p.cache.head == 64 ? few_typed<DT, 64, 0>(p, stream) : few_typed<DT, 128, 0>(p, stream);
 }
 
 }  // namespace
