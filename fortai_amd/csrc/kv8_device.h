@@ -21,8 +21,8 @@ constexpr int kKv8PairsPerLaunch = 448;  // page pairs that fit a launch's argum
 constexpr int kKv8MaxSplits = 256;       // workgroups that may share a sequence's head
 constexpr int kKv8PartialRows = 16384;   // rows of partial results that a call may have
 constexpr int kKv8SharedRows = 32768;    // that one with shared tokens may have: what a cache has room for (with as
-                                         // many as the other, 160 rows over 24,000 tokens in two groups had 204
-                                         // workgroups, not 456, and took 61 us, not 41)
+                                         // many as the other, two groups of 132 rows over up to 24,000 tokens had
+                                         // 204 workgroups, not 456, and took 61 us, not 41)
 
 
 struct Kv8View {

@@ -23,7 +23,7 @@ constexpr int kRuleThreads = 256;
 template <Dtype DT, bool VEC, int CHUNK>
 __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p) {
     typedef typename Element<DT>::type E;
-    constexpr int kFours = CHUNK / (4 * kRuleThreads), kAtOnce = 8;
+    constexpr int kFours = CHUNK / (4 * kRuleThreads), kAtOnce = 16;
     __shared__ __align__(16) int counts[CHUNK];
     // the tokens that come and go with a row, from row0 + 1 on, as places in the chunk (-1: elsewhere)
     __shared__ int comes[kRuleThreads], goes[kRuleThreads];
@@ -57,6 +57,14 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
     int64_t length = 0;  // of the history
     const int64_t *history = nullptr;
     const auto token_at = [&](int64_t place) { return place < length ? history[place] : p.tokens[begin + (place - length)]; };
+    // x / repetition where x is positive, by the reciprocal and what is left of x then: the quotient to its last place
+    // without a division each (divisions took 2 us of 27)
+    float inverse = 1.0f;
+    const auto repeated = [&](float x) {
+        const float q = x * (x > 0.0f ? inverse : repetition), left = __builtin_fmaf(-q, repetition, x);
+        const float quotient = __builtin_fmaf(left, inverse, q);
+        return x > 0.0f && fabsf(quotient) < __builtin_inff() ? quotient : q;
+    };
     const auto place_of = [&](int64_t token) {
         const int64_t at = token - first;
         return at >= 0 && at < CHUNK && token < p.vocab ? static_cast<int>(at) : -1;
@@ -73,6 +81,7 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
     };
     if (counting) {
         repetition = p.penalties[3 * seq];
+        inverse = 1.0f / repetition;
         frequency = p.penalties[3 * seq + 1];
         presence = p.penalties[3 * seq + 2];
         if (p.history) {
@@ -119,7 +128,7 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int n = counts[i + k];
-                    const float seen = (y[f][k] > 0.0f ? y[f][k] / repetition : y[f][k] * repetition) - static_cast<float>(n) * frequency - presence;
+                    const float seen = repeated(y[f][k]) - static_cast<float>(n) * frequency - presence;
                     y[f][k] = n > 0 ? seen : y[f][k];
                 }
             }
