@@ -93,14 +93,14 @@ struct Kv8Plan {
 // costs 30.5 us where two cost 25.9 (eight sequences of up to 8190 tokens); one tile a
 // wave costs 13.2 us where three cost 17.0 (600 tokens).
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length,
-    int64_t partial_rows = kKv8PartialRows) {
+    int64_t partial_rows = kKv8PartialRows, int workgroups = 512) {
     Kv8Plan p;
     const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
     const int few = fp32 || rows <= 8 ? 8 : 16;
     const bool much = rows > 2 * few && (rows + few - 1) / few * heads >= 4096 / ((max_length + 63) / 64 + 1);
     p.rows = much ? 4 * few : few;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
-    const int64_t base = p.row_tiles * heads, fill = 512 * (256 / head), least = much ? 128 : 256;
+    const int64_t base = p.row_tiles * heads, fill = workgroups * (256 / head), least = much ? 128 : 256;
     const int64_t wanted = (fill + base - 1) / base, useful = (max_length + least - 1) / least;
     const int64_t room = partial_rows / (base * p.rows);
     int64_t s = wanted < useful ? wanted : useful;
@@ -112,7 +112,11 @@ inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_
 
 // How a call is cut whose sequences share tokens: the groups' tokens and the sequences'
 // own, which have their partial results behind the groups' from row own_at on.  shares
-// is false where these do not fit.
+// is false where these do not fit.  The groups' tokens are split for one workgroup a CU
+// (half as many partial results to write and join) unless that leaves one more than 12 tiles: 4 kv
+// heads of 256 behind 8000 tokens, eight sequences' rows in fp32 17.9 us against 23.4 for
+// two a CU, 32 sequences' 33.6 against 37.5; 5 rows of 4 in bf16 behind 24,000 (11.7 tiles) 44.0 against
+// 43.6, two groups of 8 (18 tiles) 61 against 41.
 struct Kv8SharedPlan {
     Kv8Plan own, group;
     int64_t own_at = 0;
@@ -128,7 +132,9 @@ inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int gro
     // the sequences' own tokens are few: what they leave of the workspace is the groups'
     p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8SharedRows / 4);
     const int64_t own = partial(p.own, sequences);
-    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0);
+    const int64_t room = own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0;
+    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room, 256);
+    if (max_shared / 64 > 12 * p.group.splits) p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room);
     p.own_at = (partial(p.group, groups) + 63) / 64 * 64;
     p.shares = max_shared >= 64 && p.own_at + own <= kKv8SharedRows;
     return p;

@@ -10,6 +10,11 @@
 // hashing, and integer sums, whose order does not matter), and from row to row adds
 // the one token that comes and takes away the one that leaves the window, while the
 // next row's logits are on their way.
+//
+// Bound by the bytes of the rows, by the first count of a long text (every chunk's workgroup
+// reads it again, from L2) and, for one row, by a launch's latency.  33 rows of 248,320 of
+// eight sequences in fp32 (67 MB) behind texts of up to 8000 tokens, with biases and masks:
+// 25 us; one row of 16,384 4.2 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "step_kernels.h"
