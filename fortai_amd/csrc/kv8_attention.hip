@@ -971,7 +971,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_wide_kernel(Kv8A
 
 // Many rows of groups, few of each sequence's: both in one launch, so that the second
 // fills what the first leaves.  32 sequences (16 heads, 4 kv heads of 256, fp32) with up to 190
-// tokens of their own behind 8000 shared ones: 31 us, where two launches took 28 and 10.
+// tokens of their own behind 8000 shared ones: 29 us, where two launches took 28 and 10.
 template <int D, Dtype DT, bool FEW_SPLIT, bool WIDE_SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attention_both_kernel(Kv8AttentionParams p) {
     __shared__ union {
@@ -1063,7 +1063,7 @@ __global__ __launch_bounds__(THREADS) void kv8_attention_join_kernel(Kv8Attentio
 // The same where a row's tokens are its group's, then its own: the partial results of
 // both.  One wave does 64 dims where it can have a quarter of the partial results on their
 // way at once: four waves of fewer each fill the chip's places twice (32 sequences of 4 kv
-// heads, 33 partial results a row: 8.3 us against 10.0).
+// heads, 33 partial results a row: 8.3 us against 10.0; 17 of them 6.5).
 template <int D, Dtype DT, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_shared_join_kernel(Kv8AttentionParams p) {
     constexpr int kLanes = 16, kGroups = THREADS / kLanes, kEarly = THREADS == 64 ? 8 : 4;
