@@ -24,7 +24,7 @@ struct fortai_hip_gdn_cache {
     int *arrivals = nullptr, *stands = nullptr;
     _Float16 *asks = nullptr, *keys_by_dim = nullptr, *through = nullptr, *inner = nullptr;
     float *values = nullptr, *chunk_gates = nullptr, *tops = nullptr, *decay = nullptr, *rate = nullptr;
-    std::mutex launches;  // a call's launches follow each other on the stream
+    std::mutex launches;  // a call's launches follow each other on the stream, without another's between them
 
     GdnView layer(int index) const {
         GdnView v;
@@ -301,6 +301,7 @@ int fortai_hip_gdn_copy_slots(fortai_hip_gdn_cache *h, const int32_t *from, cons
         return fail(c, FORTAI_HIP_RUNTIME_ERROR, "gdn copy: out of host memory");
     }
     const DeviceScope scope(c->device);
+    const std::lock_guard<std::mutex> lock(h->launches);
     return done(c, launch_gdn_copy_slots(h->layer(0), h->shape.layers, from, to, count, c->stream), "gdn copy slots");
 }
 

@@ -139,6 +139,18 @@ def test_codes_of_gated_rows_alone(ctx, rows, width, group, dtype):
     check(run(ctx, x, None, w, group, z, dtype, want_sum=False, want_output=False), want, dtype, False, False)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,width,group", [(6, 1056, 32), (1025, 2560, 128), (3, 5120, 256), (1030, 4096, 4096), (1026, 1792, 1792), (5, 4160, None)])
+def test_sums_of_rows_with_any_norm(ctx, rows, width, group, dtype):
+    g = torch.Generator().manual_seed(rows + width)
+    x, r, z = (torch.randn(rows, width, generator=g).to(TYPES[dtype]).cuda() for _ in range(3))
+    w = None if group is None else (1.0 + 0.2 * torch.randn(group, generator=g)).cuda()
+    for gate in (None, z):
+        want = definition(x, r, w, group or width, gate, dtype)
+        check(run(ctx, x, r, w, group or width, gate, dtype), want, dtype)
+        check(run(ctx, x, r.clone(), w, group or width, gate, dtype, want_output=False, in_place=True), want, dtype, True, False)
+
+
 def test_gated_rows_near_the_ends_of_their_type(ctx):
     """Large and small gates, weights and rows, one in each block or all of one: the codes are still the nearest."""
     g = torch.Generator().manual_seed(3)
