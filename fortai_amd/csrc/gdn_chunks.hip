@@ -41,6 +41,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kRun = kGdnRun;       // rows that a wave of the first launch takes
 constexpr float kOne = 1024.0f;     // 2^10
+constexpr int kLoadsMayCross = 0x2 | 0x4 | 0x10;  // for sched_barrier: vector, scalar and memory, not matrix and LDS instructions
 constexpr float kProduct = 1.0f / (kOne * kOne);
 
 template <typename V>
@@ -526,6 +527,9 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
     typedef typename Runs<D>::Ask Ask;
     constexpr int kSlices = D / (16 * NT), kTiles = D / 64, kPitch = D + 8, kPitchD = kGdnChunk + 8, kAsk = Runs<D>::kAsk;
     constexpr int kHead = Runs<D>::kHead;
+    // two workgroups a CU: loads stand between the products and the arithmetic, not among the products, where a CU
+    // takes 64 bytes a cycle (eight prompts in all 151 -> 149 us; one workgroup by itself would lose 2 of a document's 62)
+    constexpr bool kSpread = NT == 2;
     __shared__ __align__(16) _Float16 sh[2][16 * NT * kPitch], dh[2][16 * NT * kPitchD], rh[2][16 * NT * kPitchD];
     __shared__ float tops[4][16 * NT];
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
@@ -549,15 +553,27 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
             if (stands >= 0) S[u][t] = *reinterpret_cast<const f32x4_t *>(state + 16 * u * D + 16 * t);
         }
 #pragma unroll 1
-    for (int i = 0; i < stands; ++i) {  // the pending rows that stand
-        const int64_t row = static_cast<int64_t>(s.slot) * c.pending + i;
-        const float a = c.decays[row * c.value_heads + h];
-        const float *d = c.updates + (row * c.value_heads + h) * D + r0 + m;
-        const float *k = c.keys + (row * c.key_heads + kh) * D + 16 * kTiles * wave + 4 * g;
+    for (int i = 0; i < stands; i += 2) {  // the pending rows that stand, two on their way at once
+        float a[2], d[2][NT];
+        f32x4_t k[2][kTiles];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int j = 0; j < 2; ++j) {
+            const int64_t row = static_cast<int64_t>(s.slot) * c.pending + min(i + j, stands - 1);
+            a[j] = c.decays[row * c.value_heads + h];
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) S[u][t] = S[u][t] * a + d[16 * u] * *reinterpret_cast<const f32x4_t *>(k + 16 * t);
+            for (int t = 0; t < NT; ++t) d[j][t] = c.updates[(row * c.value_heads + h) * D + r0 + m + 16 * t];
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                k[j][t] = *reinterpret_cast<const f32x4_t *>(c.keys + (row * c.key_heads + kh) * D + 16 * kTiles * wave + 4 * g + 16 * t);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (i + j >= stands) break;
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) S[u][t] = S[u][t] * a[j] + d[j][u] * k[j][t];
+        }
     }
     if (h == 0 && r0 == 0 && tid == 0) c.counts[s.slot] = 0;
 
@@ -656,16 +672,30 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
         f32x4_t asked[NT], o[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) asked[t] = o[t] = zero;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        // a step's numbers of S are read from LDS while the step before multiplies
+        Pair<Ask> of_s[2][NT];
+        const auto read_s = [&](int k) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
-                const Pair<Ask> b = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
-                asked[t] = product(w[k], b, asked[t]);
-                o[t] = product(q[k], b, o[t]);
+                of_s[k & 1][t] = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
             }
-            load_ask(next, k);
+        };
+        read_s(0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k < 3) read_s(k + 1);
+            __builtin_amdgcn_sched_barrier(kLoadsMayCross);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                asked[t] = product(w[k], of_s[k & 1][t], asked[t]);
+                o[t] = product(q[k], of_s[k & 1][t], o[t]);
+            }
+            if (!kSpread) load_ask(next, k);
+        }
+        if (kSpread) {
+            load_ask(next, 0);
+            load_ask(next, 1);
         }
         float d_from[NT];
 #pragma unroll
@@ -698,20 +728,32 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
 #pragma unroll
             for (int k = 0; k < kTiles; ++k) added[t][k] = zero;
         }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        Pair4 of_r[2][NT], of_d[2][NT];
+        const auto read_d = [&](int b) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
-                const Pair4 r = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
-#pragma unroll
-                for (int k = 0; k < kTiles; ++k) added[t][k] = product(keys[k][b], r, added[t][k]);
-                if (b <= wave) {
-                    const Pair4 d = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
-                    among[t] = product(inner[b], d, among[t]);
-                }
+                of_r[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
+                of_d[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
             }
-            load_run(next, b);
+        };
+        read_d(0);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (b < 3) read_d(b + 1);
+            __builtin_amdgcn_sched_barrier(kLoadsMayCross);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int k = 0; k < kTiles; ++k) added[t][k] = product(keys[k][b], of_r[b & 1][t], added[t][k]);
+                if (b <= wave) among[t] = product(inner[b], of_d[b & 1][t], among[t]);
+            }
+            if (!kSpread) load_run(next, b);
+            else if (b >= 2) load_ask(next, b);
+        }
+        if (kSpread) {
+            load_run(next, 0);
+            load_run(next, 1);
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -722,6 +764,10 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
                 o[t][e] = __builtin_fmaf(among[t][e], d_from[t], o[t][e]);
             }
         load_whole(next);
+        if (kSpread) {
+            load_run(next, 2);
+            load_run(next, 3);
+        }
         E *to = out + static_cast<int64_t>(chunk) * kGdnChunk * p.out_row;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
