@@ -56,6 +56,38 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
         }
     };
     load_row(row0);
+    // the chunk's biases, the same for every row, and the next row's mask, whose number is known a row before
+    const bool biased = p.bias != nullptr;
+    f32x4_t biases[kFours];
+    if (biased) {
+        const float *at = p.bias + seq * p.bias_pitch + first;
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const int i = 4 * (f * kRuleThreads + thread);
+            biases[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (VEC) {
+                if (first + i < p.vocab) biases[f] = *reinterpret_cast<const f32x4_t *>(at + i);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (first + i + k < p.vocab) biases[f][k] = at[i + k];
+            }
+        }
+    }
+    uint32_t words[kFours];
+    const auto mask_number = [&](int row) { return p.masks ? read_only(p.mask_of + min(row, row1 - 1)) : -1; };
+    const auto load_words = [&](int number) {
+        const bool held = number >= 0 && number < p.mask_count;
+        const uint32_t *allowed = p.masks + (held ? number * p.mask_pitch : 0);
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) {
+            const int i = first + 4 * (f * kRuleThreads + thread);
+            words[f] = ~0u;
+            if (held && i < p.vocab) words[f] = allowed[i >> 5] >> (i & 31);
+        }
+    };
+    load_words(mask_number(row0));
+    int next_number = mask_number(row0 + 1);
 
     const bool counting = p.penalties != nullptr;
     float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
@@ -120,10 +152,14 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
         f32x4_t y[kFours];
 #pragma unroll
         for (int f = 0; f < kFours; ++f) y[f] = x[f];
-        if (row + 1 < row1) load_row(row + 1);
-        const int mask = p.masks ? p.mask_of[row] : -1;
-        const uint32_t *allowed = mask >= 0 && mask < p.mask_count ? p.masks + mask * p.mask_pitch : nullptr;
-        const float *bias = p.bias ? p.bias + seq * p.bias_pitch + first : nullptr;
+        uint32_t bits[kFours];
+#pragma unroll
+        for (int f = 0; f < kFours; ++f) bits[f] = words[f];
+        if (row + 1 < row1) {
+            load_row(row + 1);
+            load_words(next_number);
+            next_number = mask_number(row + 2);
+        }
         E *to = static_cast<E *>(p.out) + static_cast<int64_t>(row) * p.out_row + first;
 #pragma unroll
         for (int f = 0; f < kFours; ++f) {
@@ -138,21 +174,10 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
                 }
             }
             const bool four = VEC || first + i + 3 < p.vocab;
-            if (bias) {
-                if (VEC) {
-                    y[f] += *reinterpret_cast<const f32x4_t *>(bias + i);
-                } else {
+            if (biased) y[f] += biases[f];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (first + i + k < p.vocab) y[f][k] += bias[i + k];
-                }
-            }
-            if (allowed) {
-                const uint32_t bits = allowed[(first + i) >> 5] >> ((first + i) & 31);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (!(bits >> k & 1u)) y[f][k] = -__builtin_inff();
-            }
+            for (int k = 0; k < 4; ++k)
+                if (!(bits[f] >> k & 1u)) y[f][k] = -__builtin_inff();
             if (four) {
                 store4<DT, VEC>(to + i, y[f]);
             } else {
