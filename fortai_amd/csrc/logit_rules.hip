@@ -14,7 +14,7 @@
 // Bound by the bytes of the rows, by the first count of a long text (every chunk's workgroup
 // reads it again, from L2) and, for one row, by a launch's latency.  33 rows of 248,320 of
 // eight sequences in fp32 (67 MB) behind texts of up to 8000 tokens, with biases and masks:
-// 25 us; one row of 16,384 4.2 us.
+// 22 us; one row of 16,384 4.2 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "step_kernels.h"
@@ -204,8 +204,10 @@ __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesPar
 
 template <Dtype DT, bool VEC>
 hipError_t rules_typed(const LogitRulesParams &p, hipStream_t stream) {
-    // rows of a sequence stay together up to eight: the text is counted once for them
-    const int average = (p.rows + p.sequences - 1) / p.sequences, parts = (average + 7) / 8;
+    // three rows of a sequence stay together, for which the text is counted once and whose rows follow each other:
+    // eight sequences of up to five behind 8000 tokens (16) 21.6 us (18.2), five together 22.6 (21.7), two 23.5 (19.9), one
+    // 26.0 (20.8)
+    const int average = (p.rows + p.sequences - 1) / p.sequences, parts = (average + 2) / 3;
     const int64_t groups = static_cast<int64_t>(p.sequences) * parts;
     if (groups * ((p.vocab + 4095) / 4096) >= 256)
         hipLaunchKernelGGL((logit_rules_kernel<DT, VEC, 4096>), dim3((p.vocab + 4095) / 4096, p.sequences, parts), dim3(kRuleThreads), 0, stream, p);
