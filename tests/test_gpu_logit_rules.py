@@ -108,6 +108,13 @@ def test_many_rows_of_a_sequence(ctx):
         case.check(case.run(ctx))
 
 
+@pytest.mark.parametrize("window", [0, 5, 400])
+def test_all_rows_in_one_of_many_sequences(ctx, window):
+    """One workgroup then has them all, and looks up their tokens in several turns."""
+    case = Case(4, [0] * 120 + [600] + [0] * 179, 300, [0] * 120 + [30] + [2] * 179, window, "f32")
+    case.check(case.run(ctx))
+
+
 def test_in_place_and_large(ctx):
     case = Case(4, [5] * 8, 70000, [500] * 8, 0, "f32")
     case.check(case.run(ctx, in_place=True))
