@@ -13,7 +13,7 @@
 // arithmetic.  That hides behind the memory but for the gate's exponential, which took 46 us
 // of 64 bits for 2000 rows of 4096 in bf16: gated values are computed in 32 bits first, and
 // again in 64 where a quotient of the wave's 256 may lie on either side of a half for all
-// that 32 bits say, or a scale on either side of a border of fp16 (one wave in eight): 27 us.
+// that 32 bits say, or a scale on either side of a border of fp16 (one wave in eight): 22 us.
 //
 // Bound by memory: rows of up to 4096 stay in registers from the sum to the codes (4096 rows
 // of 2560 in fp32 with a sum, 138 MB: 31 us, 4.4 TB/s; read twice 39 us; a wave a row, which
@@ -55,8 +55,7 @@ struct Codes {
 // pieces that a wave has at most, which then stay in registers; 0: any.  Where the norm is
 // of parts of a row or there is none, blockIdx.y has the row's next HELD pieces.
 // With a gate the loop over pieces is not unrolled, the held ones move down instead: a row
-// of 4096 by one wave in 16 copies of that code (64 KB) took 37 us where quarters of four
-// rows a workgroup and one copy take 27.
+// of 4096 by one wave in 16 copies of that code (64 KB) took 37 us.
 template <Dtype DT, bool VEC, int ROW_WAVES, int HELD, bool GATE>
 __global__ __launch_bounds__(kNormThreads) void norm_tokens_kernel(NormTokensParams p) {
     typedef typename Element<DT>::type E;
@@ -258,11 +257,12 @@ void norm_rows(const NormTokensParams &p, int columns, hipStream_t stream) {
 
 template <Dtype DT>
 hipError_t norm_typed(const NormTokensParams &p, bool vec, hipStream_t stream) {
-    // parts of rows are nobody else's: a wave has up to 1024 values of a row; a whole row's norm takes
+    // parts of rows are nobody else's: a wave has 256 values of a row (2000 rows of 4096, gated: 22 us, with 512 25,
+    // with 1024 27: the fewer registers, the more waves a SIMD has to choose from); a whole row's norm takes
     // a workgroup, which reads rows again that are longer than it holds, or not aligned
     const int padded = p.codes ? p.blocks_pad * 32 : p.width;
     if (!vec) norm_rows<DT, false, 4, 0>(p, 1, stream);
-    else if (!p.norm || p.group < p.width) norm_rows<DT, true, 1, 4>(p, (padded + 1023) / 1024, stream);
+    else if (!p.norm || p.group < p.width) norm_rows<DT, true, 1, 1>(p, (padded + 255) / 256, stream);
     else if (p.width <= 4096) norm_rows<DT, true, 4, 4>(p, 1, stream);
     else norm_rows<DT, true, 4, 0>(p, 1, stream);
     return hipGetLastError();
