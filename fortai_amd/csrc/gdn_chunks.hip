@@ -141,6 +141,7 @@ __device__ __forceinline__ void store_four_step(_Float16 *tile, int lane, const 
 
 // Convolution, norms and gates: a wave has 128 channels (two a lane) of a run, or every
 // gate.  TAPS: of the convolution, 0: as many as there are.  PAIRS: two elements at once.
+// Bound by memory: 2456 rows of 8192 channels in fp32, 180 MB in and out, 43 us.
 template <Dtype DT, int D, int TAPS, bool PAIRS>
 __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
@@ -287,7 +288,9 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
 // W, U and the weights of one chunk and value head.
 // Three workgroups a CU: each goes through a chain of small steps with barriers between
 // them, and waits most of the time.  Everything that comes from memory is asked for before
-// the first of them, without conditions, so that no wait is for more than it needs.
+// the first of them, without conditions, so that no wait is for more than it needs.  43
+// chunks of 32 heads: 48 us, which is 4.2 TB/s of operands read and written; 32 chunks of 16
+// heads 22 us, two chains one after the other.
 template <int D>
 __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p) {
     typedef typename Runs<D>::Ask Ask;
@@ -520,7 +523,10 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
 
 // The state of 16 NT value dims of a head through a sequence's chunks.  In the matrix
 // instructions' results a lane has value dim m and four key dims (of S) or rows (of D and
-// O).  A wave has 16 rows of the chunk and a quarter of the key dims.
+// O).  A wave has 16 rows of the chunk and a quarter of the key dims.  A chunk is a chain of
+// two products with a barrier before each: 4300 cycles for one workgroup a CU (62 us for 32
+// chunks), of which its 112 KB through the L1 are 1900; 71 us for eight sequences of up to
+// 8 chunks and 32 heads, two workgroups a CU.
 template <Dtype DT, int D, int NT>
 __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams p) {
     typedef typename Element<DT>::type E;
