@@ -209,6 +209,8 @@ hipError_t rules_typed(const LogitRulesParams &p, hipStream_t stream) {
     // 26.0 (20.8)
     const int average = (p.rows + p.sequences - 1) / p.sequences, parts = (average + 2) / 3;
     const int64_t groups = static_cast<int64_t>(p.sequences) * parts;
+    // chunks of 4096 where they fill the chip (33 rows of 248,320 21.5 us, of 1024 30.7), otherwise of 1024 (one row 7.3 us
+    // against 9.1, four sequences' 9.2 against 9.6)
     if (groups * ((p.vocab + 4095) / 4096) >= 256)
         hipLaunchKernelGGL((logit_rules_kernel<DT, VEC, 4096>), dim3((p.vocab + 4095) / 4096, p.sequences, parts), dim3(kRuleThreads), 0, stream, p);
     else
