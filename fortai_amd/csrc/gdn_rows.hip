@@ -17,8 +17,8 @@
 // the head's q and k, 2 head channels, is done by every workgroup of the head again
 // instead of a launch of its own.  What bounds it in fact is the chain of dependent loads (row starts, slot,
 // count, pending rows) in front of the arithmetic: all loads of a stage are asked for before the first
-// is waited for.  Eight sequences of one row, 16 heads of 128: 8.7 us for 17 MB; of up to five rows and five
-// pending ones, 32 heads, bf16: 16.6 us for 34 MB (21 where rows were loaded one by one).
+// is waited for.  Eight sequences of one row, 16 heads of 128: 8.3 us for 17 MB; of up to five rows and five
+// pending ones, 32 heads, bf16: 14.9 us for 34 MB; 64 of one row, 32 heads, 50 us for 268 MB.
 //
 // Who may overwrite what others read: the inputs and keys of a key head are read by all
 // its workgroups.  Each counts itself in once its reads are done, and the last one
@@ -278,8 +278,10 @@ __global__ __launch_bounds__(256) void gdn_copy_slots_kernel(float *plane, int64
 template <Dtype DT, int D, int TAPS>
 hipError_t few_typed(const GdnRowsParams &p, hipStream_t stream) {
     const GdnView &c = p.cache;
-    // 16 rows of S a workgroup do the convolution twice as often, and take longer for one sequence too (8.4 us against 7.9)
-    constexpr int kRows = 32;
+    // Fewer rows of S a workgroup do the convolution more often, and win nothing where there are few workgroups: one
+    // sequence of 16 heads 8.4 us with 16 rows, 7.5 with 32, 7.6 with 64, 7.3 with 128; eight of up to five rows and 32
+    // heads 28, 17.0, 14.9 and 14.7; 64 of one row and 32 heads with 32 rows 56, 50 and 52.
+    constexpr int kRows = 64;
     hipLaunchKernelGGL((gdn_few_kernel<DT, D, kRows, TAPS>), dim3(c.value_heads * (D / kRows), p.batch.sequences), dim3(kRows * 8), 0, stream, p);
     return hipGetLastError();
 }
