@@ -26,7 +26,8 @@
 // updates and all sums are fp32.
 //
 // The sums c are taken in 64 bits: far into a decay they are large, and their differences
-// are not.
+// are not.  A row's logarithm is -256 at least (gdn_log_decay), so that 64 of them stay below
+// 2^15 and keep 2^-38 of what lies between any two rows.
 #include "gdn_device.h"
 
 #include <type_traits>

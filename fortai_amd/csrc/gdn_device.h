@@ -43,10 +43,13 @@ __device__ __forceinline__ float gdn_silu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
 
-// ssm_a softplus(alpha + ssm_dt): the logarithm of a row's decay
+// ssm_a softplus(alpha + ssm_dt): the logarithm of a row's decay.  Below -256 the decay is nothing (fp32's last number
+// is e^-103), and so it is at -256: sums over a chunk's rows keep every row's own decay behind one that forgets
+// everything.  Sum and product are taken in 64 bits, where they stay finite (of numbers that are), and a NaN stays one.
 __device__ __forceinline__ float gdn_log_decay(float a, float alpha, float dt) {
-    const float x = alpha + dt;
-    return a * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+    const double x = static_cast<double>(alpha) + static_cast<double>(dt);
+    const double log = a * (fmax(x, 0.0) + static_cast<double>(log1pf(expf(-fabsf(static_cast<float>(x))))));
+    return log < -256.0 ? -256.0f : static_cast<float>(log);
 }
 
 __device__ __forceinline__ float gdn_sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
