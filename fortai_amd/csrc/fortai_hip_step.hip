@@ -23,7 +23,9 @@ struct fortai_hip_gdn_cache {
     // made with the cache and never again, so that a captured call keeps their addresses
     int *arrivals = nullptr, *stands = nullptr;
     _Float16 *asks = nullptr, *keys_by_dim = nullptr, *through = nullptr, *inner = nullptr;
-    float *values = nullptr, *chunk_gates = nullptr, *tops = nullptr, *decay = nullptr, *rate = nullptr;
+    float *values = nullptr, *chunk_gates = nullptr, *decay = nullptr, *rate = nullptr;
+    uint32_t *columns = nullptr;
+    int *faint = nullptr;
     std::mutex launches;  // a call's launches follow each other on the stream, without another's between them
 
     GdnView layer(int index) const {
@@ -58,7 +60,8 @@ struct fortai_hip_gdn_cache {
         release(inner);
         release(values);
         release(chunk_gates);
-        release(tops);
+        release(columns);
+        release(faint);
         release(decay);
         release(rate);
     }
@@ -212,7 +215,8 @@ int fortai_hip_gdn_create(fortai_hip_q8_context *c, int layers, int slots, int k
         if (e == hipSuccess) e = alloc(&h->inner, runs * value_heads * 2 * kGdnChunk);
         if (e == hipSuccess) e = alloc(&h->values, runs * value_heads * head_size);
         if (e == hipSuccess) e = alloc(&h->chunk_gates, runs * value_heads * 2);
-        if (e == hipSuccess) e = alloc(&h->tops, gdn_runs(rows) * value_heads * head_size);
+        if (e == hipSuccess) e = alloc(&h->columns, gdn_runs(rows) * value_heads * head_size);
+        if (e == hipSuccess) e = alloc(&h->faint, gdn_runs(rows) * value_heads * head_size);
         if (e == hipSuccess) e = alloc(&h->decay, rows * value_heads);
         if (e == hipSuccess) e = alloc(&h->rate, rows * value_heads);
     }
@@ -274,7 +278,8 @@ int fortai_hip_gdn_run_device(fortai_hip_gdn_cache *h, int layer, const fortai_h
     p.inner = h->inner;
     p.values = h->values;
     p.chunk_gates = h->chunk_gates;
-    p.tops = h->tops;
+    p.columns = h->columns;
+    p.faint = h->faint;
     p.decay = h->decay;
     p.rate = h->rate;
     p.stands = h->stands;

@@ -14,16 +14,25 @@
 //
 // Products run in fp16 matrix instructions with fp32 sums: an operand is two numbers,
 // x scale = h + l, and h h + h l + l h keeps 22 bits of either (three instructions of a
-// sixteenth of the fp32 one's time each).  That is as exact as the sums' own fp32
-// rounding, if x is not far below the largest of its kind.  q, k, W, T and the weights are
+// sixteenth of the fp32 one's time each), down to l's smallest step.  q, k, W, T and the weights are
 // at most 1 (decays are at most 1, and a row's update answers any value at most its own
-// size: the rule is a contraction) and scaled by 2^10.  V, S and D have any size: a column (one value
-// dim) is scaled by a power of two, V by its largest in the chunk, S and D by bounds: with
+// size: the rule is a contraction) and scaled by 2^15, weights by 2^18 (a query's length is at most an eighth).
+// Values (times b), S and D have any size: a column (one value
+// dim) is scaled by a power of two, b V by its largest in the chunk, S and D by bounds: with
 // s the largest of S before the chunk and u that of U,
-//   |D| <= u + sqrt(head) s,  |S after it| <= exp(c_n) s + 64 max |D|,
-// which no wave has to wait for another's numbers for.  They exceed the largest by 2^10 or
-// so; halves that are scaled to 2^15 lose bits below 2^-3, 2^-18 of the bound.  S itself, the
+//   |D| <= u + sqrt(head) s,  |S after it| <= exp(c_n) s + sum_j exp(c_n - c_j) max |D|,
+// which no wave has to wait for another's numbers for.  S itself, the
 // updates and all sums are fp32.
+//
+// So a chunk's numbers are off by 2^-38 or so of R, the largest of s and |b v| in their column (64 errors of 2^-39
+// of it that all point one way: 2^-31).  That is rounding for a row in whose text something of R's size is left: it has
+// at least 2^-20 R among b v and s up to it, with the decays since.  Where a row has less (tokens before a far louder
+// one, or behind one that is forgotten), it and the chunk's rows before it go one by one, in fp32, as few rows do, for
+// the 16 or 32 columns of a workgroup at once.  The chunk kernel looks for such rows, since it has the values, makes
+// their U in fp32 products, and says in a word a column which s is enough for them; the kernel that has s compares.
+// (Where, of ordinary values, one first row in 10^5 is that small: 4 us.)  2000 rows of 16 heads 113 us, of which
+// this is 3; with every row one by one, 0.75 us each, 1.6 ms.  Outputs of the 56 rows before one that is 1 to 2^30 times
+// as loud are off by 2^-22 of their size throughout.
 //
 // The sums c are taken in 64 bits: far into a decay they are large, and their differences
 // are not.  A row's logarithm is -256 at least (gdn_log_decay), so that 64 of them stay below
@@ -41,7 +50,9 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kRun = kGdnRun;       // rows that a wave of the first launch takes
-constexpr float kOne = 1024.0f;     // 2^10
+constexpr float kOne = 32768.0f;    // 2^15
+constexpr float kWeight = 262144.0f;  // 2^18
+constexpr float kWithin = 0x1p-20f, kWithinLog = -20.0f;  // what a row has of its column's largest, or it goes by itself
 constexpr int kLoadsMayCross = 0x2 | 0x4 | 0x10;  // for sched_barrier: vector, scalar and memory, not matrix and LDS instructions
 constexpr float kProduct = 1.0f / (kOne * kOne);
 
@@ -52,7 +63,7 @@ struct Pair {
 typedef Pair<f16x4_t> Pair4;
 typedef Pair<f16x8_t> Pair8;
 
-// scaled: x times what brings it to 2^10 at most.  It is rounded to fp32 before anything is
+// scaled: x times what brings it to 2^15 at most.  It is rounded to fp32 before anything is
 // done with it: the compiler folds a multiplication into a conversion to fp16 (one
 // rounding), but not into every use of it, and a lower half that is left over from
 // another upper half is off by a whole step.
@@ -93,13 +104,14 @@ __device__ __forceinline__ f32x4_t product32(f32x4_t a, f32x4_t b, f32x4_t c) {
 }
 
 // The power of two that brings numbers up to `top` below 2^15, and back from a product with
-// a number times 2^10 (1 for nothing).
+// a number times 2^15 (1 for nothing).
 struct Scale {
-    float to, from;
+    float to, from, least;  // least: what keeps 22 bits (2^-3, scaled), unless it is near the end of fp32
     __device__ __forceinline__ explicit Scale(float top) {
         const int e = top > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(top), -100), 128) : 0;
         to = __builtin_ldexpf(32768.0f, -e);
         from = __builtin_ldexpf(1.0f / (32768.0f * kOne), e);
+        least = __builtin_ldexpf(e > -100 ? 0x1p-18f : 0.0f, e);
     }
 };
 
@@ -213,7 +225,7 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     const int head = channel / D, dim = channel % D;
     const bool is_value = head >= 2 * c.key_heads, is_key = !is_value && head >= c.key_heads;
     const int64_t run = run_place(s, s.begin + i0);
-    // 2^10 over the length, but no more than over epsilon; queries also over sqrt(head)
+    // 2^15 over the length, but no more than over epsilon; queries also over sqrt(head)
     const float one = is_key ? kOne : kOne / sqrtf(static_cast<float>(D)), most = fminf(one / p.eps, 3e38f);
     // the head's part of the image, D * 4 units (heads of 64: two heads a wave, half its lanes each)
     constexpr int kAsk = Runs<D>::kAsk, kUnits = D * 4, kHeadLanes = D / 2;
@@ -286,12 +298,115 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
     if (channel == 0 && lane == 0) p.stands[seq] = s.begins ? -1 : s.stands;
 }
 
+// What a column's numbers ask of the state before them.  A row is faint if it has less than kWithin of the column's
+// largest number, most, in its text (b v so far, with the decays since).  A lane has rows 16 b + 4 g + e.  In binary
+// logarithms: the largest of log |v_j| - c_j up to row i, and c_i.
+struct Faint {
+    int last;     // faint row, -1: none
+    float least;  // in the text of rows at which the state is gone
+};
+
+__device__ __forceinline__ Faint faint_rows(const f32x4_t (&v)[4], float most, const float *logs, int n, int lane) {
+    Faint f = {-1, __builtin_inff()};
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        f32x4_t x = v[b];
+        if (n < kGdnChunk) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (16 * b + 4 * (lane >> 4) + e >= n) x[e] = f.least;
+        }
+        f.least = fminf(f.least, fminf(fminf(fabsf(x[0]), fabsf(x[1])), fminf(fabsf(x[2]), fabsf(x[3]))));
+    }
+    // whatever the decays, and with room for states of up to four times the largest (of ordinary values one tile in 50
+    // does not get by)
+    if (__all(f.least >= most * (8.0f * kWithin))) {
+        f.least = fminf(f.least, xor_lane<16>(f.least));
+        f.least = fminf(f.least, xor_lane<32>(f.least));
+        return f;
+    }
+    const int g = lane >> 4;
+    const float none = -__builtin_inff(), low = __builtin_amdgcn_logf(most * kWithin);
+    float before = none, least = __builtin_inff();  // before: the largest of the runs before
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const f32x4_t c = *reinterpret_cast<const f32x4_t *>(logs + 16 * b + 4 * g);
+        float up_to[4], x = none;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) up_to[e] = x = fmaxf(x, __builtin_amdgcn_logf(fabsf(v[b][e])) - c[e]);
+        // of the lanes of the rows before these, and of all of the run
+        const float one = __shfl(x, lane - 16), two = __shfl(x, lane - 32), three = __shfl(x, lane - 48);
+        float earlier = before;
+        if (g > 0) earlier = fmaxf(earlier, one);
+        if (g > 1) earlier = fmaxf(earlier, two);
+        if (g > 2) earlier = fmaxf(earlier, three);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * b + 4 * g + e;
+            const float text = fmaxf(up_to[e], earlier) + c[e];
+            if (row < n && text < low) f.last = row;
+            if (row < n && c[e] < kWithinLog) least = fminf(least, text);
+        }
+        before = fmaxf(before, largest_of_column(x));
+    }
+    f.last = max(f.last, xor_lane<16>(f.last));
+    f.last = max(f.last, xor_lane<32>(f.last));
+    least = fminf(least, xor_lane<16>(least));
+    f.least = __builtin_amdgcn_exp2f(fminf(least, xor_lane<32>(least)));
+    return f;
+}
+
+// A column of U and what its rows ask of the largest of S in it, s, as the exponents of four powers of two in a word, the
+// first in the lowest bits: need is enough of s for the faint rows (they have kWithin of the chunk's largest from it); limit
+// leaves the rows at which S is gone kWithin of it in their text, and bounds within fp32; top and left are no less than
+// the largest of U and the sum of the decays to the chunk's end.  The others' bits stand behind an exponent and
+// make its number up to twice as large (need has none).
+struct Column {
+    float need, limit, top, left;
+    __device__ __forceinline__ explicit Column(uint32_t word)
+        : need(fabsf(__builtin_bit_cast(float, word << 23))), limit(fabsf(__builtin_bit_cast(float, word << 15))),
+          top(fabsf(__builtin_bit_cast(float, word << 7))), left(__builtin_bit_cast(float, word >> 1)) {}
+    __device__ __forceinline__ bool exceeded(float s) const { return !(s <= limit); }
+    __device__ __forceinline__ bool wanting(float s) const { return s < need; }
+    static __device__ __forceinline__ uint32_t word(float top, float left, const Faint &f, float most, const float *logs) {
+        const float gone = f.last >= 0 ? logs[f.last] : 0.0f, infinite = __builtin_inff();
+        float need = f.last < 0 ? 0.0f : gone < kWithinLog ? infinite : most * kWithin * __builtin_amdgcn_exp2f(-gone);
+        float limit = fminf(logs[kGdnChunk - 1] < kWithinLog ? f.least * (0.5f / kWithin) : infinite, 0x1p100f);
+        if (!(top < 0x1p100f)) {  // no s will do
+            need = infinite;
+            limit = 0.0f;
+        }
+        const auto up = [](float x) { return (__builtin_bit_cast(uint32_t, x) + 0x7fffffu) >> 23; };
+        return up(left) << 24 | up(top) << 16 | __builtin_bit_cast(uint32_t, limit) >> 23 << 8 | up(need);
+    }
+};
+
+// One tile of U = T b V, over V, in fp32 products; its largest number.
+template <typename Rows>
+__device__ __forceinline__ float exact_updates(float *values, int64_t run_values, int last_run, const float *rates, int g, const Rows &rows_of_t) {
+    f32x4_t v[4];
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+        v[b] = *reinterpret_cast<const f32x4_t *>(values + min(b, last_run) * run_values) * *reinterpret_cast<const f32x4_t *>(rates + 16 * b + 4 * g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i > last_run) break;
+        f32x4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b <= i; ++b) u = product32(rows_of_t(i, b), v[b], u);
+        top = fmaxf(top, largest(u));
+        *reinterpret_cast<f32x4_t *>(values + i * run_values) = u;
+    }
+    return top;
+}
+
 // W, U and the weights of one chunk and value head.
 // Three workgroups a CU: each goes through a chain of small steps with barriers between
 // them, and waits most of the time.  Everything that comes from memory is asked for before
 // the first of them, without conditions, so that no wait is for more than it needs.  43
-// chunks of 32 heads: 48 us, which is 4.2 TB/s of operands read and written; 32 chunks of 16
-// heads 22 us, two chains one after the other.
+// chunks of 32 heads: 49 us, which is 4.1 TB/s of operands read and written; 32 chunks of 16
+// heads 23.7 us, two chains one after the other.  Of these the search for faint rows takes 3 and 1.9 us.
 template <int D>
 __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p) {
     typedef typename Runs<D>::Ask Ask;
@@ -301,7 +416,8 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
     static_assert(sizeof(as) >= 4 * kHead * sizeof(_Float16), "the keys of four runs");
     _Float16(*halves)[2][kGdnChunk * kPitchT] = reinterpret_cast<_Float16(*)[2][kGdnChunk * kPitchT]>(as);
     __shared__ double sums[kGdnChunk];  // binary logarithms
-    __shared__ __align__(16) float rates[kGdnChunk], asked_rates[kGdnChunk];  // b, and with exp(c)
+    __shared__ __align__(16) float rates[kGdnChunk], asked_rates[kGdnChunk], logs[kGdnChunk];  // b, with exp(c); c, in 32 bits
+    __shared__ float left_sum;  // of the decays to the chunk's end
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
@@ -337,15 +453,18 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
         }
         const double all = __shfl(sum, 63);
         if (wave == 0) {
-            const float decay = __builtin_amdgcn_exp2f(static_cast<float>(sum));
+            const float decay = __builtin_amdgcn_exp2f(static_cast<float>(sum)), left = __builtin_amdgcn_exp2f(static_cast<float>(all - sum));
             sums[lane] = sum;
+            logs[lane] = static_cast<float>(sum);
             rates[lane] = rate;
             asked_rates[lane] = rate * decay;
             if (lane / kRun <= last_run) {  // for the launch that follows
                 float *to = p.chunk_gates + ((run0 + lane / kRun) * c.value_heads + h) * (2 * kRun) + lane % kRun;
                 to[0] = decay;
-                to[kRun] = __builtin_amdgcn_exp2f(static_cast<float>(all - sum));
+                to[kRun] = left;
             }
+            const float lefts = wave_sum(lane < n ? left : 0.0f);
+            if (lane == 0) left_sum = lefts;
         }
     }
     _Float16 *keys = reinterpret_cast<_Float16 *>(as);
@@ -380,7 +499,7 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
     for (int k = 0; k < 5; ++k) {
         const int i = 16 * row_run[k] + m, j0 = 16 * key_run[k] + 4 * g;
         const double at_i = sums[i];
-        const float factor = of_queries ? kProduct * kOne : rates[i] * kProduct;
+        const float factor = of_queries ? kProduct * kWeight : rates[i] * kProduct;
         const int past = of_queries ? i : i - 1;  // the last j that counts
         f32x4_t x;
 #pragma unroll
@@ -460,22 +579,27 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
         const int i = at / kGdnChunk, j = at % kGdnChunk;
         if (j / 16 > i / 16) continue;
         const f32x4_t t = *reinterpret_cast<const f32x4_t *>(ts + i * kPitch + j) * kOne;
-        const f32x4_t of_w = t * *reinterpret_cast<const f32x4_t *>(asked_rates + j), of_u = t * *reinterpret_cast<const f32x4_t *>(rates + j);
-        const Pair4 w = split4(of_w), u = split4(of_u);
+        const Pair4 w = split4(t * *reinterpret_cast<const f32x4_t *>(asked_rates + j)), u = split4(t);
         *reinterpret_cast<f16x4_t *>(&halves[0][0][i * kPitchT + j]) = w.h;
         *reinterpret_cast<f16x4_t *>(&halves[0][1][i * kPitchT + j]) = w.l;
         *reinterpret_cast<f16x4_t *>(&halves[1][0][i * kPitchT + j]) = u.h;
         *reinterpret_cast<f16x4_t *>(&halves[1][1][i * kPitchT + j]) = u.l;
     }
-    // this wave's columns of V as operands
-    float from[kTiles];
+    // this wave's columns of b V as operands (b is 0 behind the last row)
+    float from[kTiles], largest_v[kTiles];
+    Faint faint[kTiles];
     Pair4 vs[kTiles][4];
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-        const Scale scale(largest_of_column(fmaxf(fmaxf(largest(v[t][0]), largest(v[t][1])), fmaxf(largest(v[t][2]), largest(v[t][3])))));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[t][b] *= *reinterpret_cast<const f32x4_t *>(rates + 16 * b + 4 * g);
+        const float most = largest_of_column(fmaxf(fmaxf(largest(v[t][0]), largest(v[t][1])), fmaxf(largest(v[t][2]), largest(v[t][3]))));
+        const Scale scale(most);
         from[t] = scale.from;
 #pragma unroll
         for (int b = 0; b < 4; ++b) vs[t][b] = split4(v[t][b] * scale.to);
+        largest_v[t] = most;
+        faint[t] = faint_rows(v[t], most, logs, n, lane);
     }
     lds_barrier();
     const auto half_at = [&](int which, int i, int b) {
@@ -485,8 +609,14 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
     // of W a lane has four key dims of row m, of U four rows of value dim m
     const int lane_dim = 16 * kTiles * wave + 4 * g;
     float top[kTiles];  // of U's columns
+    // where rows are faint U is made of fp32 products, which keep every row's bits
+    bool exact[kTiles];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) top[t] = 0.0f;
+    for (int t = 0; t < kTiles; ++t) {
+        top[t] = 0.0f;
+        exact[t] = __any(faint[t].last >= 0);
+        if (exact[t]) top[t] = exact_updates(values + t * 256, run_values, last_run, rates, g, [&](int i, int b) { return row_of(ts, i, b); });
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (i > last_run) break;
@@ -505,9 +635,11 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
         _Float16 *through = p.through + ((run0 + i) * c.value_heads + h) * kHead;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-            u[t] *= from[t];
-            top[t] = fmaxf(top[t], largest(u[t]));
-            *reinterpret_cast<f32x4_t *>(values + i * run_values + t * 256) = u[t];
+            if (!exact[t]) {
+                u[t] *= from[t];
+                top[t] = fmaxf(top[t], largest(u[t]));
+                *reinterpret_cast<f32x4_t *>(values + i * run_values + t * 256) = u[t];
+            }
             const Pair4 x = split4(w[t] * (kProduct * kOne));
             const int dim = lane_dim + 16 * t;
             _Float16 *to = through + (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16 + m) * kAsk + dim % kAsk;
@@ -518,15 +650,19 @@ __global__ __launch_bounds__(256, 3) void gdn_chunk_kernel(const GdnRowsParams p
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
         top[t] = largest_of_column(top[t]);
-        if (g == 0) p.tops[(run0 * c.value_heads + h) * D + 16 * (kTiles * wave + t) + m] = top[t];
+        if (g == 0) {
+            const int64_t at = (run0 * c.value_heads + h) * D + 16 * (kTiles * wave + t) + m;
+            p.columns[at] = Column::word(top[t], left_sum, faint[t], largest_v[t], logs);
+            p.faint[at] = faint[t].last;
+        }
     }
 }
 
 // The state of 16 NT value dims of a head through a sequence's chunks.  In the matrix
 // instructions' results a lane has value dim m and four key dims (of S) or rows (of D and
 // O).  A wave has 16 rows of the chunk and a quarter of the key dims.  A chunk is a chain of
-// two products with a barrier before each: 4300 cycles for one workgroup a CU (62 us for 32
-// chunks), of which its 112 KB through the L1 are 1900; 71 us for eight sequences of up to
+// two products with a barrier before each: 4400 cycles for one workgroup a CU (64 us for 32
+// chunks), of which its 112 KB through the L1 are 1900; 68 us for eight sequences of up to
 // 8 chunks and 32 heads, two workgroups a CU.
 template <Dtype DT, int D, int NT>
 __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams p) {
@@ -538,7 +674,7 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
     // takes 64 bytes a cycle (eight prompts in all 151 -> 149 us; one workgroup by itself would lose 2 of a document's 62)
     constexpr bool kSpread = NT == 2;
     __shared__ __align__(16) _Float16 sh[2][16 * NT * kPitch], dh[2][16 * NT * kPitchD], rh[2][16 * NT * kPitchD];
-    __shared__ float tops[4][16 * NT];
+    __shared__ float tops[4][16 * NT], outputs[kGdnChunk][16 * NT];  // outputs: of rows that go by themselves
     const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const GdnView &c = p.cache;
@@ -594,16 +730,18 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
     const _Float16 *inner_at = p.inner + ((run_first + wave) * c.value_heads + h) * (4 * kRun * 32);
     const float *u_at = p.values + ((run_first + wave) * c.value_heads + h) * (kRun * D) + (r0 / 16 * 64 + lane) * 4;
     const float *gates_at = p.chunk_gates + ((run_first + wave) * c.value_heads + h) * (2 * kRun) + 4 * g;
-    const float *tops_at = p.tops + (run_first * c.value_heads + h) * D + r0 + m;
+    const uint32_t *columns_at = p.columns + (run_first * c.value_heads + h) * D + r0 + m;
     const _Float16 *keys_at = p.keys_by_dim + (run_first * c.key_heads + kh) * kHead + kTiles * wave * (kRun * 32);
     const float *whole_at = p.chunk_gates + (run_first * c.value_heads + h) * (2 * kRun);
     const int64_t w_step = static_cast<int64_t>(4) * c.value_heads * kHead, q_step = static_cast<int64_t>(8) * c.key_heads * kHead;
     const int64_t inner_step = static_cast<int64_t>(4) * c.value_heads * (4 * kRun * 32), u_step = static_cast<int64_t>(4) * c.value_heads * (kRun * D);
-    const int64_t gates_step = static_cast<int64_t>(4) * c.value_heads * (2 * kRun), tops_step = static_cast<int64_t>(4) * c.value_heads * D;
+    const int64_t gates_step = static_cast<int64_t>(4) * c.value_heads * (2 * kRun), columns_step = static_cast<int64_t>(4) * c.value_heads * D;
     Pair<Ask> w[4], q[4];
     f32x4_t u[NT], through, left;
-    float u_top[NT], whole;
+    float whole;
+    uint32_t column[NT];
     Pair4 inner[4], keys[kTiles][4];
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const auto load_ask = [&](int chunk, int k) {
         w[k] = Runs<D>::row_step(w_at + chunk * w_step, k, lane);
         q[k] = Runs<D>::row_step(q_at + chunk * q_step, k, lane);
@@ -614,7 +752,7 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             u[t] = *reinterpret_cast<const f32x4_t *>(u_at + chunk * u_step + t * 256);
-            u_top[t] = tops_at[chunk * tops_step + 16 * t];
+            column[t] = columns_at[chunk * columns_step + 16 * t];
         }
     };
     const auto load_run = [&](int chunk, int b) {
@@ -627,12 +765,6 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
         const int row = min(s.count - 1, chunk * kGdnChunk + kGdnChunk - 1);
         whole = whole_at[static_cast<int64_t>(row / kRun) * c.value_heads * (2 * kRun) + row % kRun];
     };
-#pragma unroll
-    for (int k = 0; k < 4; ++k) load_ask(0, k);
-    load_updates(0);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) load_run(0, b);
-    load_whole(0);
     E *out = static_cast<E *>(p.out) + (s.begin + static_cast<int64_t>(16 * wave + 4 * g)) * p.out_row + h * D + r0 + m;
     // a column's largest number of this wave's part of S
     const auto top_of = [&](int t) {
@@ -643,144 +775,311 @@ __global__ __launch_bounds__(256, NT) void gdn_states_kernel(const GdnRowsParams
     const auto column_top = [&](int t) {
         return fmaxf(fmaxf(tops[0][16 * t + m], tops[1][16 * t + m]), fmaxf(tops[2][16 * t + m], tops[3][16 * t + m]));
     };
-    float s_to[NT], s_from[NT];
+    float s_to[NT], s_from[NT], s_least[NT];  // s_least: below it halves at this scale are cut short
+    // the first `rows` rows of a chunk one by one, in fp32, as few rows go; the whole chunk's also leave S.  A row's asking
+    // and the row before's output are one exchange between the waves, in the updates' place.
+    const auto go_by_rows = [&](int chunk, int rows, bool all) {
+        // places are worked out here, and nothing of them is held through the chunks
+        int m = tid & 15, g = lane >> 4, h = block / kSlices, first = r0;
+        asm volatile("" : "+v"(m), "+v"(g), "+s"(h), "+s"(first));
+        const int kh = h / (c.value_heads / c.key_heads);
+        float(*parts)[4][2][16 * NT] = reinterpret_cast<float(*)[4][2][16 * NT]>(dh);
+        static_assert(sizeof(dh) >= 2 * sizeof(*parts), "two rows' exchanges");
+        // U holds what the rows change of a state of nothing: `before` is what the state before them has become
+        f32x4_t before[NT][kTiles], state[NT][kTiles], k[kTiles], q[kTiles], q_before[kTiles];
+        Pair4 next_k[kTiles], next_q[kTiles];  // a row ahead
+        float next_d[NT], next_log, next_rate;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float top = top_of(t);
-        if (g == 0) tops[wave][16 * t + m] = top;
-    }
-    lds_barrier();
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const Scale scale(column_top(t));
-        s_to[t] = scale.to;
-        s_from[t] = scale.from;
-    }
-    lds_barrier();
-    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < kTiles; ++u) before[t][u] = state[t][u] = S[t][u];
+        const int64_t row0 = s.begin + static_cast<int64_t>(chunk) * kGdnChunk;
+        const auto load_row = [&](int row) {
+            const int64_t run = run_first + 4 * static_cast<int64_t>(chunk) + row / kRun;
+            const int r = row % kRun;
+            next_log = p.decay[(row0 + row) * c.value_heads + h];
+            next_rate = p.rate[(row0 + row) * c.value_heads + h];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) next_d[t] = p.values[(run * c.value_heads + h) * (kRun * D) + ((first / 16 + t) * 64 + r / 4 * 16 + m) * 4 + r % 4];
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) {
+                const int dim = 16 * (kTiles * wave + u) + 4 * g;
+                const _Float16 *at = p.asks + (run * 2 * c.key_heads + kh) * kHead + (dim / (4 * kAsk) * 2 * 64 + dim / kAsk % 4 * 16 + r) * kAsk + dim % kAsk;
+                next_q[u] = {*reinterpret_cast<const f16x4_t *>(at), *reinterpret_cast<const f16x4_t *>(at + 64 * kAsk)};
+                at += c.key_heads * kHead;
+                next_k[u] = {*reinterpret_cast<const f16x4_t *>(at), *reinterpret_cast<const f16x4_t *>(at + 64 * kAsk)};
+            }
+        };
+        const auto joined = [](const Pair4 &x) {
+            f32x4_t y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (static_cast<float>(x.h[e]) + static_cast<float>(x.l[e])) * (1.0f / kOne);
+            return y;
+        };
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) q[u] = zero;
+        load_row(0);
 #pragma unroll 1
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        const int mine = s.count - chunk * kGdnChunk - 16 * wave - 4 * g;  // this lane's rows that are there
-        const int next = min(chunk + 1, chunks - 1);
+        for (int row = 0; row <= rows; ++row) {
+            const float a = expf(next_log), rate = next_rate;
+            float d[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) d[t] = next_d[t];
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) {
+                q_before[u] = q[u];
+                q[u] = joined(next_q[u]);
+                k[u] = joined(next_k[u]);
+            }
+            load_row(min(row + 1, rows - 1));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x = 0.0f, y = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x = __builtin_fmaf(before[t][u][e], k[u][e], x);
+                        y = __builtin_fmaf(state[t][u][e], q_before[u][e], y);
+                    }
+                x += xor_lane<16>(x);
+                y += xor_lane<16>(y);
+                x += xor_lane<32>(x);
+                y += xor_lane<32>(y);
+                if (g == 0) {
+                    parts[row & 1][wave][0][16 * t + m] = x;
+                    parts[row & 1][wave][1][16 * t + m] = y;
+                }
+            }
+            lds_barrier();
+            const auto sum = [&](int which, int t) {
+                const float(*part)[2][16 * NT] = parts[row & 1];
+                const int at = 16 * t + m;
+                return (part[0][which][at] + part[1][which][at]) + (part[2][which][at] + part[3][which][at]);
+            };
+            if (row > 0 && wave == 0 && g == 0) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) outputs[row - 1][16 * t + m] = sum(1, t);
+            }
+            if (row == rows) break;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float of_before = -rate * (a * sum(0, t)), both = d[t] + of_before;
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        before[t][u][e] = __builtin_fmaf(of_before, k[u][e], before[t][u][e] * a);
+                        state[t][u][e] = __builtin_fmaf(both, k[u][e], state[t][u][e] * a);
+                    }
+            }
+        }
+        lds_barrier();  // every wave has read the last sums
+        if (!all) return;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u) S[t][u] = state[t][u];
+    };
+    const auto store_outputs = [&](int chunk, int rows) {
+        __syncthreads();  // the waves' own outputs of these rows are stored
+        E *to = static_cast<E *>(p.out) + (s.begin + static_cast<int64_t>(chunk) * kGdnChunk) * p.out_row + h * D + r0;
+        for (int at = tid; at < rows * 16 * NT; at += 256) to[at / (16 * NT) * p.out_row + at % (16 * NT)] = static_cast<E>(outputs[at / (16 * NT)][at % (16 * NT)]);
+    };
+    int chunk = 0, alone = 0;  // alone: rows of this chunk that have gone by themselves
+    bool looked_at = false;    // this chunk's rows
+#pragma unroll 1
+    while (chunk < chunks) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load_ask(chunk, k);
+        load_updates(chunk);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) load_run(chunk, b);
+        load_whole(chunk);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const float top = top_of(t);
             if (g == 0) tops[wave][16 * t + m] = top;
-#pragma unroll
-            for (int k = 0; k < kTiles; ++k) {
-                const Pair4 x = split4(S[t][k] * s_to[t]);
-                const int at = (16 * t + m) * kPitch + 16 * (kTiles * wave + k) + 4 * g;
-                *reinterpret_cast<f16x4_t *>(&sh[0][at]) = x.h;
-                *reinterpret_cast<f16x4_t *>(&sh[1][at]) = x.l;
-            }
         }
-        lds_barrier();  // every wave's part of S is there
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const Scale scale(column_top(t));
+            s_to[t] = scale.to;
+            s_from[t] = scale.from;
+            s_least[t] = 0.0f;
+        }
+        lds_barrier();
+        bool stopped = false;
+        const int end = looked_at ? chunk + 1 : chunks;
+#pragma unroll 1
+        do {
+            int mine = s.count - chunk * kGdnChunk - 16 * wave - 4 * g;  // this lane's rows that are there
+            const int next = min(chunk + 1, chunks - 1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float top = top_of(t);
+                if (g == 0) tops[wave][16 * t + m] = top;
+#pragma unroll
+                for (int k = 0; k < kTiles; ++k) {
+                    const Pair4 x = split4(S[t][k] * s_to[t]);
+                    const int at = (16 * t + m) * kPitch + 16 * (kTiles * wave + k) + 4 * g;
+                    *reinterpret_cast<f16x4_t *>(&sh[0][at]) = x.h;
+                    *reinterpret_cast<f16x4_t *>(&sh[1][at]) = x.l;
+                }
+            }
+            lds_barrier();  // every wave's part of S is there
 
-        f32x4_t asked[NT], o[NT];
+            f32x4_t asked[NT], o[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) asked[t] = o[t] = zero;
-        // a step's numbers of S are read from LDS while the step before multiplies
-        Pair<Ask> of_s[2][NT];
-        const auto read_s = [&](int k) {
+            for (int t = 0; t < NT; ++t) asked[t] = o[t] = zero;
+            // a step's numbers of S are read from LDS while the step before multiplies
+            Pair<Ask> of_s[2][NT];
+            const auto read_s = [&](int k) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
+                    of_s[k & 1][t] = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
+                }
+            };
+            read_s(0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k < 3) read_s(k + 1);
+                __builtin_amdgcn_sched_barrier(kLoadsMayCross);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    asked[t] = product(w[k], of_s[k & 1][t], asked[t]);
+                    o[t] = product(q[k], of_s[k & 1][t], o[t]);
+                }
+                if (!kSpread) load_ask(next, k);
+            }
+            if (kSpread) {
+                load_ask(next, 0);
+                load_ask(next, 1);
+            }
+            // All waves see the same numbers here and go the same way.
+            bool rare = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int at = (16 * t + m) * kPitch + 4 * kAsk * k + kAsk * g;
-                of_s[k & 1][t] = {*reinterpret_cast<const Ask *>(&sh[0][at]), *reinterpret_cast<const Ask *>(&sh[1][at])};
+                const Column col(column[t]);
+                const float top = column_top(t);
+                rare |= col.exceeded(top) | col.wanting(top) | (top < s_least[t]);  // without branches
             }
-        };
-        read_s(0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k < 3) read_s(k + 1);
-            __builtin_amdgcn_sched_barrier(kLoadsMayCross);
+            // Such a chunk goes through to its end without rows and changes nothing: the only way out of the loop is at its
+            // end, so that no wait has to allow for another (a branch here took 7 us of 62 and 12 of 68).
+            stopped = !looked_at & (__any(rare) != 0);
+            mine = stopped ? 0 : mine;
+            whole = stopped ? 1.0f : whole;
+            float d_from[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                asked[t] = product(w[k], of_s[k & 1][t], asked[t]);
-                o[t] = product(q[k], of_s[k & 1][t], o[t]);
-            }
-            if (!kSpread) load_ask(next, k);
-        }
-        if (kSpread) {
-            load_ask(next, 0);
-            load_ask(next, 1);
-        }
-        float d_from[NT];
+                const Column col(column[t]);
+                const float top = column_top(t), most = __builtin_fmaf(top, D == 128 ? 11.32f : 8.01f, col.top) * 1.001f;
+                const Scale scale(most), after(__builtin_fmaf(top, whole, col.left * most));
+                f32x4_t d, d_left;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float top = column_top(t), most = __builtin_fmaf(top, D == 128 ? 11.32f : 8.01f, u_top[t]) * 1.001f;
-            const Scale scale(most), after(__builtin_fmaf(top, whole, 64.0f * most));
-            f32x4_t d, d_left;
+                for (int e = 0; e < 4; ++e) {
+                    d[e] = e < mine ? __builtin_fmaf(asked[t][e], -s_from[t], u[t][e]) : 0.0f;
+                    d_left[e] = e < mine ? d[e] * left[e] : 0.0f;
+                    o[t][e] *= through[e] * s_from[t];
+                }
+                d_from[t] = scale.from;
+                s_to[t] = after.to;
+                s_from[t] = after.from;
+                s_least[t] = after.least;
+                const Pair4 x = split4(d * scale.to), y = split4(d_left * scale.to);
+                const int at = (16 * t + m) * kPitchD + 16 * wave + 4 * g;
+                *reinterpret_cast<f16x4_t *>(&dh[0][at]) = x.h;
+                *reinterpret_cast<f16x4_t *>(&dh[1][at]) = x.l;
+                *reinterpret_cast<f16x4_t *>(&rh[0][at]) = y.h;
+                *reinterpret_cast<f16x4_t *>(&rh[1][at]) = y.l;
+            }
+            load_updates(next);
+            lds_barrier();  // every wave's updates are there, and its reads of S done
+            f32x4_t added[NT][kTiles], among[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                among[t] = zero;
+#pragma unroll
+                for (int k = 0; k < kTiles; ++k) added[t][k] = zero;
+            }
+            Pair4 of_r[2][NT], of_d[2][NT];
+            const auto read_d = [&](int b) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
+                    of_r[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
+                    of_d[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
+                }
+            };
+            read_d(0);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (b < 3) read_d(b + 1);
+                __builtin_amdgcn_sched_barrier(kLoadsMayCross);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int k = 0; k < kTiles; ++k) added[t][k] = product(keys[k][b], of_r[b & 1][t], added[t][k]);
+                    if (b <= wave) among[t] = product(inner[b], of_d[b & 1][t], among[t]);
+                }
+                if (!kSpread) load_run(next, b);
+                else if (b >= 2) load_ask(next, b);
+            }
+            if (kSpread) {
+                load_run(next, 0);
+                load_run(next, 1);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int k = 0; k < kTiles; ++k) S[t][k][e] = __builtin_fmaf(added[t][k][e], d_from[t], S[t][k][e] * whole);
+                    o[t][e] = __builtin_fmaf(among[t][e], d_from[t] * (kOne / kWeight), o[t][e]);
+                }
+            load_whole(next);
+            if (kSpread) {
+                load_run(next, 2);
+                load_run(next, 3);
+            }
+            E *to = out + static_cast<int64_t>(chunk) * kGdnChunk * p.out_row;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                d[e] = e < mine ? __builtin_fmaf(asked[t][e], -s_from[t], u[t][e]) : 0.0f;
-                d_left[e] = e < mine ? d[e] * left[e] : 0.0f;
-                o[t][e] *= through[e] * s_from[t];
+                if (e >= mine) continue;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) to[e * p.out_row + 16 * t] = static_cast<E>(o[t][e]);
             }
-            d_from[t] = scale.from;
-            s_to[t] = after.to;
-            s_from[t] = after.from;
-            const Pair4 x = split4(d * scale.to), y = split4(d_left * scale.to);
-            const int at = (16 * t + m) * kPitchD + 16 * wave + 4 * g;
-            *reinterpret_cast<f16x4_t *>(&dh[0][at]) = x.h;
-            *reinterpret_cast<f16x4_t *>(&dh[1][at]) = x.l;
-            *reinterpret_cast<f16x4_t *>(&rh[0][at]) = y.h;
-            *reinterpret_cast<f16x4_t *>(&rh[1][at]) = y.l;
+            chunk += stopped ? 0 : 1;
+        } while (!stopped & (chunk < end));
+        if (!stopped) {
+            if (alone > 0) store_outputs(chunk - 1, alone);
+            alone = 0;
+            looked_at = false;
+            continue;
         }
-        load_updates(next);
-        lds_barrier();  // every wave's updates are there, and its reads of S done
-        f32x4_t added[NT][kTiles], among[NT];
+        // a chunk with rows that go by themselves, or a bound that was too far off: from its beginning again
+        const int rows = min(s.count - chunk * kGdnChunk, kGdnChunk);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            among[t] = zero;
-#pragma unroll
-            for (int k = 0; k < kTiles; ++k) added[t][k] = zero;
+            const int64_t at = chunk * columns_step + 16 * t;
+            const Column col(columns_at[at]);
+            const float top = column_top(t);
+            if (col.exceeded(top)) alone = rows;
+            else if (col.wanting(top)) alone = max(alone, p.faint[columns_at - p.columns + at] + 1);
         }
-        Pair4 of_r[2][NT], of_d[2][NT];
-        const auto read_d = [&](int b) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int at = (16 * t + m) * kPitchD + 16 * b + 4 * g;
-                of_r[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&rh[0][at]), *reinterpret_cast<const f16x4_t *>(&rh[1][at])};
-                of_d[b & 1][t] = {*reinterpret_cast<const f16x4_t *>(&dh[0][at]), *reinterpret_cast<const f16x4_t *>(&dh[1][at])};
-            }
-        };
-        read_d(0);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            if (b < 3) read_d(b + 1);
-            __builtin_amdgcn_sched_barrier(kLoadsMayCross);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int k = 0; k < kTiles; ++k) added[t][k] = product(keys[k][b], of_r[b & 1][t], added[t][k]);
-                if (b <= wave) among[t] = product(inner[b], of_d[b & 1][t], among[t]);
-            }
-            if (!kSpread) load_run(next, b);
-            else if (b >= 2) load_ask(next, b);
-        }
-        if (kSpread) {
-            load_run(next, 0);
-            load_run(next, 1);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int k = 0; k < kTiles; ++k) S[t][k][e] = __builtin_fmaf(added[t][k][e], d_from[t], S[t][k][e] * whole);
-                o[t][e] = __builtin_fmaf(among[t][e], d_from[t], o[t][e]);
-            }
-        load_whole(next);
-        if (kSpread) {
-            load_run(next, 2);
-            load_run(next, 3);
-        }
-        E *to = out + static_cast<int64_t>(chunk) * kGdnChunk * p.out_row;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e >= mine) continue;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) to[e * p.out_row + 16 * t] = static_cast<E>(o[t][e]);
+        alone = max(alone, xor_lane<1>(alone));
+        alone = max(alone, xor_lane<2>(alone));
+        alone = max(alone, xor_lane<4>(alone));
+        alone = __builtin_amdgcn_readfirstlane(max(alone, xor_lane<8>(alone)));
+        lds_barrier();  // every wave has read S and its largest
+        if (alone > 0) go_by_rows(chunk, alone, alone >= rows);
+        looked_at = alone < rows;
+        if (!looked_at) {
+            store_outputs(chunk, rows);
+            alone = 0;
+            ++chunk;
         }
     }
 #pragma unroll

@@ -83,14 +83,15 @@ struct GdnRowsParams {
     bool pairs = false;       // qkv allows two-element accesses
     int few = kGdnFewRows;    // sequences of more rows go through chunks
     // of these, a run of 16 rows and a head at a time (gdn_chunks.hip); numbers as two fp16
-    // halves of x 2^10:
+    // halves of x 2^15 (weights 2^18):
     _Float16 *asks = nullptr;         // [runs][queries over sqrt(head), keys][key_heads], by rows
     _Float16 *keys_by_dim = nullptr;  // [runs][key_heads], by dims
     _Float16 *through = nullptr;      // [runs][value_heads]: W, by rows
     _Float16 *inner = nullptr;        // [runs][value_heads][4]: weights of the chunk's updates, by rows
     float *values = nullptr;          // [runs][value_heads]: V, then U, by dims
     float *chunk_gates = nullptr;     // [runs][value_heads][2][kGdnRun]: decays since the chunk's start, and to its end
-    float *tops = nullptr;            // [runs][value_heads][head]: a chunk's largest |U| of each value dim, at its first run
+    uint32_t *columns = nullptr;      // [runs][value_heads][head]: of a chunk's value dims, at its first run (gdn_chunks.hip)
+    int *faint = nullptr;             // beside them: the last row with too little in its text, -1: none
     float *decay = nullptr;           // [rows][value_heads]: logarithms
     float *rate = nullptr;            // [rows][value_heads]: beta
     int *stands = nullptr;    // [kGdnMaxSequences]

@@ -768,7 +768,10 @@ int fortai_hip_logits_adjust_device(fortai_hip_q8_context *context, int dtype,
  * were.  Rows of qkv (channels), alpha and beta (value_heads) and of the output
  * [value_heads][head] at their pitches in dtype; conv [channels][conv_kernel], ssm_a
  * and ssm_dt [value_heads] in fp32, ssm_a at most 0.  Up to 16 rows of a sequence go one
- * by one, more in chunks of 64 with the same result up to rounding; a NaN, or an infinity in
+ * by one, more in chunks of 64 with the same result up to rounding, whatever the magnitudes:
+ * rows that have less than 2^-20 of a chunk's largest value in their text, with the decays since
+ * (those before a far louder token, or behind one that is forgotten), go one by one too, at
+ * 0.75 us a row.  A NaN, or an infinity in
  * qkv, makes outputs of its sequence not finite from its chunk on.  Sequences up to 16384.
  * copy_slots: slot to[i] becomes a copy of slot from[i] in every layer, pending rows
  * too; host arrays, used before the call returns.  No slot may be written twice, or
