@@ -93,10 +93,10 @@ struct Kv8Plan {
 // costs 30.5 us where two cost 25.9 (eight sequences of up to 8190 tokens); one tile a
 // wave costs 13.2 us where three cost 17.0 (600 tokens).
 inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_t rows, int64_t max_length,
-    int64_t partial_rows = kKv8PartialRows, int workgroups = 512) {
+    int64_t partial_rows = kKv8PartialRows, int workgroups = 512, int least_rows = 8) {
     Kv8Plan p;
     const int64_t heads = static_cast<int64_t>(kv_heads) * sequences;
-    const int few = fp32 || rows <= 8 ? 8 : 16;
+    const int few = fp32 || (rows <= 8 && least_rows <= 8) ? 8 : 16;
     const bool much = rows > 2 * few && (rows + few - 1) / few * heads >= 4096 / ((max_length + 63) / 64 + 1);
     p.rows = much ? 4 * few : few;
     p.row_tiles = static_cast<int>((rows + p.rows - 1) / p.rows);
@@ -130,11 +130,18 @@ inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int gro
         return static_cast<int64_t>(who) * plan.row_tiles * kv_heads * plan.rows * plan.splits;
     };
     // the sequences' own tokens are few: what they leave of the workspace is the groups'
-    p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8SharedRows / 4);
+    const auto cut = [&](int least_rows) {
+        p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8SharedRows / 4, 512, least_rows);
+        const int64_t own = partial(p.own, sequences);
+        const int64_t room = own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0;
+        p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room, 256);
+        if (max_shared / 64 > 12 * p.group.splits) p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room);
+    };
+    cut(8);
+    // groups of up to 16 rows and sequences of up to 8 are one launch where both have workgroups of 16: three answers to
+    // a question of 1000 tokens (16 bits, 4 rows of 4 kv heads) 13.5 us, in two launches 22
+    if (p.own.rows == 8 && p.group.rows == 16) cut(16);
     const int64_t own = partial(p.own, sequences);
-    const int64_t room = own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0;
-    p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room, 256);
-    if (max_shared / 64 > 12 * p.group.splits) p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room);
     p.own_at = (partial(p.group, groups) + 63) / 64 * 64;
     p.shares = max_shared >= 64 && p.own_at + own <= kKv8SharedRows;
     return p;
