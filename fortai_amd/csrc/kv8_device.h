@@ -112,30 +112,53 @@ inline Kv8Plan kv8_plan(bool fp32, int head, int sequences, int kv_heads, int64_
 
 // How a call is cut whose sequences share tokens: the groups' tokens and the sequences'
 // own, which have their partial results behind the groups' from row own_at on.  shares
-// is false where these do not fit.  The groups' tokens are split for one workgroup a CU
-// (half as many partial results to write and join) unless that leaves one more than 12 tiles: 4 kv
-// heads of 256 behind 8000 tokens, eight sequences' rows in fp32 17.9 us against 23.4 for
-// two a CU, 32 sequences' 33.6 against 37.5; 5 rows of 4 in bf16 behind 24,000 (11.7 tiles) 44.0 against
-// 43.6, two groups of 8 (18 tiles) 61 against 41.
+// is false where these do not fit, and where the call would lose by it.
 struct Kv8SharedPlan {
     Kv8Plan own, group;
     int64_t own_at = 0;
     bool shares = false;
 };
 
+// About how long a plan's workgroups take, in turns of the kernels for few rows (four tiles, one a wave): those for many
+// rows take a tile at a time in 0.55 (32 rows) or 0.7 (64) of one, and 1.5 to begin; two a CU take 1.2 times as long.
+inline double kv8_turns(const Kv8Plan &p, int64_t blocks, int64_t tokens, int head) {
+    const bool few = p.rows <= 16;
+    const int64_t tiles = (tokens + 63) / 64, workgroups = blocks * p.splits, chip = 512 * (256 / head);
+    const int64_t turns = (tiles + p.splits * (few ? 4 : 1) - 1) / (p.splits * (few ? 4 : 1));
+    const double each = 0.7 + (few ? turns : p.rows == 32 ? 1.5 + 0.55 * turns : 1.5 + 0.7 * turns);
+    return each * (2 * workgroups > chip ? 1.2 : 1.0) * (workgroups > chip ? static_cast<double>(workgroups) / chip : 1.0);
+}
+
+// The groups' tokens are split for one workgroup a CU (half as many partial results to write and join) unless that
+// leaves one more than 12 tiles: 4 kv heads of 256 behind 8000 tokens, eight sequences' rows in fp32 17.9 us against
+// 23.4 for two a CU, 32 sequences' 33.6 against 37.5; 5 rows of 4 in bf16 behind 24,000 (11.7 tiles) 44.0 against 43.6,
+// two groups of 8 (18 tiles) 61 against 41.
 inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int groups, int kv_heads, int64_t rows, int64_t group_rows,
     int64_t max_own, int64_t max_shared) {
     Kv8SharedPlan p;
-    const auto partial = [&](const Kv8Plan &plan, int who) {
-        return static_cast<int64_t>(who) * plan.row_tiles * kv_heads * plan.rows * plan.splits;
-    };
-    // the sequences' own tokens are few: what they leave of the workspace is the groups'
+    const auto blocks = [&](const Kv8Plan &plan, int who) { return static_cast<int64_t>(who) * plan.row_tiles * kv_heads; };
+    const auto partial = [&](const Kv8Plan &plan, int who) { return blocks(plan, who) * plan.rows * plan.splits; };
+    const int64_t tiles = (max_shared + 63) / 64;
     const auto cut = [&](int least_rows) {
+        // the sequences' own tokens are few: what they leave of the workspace is the groups'
         p.own = kv8_plan(fp32, head, sequences, kv_heads, rows, max_own, kKv8SharedRows / 4, 512, least_rows);
         const int64_t own = partial(p.own, sequences);
         const int64_t room = own < kKv8SharedRows ? kKv8SharedRows - own - 63 : 0;
         p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room, 256);
-        if (max_shared / 64 > 12 * p.group.splits) p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room);
+        if (tiles > 12 * p.group.splits) {
+            p.group = kv8_plan(fp32, head, groups, kv_heads, group_rows, max_shared, room);
+            // no more workgroups than the chip holds: a few more wait until the first ones end (four sequences of 20 rows of
+            // 4 kv heads in fp32 behind 24,000 tokens: 516 workgroups 60.7 us, 504 50)
+            const int64_t most = 512 * (256 / head) / blocks(p.group, groups);
+            if (most > 0 && most < p.group.splits) p.group.splits = static_cast<int>(most);
+        } else if (p.group.rows <= 16) {
+            // up to a quarter more workgroups where that saves their last turn of four tiles (four sequences of 20 rows in
+            // fp32 behind 8000 tokens of 2 kv heads: 15 splits of 2.08 turns 24.4 us, 16 20.2)
+            const int64_t turns = tiles / (4 * p.group.splits), splits = turns > 0 ? (tiles + 4 * turns - 1) / (4 * turns) : 0;
+            if (splits > p.group.splits && 4 * splits <= 5 * static_cast<int64_t>(p.group.splits) && splits <= kKv8MaxSplits &&
+                splits * blocks(p.group, groups) * p.group.rows <= room)
+                p.group.splits = static_cast<int>(splits);
+        }
     };
     cut(8);
     // groups of up to 16 rows and sequences of up to 8 are one launch where both have workgroups of 16: three answers to
@@ -143,7 +166,15 @@ inline Kv8SharedPlan kv8_shared_plan(bool fp32, int head, int sequences, int gro
     if (p.own.rows == 8 && p.group.rows == 16) cut(16);
     const int64_t own = partial(p.own, sequences);
     p.own_at = (partial(p.group, groups) + 63) / 64 * 64;
-    p.shares = max_shared >= 64 && p.own_at + own <= kKv8SharedRows;
+    // Where the plain call is one launch and so few tokens are shared, the join costs more than they do: 2 to 46 sequences
+    // behind 64 to 256 tokens 10.6 to 26 us, by themselves 6.7 to 14.  Otherwise sharing has to be as fast, by the turns
+    // of both, as nearly as they tell (two sequences of 20 rows of 2 kv heads in bf16 behind 24,000 tokens 29 us, by
+    // themselves 24; where they tell too much it costs up to a fifth, on average of 700 cases nothing).
+    const Kv8Plan plain = kv8_plan(fp32, head, sequences, kv_heads, rows, max_shared + max_own);
+    const bool little = plain.splits == 1 && max_shared <= 256;
+    const bool slower = kv8_turns(p.group, blocks(p.group, groups), max_shared, head) >
+        1.3 * kv8_turns(plain, blocks(plain, sequences), max_shared + max_own, head);
+    p.shares = max_shared >= 64 && p.own_at + own <= kKv8SharedRows && !little && !slower;
     return p;
 }
 
