@@ -296,10 +296,13 @@ class Context:
                    "fortai_hip_q8_tokens_read_device")
 
     def adjust_logits(self, logits, vocab: int, out, row_starts, sequences: int, rows: int, dtype: str = "f32", tokens=None,
-                      history=None, history_pitch: int = 0, history_lengths=None, window: int = 0, penalties=None, bias=None,
+                      history=None, history_pitch: Optional[int] = None, history_lengths=None, window: int = 0, penalties=None, bias=None,
                       bias_pitch: int = 0, masks=None, mask_count: int = 0, mask_pitch: Optional[int] = None, mask_of=None,
                       pitch: Optional[int] = None, out_pitch: Optional[int] = None) -> None:
-        """Penalties for repeated tokens, biases and masks on logits [rows][vocab] (fortai_hip_logits_adjust_device)."""
+        """Penalties for repeated tokens, biases and masks on logits [rows][vocab] (fortai_hip_logits_adjust_device).  A
+        history [sequences][history_pitch] comes with its pitch, which is all of a sequence's that can count."""
+        if history_pitch is None:
+            history_pitch = 0 if history is None else -1  # refused: a pitch of nothing would count nothing
         rules = LogitRules(window, mask_count, _dev(penalties), _dev(tokens), _dev(history), _dev(history_lengths), _dev(bias),
                            _dev(masks), _dev(mask_of), history_pitch, bias_pitch,
                            (vocab + 31) // 32 if mask_pitch is None else mask_pitch)

@@ -716,8 +716,8 @@ int fortai_hip_q8_tokens_read_device(fortai_hip_q8_context *context, int dtype,
  *   x += bias;  tokens that the row's mask does not allow: -infinity
  * device_row_starts (int32 [sequences + 1]) and device_tokens (int64 [rows], may be
  * NULL) are those of fortai_hip_verify_drafts_device.  device_history: int64
- * [sequences] at history_pitch, of which device_history_lengths[s] (int32) count, or
- * NULL.  device_penalties: fp32 [sequences][repetition above 0, frequency, presence],
+ * [sequences] at history_pitch, of which device_history_lengths[s] (int32, up to the
+ * pitch) count, or NULL.  device_penalties: fp32 [sequences][repetition above 0, frequency, presence],
  * or NULL for none.  device_bias: fp32 [vocab] a sequence at bias_pitch (0: one for
  * all), or NULL.  device_masks: mask_count masks at mask_pitch words of 32 bits, a
  * bit a token, the lowest first, set where it is allowed; device_mask_of (int32
