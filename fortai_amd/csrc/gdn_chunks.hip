@@ -244,7 +244,8 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
         for (int k = 0; k < 4; ++k) x[kTaps - 1 + k] = ahead[k];
 #pragma unroll
         for (int k = 0; k < 4; ++k) ahead[k] = input(i0 + min(4 * four + 4, kRun - 4) + k);
-        f32x4_t y[2];  // this lane's dims, four rows
+        f32x4_t y[2], inverse;  // this lane's dims, four rows
+        float most_sum = 0.0f, least_sum = 1.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float u0 = 0.0f, u1 = 0.0f;
@@ -256,10 +257,33 @@ __global__ __launch_bounds__(256) void gdn_inputs_kernel(const GdnRowsParams p) 
                 }
             u0 = gdn_silu(u0);
             u1 = gdn_silu(u1);
+            y[0][i] = u0;
+            y[1][i] = u1;
             const float sum = group_sum_up(u0 * u0 + u1 * u1, kHeadLanes);
-            const float inverse = is_value ? 1.0f : fminf(__builtin_amdgcn_rsqf(sum) * one, most);
-            y[0][i] = u0 * inverse;
-            y[1][i] = u1 * inverse;
+            inverse[i] = fminf(__builtin_amdgcn_rsqf(sum) * one, most);
+            most_sum = fmaxf(most_sum, sum);
+            least_sum = fminf(least_sum, sum);
+        }
+        if (__any((gdn_length_is_lost(most_sum, p.eps) | gdn_length_is_lost(least_sum, p.eps)) & !is_value)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float top = fmaxf(fabsf(y[0][i]), fabsf(y[1][i]));
+                top = fmaxf(top, xor_lane<1>(top));
+                top = fmaxf(top, xor_lane<2>(top));
+                top = fmaxf(top, xor_lane<4>(top));
+                top = fmaxf(top, xor_lane<8>(top));
+                top = fmaxf(top, xor_lane<16>(top));
+                if constexpr (kHeadLanes == 64) top = fmaxf(top, xor_lane<32>(top));
+                const int e = is_value ? 0 : __builtin_amdgcn_frexp_expf(top);
+                y[0][i] = __builtin_ldexpf(y[0][i], -e);
+                y[1][i] = __builtin_ldexpf(y[1][i], -e);
+                const float near_one = group_sum_up(y[0][i] * y[0][i] + y[1][i] * y[1][i], kHeadLanes);
+                inverse[i] = fminf(__builtin_amdgcn_rsqf(near_one) * one, one / __builtin_ldexpf(p.eps, -e));
+            }
+        }
+        if (!is_value) {
+            y[0] *= inverse;
+            y[1] *= inverse;
         }
 #pragma unroll
         for (int j = 0; j + 1 < kTaps; ++j) x[j] = x[j + 4];

@@ -52,6 +52,10 @@ __device__ __forceinline__ float gdn_log_decay(float a, float alpha, float dt) {
     return log < -256.0 ? -256.0f : static_cast<float>(log);
 }
 
+// Whether a sum of squares may have left fp32 where the length has not, or be short of its smallest parts where epsilon is
+// smaller still: then the numbers are brought near 1 first.
+__device__ __forceinline__ bool gdn_length_is_lost(float sum, float eps) { return !(sum < 0x1p126f) | ((sum < 0x1p-90f) & (eps < 0x1p-44f)); }
+
 __device__ __forceinline__ float gdn_sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
 // The inputs of a channel that a slot keeps, written by one thread: behind a sequence

@@ -169,7 +169,22 @@ __global__ __launch_bounds__(ROWS * 8) void gdn_few_kernel(const GdnRowsParams p
             sum += x[k] * x[k];
         }
         sum = wave_sum(sum);
-        float inverse = 1.0f / fmaxf(sqrtf(sum), p.eps);
+        float eps = p.eps;
+        if (gdn_length_is_lost(sum, eps)) {
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) top = fmaxf(top, fabsf(x[k]));
+            const int e = __builtin_amdgcn_frexp_expf(wave_max(top));
+            sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) {
+                x[k] = __builtin_ldexpf(x[k], -e);
+                sum += x[k] * x[k];
+            }
+            sum = wave_sum(sum);
+            eps = __builtin_ldexpf(eps, -e);
+        }
+        float inverse = 1.0f / fmaxf(sqrtf(sum), eps);
         if (i < r) inverse *= 1.0f / sqrtf(static_cast<float>(D));
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) v[64 * k + lane] = x[k] * inverse;
