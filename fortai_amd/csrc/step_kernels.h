@@ -104,6 +104,5 @@ hipError_t launch_gdn_few(const GdnRowsParams &p, Dtype dtype, hipStream_t strea
 hipError_t launch_gdn_many(const GdnRowsParams &p, Dtype dtype, hipStream_t stream);
 // slots to[i] become copies of slots from[i], in every layer (host arrays); cache: the first layer
 hipError_t launch_gdn_copy_slots(const GdnView &cache, int layers, const int32_t *from, const int32_t *to, int count, hipStream_t stream);
-hipError_t launch_gdn_clear(void *storage, size_t bytes, hipStream_t stream);
 
 }  // namespace fortai_hip
