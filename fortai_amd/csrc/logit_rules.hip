@@ -14,7 +14,7 @@
 // Bound by the bytes of the rows, by the first count of a long text (every chunk's workgroup
 // reads it again, from L2) and, for one row, by a launch's latency.  33 rows of 248,320 of
 // eight sequences in fp32 (67 MB) behind texts of up to 8000 tokens, with biases and masks:
-// 22 us; one row of 16,384 4.2 us.
+// 22 us; one row of 16,384 5.0 us.
 #include "fortai_hip_internal.h"
 #include "kv8_device.h"
 #include "step_kernels.h"
@@ -209,8 +209,8 @@ hipError_t rules_typed(const LogitRulesParams &p, hipStream_t stream) {
     // 26.0 (20.8)
     const int average = (p.rows + p.sequences - 1) / p.sequences, parts = (average + 2) / 3;
     const int64_t groups = static_cast<int64_t>(p.sequences) * parts;
-    // chunks of 4096 where they fill the chip (33 rows of 248,320 21.5 us, of 1024 30.7), otherwise of 1024 (one row 7.3 us
-    // against 9.1, four sequences' 9.2 against 9.6)
+    // chunks of 4096 where they fill the chip (33 rows of 248,320 21.5 us, of 1024 30.7), otherwise of 1024 (of the same
+    // rows, behind as long a text: one 7.3 us against 9.1, four sequences' 9.2 against 9.6)
     if (groups * ((p.vocab + 4095) / 4096) >= 256)
         hipLaunchKernelGGL((logit_rules_kernel<DT, VEC, 4096>), dim3((p.vocab + 4095) / 4096, p.sequences, parts), dim3(kRuleThreads), 0, stream, p);
     else

@@ -523,7 +523,8 @@ int fortai_hip_rope_device(fortai_hip_rope *rope, int dtype, const void *device_
  *   value codes  [layers][pages][kv_heads][head_size][page_tokens]
  *   key magnitudes, then value magnitudes, fp32 [layers][pages][kv_heads].
  * create: over the caller's device storage, which is taken as it is and stays
- * the caller's, or with NULL over storage of its own, cleared.
+ * the caller's, or with NULL over storage of its own, cleared.  Beside it a cache has
+ * room for 32,768 partial results of attention, 131,072 (head_size + 4) bytes.
  *
  * A batch says which rows of a call belong to which sequence and where its
  * tokens lie.  Rows row_starts[s] .. row_starts[s + 1] - 1 are sequence s's next
@@ -696,7 +697,10 @@ int fortai_hip_verify_drafts_device(fortai_hip_verifier *verifier, int dtype,
  * fortai_hip_q8_quantize_tokens_device does.  For a block of 32 values with m their
  * largest magnitude the scale is m / 127 rounded to fp32, then to fp16, the codes are
  * 127 y / m rounded to fp32, then to the nearest integer, ties to even; all in 64 bits up to
- * there.  A block with a NaN or an infinity has a scale of NaN.  The buffer's rows
+ * there.  (fortai_hip_q8_quantize_tokens_device, which the decoders use, rounds
+ * x * (127 / m) in fp32: where a quotient is next to a half, one code in some 10^4, the two
+ * differ by one, so a step through these calls does not have the decoders' bits.)
+ * A block with a NaN or an infinity has a scale of NaN.  The buffer's rows
  * past `rows` are not written (no product's output depends on them).  device_sum may be x or the
  * residual itself (same pitch).  width: a multiple of 32, up to 2^20.
  * tokens_read: the values code * scale of such a buffer as rows of dtype. */
@@ -756,7 +760,9 @@ int fortai_hip_logits_adjust_device(fortai_hip_q8_context *context, int dtype,
  * create: over the caller's device storage, which is taken as it is and stays the
  * caller's, or with NULL over storage of its own, cleared (states of sequences that
  * begin).  head_size 64 or 128; conv_kernel 2 to 8; pending 0 to 16; a call's rows up
- * to max_rows (to 2^19), for which workspaces are made.
+ * to max_rows (to 2^19), for which workspaces are made beside the storage: 64 KiB for
+ * key_heads + 1 each, and where max_rows is above 16 about 1.94 ((12 key_heads + 8.5
+ * value_heads) head_size + 264 value_heads) bytes a row, 132 KB with 16 and 32 heads of 128.
  *
  * Rows row_starts[s] .. row_starts[s + 1] - 1 of a batch are sequence s's next tokens,
  * slots[s] is its state; two sequences of a batch must not have the same.  Up to
